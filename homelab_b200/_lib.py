@@ -25,6 +25,8 @@ F32 = 0
 BF16 = 1
 SCALE_1X128 = 0
 SCALE_128X128 = 1
+KV_BF16 = 0
+KV_E4M3 = 1
 TABLES_READY = 1
 NOALLOC_SCRATCH_BYTES = 8 * 1024 * 1024
 PART_ALIGN = 256
@@ -72,6 +74,26 @@ class SharedExpert(C.Structure):
         ("hidden", C.c_int32), ("inter", C.c_int32), ("scale_layout", C.c_int32), ("pad_", C.c_int32),
         ("gate_up_q", C.c_void_p), ("gate_up_scale", C.c_void_p),
         ("down_q", C.c_void_p), ("down_scale", C.c_void_p), ("gate_w", C.c_void_p),
+    ]
+
+
+class RopeStruct(C.Structure):
+    """oomb_rope: rotated width, pair layout, factor and device frequencies."""
+
+    _fields_ = [
+        ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("mscale", C.c_float), ("pad_", C.c_int32),
+        ("turns", C.c_void_p),
+    ]
+
+
+class PagedKvStruct(C.Structure):
+    """oomb_paged_kv: a pool of pages and the block table over it."""
+
+    _fields_ = [
+        ("dtype", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+        ("num_pages", C.c_int32), ("max_pages", C.c_int32), ("table_stride", C.c_int32), ("pad_", C.c_int32),
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+        ("page_stride", C.c_int64), ("exp_page_stride", C.c_int64), ("block_table", C.c_void_p),
     ]
 
 
@@ -154,6 +176,17 @@ SIGNATURES = [
     ("oomb_moe_layer_workspace_bytes", Z, [I, C.POINTER(MoeLayer), C.POINTER(SharedExpert), I]),
     ("oomb_moe_layer_decode_fp8", I, [C.POINTER(MoeLayer), C.POINTER(SharedExpert), P, I, I, P, I, P, P, P, Z,
                                       S]),
+    ("oomb_rope_turns", I, [I, C.c_double, I, C.c_double, C.c_int64, P, C.POINTER(C.c_float)]),
+    ("oomb_rope_rows", I, [C.POINTER(RopeStruct), P, I, C.c_int64, P, P, C.c_int64, I, I, I, S]),
+    ("oomb_kv_append_paged", I, [C.POINTER(PagedKvStruct), C.POINTER(RopeStruct), P, C.c_int64, P, C.c_int64, I, P,
+                                 C.c_int64, P, C.c_int64, I, P, P, I, I, S]),
+    ("oomb_kv_read_paged", I, [C.POINTER(PagedKvStruct), P, P, I, I, P, P, I, C.c_int64, S]),
+    ("oomb_attention_paged_workspace_bytes", Z, [I, I, I, I, I, I]),
+    ("oomb_attention_paged", I, [C.POINTER(PagedKvStruct), P, C.c_int64, P, C.c_int64, I, P, P, I, I, I, C.c_float,
+                                 P, Z, S]),
+    ("oomb_attention_prompt_workspace_bytes", Z, [I, I, I, I, I, I]),
+    ("oomb_attention_prompt", I, [P, C.c_int64, P, C.c_int64, P, C.c_int64, P, C.c_int64, I, I, I, P, I, I, I,
+                                  C.c_float, P, Z, S]),
     ("oomb_attention_decode", I, [P, I, P, P, C.c_int64, P, I, P, I, I, I, I, I, I, C.c_float, P, Z, S]),
 ]
 

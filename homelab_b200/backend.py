@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import BF16, F32, SCALE_128X128, SCALE_1X128, Fp8Record, MoeLayer, check
+from .paged import PagedKv, RopePlan
 
 __all__ = ["Gpu", "Fp8Record", "MoeLayer", "SCALE_1X128", "SCALE_128X128", "F32", "BF16"]
 
@@ -62,6 +63,7 @@ class Gpu:
         self.device = torch.device("cuda", device)
         self.L = _lib.lib()
         self._tiled_ws = None  # grown on demand by moe_tiled calls without a workspace
+        self._attn_ws = {}     # per stream, grown on demand by paged and prompt attention without a workspace
 
     def _stream(self) -> int:
         return torch.cuda.current_stream(self.device).cuda_stream
@@ -242,6 +244,163 @@ class Gpu:
         starts, all_start = (None, int(start)) if isinstance(start, int) else (_ptr(start), 0)
         check(self.L.oomb_kv_append(_ptr(src), _dtype_code(src), src.stride(0), _ptr(cache), cache.stride(0), starts,
                                     all_start, B, t, Hkv, D, kv_max, self._stream()), "kv_append")
+
+    # ---- rotary positions and the paged cache --------------------------------------------
+
+    def rope_plan(self, rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                  original_len: int = 0, interleaved: bool = False) -> RopePlan:
+        """The frequencies of a rotation on this device (oomb_rope_turns), made once per model."""
+        return RopePlan(self.device, rot_dim, base, scaling, factor, original_len, interleaved)
+
+    def _rows(self, x, heads: int, dim: int, t: int, what: str, dtypes=(torch.float32, torch.bfloat16)):
+        """Checks a [t, heads, dim] tensor on this device with contiguous rows; its address and token stride."""
+        if x.dtype not in dtypes:
+            raise TypeError(f"{what} must be one of {dtypes}, got {x.dtype}")
+        if tuple(x.shape) != (t, heads, dim):
+            raise ValueError(f"{what} must be [{t}, {heads}, {dim}], got {tuple(x.shape)}")
+        if x.device != self.device:
+            raise ValueError(f"{what} must live on {self.device}, got {x.device}")
+        if t and (x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim)):
+            raise ValueError(f"the heads of a token of {what} must be contiguous")
+        return _ptr(x), (x.stride(0) if t > 1 else heads * dim)
+
+    def _index(self, x, n, what: str):
+        if x is None:
+            return None
+        if x.dtype != torch.int32 or not x.is_contiguous() or x.device != self.device or (
+                x.dim() != 1 or (n is not None and x.numel() != n)):
+            raise ValueError(f"{what} must be a contiguous int32 [{'B' if n is None else n}] tensor on {self.device}")
+        return _ptr(x)
+
+    def _step(self, cache: PagedKv, q_start, kv_len, t: int):
+        """The batch of a packed step over `cache` and its index addresses."""
+        if cache.device != self.device:
+            raise ValueError(f"the cache must live on {self.device}, got {cache.device}")
+        B = kv_len.numel()
+        if cache.batch < B:
+            raise ValueError(f"the block table has {cache.batch} rows for {B} sequences")
+        if q_start is None and B != t:
+            raise ValueError("without q_start every sequence has one token")
+        return B, self._index(q_start, B + 1, "q_start"), self._index(kv_len, B, "kv_len")
+
+    def rope(self, x, positions, plan: RopePlan, out=None):
+        """out[t, h] = x[t, h] rotated by positions[t] (x, out [T, H, D] fp32 or bf16; out may be x)."""
+        if x.dim() != 3:
+            raise ValueError("x must be [T, H, D]")
+        T, H, D = x.shape
+        if out is None:
+            out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+        xp, xs = self._rows(x, H, D, T, "x")
+        op, os_ = self._rows(out, H, D, T, "out", (x.dtype,))
+        pos = self._index(positions, T, "positions")
+        if T == 0:
+            return out
+        with torch.cuda.device(self.device):
+            check(self.L.oomb_rope_rows(C.byref(plan.struct), xp, _dtype_code(x), xs, pos, op, os_, T, H, D,
+                                        self._stream()), "rope")
+        return out
+
+    def kv_append_paged(self, cache: PagedKv, k, v, q_start, kv_len, rope: RopePlan = None, q=None, q_out=None):
+        """Writes a packed step's keys and values into their pages, the keys (and the queries q, to
+        q_out in bf16) rotated when a plan is given.  k, v [T, kv_heads, D], q [T, H, D] fp32 or bf16, views
+        of a fused projection's rows included; q_start int32 [B + 1] or None (one token a sequence);
+        kv_len int32 [B] counts the new tokens."""
+        T, D = k.shape[0], cache.head_dim
+        kp, ks = self._rows(k, cache.kv_heads, D, T, "k")
+        vp, vs = self._rows(v, cache.kv_heads, D, T, "v", (k.dtype,))
+        B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
+        qp = qo = None
+        qs = qos = H = 0
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out go together")
+        if q is not None:
+            H = q.shape[1]
+            qp, qs = self._rows(q, H, D, T, "q", (k.dtype,))
+            qo, qos = self._rows(q_out, H, D, T, "q_out", (torch.bfloat16,))
+        if T == 0 or B == 0:
+            return
+        with torch.cuda.device(self.device):
+            check(self.L.oomb_kv_append_paged(C.byref(cache.struct), C.byref(rope.struct) if rope is not None else None,
+                                              qp, qs, qo, qos, H, kp, ks, vp, vs, _dtype_code(k), qs_p, len_p, B, T,
+                                              self._stream()), "kv_append_paged")
+
+    def kv_read_paged(self, cache: PagedKv, q_start, kv_len, k_out, v_out):
+        """The cached rows at a packed step's positions (the last n_b of each sequence's kv_len) into
+        k_out, v_out [T, kv_heads, D], fp32 or bf16."""
+        T, D = k_out.shape[0], cache.head_dim
+        kp, ks = self._rows(k_out, cache.kv_heads, D, T, "k_out")
+        vp, vs = self._rows(v_out, cache.kv_heads, D, T, "v_out", (k_out.dtype,))
+        if ks != vs:
+            raise ValueError("k_out and v_out must be strided alike")
+        B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
+        if T == 0 or B == 0:
+            return
+        with torch.cuda.device(self.device):
+            check(self.L.oomb_kv_read_paged(C.byref(cache.struct), qs_p, len_p, B, T, kp, vp, _dtype_code(k_out), ks,
+                                            self._stream()), "kv_read_paged")
+
+    def attention_paged_workspace(self, batch: int, t: int, max_q: int, heads: int, kv_heads: int,
+                                  head_dim: int) -> torch.Tensor:
+        """A zeroed workspace for attention_paged and attention_prompt calls of at most these sizes."""
+        with torch.cuda.device(self.device):
+            n = max(int(f(batch, t, max_q, heads, kv_heads, head_dim)) for f in
+                    (self.L.oomb_attention_paged_workspace_bytes, self.L.oomb_attention_prompt_workspace_bytes))
+        if n == 0:
+            raise ValueError("unsupported attention shape")
+        return torch.zeros(n, dtype=torch.uint8, device=self.device)
+
+    def _attention_ws(self, need: int) -> torch.Tensor:
+        """A workspace of this object's for the current stream.  A graph gets one of its own, so that graphs
+        (and eager calls beside them) never share one."""
+        if need == 0:
+            raise ValueError("unsupported attention shape")
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(need, dtype=torch.uint8, device=self.device)
+        s = self._stream()
+        ws = self._attn_ws.get(s)
+        if ws is None or ws.numel() < need:
+            ws = self._attn_ws[s] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return ws
+
+    def attention_paged(self, q, cache: PagedKv, out, q_start, kv_len, max_q: int, scale: float, workspace=None):
+        """Causal attention of the packed new tokens over their sequences' pages (oomb_attention_paged):
+        q, out bf16 [T, H, D]; q_start int32 [B + 1] or None (one token a sequence); kv_len int32 [B]
+        counts the new tokens; max_q bounds a sequence's new tokens.  Without a workspace one is
+        kept per stream and grown as needed."""
+        T, H, D = q.shape
+        if D != cache.head_dim:
+            raise ValueError(f"q has head_dim {D}, the cache {cache.head_dim}")
+        qp, qs = self._rows(q, H, D, T, "q", (torch.bfloat16,))
+        op, os_ = self._rows(out, H, D, T, "out", (torch.bfloat16,))
+        B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
+        if T == 0 or B == 0:
+            return
+        with torch.cuda.device(self.device):
+            ws = workspace
+            if ws is None:
+                ws = self._attention_ws(int(self.L.oomb_attention_paged_workspace_bytes(B, T, max_q, H, cache.kv_heads, D)))
+            check(self.L.oomb_attention_paged(C.byref(cache.struct), qp, qs, op, os_, H, qs_p, len_p, B, T, int(max_q),
+                                              float(scale), _ptr(ws), ws.numel(), self._stream()), "attention_paged")
+
+    def attention_prompt(self, q, k, v, out, q_start, max_q: int, scale: float, workspace=None):
+        """Causal attention over packed whole prompts (oomb_attention_prompt): q, out bf16 [T, H, D],
+        k, v bf16 [T, kv_heads, D], q_start int32 [B + 1]; max_q bounds a prompt's tokens."""
+        T, H, D = q.shape
+        Hkv = k.shape[1]
+        qp, qs = self._rows(q, H, D, T, "q", (torch.bfloat16,))
+        kp, ks = self._rows(k, Hkv, D, T, "k", (torch.bfloat16,))
+        vp, vs = self._rows(v, Hkv, D, T, "v", (torch.bfloat16,))
+        op, os_ = self._rows(out, H, D, T, "out", (torch.bfloat16,))
+        qs_p = self._index(q_start, None, "q_start")
+        B = q_start.numel() - 1
+        if T == 0 or B <= 0:
+            return
+        with torch.cuda.device(self.device):
+            ws = workspace
+            if ws is None:
+                ws = self._attention_ws(int(self.L.oomb_attention_prompt_workspace_bytes(B, T, max_q, H, Hkv, D)))
+            check(self.L.oomb_attention_prompt(qp, qs, kp, ks, vp, vs, op, os_, H, Hkv, D, qs_p, B, T, int(max_q),
+                                               float(scale), _ptr(ws), ws.numel(), self._stream()), "attention_prompt")
 
     def device_error(self, clear: bool = True) -> int:
         code = C.c_int(0)

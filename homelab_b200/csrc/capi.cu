@@ -10,13 +10,13 @@
 #include <string.h>
 
 #include <mutex>
-#include <unordered_map>
 
 #include "../../include/oomb.h"
 #include "attn.cuh"
 #include "combine.cuh"
 #include "decode.cuh"
 #include "ep.cuh"
+#include "host.cuh"
 #include "quant.cuh"
 #include "route.cuh"
 #include "stream.cuh"
@@ -53,17 +53,10 @@ namespace {
 // Device error word: bounded waits that run out record a code here.
 __device__ unsigned g_device_error;
 
-constexpr int kMaxDevices = 64;
-
-struct DeviceState {
-    bool init = false;
-    bool ok = false;
-    int sms = 0;
-    unsigned* err = nullptr;
-};
-
 DeviceState g_dev[kMaxDevices];
 std::mutex g_dev_mu;
+
+}  // namespace
 
 // Per-device state: SM count, error-word address, sm_100 check.
 const DeviceState* device_state() {
@@ -86,67 +79,7 @@ const DeviceState* device_state() {
     return d.ok ? &d : nullptr;
 }
 
-// Opts a kernel into more than 48 KB of dynamic shared memory, once per
-// (kernel, device): calls made later (for instance during CUDA graph capture)
-// find it done and touch nothing but the stream.
-std::mutex g_attr_mu;
-std::unordered_map<const void*, size_t> g_attr_done[kMaxDevices];
-
-template <typename Kernel>
-bool set_smem(Kernel k, size_t bytes) {
-    // the default limit covers static and dynamic shared memory together
-    if (bytes <= 40 * 1024) return true;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
-    const void* key = reinterpret_cast<const void*>(k);
-    std::lock_guard<std::mutex> lk(g_attr_mu);
-    auto it = g_attr_done[dev].find(key);
-    if (it != g_attr_done[dev].end() && it->second >= bytes) return true;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) !=
-        cudaSuccess)
-        return false;
-    g_attr_done[dev][key] = bytes;
-    return true;
-}
-
-template <typename Kernel, typename... Args>
-int launch(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
-    if (!set_smem(kernel, smem)) return OOMB_E_LAUNCH;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? OOMB_OK : OOMB_E_LAUNCH;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// Where a caller's buffer lives.  Pinned host memory (cudaHostAlloc,
-// cudaHostRegister) is reachable from kernels at its mapped device address;
-// pageable host memory and unknown pointers are reachable by no kernel.
-enum class Mem { none, device, host };
-Mem mem_kind(const void* p, const void** dev) {
-    cudaPointerAttributes a{};
-    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return Mem::none;
-    }
-    if (a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged) {
-        *dev = p;
-        return Mem::device;
-    }
-    if (a.type == cudaMemoryTypeHost && a.devicePointer) {
-        *dev = a.devicePointer;
-        return Mem::host;
-    }
-    return Mem::none;
-}
+namespace {
 
 // ---- streaming kernels ----------------------------------------------------------
 
@@ -260,24 +193,6 @@ int launch_down(const DeviceState* d, const uint64_t* recs, const int32_t* off, 
 
 // ---- tensor-core path ------------------------------------------------------------
 
-// cuTensorMapEncodeTiled, fetched once from the driver through the runtime (the
-// library links only the CUDA runtime).
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-    static EncodeTiledFn fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            return static_cast<EncodeTiledFn>(nullptr);
-        return reinterpret_cast<EncodeTiledFn>(f);
-    }();
-    return fn;
-}
-
 // Tensor map of a byte matrix [rows, k] (row-major) in boxes of 128 bytes x
 // box_rows rows with the 128-byte swizzle the MMA descriptors expect: e4m3
 // weights (box 128 x 128; packed tiles are a [tiles * 128, 128] matrix) and the
@@ -304,7 +219,6 @@ bool encode_fp8_tiles(CUtensorMap* map, const uint8_t* q, int rows, int k) {
     return encode_u8_tiles(map, q, rows, k, kTcTile);
 }
 
-size_t align256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
 // The activation split of one call: terms image [rows_alloc, k] and term scales
 // [k/128][tc_sx_stride(rows_alloc)] at the given workspace offsets.
@@ -825,7 +739,9 @@ int oomb_device_error(int* code, int clear) {
 int oomb_set_wait_limit(uint64_t ns) {
     if (!device_state()) return OOMB_E_DEVICE;
     const unsigned long long v = ns ? static_cast<unsigned long long>(ns) : kWaitLimitNs;
-    return cudaMemcpyToSymbol(g_wait_limit_ns, &v, sizeof(v)) == cudaSuccess ? OOMB_OK : OOMB_E_LAUNCH;
+    return cudaMemcpyToSymbol(g_wait_limit_ns, &v, sizeof(v)) == cudaSuccess && paged_set_wait_limit(v) == cudaSuccess
+               ? OOMB_OK
+               : OOMB_E_LAUNCH;
 }
 
 int oomb_gemm_fp8(const void* x, int x_dtype, const uint8_t* q, const float* scale,

@@ -1,0 +1,346 @@
+// paged.cu - the extern "C" entry points of rotary positions, the paged key/value cache
+// and the attention over it (declared in include/oomb.h).  Argument checks run on the
+// host before any launch; a call with nothing to do launches nothing.
+#include <math.h>
+
+#include "host.cuh"
+#include "paged.cuh"
+#include "pattn.cuh"
+
+namespace oomb {
+
+cudaError_t paged_set_wait_limit(unsigned long long ns) { return cudaMemcpyToSymbol(g_wait_limit_ns, &ns, sizeof(ns)); }
+
+namespace {
+
+bool dtype_ok(int t) { return t == OOMB_F32 || t == OOMB_BF16; }
+bool head_dim_ok(int d) { return d == 64 || d == 128; }
+
+// A token stride (elements) that keeps every row 16-byte aligned and apart from the next.
+int check_rows(const void* p, int64_t stride, int64_t row, int dtype) {
+    if (stride < row) return OOMB_E_SHAPE;
+    if (!aligned16(p) || stride % (dtype == OOMB_F32 ? 4 : 8)) return OOMB_E_ALIGN;
+    return OOMB_OK;
+}
+
+int check_rope(const oomb_rope* r, int head_dim) {
+    if (!r->turns || (r->interleaved != 0 && r->interleaved != 1)) return OOMB_E_ARG;
+    if (!(r->mscale > 0.0f) || !(r->mscale <= 1024.0f)) return OOMB_E_ARG;
+    if (r->rot_dim <= 0 || r->rot_dim % 16 || r->rot_dim > head_dim) return OOMB_E_SHAPE;
+    if (reinterpret_cast<uintptr_t>(r->turns) & 7u) return OOMB_E_ALIGN;
+    return OOMB_OK;
+}
+
+int check_cache(const oomb_paged_kv* c, KvView& v) {
+    if (!c || !c->k || !c->v || !c->block_table) return OOMB_E_ARG;
+    if (c->dtype != OOMB_KV_BF16 && c->dtype != OOMB_KV_E4M3) return OOMB_E_ARG;
+    if (c->kv_heads <= 0 || !head_dim_ok(c->head_dim) || c->num_pages <= 0 || c->max_pages < 0 ||
+        c->table_stride < c->max_pages)
+        return OOMB_E_SHAPE;
+    int lg = 4;
+    while (lg < 7 && (1 << lg) != c->page_size) lg++;
+    if ((1 << lg) != c->page_size) return OOMB_E_SHAPE;
+    if ((static_cast<int64_t>(c->max_pages) << lg) > (1 << 30)) return OOMB_E_SHAPE;
+    const int64_t rows = static_cast<int64_t>(c->kv_heads) << lg;
+    if (c->page_stride < rows * c->head_dim) return OOMB_E_SHAPE;
+    const bool fp8 = c->dtype == OOMB_KV_E4M3;
+    if (!aligned16(c->k) || !aligned16(c->v) || c->page_stride % (fp8 ? 16 : 8)) return OOMB_E_ALIGN;
+    if (reinterpret_cast<uintptr_t>(c->block_table) & 3u) return OOMB_E_ALIGN;
+    if (fp8) {
+        if (!c->k_exp || !c->v_exp) return OOMB_E_ARG;
+        if (c->exp_page_stride < rows) return OOMB_E_SHAPE;
+        if (!aligned16(c->k_exp) || !aligned16(c->v_exp) || c->exp_page_stride % 16) return OOMB_E_ALIGN;
+    }
+    v = KvView{};
+    v.k = static_cast<const uint8_t*>(c->k);
+    v.v = static_cast<const uint8_t*>(c->v);
+    v.ke = c->k_exp;
+    v.ve = c->v_exp;
+    v.page_stride = c->page_stride;
+    v.exp_stride = c->exp_page_stride;
+    v.table = c->block_table;
+    v.table_stride = c->table_stride;
+    v.max_pages = c->max_pages;
+    v.num_pages = c->num_pages;
+    v.page_log2 = lg;
+    v.Hkv = c->kv_heads;
+    return OOMB_OK;
+}
+
+template <int D, int CACHE>
+int launch_rows_d(bool xb, const RowsParams& p, cudaStream_t s) {
+    const dim3 grid(static_cast<unsigned>((p.T + p.tpb - 1) / p.tpb));
+    return xb ? launch(rows_kernel<true, D, CACHE>, grid, dim3(kRowsThreads), 0, s, p)
+              : launch(rows_kernel<false, D, CACHE>, grid, dim3(kRowsThreads), 0, s, p);
+}
+
+template <int CACHE>
+int launch_rows(const DeviceState* d, int head_dim, bool xb, RowsParams& p, cudaStream_t s) {
+    // one token a CTA while that leaves SMs idle, else four: the angles of four tokens fill the CTA's threads
+    p.tpb = p.T <= 4 * d->sms ? 1 : kRowsMaxTpb;
+    return head_dim == 128 ? launch_rows_d<128, CACHE>(xb, p, s) : launch_rows_d<64, CACHE>(xb, p, s);
+}
+
+void set_rope(RowsParams& p, const oomb_rope* r) {
+    p.mscale = 1.0f;
+    if (!r) return;
+    p.turns = r->turns;
+    p.rot = r->rot_dim;
+    p.interleaved = r->interleaved;
+    p.mscale = r->mscale;
+}
+
+// The largest value a row may hold under scale 1 so that, rotated, it stays within 448.
+float rotated_limit(float mscale) {
+    const double limit = 448.0 / (sqrt(2.0) * static_cast<double>(mscale));
+    const float f = static_cast<float>(limit);
+    return static_cast<double>(f) > limit ? nextafterf(f, 0.0f) : f;
+}
+
+template <int KIND>
+int launch_attn(const PattnParams& p, int head_dim, cudaStream_t s) {
+    const int64_t warps = static_cast<int64_t>(p.T) * p.H;
+    const dim3 grid(static_cast<unsigned>((warps + 3) / 4));
+    return head_dim == 128 ? launch(attn_rows_kernel<KIND, 128>, grid, dim3(128), 0, s, p)
+                           : launch(attn_rows_kernel<KIND, 64>, grid, dim3(128), 0, s, p);
+}
+
+// The checks that both attentions share.
+int check_attn(const void* q, int64_t q_stride, const void* out, int64_t out_stride, int heads, int kv_heads, int head_dim,
+               int batch, int t, int max_q, float scale) {
+    if (!q || !out) return OOMB_E_ARG;
+    if (!isfinite(scale)) return OOMB_E_ARG;
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > 64 || !head_dim_ok(head_dim) || batch < 0 ||
+        t < 0 || max_q < 0)
+        return OOMB_E_SHAPE;
+    const int64_t row = static_cast<int64_t>(heads) * head_dim;
+    const int st = check_rows(q, q_stride, row, OOMB_BF16);
+    return st != OOMB_OK ? st : check_rows(out, out_stride, row, OOMB_BF16);
+}
+
+}  // namespace
+}  // namespace oomb
+
+using namespace oomb;
+
+extern "C" {
+
+int oomb_rope_turns(int rot_dim, double base, int scaling, double factor, int64_t original_len, uint64_t* turns,
+                    float* mscale) {
+    if (!turns || !mscale) return OOMB_E_ARG;
+    if (scaling < OOMB_ROPE_NONE || scaling > OOMB_ROPE_BY_PARTS) return OOMB_E_ARG;
+    if (rot_dim <= 0 || rot_dim % 16 || rot_dim > 128) return OOMB_E_SHAPE;
+    if (!(base > 1.0) || !(base <= 1e12) || !(factor >= 1.0) || !(factor <= 1e6)) return OOMB_E_ARG;
+    if (scaling == OOMB_ROPE_BY_PARTS && original_len <= 0) return OOMB_E_ARG;
+    const long double two_pi = 6.283185307179586476925286766559L;
+    long double b = base;
+    if (scaling == OOMB_ROPE_NTK) b *= powl(factor, static_cast<long double>(rot_dim) / (rot_dim - 2));
+    long double lo = 0.0L, hi = 0.0L;
+    if (scaling == OOMB_ROPE_BY_PARTS) {
+        // the (fractional) pair that turns `n` times over the original length
+        auto pair_of = [&](long double n) {
+            return rot_dim * logl(original_len / (n * two_pi)) / (2.0L * logl(b));
+        };
+        lo = fmaxl(floorl(pair_of(32.0L)), 0.0L);
+        hi = fminl(ceill(pair_of(1.0L)), static_cast<long double>(rot_dim - 1));
+    }
+    for (int i = 0; i < rot_dim / 2; i++) {
+        long double inv = powl(b, -2.0L * i / rot_dim);
+        if (scaling == OOMB_ROPE_LINEAR) inv /= factor;
+        if (scaling == OOMB_ROPE_BY_PARTS) {
+            const long double ramp = fminl(fmaxl((i - lo) / fmaxl(hi - lo, 0.001L), 0.0L), 1.0L);
+            inv = inv / factor * ramp + inv * (1.0L - ramp);
+        }
+        turns[i] = static_cast<uint64_t>(inv / two_pi * 18446744073709551616.0L + 0.5L);
+    }
+    *mscale = scaling == OOMB_ROPE_BY_PARTS ? static_cast<float>(0.1 * log(factor) + 1.0) : 1.0f;
+    return OOMB_OK;
+}
+
+int oomb_rope_rows(const oomb_rope* rope, const void* x, int x_dtype, int64_t x_stride, const int32_t* positions, void* out,
+                   int64_t out_stride, int t, int heads, int head_dim, oomb_stream stream) {
+    if (!rope || !x || !positions || !out || !dtype_ok(x_dtype)) return OOMB_E_ARG;
+    if (t < 0 || heads <= 0 || !head_dim_ok(head_dim)) return OOMB_E_SHAPE;
+    int st = check_rope(rope, head_dim);
+    const int64_t row = static_cast<int64_t>(heads) * head_dim;
+    if (st == OOMB_OK) st = check_rows(x, x_stride, row, x_dtype);
+    if (st == OOMB_OK) st = check_rows(out, out_stride, row, x_dtype);
+    if (st != OOMB_OK) return st;
+    if (t == 0) return OOMB_OK;
+    const DeviceState* d = device_state();
+    if (!d) return OOMB_E_DEVICE;
+    RowsParams p{};
+    p.q = x;
+    p.qs = x_stride;
+    p.qo = out;
+    p.qos = out_stride;
+    p.qo_bf16 = x_dtype == OOMB_BF16;
+    p.Hq = heads;
+    p.positions = positions;
+    p.T = t;
+    p.err = d->err;
+    set_rope(p, rope);
+    return launch_rows<-1>(d, head_dim, x_dtype == OOMB_BF16, p, stream);
+}
+
+int oomb_kv_append_paged(const oomb_paged_kv* cache, const oomb_rope* rope, const void* q, int64_t q_stride, void* q_out,
+                         int64_t q_out_stride, int heads, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                         int src_dtype, const int32_t* q_start, const int32_t* kv_len, int batch, int t,
+                         oomb_stream stream) {
+    if (!k || !v || !kv_len || !dtype_ok(src_dtype) || (q && !q_out) || (!q && q_out)) return OOMB_E_ARG;
+    if (batch < 0 || t < 0 || (!q_start && batch != t) || (q && heads <= 0)) return OOMB_E_SHAPE;
+    RowsParams p{};
+    int st = check_cache(cache, p.kv);
+    if (st == OOMB_OK && rope) st = check_rope(rope, cache->head_dim);
+    const int64_t row = st == OOMB_OK ? static_cast<int64_t>(cache->kv_heads) * cache->head_dim : 0;
+    if (st == OOMB_OK) st = check_rows(k, k_stride, row, src_dtype);
+    if (st == OOMB_OK) st = check_rows(v, v_stride, row, src_dtype);
+    if (st == OOMB_OK && q) st = check_rows(q, q_stride, static_cast<int64_t>(heads) * cache->head_dim, src_dtype);
+    if (st == OOMB_OK && q) st = check_rows(q_out, q_out_stride, static_cast<int64_t>(heads) * cache->head_dim, OOMB_BF16);
+    if (st != OOMB_OK) return st;
+    if (batch == 0 || t == 0) return OOMB_OK;
+    const DeviceState* d = device_state();
+    if (!d) return OOMB_E_DEVICE;
+    p.q = q;
+    p.qs = q_stride;
+    p.qo = q_out;
+    p.qos = q_out_stride;
+    p.qo_bf16 = 1;
+    p.Hq = q ? heads : 0;
+    p.k = k;
+    p.ks = k_stride;
+    p.v = v;
+    p.vs = v_stride;
+    p.Hkv = cache->kv_heads;
+    p.q_start = q_start;
+    p.kv_len = kv_len;
+    p.B = batch;
+    p.T = t;
+    p.ko = static_cast<uint8_t*>(cache->k);
+    p.vo = static_cast<uint8_t*>(cache->v);
+    p.keo = cache->k_exp;
+    p.veo = cache->v_exp;
+    p.err = d->err;
+    set_rope(p, rope);
+    p.k_limit = rope ? rotated_limit(p.mscale) : 448.0f;
+    return cache->dtype == OOMB_KV_E4M3 ? launch_rows<1>(d, cache->head_dim, src_dtype == OOMB_BF16, p, stream)
+                                        : launch_rows<0>(d, cache->head_dim, src_dtype == OOMB_BF16, p, stream);
+}
+
+int oomb_kv_read_paged(const oomb_paged_kv* cache, const int32_t* q_start, const int32_t* kv_len, int batch, int t,
+                       void* k_out, void* v_out, int out_dtype, int64_t out_stride, oomb_stream stream) {
+    if (!kv_len || !k_out || !v_out || !dtype_ok(out_dtype)) return OOMB_E_ARG;
+    if (batch < 0 || t < 0 || (!q_start && batch != t)) return OOMB_E_SHAPE;
+    ReadParams p{};
+    int st = check_cache(cache, p.kv);
+    const int64_t row = st == OOMB_OK ? static_cast<int64_t>(cache->kv_heads) * cache->head_dim : 0;
+    if (st == OOMB_OK) st = check_rows(k_out, out_stride, row, out_dtype);
+    if (st == OOMB_OK) st = check_rows(v_out, out_stride, row, out_dtype);
+    if (st != OOMB_OK) return st;
+    if (batch == 0 || t == 0) return OOMB_OK;
+    const DeviceState* d = device_state();
+    if (!d) return OOMB_E_DEVICE;
+    p.q_start = q_start;
+    p.kv_len = kv_len;
+    p.B = batch;
+    p.T = t;
+    p.ko = k_out;
+    p.vo = v_out;
+    p.out_bf16 = out_dtype == OOMB_BF16;
+    p.out_stride = out_stride;
+    p.err = d->err;
+    const dim3 grid(static_cast<unsigned>((t + kReadTokens - 1) / kReadTokens));
+    const bool fp8 = cache->dtype == OOMB_KV_E4M3;
+    if (cache->head_dim == 128)
+        return fp8 ? launch(read_kernel<true, 128>, grid, dim3(kReadThreads), 0, stream, p)
+                   : launch(read_kernel<false, 128>, grid, dim3(kReadThreads), 0, stream, p);
+    return fp8 ? launch(read_kernel<true, 64>, grid, dim3(kReadThreads), 0, stream, p)
+               : launch(read_kernel<false, 64>, grid, dim3(kReadThreads), 0, stream, p);
+}
+
+size_t oomb_attention_paged_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim) {
+    if (batch < 0 || t < 0 || max_q < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > 64 ||
+        !head_dim_ok(head_dim))
+        return 0;
+    return 256;
+}
+
+int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                         int heads, const int32_t* q_start, const int32_t* kv_len, int batch, int t, int max_q, float scale,
+                         void* workspace, size_t workspace_bytes, oomb_stream stream) {
+    if (!kv_len || !workspace) return OOMB_E_ARG;
+    PattnParams p{};
+    int st = check_cache(cache, p.kv);
+    if (st == OOMB_OK)
+        st = check_attn(q, q_stride, out, out_stride, heads, cache->kv_heads, cache->head_dim, batch, t, max_q, scale);
+    if (st != OOMB_OK) return st;
+    if (!q_start && batch != t) return OOMB_E_SHAPE;
+    if (!aligned16(workspace)) return OOMB_E_ALIGN;
+    if (workspace_bytes < oomb_attention_paged_workspace_bytes(batch, t, max_q, heads, cache->kv_heads, cache->head_dim))
+        return OOMB_E_WORKSPACE;
+    if (batch == 0 || t == 0 || max_q == 0) return OOMB_OK;
+    const DeviceState* d = device_state();
+    if (!d) return OOMB_E_DEVICE;
+    p.q = static_cast<const uint16_t*>(q);
+    p.q_stride = q_stride;
+    p.out = static_cast<uint16_t*>(out);
+    p.out_stride = out_stride;
+    p.q_start = q_start;
+    p.kv_len = kv_len;
+    p.B = batch;
+    p.T = t;
+    p.H = heads;
+    p.Hkv = cache->kv_heads;
+    p.G = heads / cache->kv_heads;
+    p.max_q = max_q;
+    p.kv_max = cache->max_pages * cache->page_size;
+    p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+    p.err = d->err;
+    return cache->dtype == OOMB_KV_E4M3 ? launch_attn<KV_E4M3>(p, cache->head_dim, stream)
+                                        : launch_attn<KV_BF16>(p, cache->head_dim, stream);
+}
+
+size_t oomb_attention_prompt_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim) {
+    return oomb_attention_paged_workspace_bytes(batch, t, max_q, heads, kv_heads, head_dim);
+}
+
+int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          void* out, int64_t out_stride, int heads, int kv_heads, int head_dim, const int32_t* q_start,
+                          int batch, int t, int max_q, float scale, void* workspace, size_t workspace_bytes,
+                          oomb_stream stream) {
+    if (!k || !v || !q_start || !workspace) return OOMB_E_ARG;
+    int st = check_attn(q, q_stride, out, out_stride, heads, kv_heads, head_dim, batch, t, max_q, scale);
+    const int64_t row = static_cast<int64_t>(kv_heads) * head_dim;
+    if (st == OOMB_OK) st = check_rows(k, k_stride, row, OOMB_BF16);
+    if (st == OOMB_OK) st = check_rows(v, v_stride, row, OOMB_BF16);
+    if (st != OOMB_OK) return st;
+    if (!aligned16(workspace)) return OOMB_E_ALIGN;
+    if (workspace_bytes < oomb_attention_prompt_workspace_bytes(batch, t, max_q, heads, kv_heads, head_dim))
+        return OOMB_E_WORKSPACE;
+    if (batch == 0 || t == 0 || max_q == 0) return OOMB_OK;
+    const DeviceState* d = device_state();
+    if (!d) return OOMB_E_DEVICE;
+    PattnParams p{};
+    p.q = static_cast<const uint16_t*>(q);
+    p.q_stride = q_stride;
+    p.out = static_cast<uint16_t*>(out);
+    p.out_stride = out_stride;
+    p.q_start = q_start;
+    p.B = batch;
+    p.T = t;
+    p.H = heads;
+    p.Hkv = kv_heads;
+    p.G = heads / kv_heads;
+    p.max_q = max_q;
+    p.kv_max = t;
+    p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+    p.kv.k = static_cast<const uint8_t*>(k);
+    p.kv.v = static_cast<const uint8_t*>(v);
+    p.kv.k_stride = k_stride;
+    p.kv.v_stride = v_stride;
+    p.kv.Hkv = kv_heads;
+    p.err = d->err;
+    return launch_attn<KV_ROWS>(p, head_dim, stream);
+}
+
+}  // extern "C"

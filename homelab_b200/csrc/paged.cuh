@@ -1,0 +1,420 @@
+// paged.cuh - rotary positions, and a paged key/value cache in bf16 or in 8 bits: its
+// write, fused with the rotation, and its read-back.
+//
+// A pool holds num_pages pages; a page holds page_size positions of every kv head, row
+// (page, head, slot) of head_dim values contiguous, so the positions of one (page, head)
+// are one run of page_size * head_dim values that attention streams.  Row b of the block
+// table names the pages of sequence b in order: position j sits in page table[b][j / ps]
+// at slot j % ps.  Three equal ways to say where a step's tokens go serve every kernel
+// here: token t of the packed step belongs to the sequence b with
+// q_start[b] <= t < q_start[b + 1], and its position is kv_len[b] - n_b + (t - q_start[b]),
+// n_b = q_start[b + 1] - q_start[b] (kv_len counts the new tokens).
+//
+// 8-bit rows: x = e4m3 * 2^e with one e per (position, head), kept as the byte e + 127.
+// A power of two keeps every code's product exact in bf16 and in fp32, so no reader
+// rounds again.  e is the least with amax * r <= 448 * 2^e over the finite values of the
+// row BEFORE rotation, r = sqrt(2) * mscale for a rotated row (a rotation grows a value
+// by at most sqrt(2)) and 1 otherwise: comparing the input's largest value with a
+// constant is exact, so the byte does not depend on how the angles were rounded.
+// e4m3 being a floating type, the factor sqrt(2) costs no precision above 2^-6 * 2^e.
+// Infinities and NaN become the NaN code; e is clamped to [-100, 120].
+//
+// Angles: the frequency of a pair is kept as turns per position in units of 2^-64; a
+// position times it modulo 2^64 is the exact phase, of which 32 bits go to sincospif:
+// no loss at far positions and no table to read (an fp32 product loses 1e-2 rad at
+// position 100,000).
+//
+// Bound: HBM for prompts (each value read once and written once), launch latency for
+// decode steps.  One CTA takes `tpb` tokens: their angles go through shared memory once
+// and serve all heads; a row is rotated by head_dim / 16 threads with two 8-value
+// chunks each, a pair's two halves in the same thread, so a rotation may be in place.
+#pragma once
+
+#include "common.cuh"
+
+namespace oomb {
+
+enum : unsigned {
+    ERR_KV_TABLE = 0x900,  // a block table entry was outside the pool (its positions skipped, or read as zeros)
+    ERR_KV_SEQ = 0x910,    // q_start or kv_len out of range (the sequence clamped or skipped)
+};
+
+// Where attention finds keys and values: packed rows of the step, or pages.
+struct KvView {
+    const uint8_t* k;
+    const uint8_t* v;
+    const uint8_t* ke;      // exponent bytes [pages][kv_heads][page], e4m3 pools only
+    const uint8_t* ve;
+    int64_t page_stride;    // elements from page to page (exponents: exp_stride)
+    int64_t exp_stride;
+    const int32_t* table;
+    int table_stride;       // entries from one sequence's row to the next
+    int max_pages;          // entries of a row in use at most
+    int num_pages;
+    int page_log2;
+    int Hkv;
+    int64_t k_stride, v_stride;  // packed rows: elements from token to token
+};
+
+// The sequence that token t belongs to: the number of b with q_start[b + 1] <= t, by a
+// 32-way search of one warp (B <= 32: one load).  Every lane gets it; B when t is behind
+// the last sequence.
+__device__ __forceinline__ int find_sequence(const int32_t* q_start, int B, int t, int lane) {
+    int lo = 0, n = B;
+    while (n > 0) {
+        const int step = (n + 31) / 32;
+        const int i = lo + (lane + 1) * step - 1;
+        const bool past = i < lo + n && __ldcg(q_start + i + 1) <= t;
+        const int c = __popc(__ballot_sync(0xffffffffu, past));
+        const int end = lo + n;
+        lo += c * step;
+        n = min(step, end - lo);
+        if (step == 1) break;
+    }
+    return lo;
+}
+
+struct Seq {
+    int q0, n, len;  // first packed token, new tokens, cached positions with them
+};
+
+// Sequence b's numbers, forced into range (and the device error word set) where they are
+// not: 0 <= q0 <= q0 + n <= T, 0 <= len <= kv_max.
+__device__ __forceinline__ Seq read_seq(const int32_t* q_start, const int32_t* kv_len, int b, int T, int kv_max,
+                                        unsigned* err) {
+    Seq s;
+    const int a = q_start ? __ldcg(q_start + b) : b, e = q_start ? __ldcg(q_start + b + 1) : b + 1;
+    s.q0 = max(0, min(a, T));
+    s.n = max(0, min(e, T) - s.q0);
+    const int len = kv_len ? __ldcg(kv_len + b) : s.n;
+    s.len = max(0, min(len, kv_max));
+    if (a < 0 || e < a || e > T || len < s.n || len > kv_max) record_error(err, ERR_KV_SEQ);
+    return s;
+}
+
+// ---- rotation and append -------------------------------------------------------------
+
+constexpr int kRowsThreads = 256;
+constexpr int kRowsMaxTpb = 4;    // tokens of a CTA
+constexpr int kRopeMaxPairs = 64;  // head_dim / 2
+
+struct RowsParams {
+    const void *q, *k, *v;  // q null: none; k null: rotation alone
+    int64_t qs, ks, vs;     // elements from token to token
+    void* qo;
+    int64_t qos;
+    int qo_bf16;
+    int Hq, Hkv;
+    const uint64_t* turns;  // null: no rotation
+    int rot, interleaved;
+    float mscale;
+    float k_limit;          // e4m3: 448, or 448 / (sqrt(2) * mscale) of rotated keys
+    const int32_t* positions;  // rotation alone: [T]
+    const int32_t* q_start;    // append: [B + 1], or null for one token a sequence
+    const int32_t* kv_len;
+    int B, T, tpb;
+    KvView kv;
+    uint8_t *ko, *vo, *keo, *veo;  // the pool, to be written
+    unsigned* err;
+};
+
+template <bool BF16>
+__device__ __forceinline__ void load8(const void* base, int64_t idx, float (&f)[8]) {
+    if constexpr (BF16) {
+        const uint4 w = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + idx));
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f[2 * i] = __uint_as_float(u[i] << 16);
+            f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    } else {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + idx);
+        const float4 a = __ldcg(p), b = __ldcg(p + 1);
+        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    }
+}
+
+__device__ __forceinline__ void store8(void* base, int64_t idx, bool bf16, const float (&f)[8]) {
+    if (bf16) {
+        uint4 o;
+        unsigned* w = reinterpret_cast<unsigned*>(&o);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned*>(&h);
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + idx) = o;
+    } else {
+        float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + idx);
+        p[0] = make_float4(f[0], f[1], f[2], f[3]);
+        p[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+}
+
+// The least e with amax <= limit * 2^e (amax, limit finite; 0 for a zero row), clamped.
+__device__ __forceinline__ int row_exponent(float amax, float limit) {
+    const unsigned a = __float_as_uint(amax), l = __float_as_uint(limit);
+    const int e = static_cast<int>(a >> 23) - static_cast<int>(l >> 23) + ((a & 0x7fffffu) > (l & 0x7fffffu) ? 1 : 0);
+    return amax > 0.0f ? max(-100, min(120, e)) : 0;
+}
+
+// Eight values times 2^-e as e4m3 codes; non-finite values become the NaN code.
+__device__ __forceinline__ uint2 codes8(const float (&f)[8], float inv) {
+    unsigned w[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        unsigned r = 0;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            float a = f[4 * i + 2 * j] * inv, b = f[4 * i + 2 * j + 1] * inv;
+            a = fabsf(a) <= 3.4e38f ? a : __uint_as_float(0x7fffffffu);
+            b = fabsf(b) <= 3.4e38f ? b : __uint_as_float(0x7fffffffu);
+            unsigned short c;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(b), "f"(a));
+            r |= static_cast<unsigned>(c) << (16 * j);
+        }
+        w[i] = r;
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// CACHE: -1 rotation alone, 0 bf16 pool, 1 e4m3 pool.
+template <bool XBF16, int D, int CACHE>
+__global__ void __launch_bounds__(kRowsThreads) rows_kernel(const RowsParams p) {
+    constexpr int TEAM = D / 16;  // threads of a row
+    constexpr int SLOTS = kRowsThreads / TEAM;
+    __shared__ __align__(16) float cs[kRowsMaxTpb][2][kRopeMaxPairs];
+    __shared__ int tok_ok[kRowsMaxTpb], tok_pos[kRowsMaxTpb];
+    __shared__ int64_t tok_row[kRowsMaxTpb], tok_exp[kRowsMaxTpb];
+    const int t0 = blockIdx.x * p.tpb, nt = min(p.tpb, p.T - t0);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (warp < nt) {
+        const int t = t0 + warp;
+        int pos = 0;
+        bool ok = true;
+        int64_t row = -1, ex = -1;
+        if constexpr (CACHE < 0) {
+            pos = __ldcg(p.positions + t);
+        } else {
+            const int b = p.q_start ? find_sequence(p.q_start, p.B, t, lane) : t;
+            ok = b < p.B && (!p.q_start || t >= __ldcg(p.q_start));
+            if (ok) {
+                const int kv_max = p.kv.max_pages << p.kv.page_log2;
+                const int q0 = p.q_start ? __ldcg(p.q_start + b) : b, q1 = p.q_start ? __ldcg(p.q_start + b + 1) : b + 1;
+                pos = __ldcg(p.kv_len + b) - (q1 - q0) + (t - q0);
+                if (pos < 0 || pos >= kv_max) {
+                    ok = false;  // nowhere to write: the token is skipped
+                    if (lane == 0) record_error(p.err, ERR_KV_SEQ);
+                } else {
+                    const int page = __ldcg(p.kv.table + static_cast<int64_t>(b) * p.kv.table_stride + (pos >> p.kv.page_log2));
+                    const int slot = pos & ((1 << p.kv.page_log2) - 1);
+                    if (page < 0 || page >= p.kv.num_pages) {
+                        if (lane == 0) record_error(p.err, ERR_KV_TABLE);
+                    } else {
+                        row = page * p.kv.page_stride + static_cast<int64_t>(slot) * D;
+                        ex = page * p.kv.exp_stride + slot;
+                    }
+                }
+            }
+        }
+        if (lane == 0) {
+            tok_ok[warp] = ok;
+            tok_pos[warp] = pos;
+            tok_row[warp] = row;
+            tok_exp[warp] = ex;
+        }
+    }
+    if (p.turns) {
+        __syncthreads();
+        const int pairs = p.rot / 2;
+        for (int i = threadIdx.x; i < nt * pairs; i += kRowsThreads) {
+            const int a = i / pairs, f = i - a * pairs;
+            const uint64_t phase = static_cast<uint64_t>(static_cast<int64_t>(tok_pos[a])) * __ldg(p.turns + f) + 0x80000000ull;
+            float s, c;
+            sincospif(static_cast<float>(static_cast<int>(phase >> 32)) * 4.656612873077393e-10f, &s, &c);  // 2^-31
+            cs[a][0][f] = c * p.mscale;
+            cs[a][1][f] = s * p.mscale;
+        }
+    }
+    __syncthreads();
+
+    const int R = p.Hq + 2 * p.Hkv, slot = threadIdx.x / TEAM, t8 = threadIdx.x % TEAM;
+    const int total = nt * R;
+    for (int r0 = 0; r0 < total; r0 += SLOTS) {
+        const int r = r0 + slot;
+        const bool in = r < total;
+        const int a = in ? r / R : 0, rr = in ? r - a * R : 0;
+        const bool is_q = rr < p.Hq, is_k = !is_q && rr < p.Hq + p.Hkv;
+        const int h = is_q ? rr : is_k ? rr - p.Hq : rr - p.Hq - p.Hkv;
+        const bool ok = in && tok_ok[a];
+        const bool turn = p.turns && (is_q || is_k);
+        // this thread's two chunks of eight values: the two halves of its pairs when the halves
+        // of a rotated row pair up, else any two
+        int ca = t8, cb = t8 + TEAM;
+        const int nr = p.rot / 16;
+        if (turn && !p.interleaved) {
+            if (t8 < nr) {
+                cb = t8 + nr;
+            } else {
+                ca = 2 * nr + (t8 - nr);
+                cb = ca + (TEAM - nr);
+            }
+        }
+        float x[8] = {}, y[8] = {};
+        if (ok) {
+            const void* src = is_q ? p.q : is_k ? p.k : p.v;
+            const int64_t base = static_cast<int64_t>(t0 + a) * (is_q ? p.qs : is_k ? p.ks : p.vs) + static_cast<int64_t>(h) * D;
+            load8<XBF16>(src, base + ca * 8, x);
+            load8<XBF16>(src, base + cb * 8, y);
+        }
+        float amax = 0.0f;
+        if constexpr (CACHE == 1) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float u = fabsf(x[i]), w = fabsf(y[i]);
+                amax = fmaxf(amax, fmaxf(u <= 3.4028235e38f ? u : 0.0f, w <= 3.4028235e38f ? w : 0.0f));
+            }
+#pragma unroll
+            for (int o = 1; o < TEAM; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        }
+        if (!ok) continue;
+        if (turn) {
+            const float* c = cs[a][0];
+            const float* s = cs[a][1];
+            if (p.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int fa = ca * 4 + i, fb = cb * 4 + i;
+                    if (2 * fa < p.rot) {
+                        const float u = x[2 * i], w = x[2 * i + 1];
+                        x[2 * i] = u * c[fa] - w * s[fa];
+                        x[2 * i + 1] = w * c[fa] + u * s[fa];
+                    }
+                    if (2 * fb < p.rot) {
+                        const float u = y[2 * i], w = y[2 * i + 1];
+                        y[2 * i] = u * c[fb] - w * s[fb];
+                        y[2 * i + 1] = w * c[fb] + u * s[fb];
+                    }
+                }
+            } else if (t8 < nr) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float cc = c[t8 * 8 + i], ss = s[t8 * 8 + i], u = x[i], w = y[i];
+                    x[i] = u * cc - w * ss;
+                    y[i] = w * cc + u * ss;
+                }
+            }
+        }
+        if (is_q) {
+            const int64_t o = static_cast<int64_t>(t0 + a) * p.qos + static_cast<int64_t>(h) * D;
+            store8(p.qo, o + ca * 8, p.qo_bf16, x);
+            store8(p.qo, o + cb * 8, p.qo_bf16, y);
+        } else if constexpr (CACHE >= 0) {
+            if (tok_row[a] < 0) continue;
+            const int64_t o = tok_row[a] + (static_cast<int64_t>(h) * D << p.kv.page_log2);
+            uint8_t* pool = is_k ? p.ko : p.vo;
+            if constexpr (CACHE == 0) {
+                store8(pool, o + ca * 8, true, x);
+                store8(pool, o + cb * 8, true, y);
+            } else {
+                const int e = row_exponent(amax, is_k ? p.k_limit : 448.0f);
+                const float inv = __int_as_float((127 - e) << 23);
+                *reinterpret_cast<uint2*>(pool + o + ca * 8) = codes8(x, inv);
+                *reinterpret_cast<uint2*>(pool + o + cb * 8) = codes8(y, inv);
+                if (t8 == 0)
+                    (is_k ? p.keo : p.veo)[tok_exp[a] + (static_cast<int64_t>(h) << p.kv.page_log2)] = static_cast<uint8_t>(e + 127);
+            }
+        }
+    }
+}
+
+// ---- read-back -----------------------------------------------------------------------
+
+constexpr int kReadThreads = 256;
+constexpr int kReadTokens = 8;  // tokens of a CTA, one warp each for the lookup
+
+struct ReadParams {
+    KvView kv;
+    const int32_t* q_start;
+    const int32_t* kv_len;
+    int B, T;
+    void *ko, *vo;
+    int out_bf16;
+    int64_t out_stride;
+    unsigned* err;
+};
+
+// 2^(byte - 127); 0 for byte 0.
+__device__ __forceinline__ float exp_byte(unsigned e) { return __uint_as_float(e << 23); }
+
+// Rows of the packed positions, keys and values: out[t][h][:] = the row's values.  A
+// thread moves 8 values: 16-byte stores of consecutive lanes are contiguous.
+template <bool FP8, int D>
+__global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) {
+    __shared__ int64_t tok_row[kReadTokens], tok_exp[kReadTokens];
+    const int t0 = blockIdx.x * kReadTokens, nt = min(kReadTokens, p.T - t0);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (warp < nt) {
+        const int t = t0 + warp;
+        const int b = p.q_start ? find_sequence(p.q_start, p.B, t, lane) : t;
+        int64_t row = -2, ex = 0;  // -2: leave the output row as it was; -1: zeros
+        if (b < p.B && (!p.q_start || t >= __ldcg(p.q_start))) {
+            const int kv_max = p.kv.max_pages << p.kv.page_log2;
+            const int q0 = p.q_start ? __ldcg(p.q_start + b) : b, q1 = p.q_start ? __ldcg(p.q_start + b + 1) : b + 1;
+            const int pos = __ldcg(p.kv_len + b) - (q1 - q0) + (t - q0);
+            row = -1;
+            if (pos < 0 || pos >= kv_max) {
+                if (lane == 0) record_error(p.err, ERR_KV_SEQ);
+            } else {
+                const int page = __ldcg(p.kv.table + static_cast<int64_t>(b) * p.kv.table_stride + (pos >> p.kv.page_log2));
+                const int slot = pos & ((1 << p.kv.page_log2) - 1);
+                if (page < 0 || page >= p.kv.num_pages) {
+                    if (lane == 0) record_error(p.err, ERR_KV_TABLE);
+                } else {
+                    row = page * p.kv.page_stride + static_cast<int64_t>(slot) * D;
+                    ex = page * p.kv.exp_stride + slot;
+                }
+            }
+        }
+        if (lane == 0) {
+            tok_row[warp] = row;
+            tok_exp[warp] = ex;
+        }
+    }
+    __syncthreads();
+    const int per_row = p.kv.Hkv * (D / 8), per_tok = 2 * per_row;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nt * per_tok; i += kReadThreads) {
+        const int a = i / per_tok, rest = i - a * per_tok;
+        const bool is_v = rest >= per_row;
+        const int c = is_v ? rest - per_row : rest, h = c / (D / 8), c8 = (c % (D / 8)) * 8;
+        const int64_t row = tok_row[a];
+        if (row == -2) continue;
+        float f[8] = {};
+        if (row >= 0) {
+            const int64_t o = row + (static_cast<int64_t>(h) * D << p.kv.page_log2) + c8;
+            const uint8_t* pool = is_v ? p.kv.v : p.kv.k;
+            if constexpr (FP8) {
+                const uint2 w = __ldcs(reinterpret_cast<const uint2*>(pool + o));
+                const float s = exp_byte((is_v ? p.kv.ve : p.kv.ke)[tok_exp[a] + (static_cast<int64_t>(h) << p.kv.page_log2)]);
+                const unsigned u[2] = {w.x, w.y};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float2 d = e4m3x2_to_float2(static_cast<unsigned short>(u[j / 2] >> (16 * (j & 1))));
+                    f[2 * j] = d.x * s;
+                    f[2 * j + 1] = d.y * s;
+                }
+            } else {
+                load8<true>(pool, o, f);
+            }
+        }
+        store8(is_v ? p.vo : p.ko, static_cast<int64_t>(t0 + a) * p.out_stride + h * D + c8, p.out_bf16, f);
+    }
+}
+
+}  // namespace oomb

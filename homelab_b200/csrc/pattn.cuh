@@ -1,0 +1,138 @@
+// pattn.cuh - causal grouped-query attention of a step's new tokens over a paged cache,
+// or over the step's own packed rows (whole prompts).
+//
+// New token i of sequence b (n_b of them, kv_len = len) sees the first
+// vis = len - n_b + i + 1 positions, clamped to [0, len]:
+//   out[i, h, :] = sum_j<vis e^(scale q.k_j - m) v_j / sum_j<vis e^(scale q.k_j - m),
+// m the largest score of the row; a row that sees nothing gets zeros.  Scores, maxima,
+// sums and outputs are kept in fp32; the output is rounded once to bf16.
+#pragma once
+
+#include "paged.cuh"
+
+namespace oomb {
+
+struct PattnParams {
+    const uint16_t* q;      // bf16 [T][H][D]
+    int64_t q_stride;       // elements from token to token
+    uint16_t* out;          // bf16 [T][H][D]
+    int64_t out_stride;
+    const int32_t* q_start;  // [B + 1], or null: one token a sequence
+    const int32_t* kv_len;   // [B]; null (packed rows): the sequence's own tokens
+    int B, T, H, Hkv, G, max_q;
+    int kv_max;
+    float scale_log2;        // scale * log2(e)
+    KvView kv;
+    unsigned* err;
+};
+
+enum : int { KV_ROWS = 0, KV_BF16 = 1, KV_E4M3 = 2 };
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Lane's D / 32 values of key (or value) row j of sequence b, kv head h, as fp32; a bad
+// block table entry reads as zeros.
+template <int KIND, int D>
+__device__ __forceinline__ void kv_row(const PattnParams& p, bool value, int b, int q0, int h, int j, int lane, float (&f)[D / 32]) {
+    constexpr int E = D / 32;
+    const uint8_t* base = value ? p.kv.v : p.kv.k;
+    int64_t o;
+    float s = 1.0f;
+    if constexpr (KIND == KV_ROWS) {
+        o = static_cast<int64_t>(q0 + j) * (value ? p.kv.v_stride : p.kv.k_stride) + static_cast<int64_t>(h) * D;
+    } else {
+        const int page = __ldcg(p.kv.table + static_cast<int64_t>(b) * p.kv.table_stride + (j >> p.kv.page_log2));
+        const int slot = j & ((1 << p.kv.page_log2) - 1);
+        if (page < 0 || page >= p.kv.num_pages) {
+            if (lane == 0) record_error(p.err, ERR_KV_TABLE);
+#pragma unroll
+            for (int i = 0; i < E; i++) f[i] = 0.0f;
+            return;
+        }
+        o = page * p.kv.page_stride + ((static_cast<int64_t>(h) << p.kv.page_log2) + slot) * D;
+        if constexpr (KIND == KV_E4M3)
+            s = exp_byte((value ? p.kv.ve : p.kv.ke)[page * p.kv.exp_stride + (static_cast<int64_t>(h) << p.kv.page_log2) + slot]);
+    }
+    o += lane * E;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+        if constexpr (KIND == KV_E4M3) {
+            const float2 d = e4m3x2_to_float2(*reinterpret_cast<const unsigned short*>(base + o + i));
+            f[i] = d.x * s;
+            f[i + 1] = d.y * s;
+        } else {
+            const unsigned w = *reinterpret_cast<const unsigned*>(base + 2 * (o + i));
+            f[i] = __uint_as_float(w << 16);
+            f[i + 1] = __uint_as_float(w & 0xffff0000u);
+        }
+    }
+}
+
+// One query row over positions [j0, j1) by one warp, in plain fp32 loops: the running
+// maximum m (in units of log2), sum l and unnormalised output acc of the row.
+template <int KIND, int D>
+__device__ __noinline__ void attend_row(const PattnParams& p, int b, int q0, int token, int head, int j0, int j1, int lane, float& m,
+                                        float& l, float (&acc)[D / 32]) {
+    constexpr int E = D / 32;
+    float q[E];
+    const uint16_t* qp = p.q + static_cast<int64_t>(token) * p.q_stride + static_cast<int64_t>(head) * D + lane * E;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        q[i] = bf16_bits_to_float(qp[i]) * p.scale_log2;
+        acc[i] = 0.0f;
+    }
+    m = -INFINITY;
+    l = 0.0f;
+    for (int j = j0; j < j1; j++) {
+        float k[E], v[E];
+        kv_row<KIND, D>(p, false, b, q0, head / p.G, j, lane, k);
+        kv_row<KIND, D>(p, true, b, q0, head / p.G, j, lane, v);
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; i++) s = fmaf(q[i], k[i], s);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        const float mn = fmaxf(m, s);
+        const float base = mn == -INFINITY ? 0.0f : mn;
+        const float c = exp2_fast(m - base), e = exp2_fast(s - base);
+        l = fmaf(l, c, e);
+#pragma unroll
+        for (int i = 0; i < E; i++) acc[i] = fmaf(acc[i], c, e * v[i]);
+        m = mn;
+    }
+}
+
+// One warp per (token, head).
+template <int KIND, int D>
+__global__ void __launch_bounds__(128) attn_rows_kernel(const PattnParams p) {
+    constexpr int E = D / 32;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (w >= static_cast<int64_t>(p.T) * p.H) return;
+    const int t = static_cast<int>(w / p.H), h = static_cast<int>(w - static_cast<int64_t>(t) * p.H);
+    const int b = p.q_start ? find_sequence(p.q_start, p.B, t, lane) : t;
+    if (b >= p.B || (p.q_start && t < __ldcg(p.q_start))) return;
+    const Seq s = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, p.err);
+    if (s.n > p.max_q) {
+        record_error(p.err, ERR_KV_SEQ);
+        return;
+    }
+    const int vis = max(0, min(s.len, s.len - s.n + (t - s.q0) + 1));
+    float m, l, acc[E];
+    attend_row<KIND, D>(p, b, s.q0, t, h, 0, vis, lane, m, l, acc);
+    const float inv = vis > 0 ? 1.0f / l : 0.0f;
+    uint16_t* o = p.out + static_cast<int64_t>(t) * p.out_stride + static_cast<int64_t>(h) * D + lane * E;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+        const __nv_bfloat162 v2 = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+        *reinterpret_cast<__nv_bfloat162*>(o + i) = v2;
+    }
+}
+
+}  // namespace oomb

@@ -267,6 +267,94 @@ int oomb_kv_append(const void* src, int src_dtype, int64_t src_row_stride, uint1
                    const int32_t* start, int start_all, int batch, int t, int kv_heads, int head_dim, int kv_max,
                    oomb_stream stream);
 
+/* ---- rotary positions and the paged key/value cache ----------------------- */
+/* Rotary positions: the first rot_dim values of a head (a positive multiple of
+ * 16, at most head_dim) turn in pairs by position * turns[i] / 2^64 full turns,
+ *   x'[a] = mscale * (x[a] cos - x[b] sin),  x'[b] = mscale * (x[b] cos + x[a] sin);
+ * pair i is (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved.  turns:
+ * device [rot_dim / 2] (oomb_rope_turns fills a host copy).  0 < mscale <= 1024. */
+#define OOMB_ROPE_NONE 0
+#define OOMB_ROPE_LINEAR 1   /* every frequency divided by factor */
+#define OOMB_ROPE_NTK 2      /* base * factor^(rot_dim / (rot_dim - 2)) */
+#define OOMB_ROPE_BY_PARTS 3 /* frequencies turning more than 32 times over original_len kept, fewer than once divided by
+                              * factor, a linear ramp over the pairs between; mscale = 0.1 ln(factor) + 1 */
+typedef struct {
+    int32_t rot_dim;
+    int32_t interleaved;
+    float mscale;
+    int32_t pad_;
+    const uint64_t* turns;
+} oomb_rope;
+/* Frequencies base^(-2 i / rot_dim), i < rot_dim / 2, scaled for long contexts, as turns per
+ * position in units of 2^-64, written to HOST memory; 1 < base <= 1e12, 1 <= factor <= 1e6,
+ * rot_dim <= 128. */
+int oomb_rope_turns(int rot_dim, double base, int scaling, double factor, int64_t original_len, uint64_t* turns,
+                    float* mscale);
+/* out[t][h][:] = rotated x[t][h][:] at positions[t] (device int32 [t], any sign), x and out [t][heads][head_dim] of x_dtype
+ * with token strides in elements; out may be x.  head_dim 64 or 128. */
+int oomb_rope_rows(const oomb_rope* rope, const void* x, int x_dtype, int64_t x_stride, const int32_t* positions, void* out,
+                   int64_t out_stride, int t, int heads, int head_dim, oomb_stream stream);
+
+/* A paged cache.  k and v: [num_pages][kv_heads][page_size][head_dim] bf16, or e4m3 codes with
+ * k_exp, v_exp [num_pages][kv_heads][page_size]: the row's value is code * 2^(byte - 127), byte 1 to
+ * 254.  page_size 16, 32, 64 or 128; head_dim 64 or 128; page_stride (elements, a multiple of 16 bytes) and
+ * exp_page_stride (bytes, a multiple of 16) lead from page to page.  block_table: device int32,
+ * row b (table_stride entries after the one before) names the pages of sequence b, of
+ * which max_pages at most are read.  An entry outside [0, num_pages) is never followed: it
+ * sets the device error word (oomb_device_error), and its positions are skipped by a write and read as zeros.
+ *
+ * The tokens of a step are packed: those of sequence b are q_start[b] .. q_start[b + 1] - 1
+ * (device int32 [batch + 1], ascending, or NULL for one token a sequence, then t == batch),
+ * at positions kv_len[b] - n_b and on, n_b their number: kv_len (device int32 [batch]) counts
+ * them.  Tokens behind the last sequence's are left alone, in inputs and outputs.  Values out
+ * of range (q_start descending or past t, kv_len below n_b or past max_pages *
+ * page_size) set the device error word; nothing outside the buffers is touched. */
+#define OOMB_KV_BF16 0
+#define OOMB_KV_E4M3 1
+typedef struct {
+    int32_t dtype;
+    int32_t kv_heads, head_dim, page_size;
+    int32_t num_pages, max_pages, table_stride;
+    int32_t pad_;
+    void *k, *v;
+    uint8_t *k_exp, *v_exp;
+    int64_t page_stride, exp_page_stride;
+    const int32_t* block_table;
+} oomb_paged_kv;
+/* Writes a step's keys and values (fp32 or bf16 [t][kv_heads][head_dim], token strides in
+ * elements) into their pages, the keys rotated first when `rope` is given; with q, also writes the step's
+ * rotated queries [t][heads][head_dim] to q_out in bf16 (q_out may be q when that is bf16).
+ * An e4m3 row takes the least e with amax * r <= 448 * 2^e over its finite values before rotation
+ * (r = sqrt(2) * mscale for rotated keys, else 1), clamped to [-100, 120], its values
+ * rounded to nearest even; infinities and NaN become the NaN code.  Two tokens of one call must not share a
+ * position of a page. */
+int oomb_kv_append_paged(const oomb_paged_kv* cache, const oomb_rope* rope, const void* q, int64_t q_stride, void* q_out,
+                         int64_t q_out_stride, int heads, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                         int src_dtype, const int32_t* q_start, const int32_t* kv_len, int batch, int t,
+                         oomb_stream stream);
+/* The inverse: k_out, v_out [t][kv_heads][head_dim] (out_dtype, token stride out_stride) get the
+ * rows at the packed positions. */
+int oomb_kv_read_paged(const oomb_paged_kv* cache, const int32_t* q_start, const int32_t* kv_len, int batch, int t,
+                       void* k_out, void* v_out, int out_dtype, int64_t out_stride, oomb_stream stream);
+/* Causal attention of the packed new tokens over their sequences' pages: q, out bf16
+ * [t][heads][head_dim] (token strides in elements), query head h reading kv head h / (heads / kv_heads), at most
+ * 64 heads a kv head.  A token at position p sees positions 0 .. p below kv_len (a token that sees none gets zeros);
+ * what it does not see never reaches its output, infinities and NaN included.
+ * max_q bounds the tokens of a sequence (a longer one sets the device error word and is left out).  The workspace
+ * holds oomb_attention_paged_workspace_bytes(...) bytes, zeroed once before first use (and after a device
+ * error); calls that share it must be ordered on one stream. */
+size_t oomb_attention_paged_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim);
+int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                         int heads, const int32_t* q_start, const int32_t* kv_len, int batch, int t, int max_q, float scale,
+                         void* workspace, size_t workspace_bytes, oomb_stream stream);
+/* The same over whole prompts whose keys and values are rows of the step itself, bf16
+ * [t][kv_heads][head_dim] packed as q: token i of a sequence sees its tokens 0 .. i. */
+size_t oomb_attention_prompt_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim);
+int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          void* out, int64_t out_stride, int heads, int kv_heads, int head_dim, const int32_t* q_start,
+                          int batch, int t, int max_q, float scale, void* workspace, size_t workspace_bytes,
+                          oomb_stream stream);
+
 /* ---- fused decode step of one resident MoE layer ------------------------ */
 /* Router GEMV, softmax top-k, grouping of the step's assignments by expert
  * (expert order, slots in slot order: Moe::begin_routed / finish_routed,
