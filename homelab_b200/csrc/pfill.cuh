@@ -1,0 +1,744 @@
+// pfill.cuh - causal grouped-query attention of many new tokens (prefill chunks over a paged
+// cache, whole prompts over their own rows) on the 5th-generation tensor cores.
+//
+// A tile is 2 x 128 query rows of one kv head: row r of a half is new token r / G, query
+// head r % G of the group, so a group's heads share every key and value that is loaded
+// (floor(128 / G) tokens a half).  Per 128 positions and half, with S and O in tensor memory:
+//   S = Q K^T          tcgen05.mma, both operands in shared memory (TMA, 128-byte swizzle)
+//   P = e^(S - m)      one thread per row, fp32, rounded to bf16 and written over S
+//   O += P V           tcgen05.mma, P from tensor memory
+// m is the running maximum; O is multiplied up only when m has grown by more than 2^8 (the
+// factor cancels in O / l, and e^8 in base 2 keeps bf16 and fp32 far from overflow), which after
+// the first tiles is rare.
+//
+// Bound: with D = 128 a pair of halves costs 4 x 512 tensor-pipe cycles per 128
+// positions and 2 x 16,384 exponentials, which at 16 a cycle and SM are 2,048 cycles as
+// well.  The two halves run in turn: while one's scores go through the exponentials,
+// the tensor cores multiply the other's.  One issuing thread orders the products
+//   S0 S1 | O0 S0' | O1 S1' | ...,
+// and since they complete in order, the barrier of S0' also says that O0 is at rest, so a
+// row's thread may rescale it without another wait, and S may be overwritten as soon as
+// P was consumed.
+//
+// Warps: 0-3 and 4-7 one softmax thread per row of half 0 and 1 (also their epilogue);
+// 8 issues the products (and zeroes value rows behind the last position, which may hold
+// anything: 0 * NaN); 9 loads by TMA through a ring of key and value tiles, page by page for a
+// paged cache (a page of 16 or more rows keeps the swizzle's 8-row pattern).
+//
+// Work: plan_kernel lists the units (a tile, or a part of its positions when there are fewer
+// tiles than SMs), longest first; the CTAs take them in turn.  Parts leave (acc, m, l) in the
+// workspace, joined in order by join_kernel.  Every wait is bounded.
+#pragma once
+
+#include "pattn.cuh"
+#include "tcptx.cuh"
+
+namespace oomb {
+
+constexpr int kFaTile = 128;
+constexpr int kFaRows = 256;       // rows of a tile pair
+constexpr int kFaMinPart = 4;      // key tiles of a part at least
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBuckets = 1024;
+
+enum : unsigned {
+    ERR_FA_WAIT = 0xa00,  // a prefill pipeline wait ran out (+ the waiting role)
+};
+
+struct FaUnit {
+    int b, i0;     // sequence, first new token (of the sequence)
+    int kv0, kv1;  // key tiles
+    int slot;      // partial outputs' slot, or -1: the unit is its tile's only one
+    int pad[3];
+};
+struct FaSplit {
+    int b, i0, slot, parts;
+};
+struct FaHead {
+    int units, splits, slots, pad;
+};
+
+struct FaWs {
+    FaHead* head;
+    FaUnit* units;
+    FaSplit* splits;
+    float* part;  // [slot][kv head][256][D + 4]: acc, m, l
+    int max_units, max_slots, sms;
+};
+
+// Tokens of a half tile.
+__host__ __device__ inline int fa_tokens(int G) { return kFaTile / G; }
+
+__device__ __forceinline__ int fa_tiles_of(const Seq& s, int tq) { return (s.n + 2 * tq - 1) / (2 * tq); }
+// Key tiles that the tokens [i0, i1) of a sequence see together.
+__device__ __forceinline__ int fa_key_tiles(const Seq& s, int i1) {
+    const int vis = max(0, min(s.len, s.len - s.n + min(i1, s.n)));
+    return (vis + kFaTile - 1) / kFaTile;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PattnParams p, const FaWs ws) {
+    __shared__ int hist[kPlanBuckets];
+    __shared__ unsigned long long total_s;
+    __shared__ int slots_s, splits_s, warp_sum[32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = kPlanThreads / 32;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (tid == 0) {
+        total_s = 0;
+        slots_s = splits_s = 0;
+    }
+    for (int i = tid; i < kPlanBuckets; i += kPlanThreads) hist[i] = 0;
+    __syncthreads();
+    const int tq = fa_tokens(p.G);
+    auto seq_of = [&](int b, unsigned* err) {
+        Seq s = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, err);
+        if (s.n > p.max_q) {
+            record_error(err, ERR_KV_SEQ);
+            s.n = 0;
+        }
+        return s;
+    };
+    unsigned long long work = 0;
+    for (int b = warp; b < p.B; b += warps) {
+        const Seq s = seq_of(b, p.err);
+        const int nt = fa_tiles_of(s, tq);
+        for (int i = lane; i < nt; i += 32) work += max(1, fa_key_tiles(s, (i + 1) * 2 * tq));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+    if (lane == 0 && work) atomicAdd(&total_s, work);
+    __syncthreads();
+    // a part is at least an SM's even share of the step, so there are at most two parts an SM
+    const unsigned long long share = (total_s * p.Hkv + ws.sms - 1) / ws.sms;
+    const int chunk = share > (1u << 30) ? (1 << 30) : max(kFaMinPart, static_cast<int>(share));
+    for (int pass = 0; pass < 2; pass++) {
+        for (int b = warp; b < p.B; b += warps) {
+            const Seq s = seq_of(b, nullptr);
+            const int nt = fa_tiles_of(s, tq);
+            for (int i = lane; i < nt; i += 32) {
+                const int keys = fa_key_tiles(s, (i + 1) * 2 * tq);
+                const int parts = max(1, (keys + chunk - 1) / chunk);
+                int slot = -1;
+                if (pass == 1 && parts > 1) {
+                    slot = atomicAdd(&slots_s, parts);
+                    const int at = atomicAdd(&splits_s, 1);
+                    ws.splits[at] = FaSplit{b, i * 2 * tq, slot, parts};
+                }
+                for (int j = 0; j < parts; j++) {
+                    const int k0 = static_cast<int>(static_cast<int64_t>(keys) * j / parts);
+                    const int k1 = static_cast<int>(static_cast<int64_t>(keys) * (j + 1) / parts);
+                    const int at = atomicAdd(&hist[kPlanBuckets - 1 - min(k1 - k0, kPlanBuckets - 1)], 1);
+                    if (pass == 1) {
+                        FaUnit u{};
+                        u.b = b;
+                        u.i0 = i * 2 * tq;
+                        u.kv0 = k0;
+                        u.kv1 = k1;
+                        u.slot = slot < 0 ? -1 : slot + j;
+                        ws.units[at] = u;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (pass == 0) {  // exclusive scan of the buckets, longest units first
+            const int v = hist[tid];
+            int inc = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += u;
+            }
+            if (lane == 31) warp_sum[warp] = inc;
+            __syncthreads();
+            int before = 0;
+            for (int w = 0; w < warp; w++) before += warp_sum[w];
+            hist[tid] = before + inc - v;
+            if (tid == kPlanThreads - 1) slots_s = before + inc;
+            __syncthreads();
+            // more units than the workspace holds: only sequences that overlap each other make so many
+            const int units = slots_s;
+            if (units > ws.max_units) {
+                if (tid == 0) {
+                    record_error(p.err, ERR_KV_SEQ);
+                    *ws.head = FaHead{};
+                }
+                return;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                ws.head->units = units;
+                slots_s = 0;
+            }
+            __syncthreads();
+        }
+    }
+    if (tid == 0) {
+        ws.head->splits = splits_s;
+        ws.head->slots = slots_s;
+    }
+}
+
+// ---- PTX ------------------------------------------------------------------------------
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_addr(dst)),
+        "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+            smem_addr(dst)),
+        "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// bf16 x bf16 -> fp32, M = 128: A and B in shared memory (B K-major), or A in tensor memory and B MN-major.
+__host__ __device__ constexpr uint32_t fa_idesc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void fa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void fa_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// An MN-major operand in the 128-byte swizzle: rows of 64 values (128 bytes) along N, 8-row groups along K 1024
+// bytes apart (stride offset), further 64-value columns `lead` bytes apart (leading offset).
+__device__ __forceinline__ uint64_t fa_desc_mn(uint32_t addr, uint32_t lead) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lead >> 4) << 16) | (64ull << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+
+__device__ __forceinline__ void tm_ld32(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- shared memory --------------------------------------------------------------------
+
+template <int D>
+struct FaGeo {
+    static constexpr int TILE = kFaTile * D * 2;         // bytes of 128 rows in bf16
+    static constexpr int HALF = kFaTile * 128;           // bytes of 64 columns of them
+    static constexpr int STAGES = (224 * 1024 - 2 * TILE) / TILE < 8 ? (224 * 1024 - 2 * TILE) / TILE : 8;
+    static constexpr int Q_OFF = 0;
+    static constexpr int KV_OFF = 2 * TILE;
+    static constexpr int BAR_OFF = KV_OFF + STAGES * TILE;
+    static constexpr int TOTAL = BAR_OFF + 256 + 1024;   // the base is aligned to 1024 at run time
+    static constexpr int THREADS = 320;
+};
+
+struct FaBars {
+    uint64_t q_full[2], q_empty, s_full[2], p_ready[2], o_full[2], kv_full[8], kv_empty[8];
+    uint32_t tmem;
+};
+
+// A role's pipeline position over a ring of N stages.
+template <int N>
+struct Ring {
+    int i = 0;
+    unsigned phase = 0;
+    __device__ void next() {
+        if (++i == N) {
+            i = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// What every role derives from a unit: the sequence and each half's key tiles.
+struct FaWork {
+    Seq s;
+    int b, i0, kvh, kv0, keys;  // keys: tiles of the unit
+    int nh[2];                  // tiles that half h multiplies (the first of the unit's)
+    int slot;
+};
+
+__device__ __forceinline__ FaWork fa_work(const PattnParams& p, const FaWs& ws, int u, int tq) {
+    FaWork w;
+    const int4 a = __ldcg(reinterpret_cast<const int4*>(ws.units + u / p.Hkv));
+    w.slot = __ldcg(&ws.units[u / p.Hkv].slot);
+    w.kvh = u % p.Hkv;
+    w.b = a.x;
+    w.i0 = a.y;
+    w.kv0 = a.z;
+    w.keys = a.w - a.z;
+    w.s = read_seq(p.q_start, p.kv_len, w.b, p.T, p.kv_max, nullptr);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int i = w.i0 + h * tq;
+        w.nh[h] = i < w.s.n ? max(0, min(w.keys, fa_key_tiles(w.s, i + tq) - w.kv0)) : 0;
+    }
+    return w;
+}
+
+template <int KIND, int D>
+__global__ void __launch_bounds__(FaGeo<D>::THREADS, 1)
+    fa_kernel(const __grid_constant__ PattnParams p, const __grid_constant__ FaWs ws, const __grid_constant__ CUtensorMap qmap,
+              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using Geo = FaGeo<D>;
+    constexpr int ST = Geo::STAGES, CH = D / 64;  // 64-column chunks of a tile
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    FaBars* bar = reinterpret_cast<FaBars*>(smem + Geo::BAR_OFF);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tq = fa_tokens(p.G);
+
+    if (tid == 0) {
+        for (int h = 0; h < 2; h++) {
+            mbar_init(&bar->q_full[h], 1);
+            mbar_init(&bar->s_full[h], 1);
+            mbar_init(&bar->p_ready[h], 4);
+            mbar_init(&bar->o_full[h], 1);
+        }
+        mbar_init(&bar->q_empty, 1);
+        for (int i = 0; i < ST; i++) {
+            mbar_init(&bar->kv_full[i], 1);
+            mbar_init(&bar->kv_empty[i], 1);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&bar->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar->tmem;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int units = __ldcg(&ws.head->units) * p.Hkv;
+
+    if (warp == 9) {
+        // ---- loader ----
+        Ring<ST> r;
+        unsigned q_phase = 0;
+        bool ok = true;
+        const int32_t* table = nullptr;
+        int ids_of = -1, ids = 0, ids_next = 0;
+        const int per_tile = kFaTile >> p.kv.page_log2;  // pages of a tile
+        auto lookup = [&](int tile) {
+            int id = 0;
+            const int at = tile * per_tile + lane;
+            if (lane < per_tile && at < p.kv.max_pages) id = __ldcg(table + at);
+            return id;
+        };
+        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            const FaWork w = fa_work(p, ws, u, tq);
+            if (w.keys == 0) continue;
+            if constexpr (KIND != KV_ROWS) {
+                table = p.kv.table + static_cast<int64_t>(w.b) * p.kv.table_stride;
+                ids_of = w.kv0;
+                ids = lookup(ids_of);
+                ids_next = w.keys > 1 ? lookup(ids_of + 1) : 0;
+            }
+            auto load = [&](bool value, int tile, int page_ids) {
+                if (!ok || !mbar_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 1)) {
+                    ok = false;
+                    return;
+                }
+                uint8_t* dst = smem + Geo::KV_OFF + r.i * Geo::TILE;
+                uint64_t* full = &bar->kv_full[r.i];
+                const CUtensorMap* map = value ? &vmap : &kmap;
+                if constexpr (KIND == KV_ROWS) {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(full, Geo::TILE);
+#pragma unroll
+                        for (int c = 0; c < CH; c++)
+                            tma_load_3d(dst + c * Geo::HALF, map, c * 64, w.kvh, w.s.q0 + tile * kFaTile, full);
+                    }
+                } else {
+                    const int page = 1 << p.kv.page_log2;
+                    const int have = min(per_tile, (w.s.len - tile * kFaTile + page - 1) >> p.kv.page_log2);
+                    if (lane == 0) mbar_arrive_expect_tx(full, have * page * D * 2);
+                    __syncwarp();
+                    if (lane < have) {
+                        int id = page_ids;
+                        if (id < 0 || id >= p.kv.num_pages) {
+                            if (!value) record_error(p.err, ERR_KV_TABLE);
+                            id = p.kv.num_pages;  // outside the map: zeros
+                        }
+#pragma unroll
+                        for (int c = 0; c < CH; c++)
+                            tma_load_4d(dst + c * Geo::HALF + lane * page * 128, map, c * 64, 0, w.kvh, id, full);
+                    }
+                }
+                r.next();
+            };
+            load(false, w.kv0, ids);
+            // the queries, once the previous unit's last scores are multiplied
+            if (ok && !mbar_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 2)) ok = false;
+            q_phase ^= 1;
+            if (!ok) break;
+            if (lane == 0) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (w.nh[h] == 0) continue;
+                    mbar_arrive_expect_tx(&bar->q_full[h], tq * p.G * D * 2);
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+                        tma_load_3d(smem + Geo::Q_OFF + h * Geo::TILE + c * Geo::HALF, &qmap, c * 64, w.kvh * p.G,
+                                    w.s.q0 + w.i0 + h * tq, &bar->q_full[h]);
+                }
+            }
+            __syncwarp();
+            for (int i = 0; i < w.keys && ok; i++) {
+                const int cur = ids;
+                if (i + 1 < w.keys) {
+                    ids = ids_next;
+                    if (KIND != KV_ROWS && i + 2 < w.keys) ids_next = lookup(w.kv0 + i + 2);
+                    load(false, w.kv0 + i + 1, ids);
+                }
+                load(true, w.kv0 + i, cur);
+            }
+        }
+        // the ring is drained before the CTA ends: nothing may still arrive in its shared memory
+        for (int i = 0; i < ST; i++) {
+            mbar_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
+            r.next();
+        }
+        mbar_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 3);
+    } else if (warp == 8) {
+        // ---- the issuing warp ----
+        Ring<ST> r;
+        unsigned q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
+        bool ok = true;
+        constexpr uint32_t id_s = fa_idesc(kFaTile, false), id_o = fa_idesc(D, true);
+        auto wait = [&](uint64_t* b, unsigned ph, int role) {
+            if (ok && !mbar_wait(b, ph, p.err, ERR_FA_WAIT + role)) ok = false;
+            return ok;
+        };
+        auto scores = [&](int h, int stage) {
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t q = smem_addr(smem + Geo::Q_OFF + h * Geo::TILE), k = smem_addr(smem + Geo::KV_OFF + stage * Geo::TILE);
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) {
+                    const uint32_t off = (i / 4) * Geo::HALF + (i % 4) * 32;
+                    fa_mma_ss(tmem + h * 128, tc_smem_desc(q + off), tc_smem_desc(k + off), id_s, i > 0);
+                }
+                tc_commit(&bar->s_full[h]);
+            }
+            __syncwarp();
+        };
+        auto outputs = [&](int h, int stage, bool first, bool final) {
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t v = smem_addr(smem + Geo::KV_OFF + stage * Geo::TILE);
+#pragma unroll
+                for (int i = 0; i < kFaTile / 16; i++)
+                    fa_mma_ts(tmem + 256 + h * 128, tmem + h * 128 + i * 8, fa_desc_mn(v + i * 2048, Geo::HALF), id_o, !first || i > 0);
+                if (final) tc_commit(&bar->o_full[h]);
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint64_t* b) {
+            if (lane == 0) tc_commit(b);
+            __syncwarp();
+        };
+        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            const FaWork w = fa_work(p, ws, u, tq);
+            if (w.keys == 0) continue;
+            if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (w.nh[h] == 0) continue;
+                if (!wait(&bar->q_full[h], q_ph[h], 5)) break;
+                q_ph[h] ^= 1;
+                scores(h, r.i);
+            }
+            if (!ok) break;
+            release(&bar->kv_empty[r.i]);
+            r.next();
+            if (w.keys == 1) release(&bar->q_empty);
+            for (int i = 0; i < w.keys && ok; i++) {
+                const bool more = i + 1 < w.keys;
+                int k_stage = 0;
+                if (more) {
+                    k_stage = r.i;
+                    if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                    r.next();
+                }
+                const int v_stage = r.i;
+                if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                r.next();
+                const int left = w.s.len - (w.kv0 + i) * kFaTile;  // positions of the tile
+                if (left < kFaTile) {
+                    // rows behind the last position: anything may be there, and 0 * NaN is NaN
+                    uint8_t* v = smem + Geo::KV_OFF + v_stage * Geo::TILE;
+                    for (int o = left * 8 + lane; o < kFaTile * 8; o += 32)
+#pragma unroll
+                        for (int c = 0; c < CH; c++) *reinterpret_cast<uint4*>(v + c * Geo::HALF + o * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_async_smem();
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (i >= w.nh[h]) continue;
+                    if (!wait(&bar->p_ready[h], p_ph[h], 6)) break;
+                    p_ph[h] ^= 1;
+                    outputs(h, v_stage, i == 0, i + 1 == w.nh[h]);
+                    if (i + 1 < w.nh[h]) scores(h, k_stage);
+                }
+                if (!ok) break;
+                release(&bar->kv_empty[v_stage]);
+                if (more) release(&bar->kv_empty[k_stage]);
+                if (i + 2 == w.keys) release(&bar->q_empty);
+            }
+        }
+    } else if (warp < 8) {
+        // ---- softmax and epilogue: one thread per row ----
+        const int h = warp >> 2, row = tid & 127;
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lane_base + h * 128, to = tmem + lane_base + 256 + h * 128;
+        unsigned s_ph = 0, o_ph = 0;
+        bool ok = true;
+        const float scale = fabsf(p.scale_log2);
+        const bool negate = p.scale_log2 < 0.0f;
+        const int token_of = row / p.G, head_of = row - token_of * p.G;
+        const bool row_in = token_of < tq;
+        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            const FaWork w = fa_work(p, ws, u, tq);
+            const int token = w.i0 + h * tq + token_of;
+            const bool valid = row_in && token < w.s.n;
+            const int vis = valid ? max(0, min(w.s.len, w.s.len - w.s.n + token + 1)) : 0;
+            float m = -INFINITY, l = 0.0f;
+            for (int i = 0; i < w.nh[h]; i++) {
+                if (!mbar_wait(&bar->s_full[h], s_ph, p.err, ERR_FA_WAIT + 7)) {
+                    ok = false;
+                    break;
+                }
+                s_ph ^= 1;
+                tc_fence_after();
+                float s[128];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tm_ld32(ts + 32 * c, s + 32 * c);
+                tc_wait_ld();
+                if (negate) {
+#pragma unroll
+                    for (int c = 0; c < 128; c++) s[c] = -s[c];
+                }
+                // rows that are no query's (and the next sequence's) are not masked: nobody reads them
+                const int lim = valid ? vis - (w.kv0 + i) * kFaTile : kFaTile;
+                if (__any_sync(0xffffffffu, lim < kFaTile)) {
+#pragma unroll
+                    for (int c = 0; c < 128; c++) s[c] = c < lim ? s[c] : -INFINITY;
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int c = 4; c < 128; c += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], s[c + e]);
+                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                if (i == 0) {
+                    m = mn;
+                } else {
+                    const bool grow = (mn - m) * scale > 8.0f;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? exp2_fast((m - mn) * scale) : 1.0f;
+                        m = grow ? mn : m;
+                        l *= f;
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            float o[32];
+                            tm_ld32(to + 32 * c, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] *= f;
+                            tm_st32(to + 32 * c, reinterpret_cast<const uint32_t*>(o));
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m * scale;
+                float2 ls = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const float2 x = ffma2(make_float2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]), make_float2(scale, scale),
+                                               make_float2(-base, -base));
+                        const float a = exp2_fast(x.x), b = exp2_fast(x.y);
+                        ls = ffma2(make_float2(a, b), make_float2(1.0f, 1.0f), ls);
+                        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);  // weights in 8 bits' mantissa, as the tensor cores take bf16
+                        pk[e] = *reinterpret_cast<const uint32_t*>(&v);
+                    }
+                    tm_st32(ts + 32 * c, pk);
+                }
+                l += ls.x + ls.y;
+                tm_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->p_ready[h]);
+            }
+            if (!ok) break;
+            // ---- the row's output ----
+            const bool any = w.nh[h] > 0;
+            if (any) {
+                if (!mbar_wait(&bar->o_full[h], o_ph, p.err, ERR_FA_WAIT + 8)) {
+                    ok = false;
+                    break;
+                }
+                o_ph ^= 1;
+                tc_fence_after();
+            }
+            const float inv = w.slot >= 0 ? 1.0f : vis > 0 ? 1.0f / l : 0.0f;
+            const int head = w.kvh * p.G + head_of;
+            uint16_t* out = p.out + static_cast<int64_t>(w.s.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D;
+            float* part = ws.part + ((static_cast<int64_t>(max(w.slot, 0)) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + row) * (D + 4);
+            bool odd = false;
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                float o[32];
+                if (any) {
+                    tm_ld32(to + 32 * c, o);
+                    tc_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0.0f;
+                }
+                float bad = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    o[e] = vis > 0 ? o[e] * inv : 0.0f;
+                    bad = fmaf(o[e], 0.0f, bad);
+                }
+                odd |= bad != 0.0f;  // NaN unless every value is finite
+                if (!valid) continue;
+                if (w.slot < 0) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const __nv_bfloat162 b2 = __floats2bfloat162_rn(o[e + 2 * k], o[e + 2 * k + 1]);
+                            v[k] = *reinterpret_cast<const uint32_t*>(&b2);
+                        }
+                        *reinterpret_cast<uint4*>(out + 32 * c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4*>(part + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+            if (w.slot >= 0 && valid) *reinterpret_cast<float2*>(part + D) = make_float2(m == -INFINITY ? m : m * scale, l);
+            // Values that are not finite, behind some row's mask, reach that row as 0 * inf through the products: such rows
+            // are done again in plain loops over what they see.
+            unsigned again = __ballot_sync(0xffffffffu, valid && (odd || !(l <= 3.4e38f)));
+            while (again) {
+                const int src = __ffs(again) - 1;
+                again &= again - 1;
+                const int tk = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
+                const int see = __shfl_sync(0xffffffffu, vis, src);
+                const int j0 = w.kv0 * kFaTile, j1 = min(see, (w.kv0 + w.keys) * kFaTile);
+                float mm, ll, a[D / 32];
+                attend_row<KIND, D>(p, w.b, w.s.q0, w.s.q0 + tk, hd, j0, j1, lane, mm, ll, a);
+                if (w.slot < 0) {
+                    uint16_t* o = p.out + static_cast<int64_t>(w.s.q0 + tk) * p.out_stride + static_cast<int64_t>(hd) * D + lane * (D / 32);
+                    const float iv = see > 0 ? 1.0f / ll : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < D / 32; e += 2) {
+                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(a[e] * iv, a[e + 1] * iv);
+                        *reinterpret_cast<__nv_bfloat162*>(o + e) = b2;
+                    }
+                } else {
+                    float* o = ws.part + ((static_cast<int64_t>(w.slot) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + (warp & 3) * 32 + src) * (D + 4);
+#pragma unroll
+                    for (int e = 0; e < D / 32; e++) o[lane * (D / 32) + e] = a[e];
+                    if (lane == 0) *reinterpret_cast<float2*>(o + D) = make_float2(mm, ll);
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Rows whose positions were split: parts joined in order, one warp a row.
+template <int KIND, int D>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ PattnParams p, const __grid_constant__ FaWs ws) {
+    constexpr int E = D / 32;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int tq = fa_tokens(p.G);
+    const int64_t rows = static_cast<int64_t>(__ldcg(&ws.head->splits)) * p.Hkv * kFaRows;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < rows; i += static_cast<int64_t>(gridDim.x) * 8) {
+        const int r = static_cast<int>(i % kFaRows);
+        const int64_t tile = i / kFaRows;
+        const int kvh = static_cast<int>(tile % p.Hkv);
+        const int4 sp = __ldcg(reinterpret_cast<const int4*>(ws.splits + tile / p.Hkv));
+        const int hr = r % kFaTile;
+        const int token = sp.y + (r / kFaTile) * tq + hr / p.G, head = kvh * p.G + hr % p.G;
+        const Seq s = read_seq(p.q_start, p.kv_len, sp.x, p.T, p.kv_max, nullptr);
+        if (hr / p.G >= tq || token >= s.n) continue;
+        const int vis = max(0, min(s.len, s.len - s.n + token + 1));
+        const float* base = ws.part + ((static_cast<int64_t>(sp.z) * p.Hkv + kvh) * kFaRows + r) * (D + 4);
+        const int64_t step = static_cast<int64_t>(p.Hkv) * kFaRows * (D + 4);
+        float M = -INFINITY;
+        for (int j = lane; j < sp.w; j += 32) M = fmaxf(M, __ldcg(base + j * step + D));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float b0 = M == -INFINITY ? 0.0f : M;
+        float a[E] = {}, l = 0.0f;
+#pragma unroll 4
+        for (int j = 0; j < sp.w; j++) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(base + j * step + D));
+            const float f = exp2_fast(ml.x - b0);
+            l = fmaf(f, ml.y, l);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(base + j * step + lane * E + e));
+                a[e] = fmaf(f, v.x, a[e]);
+                a[e + 1] = fmaf(f, v.y, a[e + 1]);
+            }
+        }
+        const float inv = vis > 0 ? 1.0f / l : 0.0f;
+        uint16_t* o = p.out + static_cast<int64_t>(s.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const __nv_bfloat162 b2 = __floats2bfloat162_rn(a[e] * inv, a[e + 1] * inv);
+            *reinterpret_cast<__nv_bfloat162*>(o + e) = b2;
+        }
+    }
+}
+
+}  // namespace oomb
