@@ -175,12 +175,13 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t n, int64_t stride, 
     return encode_map(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, true);
 }
 
-// A bf16 pool in boxes of 64 columns x one head's rows of a page.
-bool encode_pool(CUtensorMap* map, const void* base, const KvView& kv, int D) {
-    const int page = 1 << kv.page_log2;
-    const int64_t dims[4] = {D, page, kv.Hkv, kv.num_pages}, strides[4] = {0, D * 2, page * D * 2, kv.page_stride * 2};
-    const int box[4] = {64, page, 1, 1};
-    return encode_map(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 4, dims, strides, box, true);
+// A pool in boxes of one head's rows of a page: 64 swizzled columns of bf16, or whole rows of codes.
+bool encode_pool(CUtensorMap* map, const void* base, const KvView& kv, int D, bool f8) {
+    const int page = 1 << kv.page_log2, es = f8 ? 1 : 2;
+    const int64_t dims[4] = {D, page, kv.Hkv, kv.num_pages}, strides[4] = {0, D * es, page * D * es, kv.page_stride * es};
+    const int box[4] = {f8 ? D : 64, page, 1, 1};
+    return encode_map(map, base, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, 4, dims, strides, box,
+                      !f8);
 }
 
 template <int KIND, int D>
@@ -199,12 +200,12 @@ int launch_fa(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream_t s
         if (!encode_rows(&km, p.kv.k, p.T, p.kv.k_stride, p.Hkv, D, 1, kFaTile) ||
             !encode_rows(&vm, p.kv.v, p.T, p.kv.v_stride, p.Hkv, D, 1, kFaTile))
             return OOMB_E_LAUNCH;
-    } else if (!encode_pool(&km, p.kv.k, p.kv, D) || !encode_pool(&vm, p.kv.v, p.kv, D)) {
+    } else if (!encode_pool(&km, p.kv.k, p.kv, D, KIND == KV_E4M3) || !encode_pool(&vm, p.kv.v, p.kv, D, KIND == KV_E4M3)) {
         return OOMB_E_LAUNCH;
     }
     int st = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, fw);
     if (st == OOMB_OK)
-        st = launch(fa_kernel<KIND, D>, dim3(w.grid), dim3(FaGeo<D>::THREADS), FaGeo<D>::TOTAL, s, p, fw, qm, km, vm);
+        st = launch(fa_kernel<KIND, D>, dim3(w.grid), dim3(FaGeo<KIND, D>::THREADS), FaGeo<KIND, D>::TOTAL, s, p, fw, qm, km, vm);
     if (st == OOMB_OK) st = launch(join_kernel<KIND, D>, dim3(2 * w.grid), dim3(256), 0, s, p, fw);
     return st;
 }
@@ -223,9 +224,7 @@ int launch_attn_d(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream
             return launch(decode_rows_kernel<KIND, D>, dim3(grid), dim3(kDecThreads), DecodeGeo<KIND, D>::smem, s, p, dw);
         }
     }
-    if constexpr (KIND != KV_E4M3) return launch_fa<KIND, D>(p, w, ws, s);
-    const int64_t warps = static_cast<int64_t>(p.T) * p.H;
-    return launch(attn_rows_kernel<KIND, D>, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, s, p);
+    return launch_fa<KIND, D>(p, w, ws, s);
 }
 
 template <int KIND>

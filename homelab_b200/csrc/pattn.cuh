@@ -106,33 +106,4 @@ __device__ __noinline__ void attend_row(const PattnParams& p, int b, int q0, int
     }
 }
 
-// One warp per (token, head).
-template <int KIND, int D>
-__global__ void __launch_bounds__(128) attn_rows_kernel(const PattnParams p) {
-    constexpr int E = D / 32;
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (w >= static_cast<int64_t>(p.T) * p.H) return;
-    const int t = static_cast<int>(w / p.H), h = static_cast<int>(w - static_cast<int64_t>(t) * p.H);
-    const int b = p.q_start ? find_sequence(p.q_start, p.B, t, lane) : t;
-    if (b >= p.B || (p.q_start && t < __ldcg(p.q_start))) return;
-    const Seq s = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, p.err);
-    if (s.n > p.max_q) {
-        record_error(p.err, ERR_KV_SEQ);
-        return;
-    }
-    const int vis = max(0, min(s.len, s.len - s.n + (t - s.q0) + 1));
-    float m, l, acc[E];
-    attend_row<KIND, D>(p, b, s.q0, t, h, 0, vis, lane, m, l, acc);
-    const float inv = vis > 0 ? 1.0f / l : 0.0f;
-    uint16_t* o = p.out + static_cast<int64_t>(t) * p.out_stride + static_cast<int64_t>(h) * D + lane * E;
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-        const __nv_bfloat162 v2 = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
-        *reinterpret_cast<__nv_bfloat162*>(o + i) = v2;
-    }
-}
-
 }  // namespace oomb

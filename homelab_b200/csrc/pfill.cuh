@@ -23,7 +23,8 @@
 // Warps: 0-3 and 4-7 one softmax thread per row of half 0 and 1 (also their epilogue);
 // 8 issues the products (and zeroes value rows behind the last position, which may hold
 // anything: 0 * NaN); 9 loads by TMA through a ring of key and value tiles, page by page for a
-// paged cache (a page of 16 or more rows keeps the swizzle's 8-row pattern).
+// paged cache (a page of 16 or more rows keeps the swizzle's 8-row pattern); for an e4m3 cache 12-15
+// turn the loaded codes into bf16 tiles on the way (once per tile, for all 256 rows).
 //
 // Work: plan_kernel lists the units (a tile, or a part of its positions when there are fewer
 // tiles than SMs), longest first; the CTAs take them in turn.  Parts leave (acc, m, l) in the
@@ -234,34 +235,51 @@ __device__ __forceinline__ void tm_ld32(uint32_t taddr, float* v) {
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tm_ld16(uint32_t taddr, float* v) {
+    uint32_t r[16];
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- shared memory --------------------------------------------------------------------
 
-template <int D>
+template <int KIND, int D>
 struct FaGeo {
+    static constexpr bool F8 = KIND == KV_E4M3;
     static constexpr int TILE = kFaTile * D * 2;         // bytes of 128 rows in bf16
     static constexpr int HALF = kFaTile * 128;           // bytes of 64 columns of them
-    static constexpr int STAGES = (224 * 1024 - 2 * TILE) / TILE < 8 ? (224 * 1024 - 2 * TILE) / TILE : 8;
+    static constexpr int CODES = kFaTile * D;            // bytes of 128 rows in e4m3
+    static constexpr int RAW = F8 ? 2 : 0;               // slots of codes before their conversion
+    static constexpr int ROOM = 224 * 1024 - 2 * TILE - RAW * CODES;
+    static constexpr int STAGES = ROOM / TILE < 8 ? ROOM / TILE : 8;
     static constexpr int Q_OFF = 0;
     static constexpr int KV_OFF = 2 * TILE;
-    static constexpr int BAR_OFF = KV_OFF + STAGES * TILE;
-    static constexpr int TOTAL = BAR_OFF + 256 + 1024;   // the base is aligned to 1024 at run time
-    static constexpr int THREADS = 320;
+    static constexpr int RAW_OFF = KV_OFF + STAGES * TILE;
+    static constexpr int EXP_OFF = RAW_OFF + RAW * CODES;
+    static constexpr int BAR_OFF = EXP_OFF + RAW * kFaTile;
+    static constexpr int TOTAL = BAR_OFF + 320 + 1024;   // the base is aligned to 1024 at run time
+    // registers: the softmax threads hold a row of scores; the rest give theirs up (the sums equal the launch's)
+    static constexpr int THREADS = F8 ? 512 : 384;
+    static constexpr int SOFT_REGS = F8 ? 192 : 208;
+    static constexpr int REST_REGS = F8 ? 64 : 88;
+    static_assert(256 * SOFT_REGS + (THREADS - 256) * REST_REGS <= THREADS * (F8 ? 128 : 168), "register split");
+    static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
 struct FaBars {
-    uint64_t q_full[2], q_empty, s_full[2], p_ready[2], o_full[2], kv_full[8], kv_empty[8];
+    uint64_t q_full[2], q_empty, s_full[2], p_ready[2], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2];
     uint32_t tmem;
 };
 
@@ -305,10 +323,11 @@ __device__ __forceinline__ FaWork fa_work(const PattnParams& p, const FaWs& ws, 
 }
 
 template <int KIND, int D>
-__global__ void __launch_bounds__(FaGeo<D>::THREADS, 1)
+__global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
     fa_kernel(const __grid_constant__ PattnParams p, const __grid_constant__ FaWs ws, const __grid_constant__ CUtensorMap qmap,
               const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using Geo = FaGeo<D>;
+    using Geo = FaGeo<KIND, D>;
+    constexpr bool F8 = Geo::F8;
     constexpr int ST = Geo::STAGES, CH = D / 64;  // 64-column chunks of a tile
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -325,8 +344,12 @@ __global__ void __launch_bounds__(FaGeo<D>::THREADS, 1)
         }
         mbar_init(&bar->q_empty, 1);
         for (int i = 0; i < ST; i++) {
-            mbar_init(&bar->kv_full[i], 1);
+            mbar_init(&bar->kv_full[i], F8 ? 4 : 1);
             mbar_init(&bar->kv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bar->raw_full[i], 1);
+            mbar_init(&bar->raw_empty[i], 4);
         }
         fence_barrier_init();
     }
@@ -341,185 +364,9 @@ __global__ void __launch_bounds__(FaGeo<D>::THREADS, 1)
     pdl_wait();
     pdl_launch_dependents();
     const int units = __ldcg(&ws.head->units) * p.Hkv;
-
-    if (warp == 9) {
-        // ---- loader ----
-        Ring<ST> r;
-        unsigned q_phase = 0;
-        bool ok = true;
-        const int32_t* table = nullptr;
-        int ids_of = -1, ids = 0, ids_next = 0;
-        const int per_tile = kFaTile >> p.kv.page_log2;  // pages of a tile
-        auto lookup = [&](int tile) {
-            int id = 0;
-            const int at = tile * per_tile + lane;
-            if (lane < per_tile && at < p.kv.max_pages) id = __ldcg(table + at);
-            return id;
-        };
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-            const FaWork w = fa_work(p, ws, u, tq);
-            if (w.keys == 0) continue;
-            if constexpr (KIND != KV_ROWS) {
-                table = p.kv.table + static_cast<int64_t>(w.b) * p.kv.table_stride;
-                ids_of = w.kv0;
-                ids = lookup(ids_of);
-                ids_next = w.keys > 1 ? lookup(ids_of + 1) : 0;
-            }
-            auto load = [&](bool value, int tile, int page_ids) {
-                if (!ok || !mbar_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 1)) {
-                    ok = false;
-                    return;
-                }
-                uint8_t* dst = smem + Geo::KV_OFF + r.i * Geo::TILE;
-                uint64_t* full = &bar->kv_full[r.i];
-                const CUtensorMap* map = value ? &vmap : &kmap;
-                if constexpr (KIND == KV_ROWS) {
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(full, Geo::TILE);
-#pragma unroll
-                        for (int c = 0; c < CH; c++)
-                            tma_load_3d(dst + c * Geo::HALF, map, c * 64, w.kvh, w.s.q0 + tile * kFaTile, full);
-                    }
-                } else {
-                    const int page = 1 << p.kv.page_log2;
-                    const int have = min(per_tile, (w.s.len - tile * kFaTile + page - 1) >> p.kv.page_log2);
-                    if (lane == 0) mbar_arrive_expect_tx(full, have * page * D * 2);
-                    __syncwarp();
-                    if (lane < have) {
-                        int id = page_ids;
-                        if (id < 0 || id >= p.kv.num_pages) {
-                            if (!value) record_error(p.err, ERR_KV_TABLE);
-                            id = p.kv.num_pages;  // outside the map: zeros
-                        }
-#pragma unroll
-                        for (int c = 0; c < CH; c++)
-                            tma_load_4d(dst + c * Geo::HALF + lane * page * 128, map, c * 64, 0, w.kvh, id, full);
-                    }
-                }
-                r.next();
-            };
-            load(false, w.kv0, ids);
-            // the queries, once the previous unit's last scores are multiplied
-            if (ok && !mbar_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 2)) ok = false;
-            q_phase ^= 1;
-            if (!ok) break;
-            if (lane == 0) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if (w.nh[h] == 0) continue;
-                    mbar_arrive_expect_tx(&bar->q_full[h], tq * p.G * D * 2);
-#pragma unroll
-                    for (int c = 0; c < CH; c++)
-                        tma_load_3d(smem + Geo::Q_OFF + h * Geo::TILE + c * Geo::HALF, &qmap, c * 64, w.kvh * p.G,
-                                    w.s.q0 + w.i0 + h * tq, &bar->q_full[h]);
-                }
-            }
-            __syncwarp();
-            for (int i = 0; i < w.keys && ok; i++) {
-                const int cur = ids;
-                if (i + 1 < w.keys) {
-                    ids = ids_next;
-                    if (KIND != KV_ROWS && i + 2 < w.keys) ids_next = lookup(w.kv0 + i + 2);
-                    load(false, w.kv0 + i + 1, ids);
-                }
-                load(true, w.kv0 + i, cur);
-            }
-        }
-        // the ring is drained before the CTA ends: nothing may still arrive in its shared memory
-        for (int i = 0; i < ST; i++) {
-            mbar_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
-            r.next();
-        }
-        mbar_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 3);
-    } else if (warp == 8) {
-        // ---- the issuing warp ----
-        Ring<ST> r;
-        unsigned q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
-        bool ok = true;
-        constexpr uint32_t id_s = fa_idesc(kFaTile, false), id_o = fa_idesc(D, true);
-        auto wait = [&](uint64_t* b, unsigned ph, int role) {
-            if (ok && !mbar_wait(b, ph, p.err, ERR_FA_WAIT + role)) ok = false;
-            return ok;
-        };
-        auto scores = [&](int h, int stage) {
-            tc_fence_after();
-            if (lane == 0) {
-                const uint32_t q = smem_addr(smem + Geo::Q_OFF + h * Geo::TILE), k = smem_addr(smem + Geo::KV_OFF + stage * Geo::TILE);
-#pragma unroll
-                for (int i = 0; i < D / 16; i++) {
-                    const uint32_t off = (i / 4) * Geo::HALF + (i % 4) * 32;
-                    fa_mma_ss(tmem + h * 128, tc_smem_desc(q + off), tc_smem_desc(k + off), id_s, i > 0);
-                }
-                tc_commit(&bar->s_full[h]);
-            }
-            __syncwarp();
-        };
-        auto outputs = [&](int h, int stage, bool first, bool final) {
-            tc_fence_after();
-            if (lane == 0) {
-                const uint32_t v = smem_addr(smem + Geo::KV_OFF + stage * Geo::TILE);
-#pragma unroll
-                for (int i = 0; i < kFaTile / 16; i++)
-                    fa_mma_ts(tmem + 256 + h * 128, tmem + h * 128 + i * 8, fa_desc_mn(v + i * 2048, Geo::HALF), id_o, !first || i > 0);
-                if (final) tc_commit(&bar->o_full[h]);
-            }
-            __syncwarp();
-        };
-        auto release = [&](uint64_t* b) {
-            if (lane == 0) tc_commit(b);
-            __syncwarp();
-        };
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-            const FaWork w = fa_work(p, ws, u, tq);
-            if (w.keys == 0) continue;
-            if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if (w.nh[h] == 0) continue;
-                if (!wait(&bar->q_full[h], q_ph[h], 5)) break;
-                q_ph[h] ^= 1;
-                scores(h, r.i);
-            }
-            if (!ok) break;
-            release(&bar->kv_empty[r.i]);
-            r.next();
-            if (w.keys == 1) release(&bar->q_empty);
-            for (int i = 0; i < w.keys && ok; i++) {
-                const bool more = i + 1 < w.keys;
-                int k_stage = 0;
-                if (more) {
-                    k_stage = r.i;
-                    if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
-                    r.next();
-                }
-                const int v_stage = r.i;
-                if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
-                r.next();
-                const int left = w.s.len - (w.kv0 + i) * kFaTile;  // positions of the tile
-                if (left < kFaTile) {
-                    // rows behind the last position: anything may be there, and 0 * NaN is NaN
-                    uint8_t* v = smem + Geo::KV_OFF + v_stage * Geo::TILE;
-                    for (int o = left * 8 + lane; o < kFaTile * 8; o += 32)
-#pragma unroll
-                        for (int c = 0; c < CH; c++) *reinterpret_cast<uint4*>(v + c * Geo::HALF + o * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    fence_async_smem();
-                    __syncwarp();
-                }
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if (i >= w.nh[h]) continue;
-                    if (!wait(&bar->p_ready[h], p_ph[h], 6)) break;
-                    p_ph[h] ^= 1;
-                    outputs(h, v_stage, i == 0, i + 1 == w.nh[h]);
-                    if (i + 1 < w.nh[h]) scores(h, k_stage);
-                }
-                if (!ok) break;
-                release(&bar->kv_empty[v_stage]);
-                if (more) release(&bar->kv_empty[k_stage]);
-                if (i + 2 == w.keys) release(&bar->q_empty);
-            }
-        }
-    } else if (warp < 8) {
+    // the register split stands inside the roles' branches: behind a join the smaller share would bind them all
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Geo::SOFT_REGS));
         // ---- softmax and epilogue: one thread per row ----
         const int h = warp >> 2, row = tid & 127;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -572,31 +419,31 @@ __global__ void __launch_bounds__(FaGeo<D>::THREADS, 1)
                         m = grow ? mn : m;
                         l *= f;
 #pragma unroll
-                        for (int c = 0; c < D / 32; c++) {
-                            float o[32];
-                            tm_ld32(to + 32 * c, o);
+                        for (int c = 0; c < D / 16; c++) {
+                            float o[16];
+                            tm_ld16(to + 16 * c, o);
                             tc_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] *= f;
-                            tm_st32(to + 32 * c, reinterpret_cast<const uint32_t*>(o));
+                            for (int e = 0; e < 16; e++) o[e] *= f;
+                            tm_st16(to + 16 * c, reinterpret_cast<const uint32_t*>(o));
                         }
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : m * scale;
                 float2 ls = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t pk[32];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t pk[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const float2 x = ffma2(make_float2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]), make_float2(scale, scale),
+                    for (int e = 0; e < 16; e++) {
+                        const float2 x = ffma2(make_float2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), make_float2(scale, scale),
                                                make_float2(-base, -base));
                         const float a = exp2_fast(x.x), b = exp2_fast(x.y);
                         ls = ffma2(make_float2(a, b), make_float2(1.0f, 1.0f), ls);
                         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);  // weights in 8 bits' mantissa, as the tensor cores take bf16
                         pk[e] = *reinterpret_cast<const uint32_t*>(&v);
                     }
-                    tm_st32(ts + 32 * c, pk);
+                    tm_st16(ts + 16 * c, pk);
                 }
                 l += ls.x + ls.y;
                 tm_wait_st();
@@ -683,6 +530,262 @@ __global__ void __launch_bounds__(FaGeo<D>::THREADS, 1)
                 }
             }
             tc_fence_before();
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Geo::REST_REGS));
+        if (warp == 9) {
+            // ---- loader (of the codes' slots when they are to be converted) ----
+            Ring<F8 ? 2 : ST> r;
+            uint64_t* const full_bar = F8 ? bar->raw_full : bar->kv_full;
+            uint64_t* const empty_bar = F8 ? bar->raw_empty : bar->kv_empty;
+            unsigned q_phase = 0;
+            bool ok = true;
+            const int32_t* table = nullptr;
+            int ids_of = -1, ids = 0, ids_next = 0;
+            const int per_tile = kFaTile >> p.kv.page_log2;  // pages of a tile
+            auto lookup = [&](int tile) {
+                int id = 0;
+                const int at = tile * per_tile + lane;
+                if (lane < per_tile && at < p.kv.max_pages) id = __ldcg(table + at);
+                return id;
+            };
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                const FaWork w = fa_work(p, ws, u, tq);
+                if (w.keys == 0) continue;
+                if constexpr (KIND != KV_ROWS) {
+                    table = p.kv.table + static_cast<int64_t>(w.b) * p.kv.table_stride;
+                    ids_of = w.kv0;
+                    ids = lookup(ids_of);
+                    ids_next = w.keys > 1 ? lookup(ids_of + 1) : 0;
+                }
+                auto load = [&](bool value, int tile, int page_ids) {
+                    if (!ok || !mbar_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 1)) {
+                        ok = false;
+                        return;
+                    }
+                    uint8_t* dst = smem + (F8 ? Geo::RAW_OFF + r.i * Geo::CODES : Geo::KV_OFF + r.i * Geo::TILE);
+                    uint64_t* full = &full_bar[r.i];
+                    const CUtensorMap* map = value ? &vmap : &kmap;
+                    if constexpr (KIND == KV_ROWS) {
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(full, Geo::TILE);
+#pragma unroll
+                            for (int c = 0; c < CH; c++)
+                                tma_load_3d(dst + c * Geo::HALF, map, c * 64, w.kvh, w.s.q0 + tile * kFaTile, full);
+                        }
+                    } else {
+                        const int page = 1 << p.kv.page_log2;
+                        const int have = min(per_tile, (w.s.len - tile * kFaTile + page - 1) >> p.kv.page_log2);
+                        const bool mine = lane < have;
+                        const bool good = mine && page_ids >= 0 && page_ids < p.kv.num_pages;
+                        if (mine && !good && !value) record_error(p.err, ERR_KV_TABLE);
+                        const int exps = F8 ? __popc(__ballot_sync(0xffffffffu, good)) * page : 0;
+                        if (lane == 0) mbar_arrive_expect_tx(full, have * page * D * (F8 ? 1 : 2) + exps);
+                        __syncwarp();
+                        if (mine) {
+                            const int id = good ? page_ids : p.kv.num_pages;  // outside the map: zeros
+                            if constexpr (F8) {
+                                tma_load_4d(dst + lane * page * D, map, 0, 0, w.kvh, id, full);
+                                if (good)
+                                    bulk_g2s_plain(smem + Geo::EXP_OFF + r.i * kFaTile + lane * page,
+                                                   (value ? p.kv.ve : p.kv.ke) + id * p.kv.exp_stride + (static_cast<int64_t>(w.kvh) << p.kv.page_log2),
+                                                   page, full);
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < CH; c++)
+                                    tma_load_4d(dst + c * Geo::HALF + lane * page * 128, map, c * 64, 0, w.kvh, id, full);
+                            }
+                        }
+                    }
+                    r.next();
+                };
+                load(false, w.kv0, ids);
+                // the queries, once the previous unit's last scores are multiplied
+                if (ok && !mbar_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 2)) ok = false;
+                q_phase ^= 1;
+                if (!ok) break;
+                if (lane == 0) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (w.nh[h] == 0) continue;
+                        mbar_arrive_expect_tx(&bar->q_full[h], tq * p.G * D * 2);
+#pragma unroll
+                        for (int c = 0; c < CH; c++)
+                            tma_load_3d(smem + Geo::Q_OFF + h * Geo::TILE + c * Geo::HALF, &qmap, c * 64, w.kvh * p.G,
+                                        w.s.q0 + w.i0 + h * tq, &bar->q_full[h]);
+                    }
+                }
+                __syncwarp();
+                for (int i = 0; i < w.keys && ok; i++) {
+                    const int cur = ids;
+                    if (i + 1 < w.keys) {
+                        ids = ids_next;
+                        if (KIND != KV_ROWS && i + 2 < w.keys) ids_next = lookup(w.kv0 + i + 2);
+                        load(false, w.kv0 + i + 1, ids);
+                    }
+                    load(true, w.kv0 + i, cur);
+                }
+            }
+            // the ring is drained before the CTA ends: nothing may still arrive in its shared memory
+            for (int i = 0; i < (F8 ? 2 : ST); i++) {
+                mbar_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
+                r.next();
+            }
+            mbar_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 3);
+        } else if (F8 && warp >= 12) {
+            // ---- conversion: codes times their row's power of two, exact in bf16, into the swizzled tile ----
+            Ring<2> rr;
+            Ring<ST> r;
+            bool ok = true;
+            constexpr int RC = D / 16;  // 16-code chunks of a row
+            const int ct = tid - 384;
+            auto convert = [&](int left) {
+                if (!ok || !mbar_wait(&bar->raw_full[rr.i], rr.phase, p.err, ERR_FA_WAIT + 9) ||
+                    !mbar_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 10)) {
+                    ok = false;
+                    return;
+                }
+                const uint8_t* codes = smem + Geo::RAW_OFF + rr.i * Geo::CODES;
+                const uint8_t* exps = smem + Geo::EXP_OFF + rr.i * kFaTile;
+                uint8_t* dst = smem + Geo::KV_OFF + r.i * Geo::TILE;
+#pragma unroll 2
+                for (int o = ct; o < kFaTile * RC; o += 128) {
+                    const int row = o / RC, c = o % RC;
+                    const uint4 w = *reinterpret_cast<const uint4*>(codes + o * 16);
+                    // a byte of 255 (a slot that was never written, or a page outside the pool) must not make NaN of zeros
+                    const float sc = exp_byte(min(static_cast<unsigned>(exps[row]), 254u));
+                    const unsigned u[4] = {w.x, w.y, w.z, w.w};
+                    uint32_t v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float2 f = e4m3x2_to_float2(static_cast<unsigned short>(u[i / 2] >> (16 * (i & 1))));
+                        const float2 g = fmul2(f, make_float2(sc, sc));
+                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(g.x, g.y);
+                        v[i] = *reinterpret_cast<const uint32_t*>(&b2);
+                    }
+                    if (row >= left) {  // behind the last position: anything may be there, and 0 * NaN is NaN
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[i] = 0u;
+                    }
+                    // chunks 2 (c % 4) and + 1 of the row's 64-column half; the upper half writes them in the other order, so
+                    // that eight lanes of a row meet eight bank groups
+                    uint8_t* at = dst + (c / 4) * Geo::HALF + row * 128;
+                    const int first = c / 4, k0 = 2 * (c % 4) + first, k1 = 2 * (c % 4) + 1 - first;
+                    const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
+                    *reinterpret_cast<uint4*>(at + ((k0 ^ (row & 7)) << 4)) = first ? hi : lo;
+                    *reinterpret_cast<uint4*>(at + ((k1 ^ (row & 7)) << 4)) = first ? lo : hi;
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&bar->kv_full[r.i]);
+                    mbar_arrive(&bar->raw_empty[rr.i]);
+                }
+                rr.next();
+                r.next();
+            };
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                const FaWork w = fa_work(p, ws, u, tq);
+                if (w.keys == 0) continue;
+                convert(w.s.len - w.kv0 * kFaTile);
+                for (int i = 0; i < w.keys && ok; i++) {
+                    const int left = w.s.len - (w.kv0 + i) * kFaTile;
+                    if (i + 1 < w.keys) convert(left - kFaTile);
+                    convert(left);
+                }
+            }
+            for (int i = 0; i < ST; i++) {  // every tile released before the CTA ends
+                mbar_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
+                r.next();
+            }
+        } else if (warp == 8) {
+            // ---- the issuing warp ----
+            Ring<ST> r;
+            unsigned q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
+            bool ok = true;
+            constexpr uint32_t id_s = fa_idesc(kFaTile, false), id_o = fa_idesc(D, true);
+            auto wait = [&](uint64_t* b, unsigned ph, int role) {
+                if (ok && !mbar_wait(b, ph, p.err, ERR_FA_WAIT + role)) ok = false;
+                return ok;
+            };
+            auto scores = [&](int h, int stage) {
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t q = smem_addr(smem + Geo::Q_OFF + h * Geo::TILE), k = smem_addr(smem + Geo::KV_OFF + stage * Geo::TILE);
+#pragma unroll
+                    for (int i = 0; i < D / 16; i++) {
+                        const uint32_t off = (i / 4) * Geo::HALF + (i % 4) * 32;
+                        fa_mma_ss(tmem + h * 128, tc_smem_desc(q + off), tc_smem_desc(k + off), id_s, i > 0);
+                    }
+                    tc_commit(&bar->s_full[h]);
+                }
+                __syncwarp();
+            };
+            auto outputs = [&](int h, int stage, bool first, bool final) {
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t v = smem_addr(smem + Geo::KV_OFF + stage * Geo::TILE);
+#pragma unroll
+                    for (int i = 0; i < kFaTile / 16; i++)
+                        fa_mma_ts(tmem + 256 + h * 128, tmem + h * 128 + i * 8, fa_desc_mn(v + i * 2048, Geo::HALF), id_o, !first || i > 0);
+                    if (final) tc_commit(&bar->o_full[h]);
+                }
+                __syncwarp();
+            };
+            auto release = [&](uint64_t* b) {
+                if (lane == 0) tc_commit(b);
+                __syncwarp();
+            };
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                const FaWork w = fa_work(p, ws, u, tq);
+                if (w.keys == 0) continue;
+                if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (w.nh[h] == 0) continue;
+                    if (!wait(&bar->q_full[h], q_ph[h], 5)) break;
+                    q_ph[h] ^= 1;
+                    scores(h, r.i);
+                }
+                if (!ok) break;
+                release(&bar->kv_empty[r.i]);
+                r.next();
+                if (w.keys == 1) release(&bar->q_empty);
+                for (int i = 0; i < w.keys && ok; i++) {
+                    const bool more = i + 1 < w.keys;
+                    int k_stage = 0;
+                    if (more) {
+                        k_stage = r.i;
+                        if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                        r.next();
+                    }
+                    const int v_stage = r.i;
+                    if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                    r.next();
+                    const int left = w.s.len - (w.kv0 + i) * kFaTile;  // positions of the tile
+                    if (!F8 && left < kFaTile) {
+                        // rows behind the last position: anything may be there, and 0 * NaN is NaN
+                        uint8_t* v = smem + Geo::KV_OFF + v_stage * Geo::TILE;
+                        for (int o = left * 8 + lane; o < kFaTile * 8; o += 32)
+#pragma unroll
+                            for (int c = 0; c < CH; c++) *reinterpret_cast<uint4*>(v + c * Geo::HALF + o * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        fence_async_smem();
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (i >= w.nh[h]) continue;
+                        if (!wait(&bar->p_ready[h], p_ph[h], 6)) break;
+                        p_ph[h] ^= 1;
+                        outputs(h, v_stage, i == 0, i + 1 == w.nh[h]);
+                        if (i + 1 < w.nh[h]) scores(h, k_stage);
+                    }
+                    if (!ok) break;
+                    release(&bar->kv_empty[v_stage]);
+                    if (more) release(&bar->kv_empty[k_stage]);
+                    if (i + 2 == w.keys) release(&bar->q_empty);
+                }
+            }
         }
     }
     __syncthreads();
