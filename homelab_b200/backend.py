@@ -56,6 +56,14 @@ def _ptr_or_host(t) -> int:
     return t.data_ptr()
 
 
+# the current device and a device's current stream as plain integers (a launch-bound call spends as long on
+# torch's Stream and device-guard objects as on its launch)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
+_ANY, _BF16 = (torch.float32, torch.bfloat16), (torch.bfloat16,)
+
+
 class Gpu:
     """One device's backend (the counterpart of `oominf_cuda::Gpu`)."""
 
@@ -63,10 +71,20 @@ class Gpu:
         self.device = torch.device("cuda", device)
         self.L = _lib.lib()
         self._tiled_ws = None  # grown on demand by moe_tiled calls without a workspace
-        self._attn_ws = {}     # per stream, grown on demand by paged and prompt attention without a workspace
+        # paged and prompt attention without a workspace: one per stream, grown on demand, and the shapes known to fit it
+        self._attn_ws = {}
 
     def _stream(self) -> int:
         return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _launch(self, fn, what: str, *args):
+        """fn(*args, current stream of this device), with this device the current one."""
+        i = self.device.index
+        if torch.cuda.is_initialized() and _current_device() == i:
+            check(fn(*args, _raw_stream(i)), what)
+            return
+        with torch.cuda.device(self.device):
+            check(fn(*args, self._stream()), what)
 
     # ---- Linear -------------------------------------------------------------------------
     def gemm_fp8(self, x, q, scale, y, t: int, n: int, k: int, layout: int = SCALE_128X128, workspace=None):
@@ -252,31 +270,34 @@ class Gpu:
         """The frequencies of a rotation on this device (oomb_rope_turns), made once per model."""
         return RopePlan(self.device, rot_dim, base, scaling, factor, original_len, interleaved)
 
-    def _rows(self, x, heads: int, dim: int, t: int, what: str, dtypes=(torch.float32, torch.bfloat16)):
+    def _rows(self, x, heads: int, dim: int, t: int, what: str, dtypes=_ANY):
         """Checks a [t, heads, dim] tensor on this device with contiguous rows; its address and token stride."""
+        st = x.stride()
+        if x.dtype in dtypes and x.shape == (t, heads, dim) and x.device == self.device:
+            if t > 1 and st[1] == dim and st[2] == 1:
+                return x.data_ptr(), st[0]
+            if t == 0 or (st[2] == 1 and (heads == 1 or st[1] == dim)):
+                return x.data_ptr(), (st[0] if t > 1 else heads * dim)
+            raise ValueError(f"the heads of a token of {what} must be contiguous")
         if x.dtype not in dtypes:
             raise TypeError(f"{what} must be one of {dtypes}, got {x.dtype}")
-        if tuple(x.shape) != (t, heads, dim):
+        if x.shape != (t, heads, dim):
             raise ValueError(f"{what} must be [{t}, {heads}, {dim}], got {tuple(x.shape)}")
-        if x.device != self.device:
-            raise ValueError(f"{what} must live on {self.device}, got {x.device}")
-        if t and (x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim)):
-            raise ValueError(f"the heads of a token of {what} must be contiguous")
-        return _ptr(x), (x.stride(0) if t > 1 else heads * dim)
+        raise ValueError(f"{what} must live on {self.device}, got {x.device}")
 
     def _index(self, x, n, what: str):
         if x is None:
             return None
-        if x.dtype != torch.int32 or not x.is_contiguous() or x.device != self.device or (
-                x.dim() != 1 or (n is not None and x.numel() != n)):
+        if x.dtype != torch.int32 or x.device != self.device or x.dim() != 1 or not x.is_contiguous() or (
+                n is not None and x.shape[0] != n):
             raise ValueError(f"{what} must be a contiguous int32 [{'B' if n is None else n}] tensor on {self.device}")
-        return _ptr(x)
+        return x.data_ptr()
 
     def _step(self, cache: PagedKv, q_start, kv_len, t: int):
         """The batch of a packed step over `cache` and its index addresses."""
         if cache.device != self.device:
             raise ValueError(f"the cache must live on {self.device}, got {cache.device}")
-        B = kv_len.numel()
+        B = kv_len.shape[0] if kv_len.dim() == 1 else -1
         if cache.batch < B:
             raise ValueError(f"the block table has {cache.batch} rows for {B} sequences")
         if q_start is None and B != t:
@@ -295,9 +316,7 @@ class Gpu:
         pos = self._index(positions, T, "positions")
         if T == 0:
             return out
-        with torch.cuda.device(self.device):
-            check(self.L.oomb_rope_rows(C.byref(plan.struct), xp, _dtype_code(x), xs, pos, op, os_, T, H, D,
-                                        self._stream()), "rope")
+        self._launch(self.L.oomb_rope_rows, "rope", plan.ref, xp, _dtype_code(x), xs, pos, op, os_, T, H, D)
         return out
 
     def kv_append_paged(self, cache: PagedKv, k, v, q_start, kv_len, rope: RopePlan = None, q=None, q_out=None):
@@ -316,13 +335,11 @@ class Gpu:
         if q is not None:
             H = q.shape[1]
             qp, qs = self._rows(q, H, D, T, "q", (k.dtype,))
-            qo, qos = self._rows(q_out, H, D, T, "q_out", (torch.bfloat16,))
+            qo, qos = self._rows(q_out, H, D, T, "q_out", _BF16)
         if T == 0 or B == 0:
             return
-        with torch.cuda.device(self.device):
-            check(self.L.oomb_kv_append_paged(C.byref(cache.struct), C.byref(rope.struct) if rope is not None else None,
-                                              qp, qs, qo, qos, H, kp, ks, vp, vs, _dtype_code(k), qs_p, len_p, B, T,
-                                              self._stream()), "kv_append_paged")
+        self._launch(self.L.oomb_kv_append_paged, "kv_append_paged", cache.ref, None if rope is None else rope.ref, qp, qs,
+                     qo, qos, H, kp, ks, vp, vs, _dtype_code(k), qs_p, len_p, B, T)
 
     def kv_read_paged(self, cache: PagedKv, q_start, kv_len, k_out, v_out):
         """The cached rows at a packed step's positions (the last n_b of each sequence's kv_len) into
@@ -335,9 +352,7 @@ class Gpu:
         B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
         if T == 0 or B == 0:
             return
-        with torch.cuda.device(self.device):
-            check(self.L.oomb_kv_read_paged(C.byref(cache.struct), qs_p, len_p, B, T, kp, vp, _dtype_code(k_out), ks,
-                                            self._stream()), "kv_read_paged")
+        self._launch(self.L.oomb_kv_read_paged, "kv_read_paged", cache.ref, qs_p, len_p, B, T, kp, vp, _dtype_code(k_out), ks)
 
     def attention_paged_workspace(self, batch: int, t: int, max_q: int, heads: int, kv_heads: int,
                                   head_dim: int) -> torch.Tensor:
@@ -349,17 +364,27 @@ class Gpu:
             raise ValueError("unsupported attention shape")
         return torch.zeros(n, dtype=torch.uint8, device=self.device)
 
-    def _attention_ws(self, need: int) -> torch.Tensor:
-        """A workspace of this object's for the current stream.  A graph gets one of its own, so that graphs
-        (and eager calls beside them) never share one."""
-        if need == 0:
-            raise ValueError("unsupported attention shape")
-        if torch.cuda.is_current_stream_capturing():
-            return torch.zeros(need, dtype=torch.uint8, device=self.device)
-        s = self._stream()
-        ws = self._attn_ws.get(s)
-        if ws is None or ws.numel() < need:
-            ws = self._attn_ws[s] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+    def _attention_ws(self, paged: bool, *shape) -> torch.Tensor:
+        """A workspace of this object's for a call of this shape on the current stream.  A graph gets one of its
+        own, so that graphs (and eager calls beside them) never share one."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        key = (_raw_stream(self.device.index), paged, *shape)
+        if not capturing and key in self._attn_ws:
+            return self._attn_ws[key]
+        with torch.cuda.device(self.device):
+            need = int((self.L.oomb_attention_paged_workspace_bytes if paged else
+                        self.L.oomb_attention_prompt_workspace_bytes)(*shape))
+            if need == 0:
+                raise ValueError("unsupported attention shape")
+            if capturing:
+                return torch.zeros(need, dtype=torch.uint8, device=self.device)
+            ws = self._attn_ws.get(key[0])
+            if ws is None or ws.numel() < need:
+                self._attn_ws = {k: w for k, w in self._attn_ws.items() if k != key[0] and (
+                    isinstance(k, int) or k[0] != key[0])}
+                ws = self._attn_ws[key[0]] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        if len(self._attn_ws) < 4096:
+            self._attn_ws[key] = ws
         return ws
 
     def attention_paged(self, q, cache: PagedKv, out, q_start, kv_len, max_q: int, scale: float, workspace=None):
@@ -370,37 +395,31 @@ class Gpu:
         T, H, D = q.shape
         if D != cache.head_dim:
             raise ValueError(f"q has head_dim {D}, the cache {cache.head_dim}")
-        qp, qs = self._rows(q, H, D, T, "q", (torch.bfloat16,))
-        op, os_ = self._rows(out, H, D, T, "out", (torch.bfloat16,))
+        qp, qs = self._rows(q, H, D, T, "q", _BF16)
+        op, os_ = self._rows(out, H, D, T, "out", _BF16)
         B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
         if T == 0 or B == 0:
             return
-        with torch.cuda.device(self.device):
-            ws = workspace
-            if ws is None:
-                ws = self._attention_ws(int(self.L.oomb_attention_paged_workspace_bytes(B, T, max_q, H, cache.kv_heads, D)))
-            check(self.L.oomb_attention_paged(C.byref(cache.struct), qp, qs, op, os_, H, qs_p, len_p, B, T, int(max_q),
-                                              float(scale), _ptr(ws), ws.numel(), self._stream()), "attention_paged")
+        ws = self._attention_ws(True, B, T, max_q, H, cache.kv_heads, D) if workspace is None else workspace
+        self._launch(self.L.oomb_attention_paged, "attention_paged", cache.ref, qp, qs, op, os_, H, qs_p, len_p, B, T, max_q,
+                     scale, _ptr(ws), ws.numel())
 
     def attention_prompt(self, q, k, v, out, q_start, max_q: int, scale: float, workspace=None):
         """Causal attention over packed whole prompts (oomb_attention_prompt): q, out bf16 [T, H, D],
         k, v bf16 [T, kv_heads, D], q_start int32 [B + 1]; max_q bounds a prompt's tokens."""
         T, H, D = q.shape
         Hkv = k.shape[1]
-        qp, qs = self._rows(q, H, D, T, "q", (torch.bfloat16,))
-        kp, ks = self._rows(k, Hkv, D, T, "k", (torch.bfloat16,))
-        vp, vs = self._rows(v, Hkv, D, T, "v", (torch.bfloat16,))
-        op, os_ = self._rows(out, H, D, T, "out", (torch.bfloat16,))
+        qp, qs = self._rows(q, H, D, T, "q", _BF16)
+        kp, ks = self._rows(k, Hkv, D, T, "k", _BF16)
+        vp, vs = self._rows(v, Hkv, D, T, "v", _BF16)
+        op, os_ = self._rows(out, H, D, T, "out", _BF16)
         qs_p = self._index(q_start, None, "q_start")
         B = q_start.numel() - 1
         if T == 0 or B <= 0:
             return
-        with torch.cuda.device(self.device):
-            ws = workspace
-            if ws is None:
-                ws = self._attention_ws(int(self.L.oomb_attention_prompt_workspace_bytes(B, T, max_q, H, Hkv, D)))
-            check(self.L.oomb_attention_prompt(qp, qs, kp, ks, vp, vs, op, os_, H, Hkv, D, qs_p, B, T, int(max_q),
-                                               float(scale), _ptr(ws), ws.numel(), self._stream()), "attention_prompt")
+        ws = self._attention_ws(False, B, T, max_q, H, Hkv, D) if workspace is None else workspace
+        self._launch(self.L.oomb_attention_prompt, "attention_prompt", qp, qs, kp, ks, vp, vs, op, os_, H, Hkv, D, qs_p, B, T,
+                     max_q, scale, _ptr(ws), ws.numel())
 
     def device_error(self, clear: bool = True) -> int:
         code = C.c_int(0)

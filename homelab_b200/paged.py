@@ -13,6 +13,7 @@ import torch
 from . import _lib
 from ._lib import KV_BF16, KV_E4M3, PagedKvStruct, RopeStruct, check
 
+_CODES = (torch.float8_e4m3fn, torch.uint8)
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "by_parts": 3}
 
 
@@ -38,6 +39,7 @@ class RopePlan:
         self.turns = turns.to(device)
         self.struct = RopeStruct(rot_dim=self.rot_dim, interleaved=int(self.interleaved), mscale=m,
                                  turns=self.turns.data_ptr())
+        self.ref = C.byref(self.struct)
 
 
 class PagedKv:
@@ -52,38 +54,38 @@ class PagedKv:
 
     def __init__(self, k_pages, v_pages, block_table, k_exp=None, v_exp=None):
         fp8 = k_exp is not None or v_exp is not None
-        kinds = (torch.float8_e4m3fn, torch.uint8) if fp8 else (torch.bfloat16,)
-        if k_pages.dtype not in kinds or v_pages.dtype != k_pages.dtype:
-            raise TypeError(f"pages must both be one of {kinds}, got {k_pages.dtype} and {v_pages.dtype}")
-        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        kind, shape, ks, device = k_pages.dtype, k_pages.shape, k_pages.stride(), k_pages.device
+        if (kind not in _CODES if fp8 else kind is not torch.bfloat16) or v_pages.dtype is not kind:
+            raise TypeError(f"pages must both be {'e4m3 codes' if fp8 else 'bf16'}, got {kind} and {v_pages.dtype}")
+        if len(shape) != 4 or v_pages.shape != shape:
             raise ValueError("k_pages and v_pages must be [pages, kv_heads, page_size, head_dim], of one shape")
-        pages, heads, size, dim = k_pages.shape
-        for x in (k_pages, v_pages):
-            if x.stride()[1:] != (size * dim, dim, 1) or x.stride(0) != k_pages.stride(0):
-                raise ValueError("the rows of a page must be contiguous, and both pools strided alike")
+        pages, heads, size, dim = shape
+        if ks[1:] != (size * dim, dim, 1) or v_pages.stride() != ks:
+            raise ValueError("the rows of a page must be contiguous, and both pools strided alike")
+        es = (0, 0, 0)
         if fp8:
             for x in (k_exp, v_exp):
-                if x is None or x.dtype != torch.uint8 or x.shape != (pages, heads, size):
+                if x is None or x.dtype is not torch.uint8 or x.shape != (pages, heads, size):
                     raise ValueError("k_exp and v_exp must be uint8 [pages, kv_heads, page_size]")
-                if x.stride()[1:] != (size, 1) or x.stride(0) != k_exp.stride(0):
-                    raise ValueError("the exponents of a page must be contiguous, and both strided alike")
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or (
-                block_table.shape[1] > 1 and block_table.stride(1) != 1):
+            es = k_exp.stride()
+            if es[1:] != (size, 1) or v_exp.stride() != es:
+                raise ValueError("the exponents of a page must be contiguous, and both strided alike")
+            if k_exp.device != device or v_exp.device != device:
+                raise ValueError("the pages, exponents and block table must live on one device")
+        ts = block_table.stride()
+        if block_table.dtype is not torch.int32 or len(ts) != 2 or (ts[1] != 1 and block_table.shape[1] > 1):
             raise ValueError("block_table must be int32 [batch, max_pages] with contiguous rows")
-        tensors = [x for x in (k_pages, v_pages, block_table, k_exp, v_exp) if x is not None]
-        if len({x.device for x in tensors}) != 1:
+        if v_pages.device != device or block_table.device != device:
             raise ValueError("the pages, exponents and block table must live on one device")
         self.k_pages, self.v_pages, self.k_exp, self.v_exp, self.block_table = k_pages, v_pages, k_exp, v_exp, block_table
-        self.kv_heads, self.page_size, self.head_dim, self.fp8 = heads, size, dim, fp8
+        self.kv_heads, self.page_size, self.head_dim, self.fp8, self.device = heads, size, dim, fp8, device
         self.batch, self.max_pages = block_table.shape
-        self.device = k_pages.device
         self.struct = PagedKvStruct(
-            dtype=KV_E4M3 if fp8 else KV_BF16, kv_heads=heads, head_dim=dim, page_size=size, num_pages=pages,
-            max_pages=self.max_pages, table_stride=max(block_table.stride(0), self.max_pages),
-            k=k_pages.data_ptr(), v=v_pages.data_ptr(), k_exp=k_exp.data_ptr() if fp8 else None,
-            v_exp=v_exp.data_ptr() if fp8 else None, page_stride=k_pages.stride(0) if pages > 1 else heads * size * dim,
-            exp_page_stride=(k_exp.stride(0) if pages > 1 else heads * size) if fp8 else 0,
-            block_table=block_table.data_ptr())
+            KV_E4M3 if fp8 else KV_BF16, heads, dim, size, pages, self.max_pages, max(ts[0], self.max_pages), 0,
+            k_pages.data_ptr(), v_pages.data_ptr(), k_exp.data_ptr() if fp8 else None, v_exp.data_ptr() if fp8 else None,
+            ks[0] if pages > 1 else heads * size * dim, (es[0] if pages > 1 else heads * size) if fp8 else 0,
+            block_table.data_ptr())
+        self.ref = C.byref(self.struct)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, block_table, fp8: bool = False):
