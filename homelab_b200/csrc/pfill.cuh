@@ -202,21 +202,24 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 __host__ __device__ constexpr uint32_t fa_idesc(int n, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void fa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
+// Descriptors by their low words and a common high word.
+__device__ __forceinline__ void fa_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, int acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %5, 0;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}" ::"r"(d),
+        "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void fa_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+__device__ __forceinline__ void fa_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, int acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n mov.b64 db, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}" ::"r"(d),
+        "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(acc)
         : "memory");
 }
 // An MN-major operand in the 128-byte swizzle: rows of 64 values (128 bytes) along N, 8-row groups along K 1024
 // bytes apart (stride offset), further 64-value columns `lead` bytes apart (leading offset).
-__device__ __forceinline__ uint64_t fa_desc_mn(uint32_t addr, uint32_t lead) {
+__host__ __device__ constexpr uint64_t fa_desc_mn(uint32_t addr, uint32_t lead) {
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lead >> 4) << 16) | (64ull << 32) | (1ull << 46) |
            (2ull << 61);
 }
@@ -283,6 +286,15 @@ struct FaBars {
     uint32_t tmem;
 };
 
+// The value of lane 0 in every lane: the compiler then keeps it, and what it makes of it, in uniform
+// registers, which the tensor instructions take their descriptors from.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ bool elect_one() {
+    unsigned r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+    return r != 0;
+}
+
 // A role's pipeline position over a ring of N stages.
 template <int N>
 struct Ring {
@@ -295,6 +307,14 @@ struct Ring {
         }
     }
 };
+
+// As mbar_wait, but the clock and the limit (a load from global memory, some 600 cycles) are read only
+// after many polls: a wait of a tile's length must not pay for them.
+__device__ __forceinline__ bool fa_wait(uint64_t* bar, unsigned parity, unsigned* err, unsigned code) {
+    for (int i = 0; i < 64; i++)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait(bar, parity, err, code);
+}
 
 // What every role derives from a unit: the sequence and each half's key tiles.
 struct FaWork {
@@ -384,7 +404,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             const int vis = valid ? max(0, min(w.s.len, w.s.len - w.s.n + token + 1)) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < w.nh[h]; i++) {
-                if (!mbar_wait(&bar->s_full[h], s_ph, p.err, ERR_FA_WAIT + 7)) {
+                if (!fa_wait(&bar->s_full[h], s_ph, p.err, ERR_FA_WAIT + 7)) {
                     ok = false;
                     break;
                 }
@@ -455,7 +475,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             // ---- the row's output ----
             const bool any = w.nh[h] > 0;
             if (any) {
-                if (!mbar_wait(&bar->o_full[h], o_ph, p.err, ERR_FA_WAIT + 8)) {
+                if (!fa_wait(&bar->o_full[h], o_ph, p.err, ERR_FA_WAIT + 8)) {
                     ok = false;
                     break;
                 }
@@ -559,7 +579,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                     ids_next = w.keys > 1 ? lookup(ids_of + 1) : 0;
                 }
                 auto load = [&](bool value, int tile, int page_ids) {
-                    if (!ok || !mbar_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 1)) {
+                    if (!ok || !fa_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 1)) {
                         ok = false;
                         return;
                     }
@@ -601,7 +621,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 };
                 load(false, w.kv0, ids);
                 // the queries, once the previous unit's last scores are multiplied
-                if (ok && !mbar_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 2)) ok = false;
+                if (ok && !fa_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 2)) ok = false;
                 q_phase ^= 1;
                 if (!ok) break;
                 if (lane == 0) {
@@ -628,10 +648,10 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             }
             // the ring is drained before the CTA ends: nothing may still arrive in its shared memory
             for (int i = 0; i < (F8 ? 2 : ST); i++) {
-                mbar_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
+                fa_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
                 r.next();
             }
-            mbar_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 3);
+            fa_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 3);
         } else if (F8 && warp >= 12) {
             // ---- conversion: codes times their row's power of two, exact in bf16, into the swizzled tile ----
             Ring<2> rr;
@@ -640,8 +660,8 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             constexpr int RC = D / 16;  // 16-code chunks of a row
             const int ct = tid - 384;
             auto convert = [&](int left) {
-                if (!ok || !mbar_wait(&bar->raw_full[rr.i], rr.phase, p.err, ERR_FA_WAIT + 9) ||
-                    !mbar_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 10)) {
+                if (!ok || !fa_wait(&bar->raw_full[rr.i], rr.phase, p.err, ERR_FA_WAIT + 9) ||
+                    !fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 10)) {
                     ok = false;
                     return;
                 }
@@ -695,7 +715,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 }
             }
             for (int i = 0; i < ST; i++) {  // every tile released before the CTA ends
-                mbar_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
+                fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
                 r.next();
             }
         } else if (warp == 8) {
@@ -705,17 +725,22 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             bool ok = true;
             constexpr uint32_t id_s = fa_idesc(kFaTile, false), id_o = fa_idesc(D, true);
             auto wait = [&](uint64_t* b, unsigned ph, int role) {
-                if (ok && !mbar_wait(b, ph, p.err, ERR_FA_WAIT + role)) ok = false;
+                if (ok && !fa_wait(b, ph, p.err, ERR_FA_WAIT + role)) ok = false;
                 return ok;
             };
+            const uint32_t q_lo = uniform(static_cast<uint32_t>(tc_smem_desc(smem_addr(smem + Geo::Q_OFF))));
+            const uint32_t k_lo = uniform(static_cast<uint32_t>(tc_smem_desc(smem_addr(smem + Geo::KV_OFF))));
+            const uint32_t v_lo = uniform(static_cast<uint32_t>(fa_desc_mn(smem_addr(smem + Geo::KV_OFF), Geo::HALF)));
+            constexpr uint32_t k_hi = static_cast<uint32_t>(tc_smem_desc(0) >> 32), v_hi = static_cast<uint32_t>(fa_desc_mn(0, 0) >> 32);
+            const uint32_t tm = uniform(tmem);
             auto scores = [&](int h, int stage) {
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t q = smem_addr(smem + Geo::Q_OFF + h * Geo::TILE), k = smem_addr(smem + Geo::KV_OFF + stage * Geo::TILE);
+                const uint32_t q = q_lo + h * (Geo::TILE >> 4), k = uniform(k_lo + stage * (Geo::TILE >> 4));
+                if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < D / 16; i++) {
-                        const uint32_t off = (i / 4) * Geo::HALF + (i % 4) * 32;
-                        fa_mma_ss(tmem + h * 128, tc_smem_desc(q + off), tc_smem_desc(k + off), id_s, i > 0);
+                        const uint32_t off = ((i / 4) * Geo::HALF + (i % 4) * 32) >> 4;
+                        fa_mma_ss(tm + h * 128, q + off, k + off, k_hi, id_s, i > 0);
                     }
                     tc_commit(&bar->s_full[h]);
                 }
@@ -723,17 +748,18 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             };
             auto outputs = [&](int h, int stage, bool first, bool final) {
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t v = smem_addr(smem + Geo::KV_OFF + stage * Geo::TILE);
+                const uint32_t v = uniform(v_lo + stage * (Geo::TILE >> 4));
+                const int more = uniform(!first);
+                if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < kFaTile / 16; i++)
-                        fa_mma_ts(tmem + 256 + h * 128, tmem + h * 128 + i * 8, fa_desc_mn(v + i * 2048, Geo::HALF), id_o, !first || i > 0);
+                        fa_mma_ts(tm + 256 + h * 128, tm + h * 128 + i * 8, v + i * (2048 >> 4), v_hi, id_o, i > 0 ? 1 : more);
                     if (final) tc_commit(&bar->o_full[h]);
                 }
                 __syncwarp();
             };
             auto release = [&](uint64_t* b) {
-                if (lane == 0) tc_commit(b);
+                if (elect_one()) tc_commit(b);
                 __syncwarp();
             };
             for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {

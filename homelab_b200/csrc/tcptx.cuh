@@ -23,7 +23,7 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 // Shared-memory matrix descriptor of a K-major operand in the 128-byte swizzled
 // canonical layout: 128-byte rows, 8-row groups 1024 bytes apart (stride byte
 // offset 64 x 16 B), descriptor version 1, layout type 2 (128-byte swizzle).
-__device__ __forceinline__ uint64_t tc_smem_desc(uint32_t addr) {
+__host__ __device__ constexpr uint64_t tc_smem_desc(uint32_t addr) {
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) |
            (2ull << 61);
 }
