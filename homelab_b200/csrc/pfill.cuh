@@ -11,16 +11,20 @@
 // factor cancels in O / l, and e^8 in base 2 keeps bf16 and fp32 far from overflow), which after
 // the first tiles is rare.
 //
-// Bound: with D = 128 a pair of halves costs 4 x 512 tensor-pipe cycles per 128
-// positions and 2 x 16,384 exponentials, which at 16 a cycle and SM are 2,048 cycles as
+// Bound: with D = 128 a pair of halves costs 32 products of 64 tensor-pipe cycles per 128
+// positions (a product of M = 128 takes about 64 cycles for any N up to 128: its operands come
+// out of shared memory) and 2 x 16,384 exponentials, which at 16 a cycle and SM are 2,048 cycles as
 // well.  The two halves run in turn: while one's scores go through the exponentials,
-// the tensor cores multiply the other's.  One issuing thread orders the products
+// the tensor cores multiply the other's.  One issuing warp orders the products
 //   S0 S1 | O0 S0' | O1 S1' | ...,
 // and since they complete in order, the barrier of S0' also says that O0 is at rest, so a
 // row's thread may rescale it without another wait, and S may be overwritten as soon as
-// P was consumed.
+// P was consumed.  Scores, maxima, exponentials and products of one half still follow one
+// another (tensor memory has no room for second scores beside two outputs of 128 columns), which leaves
+// the tensor cores idle about a third of the time.  Tried and no faster: two threads a row (619 us),
+// scores of 64 positions at a time, made ahead (633 us: the products cost the same at N = 64).
 //
-// Warps: 0-3 and 4-7 one softmax thread per row of half 0 and 1 (also their epilogue);
+// Warps: 0-3 and 4-7 the softmax of half 0 and 1 (and their epilogue), one thread a row;
 // 8 issues the products (and zeroes value rows behind the last position, which may hold
 // anything: 0 * NaN); 9 loads by TMA through a ring of key and value tiles, page by page for a
 // paged cache (a page of 16 or more rows keeps the swizzle's 8-row pattern); for an e4m3 cache 12-15
@@ -38,6 +42,10 @@ namespace oomb {
 
 constexpr int kFaTile = 128;
 constexpr int kFaRows = 256;       // rows of a tile pair
+// Parts of a tile's weights that are handed to the product on their own; measured on two packed prompts of 8192 and 3001
+// tokens (32 heads over 8, D = 128): one part 610 us, two 569-600, four 601-625 (each hand-over waits for its stores).
+constexpr int kFaParts = 2;
+constexpr int kFaSoft = 8;         // softmax warps
 constexpr int kFaMinPart = 4;      // key tiles of a part at least
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBuckets = 1024;
@@ -272,17 +280,17 @@ struct FaGeo {
     static constexpr int RAW_OFF = KV_OFF + STAGES * TILE;
     static constexpr int EXP_OFF = RAW_OFF + RAW * CODES;
     static constexpr int BAR_OFF = EXP_OFF + RAW * kFaTile;
-    static constexpr int TOTAL = BAR_OFF + 320 + 1024;   // the base is aligned to 1024 at run time
+    static constexpr int TOTAL = BAR_OFF + 320;
     // registers: the softmax threads hold a row of scores; the rest give theirs up (the sums equal the launch's)
-    static constexpr int THREADS = F8 ? 512 : 384;
+    static constexpr int THREADS = kFaSoft * 32 + (F8 ? 256 : 128);
     static constexpr int SOFT_REGS = F8 ? 192 : 208;
     static constexpr int REST_REGS = F8 ? 64 : 88;
-    static_assert(256 * SOFT_REGS + (THREADS - 256) * REST_REGS <= THREADS * (F8 ? 128 : 168), "register split");
+    static_assert(kFaSoft * 32 * SOFT_REGS + (THREADS - kFaSoft * 32) * REST_REGS <= THREADS * (F8 ? 128 : 168), "register split");
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
 struct FaBars {
-    uint64_t q_full[2], q_empty, s_full[2], p_ready[2], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2];
+    uint64_t q_full[2], q_empty, s_full[2], p_ready[2][kFaParts], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2];
     uint32_t tmem;
 };
 
@@ -307,6 +315,33 @@ struct Ring {
         }
     }
 };
+
+// The larger of three (one instruction on sm_100).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^x of two values on the FMA units: x = r + f, r the nearest integer, 2^f by a polynomial of degree 4
+// fitted to it on [-1/2, 1/2] (Remez exchange on the relative error: 2.7e-6, an 800th of the weights'
+// rounding to bf16), r added to the exponent.  Below -126 it stays at 2^-126; NaN gives a huge
+// value, which the epilogue's check for values that are not finite finds.  -inf < x < 128.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.0f));
+    const float2 one = make_float2(1.0f, 1.0f);
+    const float2 t = ffma2(x, one, make_float2(kMagic, kMagic));
+    const float2 r = ffma2(t, one, make_float2(-kMagic, -kMagic));
+    const float2 f = ffma2(r, make_float2(-1.0f, -1.0f), x);
+    float2 y = ffma2(make_float2(9.570102207e-03f, 9.570102207e-03f), f, make_float2(5.591785908e-02f, 5.591785908e-02f));
+    y = ffma2(y, f, make_float2(2.402474433e-01f, 2.402474433e-01f));
+    y = ffma2(y, f, make_float2(6.931217909e-01f, 6.931217909e-01f));
+    y = ffma2(y, f, make_float2(9.999992847e-01f, 9.999992847e-01f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
 
 // As mbar_wait, but the clock and the limit (a load from global memory, some 600 cycles) are read only
 // after many polls: a wait of a tile's length must not pay for them.
@@ -349,17 +384,20 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
     using Geo = FaGeo<KIND, D>;
     constexpr bool F8 = Geo::F8;
     constexpr int ST = Geo::STAGES, CH = D / 64;  // 64-column chunks of a tile
-    extern __shared__ uint8_t raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     FaBars* bar = reinterpret_cast<FaBars*>(smem + Geo::BAR_OFF);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int tq = fa_tokens(p.G);
 
+    if (smem_addr(smem) & 1023u) {  // the swizzle's pattern starts there
+        if (tid == 0) record_error(p.err, ERR_FA_WAIT + 15);
+        return;
+    }
     if (tid == 0) {
         for (int h = 0; h < 2; h++) {
             mbar_init(&bar->q_full[h], 1);
             mbar_init(&bar->s_full[h], 1);
-            mbar_init(&bar->p_ready[h], 4);
+            for (int part = 0; part < kFaParts; part++) mbar_init(&bar->p_ready[h][part], 4);
             mbar_init(&bar->o_full[h], 1);
         }
         mbar_init(&bar->q_empty, 1);
@@ -373,7 +411,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         }
         fence_barrier_init();
     }
-    if (warp == 8) {
+    if (warp == kFaSoft) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&bar->tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -385,7 +423,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
     pdl_launch_dependents();
     const int units = __ldcg(&ws.head->units) * p.Hkv;
     // the register split stands inside the roles' branches: behind a join the smaller share would bind them all
-    if (warp < 8) {
+    if (warp < kFaSoft) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Geo::SOFT_REGS));
         // ---- softmax and epilogue: one thread per row ----
         const int h = warp >> 2, row = tid & 127;
@@ -414,27 +452,28 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
 #pragma unroll
                 for (int c = 0; c < 4; c++) tm_ld32(ts + 32 * c, s + 32 * c);
                 tc_wait_ld();
+                // rows that are no query's (and the next sequence's) are not masked: nobody reads them
+                const int lim = valid ? vis - (w.kv0 + i) * kFaTile : kFaTile;
                 if (negate) {
 #pragma unroll
                     for (int c = 0; c < 128; c++) s[c] = -s[c];
                 }
-                // rows that are no query's (and the next sequence's) are not masked: nobody reads them
-                const int lim = valid ? vis - (w.kv0 + i) * kFaTile : kFaTile;
                 if (__any_sync(0xffffffffu, lim < kFaTile)) {
 #pragma unroll
                     for (int c = 0; c < 128; c++) s[c] = c < lim ? s[c] : -INFINITY;
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
+                float mx[4] = {max3(s[0], s[4], s[8]), max3(s[1], s[5], s[9]), max3(s[2], s[6], s[10]), max3(s[3], s[7], s[11])};
 #pragma unroll
-                for (int c = 4; c < 128; c += 4)
+                for (int c = 12; c < 124; c += 8)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], s[c + e]);
-                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+                const float mn = max3(max3(mx[0], mx[1], max3(s[124], s[125], s[126])), max3(mx[2], mx[3], s[127]), m);
                 if (i == 0) {
                     m = mn;
                 } else {
                     const bool grow = (mn - m) * scale > 8.0f;
                     if (__any_sync(0xffffffffu, grow)) {
+                        // these scores came after the product before them: the output is at rest
                         const float f = grow ? exp2_fast((m - mn) * scale) : 1.0f;
                         m = grow ? mn : m;
                         l *= f;
@@ -458,18 +497,22 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                     for (int e = 0; e < 16; e++) {
                         const float2 x = ffma2(make_float2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), make_float2(scale, scale),
                                                make_float2(-base, -base));
-                        const float a = exp2_fast(x.x), b = exp2_fast(x.y);
-                        ls = ffma2(make_float2(a, b), make_float2(1.0f, 1.0f), ls);
-                        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);  // weights in 8 bits' mantissa, as the tensor cores take bf16
+                        // every eighth pair on the FMA units (the same prompts: none 584-600 us, an eighth 569, a quarter
+                        // 610-630); not beside the conversion warps, which need those units (609 us none, 636 an eighth)
+                        const float2 y = !F8 && e % 8 == 0 ? exp2_fma(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        ls = ffma2(y, make_float2(1.0f, 1.0f), ls);
+                        const __nv_bfloat162 v = __floats2bfloat162_rn(y.x, y.y);  // weights in 8 bits' mantissa, as the tensor cores take bf16
                         pk[e] = *reinterpret_cast<const uint32_t*>(&v);
                     }
                     tm_st16(ts + 16 * c, pk);
+                    if ((c + 1) % (4 / kFaParts) == 0) {  // the product takes these positions while the next weights are made
+                        tm_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar->p_ready[h][(c + 1) / (4 / kFaParts) - 1]);
+                    }
                 }
                 l += ls.x + ls.y;
-                tm_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar->p_ready[h]);
             }
             if (!ok) break;
             // ---- the row's output ----
@@ -485,8 +528,8 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             const float inv = w.slot >= 0 ? 1.0f : vis > 0 ? 1.0f / l : 0.0f;
             const int head = w.kvh * p.G + head_of;
             uint16_t* out = p.out + static_cast<int64_t>(w.s.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D;
-            float* part = ws.part + ((static_cast<int64_t>(max(w.slot, 0)) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + row) * (D + 4);
-            bool odd = false;
+            float* line = ws.part + ((static_cast<int64_t>(max(w.slot, 0)) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + row) * (D + 4);
+            bool odd = !(l <= 3.4e38f);
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
                 float o[32];
@@ -519,13 +562,13 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4*>(part + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        *reinterpret_cast<float4*>(line + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
             }
-            if (w.slot >= 0 && valid) *reinterpret_cast<float2*>(part + D) = make_float2(m == -INFINITY ? m : m * scale, l);
+            if (w.slot >= 0 && valid) *reinterpret_cast<float2*>(line + D) = make_float2(m == -INFINITY ? m : m * scale, l);
             // Values that are not finite, behind some row's mask, reach that row as 0 * inf through the products: such rows
             // are done again in plain loops over what they see.
-            unsigned again = __ballot_sync(0xffffffffu, valid && (odd || !(l <= 3.4e38f)));
+            unsigned again = __ballot_sync(0xffffffffu, valid && odd);
             while (again) {
                 const int src = __ffs(again) - 1;
                 again &= again - 1;
@@ -553,7 +596,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Geo::REST_REGS));
-        if (warp == 9) {
+        if (warp == kFaSoft + 1) {
             // ---- loader (of the codes' slots when they are to be converted) ----
             Ring<F8 ? 2 : ST> r;
             uint64_t* const full_bar = F8 ? bar->raw_full : bar->kv_full;
@@ -652,13 +695,13 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 r.next();
             }
             fa_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 3);
-        } else if (F8 && warp >= 12) {
+        } else if (F8 && warp >= kFaSoft + 4) {
             // ---- conversion: codes times their row's power of two, exact in bf16, into the swizzled tile ----
             Ring<2> rr;
             Ring<ST> r;
             bool ok = true;
             constexpr int RC = D / 16;  // 16-code chunks of a row
-            const int ct = tid - 384;
+            const int ct = tid - (kFaSoft + 4) * 32;
             auto convert = [&](int left) {
                 if (!ok || !fa_wait(&bar->raw_full[rr.i], rr.phase, p.err, ERR_FA_WAIT + 9) ||
                     !fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 10)) {
@@ -718,7 +761,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
                 r.next();
             }
-        } else if (warp == 8) {
+        } else if (warp == kFaSoft) {
             // ---- the issuing warp ----
             Ring<ST> r;
             unsigned q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
@@ -746,14 +789,17 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 }
                 __syncwarp();
             };
-            auto outputs = [&](int h, int stage, bool first, bool final) {
+            // the product with a part of the tile's positions
+            auto outputs = [&](int h, int stage, int part, bool first, bool final) {
                 tc_fence_after();
-                const uint32_t v = uniform(v_lo + stage * (Geo::TILE >> 4));
-                const int more = uniform(!first);
+                constexpr int N = kFaTile / 16 / kFaParts;
+                const uint32_t v = uniform(v_lo + stage * (Geo::TILE >> 4) + part * (N * 2048 >> 4));
+                const uint32_t a = uniform(tm + h * 128 + part * N * 8);
+                const int more = uniform(part > 0 || !first);
                 if (elect_one()) {
 #pragma unroll
-                    for (int i = 0; i < kFaTile / 16; i++)
-                        fa_mma_ts(tm + 256 + h * 128, tm + h * 128 + i * 8, v + i * (2048 >> 4), v_hi, id_o, i > 0 ? 1 : more);
+                    for (int i = 0; i < N; i++)
+                        fa_mma_ts(tm + 256 + h * 128, a + i * 8, v + i * (2048 >> 4), v_hi, id_o, i > 0 ? 1 : more);
                     if (final) tc_commit(&bar->o_full[h]);
                 }
                 __syncwarp();
@@ -800,11 +846,13 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                     }
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        if (i >= w.nh[h]) continue;
-                        if (!wait(&bar->p_ready[h], p_ph[h], 6)) break;
+                        if (!ok || i >= w.nh[h]) continue;
+                        for (int part = 0; part < kFaParts; part++) {
+                            if (!wait(&bar->p_ready[h][part], p_ph[h], 6)) break;
+                            outputs(h, v_stage, part, i == 0, part + 1 == kFaParts && i + 1 == w.nh[h]);
+                        }
                         p_ph[h] ^= 1;
-                        outputs(h, v_stage, i == 0, i + 1 == w.nh[h]);
-                        if (i + 1 < w.nh[h]) scores(h, k_stage);
+                        if (ok && i + 1 < w.nh[h]) scores(h, k_stage);
                     }
                     if (!ok) break;
                     release(&bar->kv_empty[v_stage]);
@@ -815,7 +863,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         }
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kFaSoft) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
