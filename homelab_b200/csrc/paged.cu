@@ -104,7 +104,7 @@ float rotated_limit(float mscale) {
 // most this batch, t and max_q.
 struct AttnWs {
     bool few;  // up to kDecRows query rows a kv head: decode_rows_kernel
-    int grid;
+    int grid;  // of the decode kernel
     size_t part_off;  // few
     size_t head_off, unit_off, split_off, fa_part_off;
     int max_units, max_slots;
@@ -116,7 +116,7 @@ AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int
     const int G = heads / kv_heads;
     const int64_t rows = static_cast<int64_t>(max_q) * G;
     w.few = paged && rows <= kDecRows;
-    w.grid = d->sms;
+    w.grid = kDecCtas * d->sms;
     // the counters keep their place, and nothing else comes there, whatever the calls that share a workspace
     const size_t base = align256(static_cast<size_t>(w.grid) * 4);
     w.bytes = base;
@@ -140,9 +140,9 @@ AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int
     return w;
 }
 
-// A tensor map of `rank` dimensions (innermost first; strides in bytes from the second on), 128-byte swizzle.
+// A tensor map of `rank` dimensions (innermost first; strides in bytes from the second on).
 bool encode_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int es, int rank, const int64_t* dims,
-                const int64_t* strides, const int* box, bool swizzle) {
+                const int64_t* strides, const int* box, CUtensorMapSwizzle swizzle) {
     EncodeTiledFn enc = encode_tiled();
     if (!enc) return false;
     cuuint64_t gd[5], gs[4];
@@ -158,7 +158,7 @@ bool encode_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, in
         }
     }
     if (enc(map, type, rank, const_cast<void*>(base), gd, gs, bd, est, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
     // as for the weight tiles: drivers up to 13.1 on tensors under 128 KiB
@@ -175,16 +175,16 @@ bool encode_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, in
 bool encode_rows(CUtensorMap* map, const void* base, int64_t n, int64_t stride, int heads, int D, int box_heads, int box_rows) {
     const int64_t dims[3] = {D, heads, n}, strides[3] = {0, D * 2, stride * 2};
     const int box[3] = {64, box_heads, box_rows};
-    return encode_map(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, true);
+    return encode_map(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// A pool in boxes of one head's rows of a page: 64 swizzled columns of bf16, or whole rows of codes.
-bool encode_pool(CUtensorMap* map, const void* base, const KvView& kv, int D, bool f8) {
+// A pool in boxes of one head's rows of a page: 64 swizzled columns of bf16, or whole rows of codes, swizzled or not.
+bool encode_pool(CUtensorMap* map, const void* base, const KvView& kv, int D, bool f8, bool swizzle) {
     const int page = 1 << kv.page_log2, es = f8 ? 1 : 2;
     const int64_t dims[4] = {D, page, kv.Hkv, kv.num_pages}, strides[4] = {0, D * es, page * D * es, kv.page_stride * es};
     const int box[4] = {f8 ? D : 64, page, 1, 1};
     return encode_map(map, base, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, es, 4, dims, strides, box,
-                      !f8);
+                      !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE : box[0] * es == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int KIND, int D>
@@ -196,36 +196,47 @@ int launch_fa(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream_t s
     fw.part = reinterpret_cast<float*>(ws + w.fa_part_off);
     fw.max_units = w.max_units;
     fw.max_slots = w.max_slots;
-    fw.sms = w.grid;
+    fw.sms = w.grid / kDecCtas;
     CUtensorMap qm, km, vm;
     if (!encode_rows(&qm, p.q, p.T, p.q_stride, p.H, D, p.G, fa_tokens(p.G))) return OOMB_E_LAUNCH;
     if (KIND == KV_ROWS) {
         if (!encode_rows(&km, p.kv.k, p.T, p.kv.k_stride, p.Hkv, D, 1, kFaTile) ||
             !encode_rows(&vm, p.kv.v, p.T, p.kv.v_stride, p.Hkv, D, 1, kFaTile))
             return OOMB_E_LAUNCH;
-    } else if (!encode_pool(&km, p.kv.k, p.kv, D, KIND == KV_E4M3) || !encode_pool(&vm, p.kv.v, p.kv, D, KIND == KV_E4M3)) {
+    } else if (!encode_pool(&km, p.kv.k, p.kv, D, KIND == KV_E4M3, KIND != KV_E4M3) ||
+               !encode_pool(&vm, p.kv.v, p.kv, D, KIND == KV_E4M3, KIND != KV_E4M3)) {
         return OOMB_E_LAUNCH;
     }
     int st = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, fw);
     if (st == OOMB_OK)
-        st = launch(fa_kernel<KIND, D>, dim3(w.grid), dim3(FaGeo<KIND, D>::THREADS), FaGeo<KIND, D>::TOTAL, s, p, fw, qm, km, vm);
-    if (st == OOMB_OK) st = launch(join_kernel<KIND, D>, dim3(2 * w.grid), dim3(256), 0, s, p, fw);
+        st = launch(fa_kernel<KIND, D>, dim3(fw.sms), dim3(FaGeo<KIND, D>::THREADS), FaGeo<KIND, D>::TOTAL, s, p, fw, qm, km, vm);
+    if (st == OOMB_OK) st = launch(join_kernel<KIND, D>, dim3(2 * fw.sms), dim3(256), 0, s, p, fw);
     return st;
+}
+
+template <int KIND, int D, int R>
+int launch_decode(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream_t s) {
+    DecodeWs dw{};
+    dw.counters = reinterpret_cast<unsigned*>(ws);
+    dw.part = reinterpret_cast<float*>(ws + w.part_off);
+    dw.rows = p.max_q * p.G;
+    CUtensorMap km, vm;
+    if (!encode_pool(&km, p.kv.k, p.kv, D, KIND == KV_E4M3, true) || !encode_pool(&vm, p.kv.v, p.kv, D, KIND == KV_E4M3, true))
+        return OOMB_E_LAUNCH;
+    // never more CTAs than there can be blocks
+    const int64_t most = static_cast<int64_t>(p.B) * p.Hkv * (p.kv_max / kDecBlock + 1);
+    const int grid = most < w.grid ? static_cast<int>(most) : w.grid;
+    return launch(decode_rows_kernel<KIND, D, R>, dim3(grid), dim3(kDecThreads), DecodeGeo<KIND, D, R>::TOTAL, s, p, dw, km, vm);
 }
 
 template <int KIND, int D>
 int launch_attn_d(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream_t s) {
     if constexpr (KIND != KV_ROWS) {
-        if (w.few) {
-            DecodeWs dw{};
-            dw.counters = reinterpret_cast<unsigned*>(ws);
-            dw.part = reinterpret_cast<float*>(ws + w.part_off);
-            dw.rows = p.max_q * p.G;
-            // never more CTAs than there can be blocks
-            const int64_t most = static_cast<int64_t>(p.B) * p.Hkv * (p.kv_max / kDecBlock + 1);
-            const int grid = most < w.grid ? static_cast<int>(most) : w.grid;
-            return launch(decode_rows_kernel<KIND, D>, dim3(grid), dim3(kDecThreads), DecodeGeo<KIND, D>::smem, s, p, dw);
-        }
+        const int rows = p.max_q * p.G;
+        if (w.few)
+            return rows <= 4   ? launch_decode<KIND, D, 4>(p, w, ws, s)
+                   : rows <= 8 ? launch_decode<KIND, D, 8>(p, w, ws, s)
+                               : launch_decode<KIND, D, 16>(p, w, ws, s);
     }
     return launch_fa<KIND, D>(p, w, ws, s);
 }

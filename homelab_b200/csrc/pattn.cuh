@@ -34,6 +34,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// 2^e, e in [-126, 127].
+__device__ __forceinline__ float power_of(int e) { return __int_as_float((e + 127) << 23); }
+
 // Lane's D / 32 values of key (or value) row j of sequence b, kv head h, as fp32; a bad
 // block table entry reads as zeros.
 template <int KIND, int D>

@@ -2,55 +2,73 @@
 // steps and short drafts, up to 16 rows (new tokens x query heads of a kv head).
 //
 // Bound: HBM; every key and value byte is read once and used for all rows at once.  The
-// 16 rows are one M = 16 tile of the warp-level matrix instructions (mma.m16n8k16); the
-// 128-row tiles of the 5th-generation tensor cores would leave 7/8 of their rows empty
-// and pass every key through tensor memory for nothing: at the measured HBM rate an SM gets
-// 16 positions (8 KB in bf16) every ~185 ns and needs 32 such instructions for them.
+// positions, not the rows, fill the 128 rows of the tensor cores' tile:
+//   S^T [128 positions x rows] = K Q^T     A: the key tile as it lies in the pages
+//   O^T [head_dim x rows]     += V^T P^T   A: the value tile, read along positions
+// so a tile of 128 positions costs 16 products (bf16; 8 for e4m3) of about 70-90 cycles whatever the number of rows,
+// against the ~2,800 (1,400) cycles that its bytes take at an SM's share of the measured
+// HBM rate, and one thread per position has all rows' scores: its maximum over the
+// positions is needed only when a score passes the running one, which one barrier with
+// an "or" finds out.  A first version on warp-level matrix instructions with the rows as
+// M = 16 spent 437 instructions per 16 positions and head, and took 228 us where this takes 106
+// (32 sequences of 1,001 to 16,098 positions, 32 heads over 8, e4m3 pages).
+//
+// e4m3 codes are multiplied as they are.  A row of queries, scaled by a power of two into
+// [128, 256), is two e4m3 rows q1 = rn(q), q2 = rn(q - q1): a bf16 value's eight bits, exact
+// down to 2^-9 of the scaled row (beyond, off by 2^-10 of it, 2^-18 of the row's largest).  A weight
+// w = 2^(x - m + 11) 2^(e - X), e its value row's exponent and X the largest met, is three e5m2 rows of
+// three bits each: off by at most 2^-9 of itself, or by 2^-28 of 2^-... of the largest: e5m2 reaches
+// from 2^15 down to 2^-16.
 //
 // Work split: the batch's positions are cut into blocks of 128 (per sequence and kv head)
-// and the blocks, laid end to end, evenly over the CTAs (one per SM), whatever the lengths;
+// and the blocks, laid end to end, evenly over the CTAs, whatever the lengths;
 // a (sequence, kv head) spread over several CTAs is joined by the last of them
-// to finish, in order, so a call's bits do not depend on timing.  Within a CTA each warp
-// takes every eighth group of 16 positions with a running maximum and sum of its own.
+// to finish, in order, so a call's bits do not depend on timing.
 //
-// Loads: each warp keeps a ring of groups in flight with cp.async, and every byte is
-// fetched by the one lane that will use it, so the ring needs no barrier and no
-// transpose.  That works because both products may order their inner index freely:
-//  - scores: lane (g = lane / 4, t = lane % 4) is the B fragment's column g (a position) and
-//    four inner indices a step; it takes 16-byte chunks of the rows of positions g and
-//    8 + g, and the query fragment is laid out with the same order of dimensions;
-//  - values: the lane holds positions 2t, 2t + 1, 2t + 8, 2t + 9 (the inner index) and column g,
-//    and a column may stand for any dimension: it takes whole chunks of those four rows
-//    and pairs two positions' values with byte permutes.
-// e4m3 codes become f16 exactly (one conversion a pair); queries are then f16 too, each
-// row scaled by a power of two so that its largest value lies in [2^13, 2^14): their eight
-// bits stay exact down to 2^-28 of it.  Keys' exponents multiply the scores; values'
-// join the weights as w = p 2^(e - X), X the largest exponent met so far, so w <= 1 and fits f16.
+// Warps: 0-3 softmax, one thread per position of a tile and then per output dimension; 4
+// issues the products (scores of the next tile before this tile's outputs); 5 loads by TMA, page by
+// page, through a ring of tiles.  Every wait is bounded.
 #pragma once
 
-#include "pattn.cuh"
+#include "pfill.cuh"
 
 namespace oomb {
 
-constexpr int kDecWarps = 8;
-constexpr int kDecThreads = kDecWarps * 32;
-constexpr int kDecBlock = 128;   // positions of a work block: one group of 16 a warp
+constexpr int kDecSoft = 128;               // softmax threads
+constexpr int kDecThreads = kDecSoft + 64;
+constexpr int kDecBlock = 128;              // positions of a work block: one tile
 constexpr int kDecRows = 16;
-constexpr int kDecRingBytes = 192 * 1024;
+constexpr int kDecCtas = 2;                 // CTAs of an SM
 
-template <int KIND, int D>
+enum : unsigned {
+    ERR_DEC_WAIT = 0xb00,  // a decode pipeline wait ran out (+ the waiting role)
+};
+
+// R: rows a tile is made for (4, 8 or 16; a call's rows at most).
+template <int KIND, int D, int R>
 struct DecodeGeo {
     static constexpr bool F8 = KIND == KV_E4M3;
-    static constexpr int ROW = F8 ? D : 2 * D;                 // bytes of a position's row
-    static constexpr int KC = ROW / 64;                        // 16-byte chunks of a key row a lane takes
-    static constexpr int VB = ROW / 8 < 16 ? ROW / 8 : 16;     // bytes of a value chunk (8 lanes a row)
-    static constexpr int VC = ROW / 8 / VB;                    // value chunks of a row a lane takes
-    static constexpr int STAGE = 16 * ROW * 2;                 // keys and values of a group
-    static constexpr int STAGES = kDecRingBytes / (kDecWarps * STAGE) < 8 ? kDecRingBytes / (kDecWarps * STAGE) : 8;
-    static constexpr int PAD = D + 4;                          // floats of a merge row
-    static constexpr size_t smem = static_cast<size_t>(kDecWarps) * STAGE * STAGES + kDecWarps * STAGES * 32;
-    static_assert(static_cast<size_t>(kDecWarps) * kDecRows * PAD * 4 <= static_cast<size_t>(kDecWarps) * STAGE * STAGES,
-                  "the merge rows reuse the ring");
+    static constexpr int ROW = F8 ? D : 2 * D;                  // bytes of a position's row
+    static constexpr int CHUNK = ROW < 128 ? ROW : 128;         // bytes of a swizzled row
+    static constexpr int CH = ROW / CHUNK;
+    static constexpr int TILE = kDecBlock * ROW;
+    static constexpr int QT = F8 ? 2 : 1, PT = F8 ? 3 : 1;      // terms of a query and of a weight
+    static constexpr int NQ = (R * QT + 15) / 16 * 16, NP = (R * PT + 15) / 16 * 16;
+    static constexpr int Q_BYTES = (CH * NQ * CHUNK + 1023) / 1024 * 1024;
+    static constexpr int P_STEP = (NP * kDecBlock * (F8 ? 1 : 2) + 1023) / 1024 * 1024;
+    static constexpr int EXPS = 8;                              // tiles whose exponents are kept
+    static constexpr int REST = Q_BYTES + 2 * P_STEP + (F8 ? EXPS * 2 * kDecBlock : 0) + 1024;
+    static constexpr int ROOM = 228 * 1024 / kDecCtas - 1024 - REST;
+    static constexpr int STAGES = ROOM / TILE < 8 ? ROOM / TILE : 8;
+    static constexpr int Q_OFF = STAGES * TILE;
+    static constexpr int P_OFF = Q_OFF + Q_BYTES;
+    static constexpr int EXP_OFF = P_OFF + 2 * P_STEP;
+    static constexpr int BAR_OFF = EXP_OFF + (F8 ? EXPS * 2 * kDecBlock : 0);
+    static constexpr int TOTAL = BAR_OFF + 1024;
+    static constexpr int S_COLS = 32;                           // tensor-memory columns of a score buffer
+    static constexpr int PAD = D + 4;                           // floats of a partial row
+    static_assert(NQ <= S_COLS && NP <= 64, "tensor memory");
+    static_assert(kDecCtas * (TOTAL + 1024) <= 228 * 1024, "shared memory");
 };
 
 struct DecodeWs {
@@ -59,48 +77,16 @@ struct DecodeWs {
     int rows;
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, unsigned bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src, unsigned bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, unsigned bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-template <bool F16>
-__device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                                         unsigned b1) {
-    if constexpr (F16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// Two e4m3 codes (low half of w) as two f16.
-__device__ __forceinline__ unsigned f16x2_of(unsigned w) {
-    unsigned r;
-    asm("{\n .reg .b16 l;\n cvt.u16.u32 l, %1;\n cvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(r) : "r"(w));
-    return r;
-}
-__device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const unsigned*>(&h);
-}
-__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const unsigned*>(&h);
-}
+struct DecodeBars {
+    uint64_t kv_full[8], kv_empty[8], s_full[2], p_ready[2], p_free[2], q_ready, e_full[8];
+    uint32_t tmem;
+    int dead;                 // a softmax thread's wait ran out
+    float red[4][kDecRows];
+    int redx[4];
+    unsigned last;
+    int start_b;
+    long long start_prefix, sum[kDecThreads / 32];
+};
 
 // First block of CTA c of n over `total` blocks, and the CTA that owns a block.
 __device__ __forceinline__ int64_t dec_lo(int64_t total, int c, int n) { return total * c / n; }
@@ -111,466 +97,666 @@ __device__ __forceinline__ int dec_owner(int64_t total, int64_t block, int n) {
     return c;
 }
 
-template <int KIND, int D>
-__global__ void __launch_bounds__(kDecThreads, 1) decode_rows_kernel(const __grid_constant__ PattnParams p, const DecodeWs ws) {
-    using Geo = DecodeGeo<KIND, D>;
-    constexpr bool F8 = Geo::F8;
-    constexpr int KC = Geo::KC, VC = Geo::VC, VB = Geo::VB, STAGES = Geo::STAGES, PAD = Geo::PAD;
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int64_t scan_sum[kDecWarps];
-    __shared__ int64_t start_prefix;
-    __shared__ int start_b;
-    __shared__ float mls[kDecWarps][kDecRows][2];
-    __shared__ bool last;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint8_t* ring = smem + warp * Geo::STAGE * STAGES;
-    const uint32_t ring_s = smem_addr(ring);
-    uint8_t* exps = smem + static_cast<size_t>(kDecWarps) * Geo::STAGE * STAGES + warp * STAGES * 32;
-    const uint32_t exps_s = smem_addr(exps);
+// Descriptors' high words: 128-byte rows in the 128-byte swizzle (8-row groups 1024 bytes apart), or 64-byte rows in the
+// 64-byte one (512).
+__host__ __device__ constexpr uint32_t dec_desc_hi(int chunk) {
+    return chunk == 128 ? (64u | (1u << 14) | (2u << 29)) : (32u | (1u << 14) | (4u << 29));
+}
+// Byte of 16-byte chunk c of row r in such a layout.
+__device__ __forceinline__ int dec_swizzle(int chunk, int r, int c) {
+    return chunk == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
 
+template <bool F8>
+__device__ __forceinline__ void dec_mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t a_hi, uint32_t b_hi, uint32_t idesc, int acc) {
+    if constexpr (F8)
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %6, 0;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %4};\n"
+            " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n}" ::"r"(d),
+            "r"(a_lo), "r"(b_lo), "r"(a_hi), "r"(b_hi), "r"(idesc), "r"(acc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %6, 0;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %4};\n"
+            " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n}" ::"r"(d),
+            "r"(a_lo), "r"(b_lo), "r"(a_hi), "r"(b_hi), "r"(idesc), "r"(acc)
+            : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void tm_ld(uint32_t t, float* v) {
+    static_assert(N % 16 == 0, "sixteen columns at a time");
+#pragma unroll
+    for (int c = 0; c < N; c += 16) tm_ld16(t + c, v + c);
+    tc_wait_ld();
+}
+
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+// (lo, hi) to two e5m2 codes (or e4m3), and what they leave of the two values.
+__device__ __forceinline__ unsigned split_e5m2(float& lo, float& hi) {
+    unsigned short c;
+    unsigned h;
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
+    asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"(c));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    lo -= f.x;
+    hi -= f.y;
+    return c;
+}
+__device__ __forceinline__ unsigned split_e4m3(float& lo, float& hi) {
+    unsigned short c;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
+    const float2 f = e4m3x2_to_float2(c);
+    lo -= f.x;
+    hi -= f.y;
+    return c;
+}
+
+// One CTA's place in the batch's blocks.
+struct DecodeSpan {
+    int64_t W, lo, hi, b_first;  // all blocks; this CTA's [lo, hi); the first block of sequence b
+    int b, S;                    // CTAs with work
+};
+// A run of blocks of one (sequence, kv head).
+struct DecodeSeg {
+    Seq sq;
+    int b, kvh, tok0, tok1, tiles;
+    int64_t pair_first, pair_end, lo;
+};
+
+// Walks a CTA's segments in order; every role does so on its own.
+struct DecodeWalk {
+    DecodeSpan sp;
+    Seq sq;
+    int nb;
+    __device__ void open(const PattnParams& p) {
+        sq = read_seq(p.q_start, p.kv_len, sp.b, p.T, p.kv_max, nullptr);
+        nb = sq.n == 0 || sq.n > p.max_q ? 0 : max(1, (sq.len + kDecBlock - 1) / kDecBlock);
+    }
+    __device__ bool next(const PattnParams& p, DecodeSeg& g) {
+        if (sp.lo >= sp.hi) return false;
+        while (sp.lo >= sp.b_first + static_cast<int64_t>(nb) * p.Hkv) {
+            sp.b_first += static_cast<int64_t>(nb) * p.Hkv;
+            sp.b++;
+            open(p);
+        }
+        g.sq = sq;
+        g.b = sp.b;
+        g.kvh = static_cast<int>((sp.lo - sp.b_first) / nb);
+        g.pair_first = sp.b_first + static_cast<int64_t>(g.kvh) * nb;
+        g.pair_end = g.pair_first + nb;
+        g.lo = sp.lo;
+        const int64_t end = g.pair_end < sp.hi ? g.pair_end : sp.hi;
+        g.tok0 = static_cast<int>(sp.lo - g.pair_first) * kDecBlock;
+        g.tok1 = min(sq.len, static_cast<int>(end - g.pair_first) * kDecBlock);
+        g.tiles = g.tok1 > g.tok0 ? (g.tok1 - g.tok0 + kDecBlock - 1) / kDecBlock : 0;
+        sp.lo = end;
+        return true;
+    }
+};
+
+template <int KIND, int D, int R>
+__global__ void __launch_bounds__(kDecThreads, kDecCtas)
+    decode_rows_kernel(const __grid_constant__ PattnParams p, const __grid_constant__ DecodeWs ws, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap) {
+    using Geo = DecodeGeo<KIND, D, R>;
+    constexpr bool F8 = Geo::F8;
+    constexpr int ST = Geo::STAGES, CHUNK = Geo::CHUNK, CH = Geo::CH, PAD = Geo::PAD;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    DecodeBars* bar = reinterpret_cast<DecodeBars*>(smem + Geo::BAR_OFF);
+    static_assert(sizeof(DecodeBars) <= 1024, "barriers");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_addr(smem) & 1023u) {  // the swizzle's pattern starts there
+        if (tid == 0) record_error(p.err, ERR_DEC_WAIT + 15);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < ST; i++) {
+            mbar_init(&bar->kv_full[i], 1);
+            mbar_init(&bar->kv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bar->s_full[i], 1);
+            mbar_init(&bar->p_ready[i], 4);
+            mbar_init(&bar->p_free[i], 1);
+        }
+        for (int i = 0; i < Geo::EXPS; i++) mbar_init(&bar->e_full[i], 1);
+        mbar_init(&bar->q_ready, 4);
+        bar->dead = 0;
+        fence_barrier_init();
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 128;" ::"r"(smem_addr(&bar->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar->tmem, o_col = tmem + 2 * Geo::S_COLS;
     pdl_wait();
     pdl_launch_dependents();
 
     // ---- this CTA's blocks of the batch ----
-    auto blocks_of = [&](int b) {
-        if (b >= p.B) return 0;
-        const Seq s = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, p.err);
-        if (s.n > p.max_q) record_error(p.err, ERR_KV_SEQ);
-        if (s.n == 0 || s.n > p.max_q) return 0;
-        return max(1, (s.len + kDecBlock - 1) / kDecBlock);  // a sequence without positions still gets its zeros
-    };
-    int64_t total = 0;
-    int mine = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kDecThreads) {
-        mine = blocks_of(b0 + tid);
-        int v = mine;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) scan_sum[warp] = v;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kDecWarps; w++) total += scan_sum[w];
-        __syncthreads();
-    }
-    const int64_t W = total * p.Hkv;
-    const int S = static_cast<int>(W < static_cast<int64_t>(gridDim.x) ? W : static_cast<int64_t>(gridDim.x));
-    const int cta = blockIdx.x;
-    if (cta >= S) return;
-    int64_t lo = dec_lo(W, cta, S);
-    const int64_t hi = dec_lo(W, cta + 1, S);
-    int64_t prefix = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kDecThreads) {
-        if (p.B > kDecThreads) mine = blocks_of(b0 + tid);
-        int inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
-        }
-        if (lane == 31) scan_sum[warp] = inc;
-        __syncthreads();
-        int64_t before = prefix;
-        for (int w = 0; w < warp; w++) before += scan_sum[w];
-        const int64_t end = before + inc;
-        if (mine > 0 && (end - mine) * p.Hkv <= lo && lo < end * p.Hkv) {
-            start_b = b0 + tid;
-            start_prefix = end - mine;
-        }
-#pragma unroll
-        for (int w = 0; w < kDecWarps; w++) prefix += scan_sum[w];
-        __syncthreads();
-    }
-    int b = start_b;
-    int64_t b_first = start_prefix * p.Hkv;  // first block of sequence b
-
-    // ---- segments: the CTA's blocks of one (sequence, kv head) at a time ----
-    while (lo < hi) {
-        Seq sq = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, nullptr);
-        const int nb = sq.n == 0 || sq.n > p.max_q ? 0 : max(1, (sq.len + kDecBlock - 1) / kDecBlock);
-        if (lo >= b_first + static_cast<int64_t>(nb) * p.Hkv) {
-            b_first += static_cast<int64_t>(nb) * p.Hkv;
-            b++;
-            continue;
-        }
-        const int kvh = static_cast<int>((lo - b_first) / nb);
-        const int64_t pair_first = b_first + static_cast<int64_t>(kvh) * nb, pair_end = pair_first + nb;
-        const int64_t seg_end = pair_end < hi ? pair_end : hi;
-        const int tok0 = static_cast<int>(lo - pair_first) * kDecBlock;
-        const int tok1 = min(sq.len, static_cast<int>(seg_end - pair_first) * kDecBlock);
-        const int rows = sq.n * p.G;
-        const int groups = tok1 > tok0 ? (tok1 - tok0 + 15) / 16 : 0;
-        const int count = groups > warp ? (groups - warp + kDecWarps - 1) / kDecWarps : 0;  // this warp's groups
-
-        // the queries' fragments: rows g and 8 + g
-        unsigned qa[D / 16][4];
-        float row_scale[2];
-        int vis[2];
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const int r = g + 8 * half;
-            const bool ok = r < rows;
-            const int token = ok ? r / p.G : 0;
-            vis[half] = ok ? max(0, min(sq.len, sq.len - sq.n + token + 1)) : 0;
-            const uint16_t* qp = p.q + static_cast<int64_t>(sq.q0 + token) * p.q_stride + static_cast<int64_t>(kvh * p.G + (ok ? r - token * p.G : 0)) * D;
-            row_scale[half] = p.scale_log2;
-            if constexpr (!F8) {
-#pragma unroll
-                for (int c = 0; c < D / 32; c++) {
-                    const uint4 w = ok ? __ldcg(reinterpret_cast<const uint4*>(qp + c * 32 + t * 8)) : make_uint4(0u, 0u, 0u, 0u);
-                    qa[2 * c][half] = w.x;
-                    qa[2 * c][half + 2] = w.y;
-                    qa[2 * c + 1][half] = w.z;
-                    qa[2 * c + 1][half + 2] = w.w;
-                }
-            } else {
-                unsigned u[D / 64][8];
-                float amax = 0.0f;
-#pragma unroll
-                for (int c = 0; c < D / 64; c++) {
-                    const uint4* src = reinterpret_cast<const uint4*>(qp + c * 64 + t * 16);
-                    const uint4 w0 = ok ? __ldcg(src) : make_uint4(0u, 0u, 0u, 0u), w1 = ok ? __ldcg(src + 1) : make_uint4(0u, 0u, 0u, 0u);
-                    u[c][0] = w0.x, u[c][1] = w0.y, u[c][2] = w0.z, u[c][3] = w0.w;
-                    u[c][4] = w1.x, u[c][5] = w1.y, u[c][6] = w1.z, u[c][7] = w1.w;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(u[c][i] << 16)), fabsf(__uint_as_float(u[c][i] & 0xffff0000u))));
-                }
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const int ex = max(-100, min(100, static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 13));
-                const float up = __int_as_float((127 - ex) << 23);
-                row_scale[half] = p.scale_log2 * __int_as_float((127 + ex) << 23);
-#pragma unroll
-                for (int c = 0; c < D / 64; c++)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        // element pair i of the chunk: step c * 4 + i / 2, its first or second inner half
-                        qa[c * 4 + i / 2][half + 2 * (i & 1)] =
-                            pack_f16(__uint_as_float(u[c][i] << 16) * up, __uint_as_float(u[c][i] & 0xffff0000u) * up);
-                    }
-            }
-        }
-        const int vis_least = max(0, min(sq.len, sq.len - sq.n + 1));
-
-        // ---- the ring of groups ----
-        const int32_t* table = p.kv.table + static_cast<int64_t>(b) * p.kv.table_stride;
-        const int page_mask = (1 << p.kv.page_log2) - 1;
-        int ids = 0, ids_base = -32;  // lane l holds the page of the warp's group ids_base + l
-        auto issue = [&](int i) {
-            if (i < count) {
-                if (i >= ids_base + 32) {
-                    ids_base += 32;
-                    const int gi = ids_base + lane;
-                    ids = gi < count ? __ldcg(table + ((tok0 + (warp + gi * kDecWarps) * 16) >> p.kv.page_log2)) : 0;
-                    if (ids < 0 || ids >= p.kv.num_pages) {
-                        record_error(p.err, ERR_KV_TABLE);
-                        ids = -1;
-                    }
-                }
-                const int page = __shfl_sync(0xffffffffu, ids, i - ids_base);
-                const int tok = tok0 + (warp + i * kDecWarps) * 16;
-                const int have = page < 0 ? 0 : tok1 - tok;  // positions of the group present
-                const int64_t row0 = max(page, 0) * p.kv.page_stride + ((static_cast<int64_t>(kvh) << p.kv.page_log2) + (tok & page_mask)) * D;
-                const int es = F8 ? 1 : 2;
-                const uint8_t* kb = p.kv.k + row0 * es;
-                const uint8_t* vb = p.kv.v + row0 * es;
-                const uint32_t dst = ring_s + (i % STAGES) * Geo::STAGE;
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int c = 0; c < KC; c++) {
-                        const int pos = 8 * j + g;
-                        cp16(dst + (j * KC + c) * 512 + lane * 16, kb + pos * Geo::ROW + c * 64 + t * 16, pos < have ? 16u : 0u);
-                    }
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int c = 0; c < VC; c++) {
-                        const int pos = 2 * t + (j & 1) + 8 * (j >> 1);
-                        const uint32_t d = dst + 16 * Geo::ROW + (j * VC + c) * 32 * VB + lane * VB;
-                        const uint8_t* s = vb + pos * Geo::ROW + c * 8 * VB + g * VB;
-                        if constexpr (VB == 16) cp16(d, s, pos < have ? 16u : 0u);
-                        else cp8(d, s, pos < have ? 8u : 0u);
-                    }
-                if constexpr (F8) {
-                    if (lane < 8) {
-                        const uint8_t* e = lane < 4 ? p.kv.ke : p.kv.ve;
-                        const int64_t at = max(page, 0) * p.kv.exp_stride + (static_cast<int64_t>(kvh) << p.kv.page_log2) + (tok & page_mask);
-                        cp4(exps_s + (i % STAGES) * 32 + lane * 4, e + at + (lane & 3) * 4, page < 0 ? 0u : 4u);
-                    }
-                }
-            }
-            cp_commit();
+    DecodeWalk walk{};
+    {
+        auto blocks_of = [&](int b) {
+            if (b >= p.B) return 0;
+            const Seq s = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, p.err);
+            if (s.n > p.max_q) record_error(p.err, ERR_KV_SEQ);
+            if (s.n == 0 || s.n > p.max_q) return 0;
+            return max(1, (s.len + kDecBlock - 1) / kDecBlock);  // a sequence without positions still gets its zeros
         };
-
-        float acc[D / 8][4];
+        int64_t total = 0;
+        int mine = 0;
+        for (int b0 = 0; b0 < p.B; b0 += kDecThreads) {
+            mine = blocks_of(b0 + tid);
+            const int v = __reduce_add_sync(0xffffffffu, mine);
+            if (lane == 0) bar->sum[warp] = v;
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < D / 8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-        int X = -1000;  // e4m3: the exponent that the accumulators are counted in
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; i++) issue(i);
-        for (int i = 0; i < count; i++) {
-            issue(i + STAGES - 1);
-            cp_wait<STAGES - 1>();
-            const uint8_t* st = ring + (i % STAGES) * Geo::STAGE;
-            const int tok = tok0 + (warp + i * kDecWarps) * 16;
-            float s[2][4] = {};
-            unsigned ke[2], ve[2];
-            if constexpr (F8) {
-                __syncwarp();  // the exponents were fetched by other lanes
-                const uint8_t* ep = exps + (i % STAGES) * 32;
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    ke[j] = *reinterpret_cast<const uint16_t*>(ep + 8 * j + 2 * t);
-                    ve[j] = *reinterpret_cast<const uint16_t*>(ep + 16 + 8 * j + 2 * t);
-                    // a slot behind the last position may hold any byte: it must not set X
-                    const int left = tok1 - (tok + 8 * j + 2 * t);
-                    if (left < 2) ve[j] = left < 1 ? 0u : ve[j] & 0xffu;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int c = 0; c < KC; c++) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(st + (j * KC + c) * 512 + lane * 16);
-                    if constexpr (!F8) {
-                        mma16816<false>(s[j], qa[2 * c][0], qa[2 * c][1], qa[2 * c][2], qa[2 * c][3], w.x, w.y);
-                        mma16816<false>(s[j], qa[2 * c + 1][0], qa[2 * c + 1][1], qa[2 * c + 1][2], qa[2 * c + 1][3], w.z, w.w);
-                    } else {
-                        const unsigned u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            mma16816<true>(s[j], qa[4 * c + q][0], qa[4 * c + q][1], qa[4 * c + q][2], qa[4 * c + q][3],
-                                           f16x2_of(u[q]), f16x2_of(u[q] >> 16));
-                    }
-                }
-            // scores in units of log2; rows g (half 0) and 8 + g (half 1), positions 8 j + 2 t + (0, 1)
-            float mx[2] = {-INFINITY, -INFINITY};
-            const bool masked = tok + 16 > vis_least;
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int half = e >> 1;
-                    float f = row_scale[half];
-                    if constexpr (F8) f *= exp_byte((ke[j] >> (8 * (e & 1))) & 0xffu);
-                    float x = s[j][e] * f;
-                    if (masked && tok + 8 * j + 2 * t + (e & 1) >= vis[half]) x = -INFINITY;
-                    s[j][e] = x;
-                    mx[half] = fmaxf(mx[half], x);
-                }
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
-                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
-            }
-            int xm = X;
-            if constexpr (F8) {
-                int e4 = max(max(static_cast<int>(ve[0] & 0xffu), static_cast<int>(ve[0] >> 8)),
-                             max(static_cast<int>(ve[1] & 0xffu), static_cast<int>(ve[1] >> 8)));
-                e4 = max(e4, __shfl_xor_sync(0xffffffffu, e4, 1));
-                e4 = max(e4, __shfl_xor_sync(0xffffffffu, e4, 2));
-                xm = max(X, e4);
-            }
-            if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || xm > X)) {
-                float grow = 1.0f;
-                if constexpr (F8) {
-                    grow = X < -500 ? 1.0f : exp2_fast(static_cast<float>(X - xm));
-                    X = xm;
-                }
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const float mn = fmaxf(m[half], mx[half]);
-                    const float c = m[half] == -INFINITY ? 0.0f : exp2_fast(m[half] - mn);
-                    m[half] = mn;
-                    l[half] *= c;
-                    const float cg = c * grow;
-#pragma unroll
-                    for (int n = 0; n < D / 8; n++) {
-                        acc[n][2 * half] *= cg;
-                        acc[n][2 * half + 1] *= cg;
-                    }
-                }
-            }
-            const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-            unsigned pa[4];
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    float e0 = exp2_fast(s[j][2 * half] - base[half]), e1 = exp2_fast(s[j][2 * half + 1] - base[half]);
-                    l[half] += e0 + e1;
-                    if constexpr (F8) {
-                        // weight times 2^(e - X) <= 1; f16 keeps it to 2^-11, or to 2^-25 absolute
-                        e0 *= exp2_fast(static_cast<float>(static_cast<int>(ve[j] & 0xffu) - X));
-                        e1 *= exp2_fast(static_cast<float>(static_cast<int>(ve[j] >> 8) - X));
-                        pa[2 * j + half] = pack_f16(e0, e1);
-                    } else {
-                        pa[2 * j + half] = pack_bf16(e0, e1);  // weights in 8 bits' mantissa, as the tensor cores take bf16
-                    }
-                }
-            const uint8_t* sv = st + 16 * Geo::ROW;
-#pragma unroll
-            for (int c = 0; c < VC; c++) {
-                unsigned w[4][VB / 4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if constexpr (VB == 16) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(sv + (j * VC + c) * 512 + lane * 16);
-                        w[j][0] = x.x, w[j][1] = x.y, w[j][2] = x.z, w[j][3] = x.w;
-                    } else {
-                        const uint2 x = *reinterpret_cast<const uint2*>(sv + (j * VC + c) * 256 + lane * 8);
-                        w[j][0] = x.x, w[j][1] = x.y;
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < VB / 4; q++) {
-                    if constexpr (F8) {
-                        // bytes of positions (2t, 2t + 1) and (2t + 8, 2t + 9) interleaved: four dimensions
-                        const unsigned a = __byte_perm(w[0][q], w[1][q], 0x5140), a2 = __byte_perm(w[0][q], w[1][q], 0x7362);
-                        const unsigned d = __byte_perm(w[2][q], w[3][q], 0x5140), d2 = __byte_perm(w[2][q], w[3][q], 0x7362);
-                        const int n = c * VB + 4 * q;
-                        mma16816<true>(acc[n], pa[0], pa[1], pa[2], pa[3], f16x2_of(a), f16x2_of(d));
-                        mma16816<true>(acc[n + 1], pa[0], pa[1], pa[2], pa[3], f16x2_of(a >> 16), f16x2_of(d >> 16));
-                        mma16816<true>(acc[n + 2], pa[0], pa[1], pa[2], pa[3], f16x2_of(a2), f16x2_of(d2));
-                        mma16816<true>(acc[n + 3], pa[0], pa[1], pa[2], pa[3], f16x2_of(a2 >> 16), f16x2_of(d2 >> 16));
-                    } else {
-                        const int n = c * (VB / 2) + 2 * q;
-                        mma16816<false>(acc[n], pa[0], pa[1], pa[2], pa[3], __byte_perm(w[0][q], w[1][q], 0x5410),
-                                        __byte_perm(w[2][q], w[3][q], 0x5410));
-                        mma16816<false>(acc[n + 1], pa[0], pa[1], pa[2], pa[3], __byte_perm(w[0][q], w[1][q], 0x7632),
-                                        __byte_perm(w[2][q], w[3][q], 0x7632));
-                    }
-                }
-            }
-            if constexpr (F8) __syncwarp();  // exponents read before a later group overwrites them
+            for (int w = 0; w < kDecThreads / 32; w++) total += bar->sum[w];
+            __syncthreads();
         }
-        cp_wait<0>();
-
-        // ---- the CTA's partial: its warps' joined in warp order ----
+        DecodeSpan& sp = walk.sp;
+        sp.W = total * p.Hkv;
+        sp.S = static_cast<int>(sp.W < static_cast<int64_t>(gridDim.x) ? sp.W : static_cast<int64_t>(gridDim.x));
+        const bool idle = static_cast<int>(blockIdx.x) >= sp.S;
+        if (!idle) {
+            sp.lo = dec_lo(sp.W, blockIdx.x, sp.S);
+            sp.hi = dec_lo(sp.W, blockIdx.x + 1, sp.S);
+            int64_t prefix = 0;
+            for (int b0 = 0; b0 < p.B; b0 += kDecThreads) {
+                if (p.B > kDecThreads) mine = blocks_of(b0 + tid);
+                int inc = mine;
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-            if (t == 0) {
-                mls[warp][g + 8 * half][0] = m[half];
-                mls[warp][g + 8 * half][1] = l[half];
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += u;
+                }
+                if (lane == 31) bar->sum[warp] = inc;
+                __syncthreads();
+                int64_t before = prefix;
+                for (int w = 0; w < warp; w++) before += bar->sum[w];
+                const int64_t end = before + inc;
+                if (mine > 0 && (end - mine) * p.Hkv <= sp.lo && sp.lo < end * p.Hkv) {
+                    bar->start_b = b0 + tid;
+                    bar->start_prefix = end - mine;
+                }
+#pragma unroll
+                for (int w = 0; w < kDecThreads / 32; w++) prefix += bar->sum[w];
+                __syncthreads();
+            }
+            sp.b = bar->start_b;
+            sp.b_first = bar->start_prefix * p.Hkv;
+            walk.open(p);
+        }
+    }
+    DecodeSeg g;
+    if (warp == 5) {
+        // ---- loader ----
+        Ring<ST> r;
+        bool ok = true;
+        unsigned tile_no = 0;
+        const int per_tile = kDecBlock >> p.kv.page_log2, page = 1 << p.kv.page_log2;
+        while (ok && walk.next(p, g)) {
+            if (g.tiles == 0) continue;
+            const int32_t* table = p.kv.table + static_cast<int64_t>(g.b) * p.kv.table_stride;
+            auto lookup = [&](int i) {
+                const int at = (g.tok0 >> p.kv.page_log2) + i * per_tile + lane;
+                return i < g.tiles && lane < per_tile && at < p.kv.max_pages ? __ldcg(table + at) : 0;
+            };
+            auto load = [&](bool value, int i, int id) {
+                if (!ok || !fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_DEC_WAIT + 1)) {
+                    ok = false;
+                    return;
+                }
+                uint8_t* dst = smem + r.i * Geo::TILE;
+                uint64_t* full = &bar->kv_full[r.i];
+                const int have = min(per_tile, (g.tok1 - g.tok0 - i * kDecBlock + page - 1) >> p.kv.page_log2);
+                const bool mine = lane < have, good = mine && id >= 0 && id < p.kv.num_pages;
+                if (mine && !good && !value) record_error(p.err, ERR_KV_TABLE);
+                if (lane == 0) mbar_arrive_expect_tx(full, have * page * Geo::ROW);
+                const unsigned e = tile_no & (Geo::EXPS - 1);
+                uint8_t* exps = smem + Geo::EXP_OFF + e * 2 * kDecBlock;
+                if (F8 && !value) {  // both kinds' exponents come with the keys
+                    if (mine && !good)
+                        for (int o = 0; o < page; o += 16) {
+                            *reinterpret_cast<uint4*>(exps + lane * page + o) = make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint4*>(exps + kDecBlock + lane * page + o) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    const int n = __popc(__ballot_sync(0xffffffffu, good));
+                    if (lane == 0) mbar_arrive_expect_tx(&bar->e_full[e], n * page * 2);
+                }
+                __syncwarp();
+                if (mine) {
+                    const int at = good ? id : p.kv.num_pages;  // outside the map: zeros
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+                        tma_load_4d(dst + c * kDecBlock * CHUNK + lane * page * CHUNK, value ? &vmap : &kmap, c * 64, 0, g.kvh, at, full);
+                    if (F8 && !value && good) {
+                        const int64_t from = id * p.kv.exp_stride + (static_cast<int64_t>(g.kvh) << p.kv.page_log2);
+                        bulk_g2s_plain(exps + lane * page, p.kv.ke + from, page, &bar->e_full[e]);
+                        bulk_g2s_plain(exps + kDecBlock + lane * page, p.kv.ve + from, page, &bar->e_full[e]);
+                    }
+                }
+                if (!value) tile_no++;
+                r.next();
+            };
+            int cur = lookup(0), nxt = lookup(1);
+            load(false, 0, cur);
+            for (int i = 0; i < g.tiles && ok; i++) {
+                const int was = cur;
+                if (i + 1 < g.tiles) {
+                    cur = nxt;
+                    nxt = lookup(i + 2);
+                    load(false, i + 1, cur);
+                }
+                load(true, i, was);
             }
         }
-        __syncthreads();  // every warp is done with the ring
-        float* merge = reinterpret_cast<float*>(smem);  // [warp][16][PAD]
-        {
-            const float un = F8 ? (X < -500 ? 0.0f : exp_byte(static_cast<unsigned>(X))) : 1.0f;
-            // column n of the tile c (VB bytes a lane: NV dimensions) is dimension c * 8 NV + n NV + i
-            constexpr int NV = F8 ? VB : VB / 2;
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                if (g + 8 * half >= rows) continue;
-                float* row = merge + (warp * kDecRows + g + 8 * half) * PAD;
-#pragma unroll
-                for (int c = 0; c < VC; c++)
-#pragma unroll
-                    for (int col = 0; col < 2; col++)
-#pragma unroll
-                        for (int i = 0; i < NV; i += 4)
-                            *reinterpret_cast<float4*>(row + c * 8 * NV + (2 * t + col) * NV + i) =
-                                make_float4(acc[c * NV + i][2 * half + col] * un, acc[c * NV + i + 1][2 * half + col] * un,
-                                            acc[c * NV + i + 2][2 * half + col] * un, acc[c * NV + i + 3][2 * half + col] * un);
-            }
+        // the ring is drained before the CTA ends: nothing may still arrive in its shared memory
+        for (int i = 0; i < ST; i++) {
+            fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_DEC_WAIT + 2);
+            r.next();
         }
-        __syncthreads();
-        const int first = dec_owner(W, pair_first, S), final_cta = dec_owner(W, pair_end - 1, S);
-        const int parts = final_cta - first + 1;
-        const int quads = rows * (D / 4);
-        float* my_part = ws.part + static_cast<int64_t>(2 * cta + (lo == pair_first ? 1 : 0)) * ws.rows * PAD;
-        bool odd = false;
-        auto finish = [&](int r, int d, float4 o, float lsum) {
-            const int token = r / p.G;
-            const bool sees = sq.len - sq.n + token >= 0 && sq.len > 0;
-            const float inv = sees ? 1.0f / lsum : 0.0f;
-            o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-            if (!sees) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            odd |= !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) <= 3.4e38f);
-            uint2 v;
-            v.x = pack_bf16(o.x, o.y);
-            v.y = pack_bf16(o.z, o.w);
-            *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(sq.q0 + token) * p.out_stride +
-                                      static_cast<int64_t>(kvh * p.G + r - token * p.G) * D + d) = v;
+    } else if (warp == 4) {
+        // ---- the issuing warp ----
+        Ring<ST> r;
+        unsigned t = 0, q_ph = 0;  // tiles so far
+        bool ok = true;
+        auto wait = [&](uint64_t* b, unsigned ph, int role) {
+            if (ok && !fa_wait(b, ph, p.err, ERR_DEC_WAIT + role)) ok = false;
+            return ok;
         };
-        for (int o = tid; o < quads; o += kDecThreads) {
-            const int r = o / (D / 4), d = (o % (D / 4)) * 4;
-            float M = -INFINITY;
+        constexpr uint32_t fmt = F8 ? 0u : (1u << 7) | (1u << 10);
+        constexpr uint32_t id_s = (1u << 4) | fmt | (static_cast<uint32_t>(Geo::NQ >> 3) << 17) | (8u << 24);
+        // A along positions (bit 15); e4m3 values with e5m2 weights
+        constexpr uint32_t id_o = (1u << 4) | fmt | (F8 ? 1u << 10 : 0u) | (1u << 15) | (static_cast<uint32_t>(Geo::NP >> 3) << 17) | (8u << 24);
+        constexpr uint32_t hi = dec_desc_hi(CHUNK), p_hi = dec_desc_hi(128);
+        // the next 64-column chunk of a bf16 value tile; with one chunk of 64 dimensions the rows above repeat it, unread
+        constexpr uint32_t lead = D == 128 && !F8 ? (kDecBlock * CHUNK) >> 4 : 0;
+        const uint32_t base = uniform(smem_addr(smem) >> 4), tm = uniform(tmem), oc = uniform(o_col);
+        auto scores = [&](int stage, unsigned tile) {
+            tc_fence_after();
+            const uint32_t a = uniform((base + stage * (Geo::TILE >> 4)) | (1u << 16)), q = (base + (Geo::Q_OFF >> 4)) | (1u << 16);
+            const uint32_t d = uniform(tm + (tile & 1) * Geo::S_COLS);
+            uint64_t* const done = &bar->s_full[tile & 1];
+            if (elect_one()) {
 #pragma unroll
-            for (int w = 0; w < kDecWarps; w++) M = fmaxf(M, mls[w][r][0]);
-            const float base = M == -INFINITY ? 0.0f : M;
-            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float ls = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kDecWarps; w++) {
-                const float f = exp2_fast(mls[w][r][0] - base);
-                const float4 v = *reinterpret_cast<const float4*>(merge + (w * kDecRows + r) * PAD + d);
-                a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
-                ls = fmaf(f, mls[w][r][1], ls);
+                for (int i = 0; i < Geo::ROW / 32; i++) {
+                    const uint32_t ao = ((i * 32 / CHUNK) * kDecBlock * CHUNK + i * 32 % CHUNK) >> 4;
+                    const uint32_t bo = ((i * 32 / CHUNK) * Geo::NQ * CHUNK + i * 32 % CHUNK) >> 4;
+                    dec_mma<F8>(d, a + ao, q + bo, hi, hi, id_s, i > 0);
+                }
+                tc_commit(done);
             }
-            if (parts == 1) {
-                finish(r, d, a, ls);
-            } else {
-                *reinterpret_cast<float4*>(my_part + r * PAD + d) = a;
-                if (d == 0) *reinterpret_cast<float2*>(my_part + r * PAD + D) = make_float2(M, ls);
+            __syncwarp();
+        };
+        auto outputs = [&](int stage, unsigned tile, bool first) {
+            tc_fence_after();
+            const uint32_t a = uniform((base + stage * (Geo::TILE >> 4)) | (lead << 16));
+            const uint32_t w = uniform((base + (Geo::P_OFF >> 4) + (tile & 1) * (Geo::P_STEP >> 4)) | (1u << 16));
+            const int more = uniform(!first);
+            uint64_t* const done = &bar->p_free[tile & 1];
+            if (elect_one()) {
+                constexpr int K = F8 ? 32 : 16;  // positions of a product
+#pragma unroll
+                for (int i = 0; i < kDecBlock / K; i++) {
+                    const uint32_t bo = F8 ? (i * 32) >> 4 : ((i / 4) * Geo::NP * 128 + (i % 4) * 32) >> 4;
+                    dec_mma<F8>(oc, a + ((i * K * CHUNK) >> 4), w + bo, hi, p_hi, id_o, i > 0 ? 1 : more);
+                }
+                tc_commit(done);
+            }
+            __syncwarp();
+        };
+        auto release = [&](int stage) {
+            if (elect_one()) tc_commit(&bar->kv_empty[stage]);
+            __syncwarp();
+        };
+        while (ok && walk.next(p, g)) {
+            if (g.tiles == 0) continue;
+            if (!wait(&bar->q_ready, q_ph, 3)) break;
+            q_ph ^= 1;
+            if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+            scores(r.i, t);
+            release(r.i);
+            r.next();
+            for (int i = 0; i < g.tiles && ok; i++, t++) {
+                if (i + 1 < g.tiles) {
+                    if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                    scores(r.i, t + 1);
+                    release(r.i);
+                    r.next();
+                }
+                if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                const int left = g.tok1 - g.tok0 - i * kDecBlock;
+                if (left < kDecBlock) {
+                    // rows behind the last position: anything may be there, and 0 * NaN is NaN
+                    uint8_t* v = smem + r.i * Geo::TILE;
+                    for (int o = left * (CHUNK / 16) + lane; o < kDecBlock * (CHUNK / 16); o += 32)
+#pragma unroll
+                        for (int c = 0; c < CH; c++) *reinterpret_cast<uint4*>(v + c * kDecBlock * CHUNK + o * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_async_smem();
+                    __syncwarp();
+                }
+                if (!wait(&bar->p_ready[t & 1], (t >> 1) & 1, 5)) break;
+                outputs(r.i, t, i == 0);
+                release(r.i);
+                r.next();
             }
         }
-        if (parts > 1) {
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                unsigned* counter = ws.counters + first;  // a CTA starts at most one (sequence, kv head) that it does not end
-                last = atomicAdd(counter, 1u) == static_cast<unsigned>(parts - 1);
-                if (last) *counter = 0u;
+    } else {
+        // ---- softmax: a position's thread, then an output dimension's ----
+        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+        constexpr float kSlack = F8 ? 4.0f : 8.0f, kLift = F8 ? 11.0f : 0.0f;
+        unsigned t = 0;
+        bool stop = false;
+        // the four warps meet; whether any says so
+        auto meet = [&](bool any) {
+            unsigned x;
+            asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 q, %1, 0;\n bar.red.or.pred p, 1, 128, q;\n selp.u32 %0, 1, 0, p;\n}"
+                         : "=r"(x)
+                         : "r"(static_cast<unsigned>(any))
+                         : "memory");
+            return x != 0;
+        };
+        // a wait that ran out is told to all at the next meeting: none leaves the loop alone
+        auto wait = [&](uint64_t* b, unsigned ph, int role) {
+            if (!fa_wait(b, ph, p.err, ERR_DEC_WAIT + role)) *static_cast<volatile int*>(&bar->dead) = 1;
+        };
+        auto dead = [&]() { return *static_cast<volatile int*>(&bar->dead) != 0; };
+        while (!stop && walk.next(p, g)) {
+            const Seq sq = g.sq;
+            const int rows = sq.n * p.G;
+            float m[R], l[R], scale[R];
+            int vis[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                m[r] = -INFINITY;
+                l[r] = 0.0f;
+                scale[r] = p.scale_log2;
+                vis[r] = r < rows ? max(0, min(sq.len, sq.len - sq.n + r / p.G + 1)) : 0;
             }
-            __syncthreads();
-            if (last) {
+            int X = 0;  // e4m3: the exponent byte that the outputs are counted in
+            if (g.tiles > 0) {
+                // ---- the queries as the scores' second operand; the last segment's scores are all made ----
+                if constexpr (!F8) {
+                    for (int o = tid; o < R * (D / 8); o += kDecSoft) {
+                        const int r = o / (D / 8), c = o % (D / 8);
+                        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                        if (r < rows)
+                            x = __ldcg(reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(sq.q0 + r / p.G) * p.q_stride +
+                                                                      static_cast<int64_t>(g.kvh * p.G + r % p.G) * D + c * 8));
+                        *reinterpret_cast<uint4*>(smem + Geo::Q_OFF + (c / 8) * Geo::NQ * 128 + dec_swizzle(128, r, c % 8)) = x;
+                    }
+                } else {
+                    // a row by 8 threads, D / 8 values each
+                    constexpr int V = D / 8;
+                    for (int r0 = 0; r0 < R; r0 += kDecSoft / 8) {
+                        const int r = r0 + tid / 8, c = tid % 8;
+                        float f[V];
+                        float big = 0.0f;
+                        const bool in = r < rows;
+                        const uint16_t* q = p.q + static_cast<int64_t>(sq.q0 + (in ? r / p.G : 0)) * p.q_stride +
+                                            static_cast<int64_t>(g.kvh * p.G + (in ? r % p.G : 0)) * D + c * V;
+#pragma unroll
+                        for (int i = 0; i < V; i += 8) {
+                            const uint4 x = in ? __ldcg(reinterpret_cast<const uint4*>(q + i)) : make_uint4(0u, 0u, 0u, 0u);
+                            const unsigned u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                f[i + 2 * k] = __uint_as_float(u[k] << 16);
+                                f[i + 2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+                                big = fmaxf(big, fmaxf(fabsf(f[i + 2 * k]), fabsf(f[i + 2 * k + 1])));
+                            }
+                        }
+#pragma unroll
+                        for (int o = 1; o < 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                        const int ex = max(-100, min(100, static_cast<int>(__float_as_uint(big) >> 23) - 127 - 7));
+                        const float up = power_of(-ex);
+                        if (r < R) {
+                            if (c == 0) bar->red[0][r] = power_of(ex);
+                            // a value that is not finite has no code: its row's scores become NaN
+                            const bool bad = !(big <= 3.4e38f);
+                            uint8_t* q1 = smem + Geo::Q_OFF;
+#pragma unroll
+                            for (int i = 0; i < V; i += 4) {
+                                float a = f[i] * up, b = f[i + 1] * up, d = f[i + 2] * up, e = f[i + 3] * up;
+                                if (a != a || b != b || d != d || e != e || bad) a = __uint_as_float(0x7fffffffu);
+                                const unsigned h0 = split_e4m3(a, b), h1 = split_e4m3(d, e);
+                                const unsigned l0 = split_e4m3(a, b), l1 = split_e4m3(d, e);
+                                const int at = c * V + i;  // byte of the row
+                                *reinterpret_cast<unsigned*>(q1 + dec_swizzle(CHUNK, r, at / 16) + at % 16) = h0 | (h1 << 16);
+                                *reinterpret_cast<unsigned*>(q1 + dec_swizzle(CHUNK, R + r, at / 16) + at % 16) = l0 | (l1 << 16);
+                            }
+                        }
+                    }
+                }
+                fence_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->q_ready);
+                if constexpr (F8) {
+                    meet(false);
+#pragma unroll
+                    for (int r = 0; r < R; r++) scale[r] *= bar->red[0][r];
+                }
+            }
+            for (int i = 0; i < g.tiles; i++, t++) {
+                wait(&bar->s_full[t & 1], (t >> 1) & 1, 6);
+                tc_fence_after();
+                float s[Geo::NQ];
+                tm_ld<Geo::NQ>(tmem + lanes + (t & 1) * Geo::S_COLS, s);
+                const int tok = g.tok0 + i * kDecBlock + tid;
+                int ve = 0;
+                float kf = 1.0f;
+                if constexpr (F8) {
+                    const unsigned e = t & (Geo::EXPS - 1);
+                    wait(&bar->e_full[e], (t / Geo::EXPS) & 1, 7);
+                    const uint8_t* ep = smem + Geo::EXP_OFF + e * 2 * kDecBlock;
+                    kf = exp_byte(ep[tid]);
+                    ve = tok < g.tok1 ? ep[kDecBlock + tid] : 0;
+                }
+                bool over = ve > X;
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    float x = F8 ? (s[r] + s[R + r]) * (scale[r] * kf) : s[r] * scale[r];
+                    if (tok >= vis[r]) x = -INFINITY;
+                    s[r] = x;
+                    over |= x > m[r] + kSlack || (m[r] == -INFINITY && x != -INFINITY);
+                }
+                const bool update = meet(over);
+                if (dead()) {
+                    stop = true;
+                    break;
+                }
+                if (update) {
+                    // the tile's maxima over its positions, and the outputs so far brought to them
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        float x = s[r];
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                        if (lane == 0) bar->red[warp][r] = x;
+                    }
+                    if constexpr (F8) {
+                        const int x = __reduce_max_sync(0xffffffffu, ve);
+                        if (lane == 0) bar->redx[warp] = x;
+                    }
+                    if (i > 0) wait(&bar->p_free[(t - 1) & 1], ((t - 1) >> 1) & 1, 8);  // the outputs are at rest
+                    meet(false);
+                    if (dead()) {
+                        stop = true;
+                        break;
+                    }
+                    float f[R];
+                    int xn = X;
+                    if constexpr (F8) xn = max(max(X, max(bar->redx[0], bar->redx[1])), max(bar->redx[2], bar->redx[3]));
+                    const float fx = F8 && i > 0 ? exp2_fast(static_cast<float>(X - xn)) : 1.0f;
+                    X = xn;
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        const float mn = fmaxf(m[r], fmaxf(fmaxf(bar->red[0][r], bar->red[1][r]), fmaxf(bar->red[2][r], bar->red[3][r])));
+                        const float c = m[r] == -INFINITY ? 0.0f : exp2_fast(m[r] - mn);
+                        l[r] *= c;
+                        f[r] = c * fx;
+                        m[r] = mn;
+                    }
+                    if (i > 0) {
+                        tc_fence_after();
+                        float o[Geo::NP];
+                        tm_ld<Geo::NP>(o_col + lanes, o);
+#pragma unroll
+                        for (int c = 0; c < R * Geo::PT; c++) o[c] *= f[c % R];
+#pragma unroll
+                        for (int c = 0; c < Geo::NP; c += 16) tm_st16(o_col + lanes + c, reinterpret_cast<const uint32_t*>(o + c));
+                        tm_wait_st();
+                    }
+                }
+                // ---- weights, as the outputs' second operand ----
+                wait(&bar->p_free[t & 1], ((t >> 1) & 1) ^ 1, 9);
+                uint8_t* pw = smem + Geo::P_OFF + (t & 1) * Geo::P_STEP;
+                const float vf = F8 ? exp2_fast(static_cast<float>(ve - X)) : 1.0f;
+#pragma unroll
+                for (int r = 0; r < R; r += 2) {
+                    float a = exp2_fast(s[r] - (m[r] == -INFINITY ? 0.0f : m[r]) + kLift);
+                    float b = exp2_fast(s[r + 1] - (m[r + 1] == -INFINITY ? 0.0f : m[r + 1]) + kLift);
+                    l[r] += a;
+                    l[r + 1] += b;
+                    if constexpr (F8) {
+                        a *= vf;
+                        b *= vf;
+#pragma unroll
+                        for (int k = 0; k < 3; k++) {
+                            const unsigned c = split_e5m2(a, b);
+                            const int n0 = k * R + r;
+                            pw[dec_swizzle(128, n0, tid / 16) + tid % 16] = static_cast<uint8_t>(c);
+                            pw[dec_swizzle(128, n0 + 1, tid / 16) + tid % 16] = static_cast<uint8_t>(c >> 8);
+                        }
+                    } else {
+                        const unsigned c = pack_bf16(a, b);  // weights in 8 bits' mantissa, as the tensor cores take bf16
+                        uint8_t* at = pw + (tid / 64) * Geo::NP * 128;
+                        const int k = tid % 64;
+                        *reinterpret_cast<uint16_t*>(at + dec_swizzle(128, r, k / 8) + (k % 8) * 2) = static_cast<uint16_t>(c);
+                        *reinterpret_cast<uint16_t*>(at + dec_swizzle(128, r + 1, k / 8) + (k % 8) * 2) = static_cast<uint16_t>(c >> 16);
+                    }
+                }
+                fence_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->p_ready[t & 1]);
+            }
+            if (stop) break;
+            // ---- the segment's outputs: thread d has dimension d of every row ----
+            float o[Geo::NP];
+            if (g.tiles > 0) {
+                wait(&bar->p_free[(t - 1) & 1], ((t - 1) >> 1) & 1, 8);
+                tc_fence_after();
+                tm_ld<Geo::NP>(o_col + lanes, o);
+            } else {
+#pragma unroll
+                for (int c = 0; c < Geo::NP; c++) o[c] = 0.0f;
+            }
+            meet(false);  // the last maxima are read
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float x = l[r];
+#pragma unroll
+                for (int k = 16; k > 0; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
+                if (lane == 0) bar->red[warp][r] = x;
+            }
+            meet(false);
+            if (dead()) break;
+            const float unit = F8 ? exp_byte(static_cast<unsigned>(X)) : 1.0f;
+            const int first = dec_owner(walk.sp.W, g.pair_first, walk.sp.S), final_cta = dec_owner(walk.sp.W, g.pair_end - 1, walk.sp.S);
+            const int parts = final_cta - first + 1;
+            float* my_part = ws.part + static_cast<int64_t>(2 * blockIdx.x + (g.lo == g.pair_first ? 1 : 0)) * ws.rows * PAD;
+            bool odd = false;
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                if (r >= rows) continue;
+                const float ls = bar->red[0][r] + bar->red[1][r] + bar->red[2][r] + bar->red[3][r];
+                float x = o[r];
+                if constexpr (F8) x = (o[r] + o[R + r] + o[2 * R + r]) * unit;
+                if (parts == 1) {
+                    x = vis[r] > 0 ? x / ls : 0.0f;
+                    odd |= tid < D && !(fabsf(x) <= 3.4e38f);
+                    const __nv_bfloat16 v = __float2bfloat16_rn(x);
+                    if (tid < D)
+                        *reinterpret_cast<__nv_bfloat16*>(p.out + static_cast<int64_t>(sq.q0 + r / p.G) * p.out_stride +
+                                                          static_cast<int64_t>(g.kvh * p.G + r % p.G) * D + tid) = v;
+                } else {
+                    if (tid < D) my_part[r * PAD + tid] = x;
+                    if (tid == 0) *reinterpret_cast<float2*>(my_part + r * PAD + D) = make_float2(m[r], ls);
+                }
+            }
+            if (parts > 1) {
                 __threadfence();
-                auto part_of = [&](int i) {
-                    // the first CTA's blocks of the pair are its last segment unless the pair starts it
-                    return ws.part + static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * ws.rows * PAD;
-                };
-                for (int o = tid; o < quads; o += kDecThreads) {
-                    const int r = o / (D / 4), d = (o % (D / 4)) * 4;
-                    float M = -INFINITY;
-#pragma unroll 4
-                    for (int i = 0; i < parts; i++) M = fmaxf(M, __ldcg(part_of(i) + r * PAD + D));
-                    const float base = M == -INFINITY ? 0.0f : M;
-                    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float ls = 0.0f;
-#pragma unroll 4
-                    for (int i = 0; i < parts; i++) {
-                        const float* pr = part_of(i) + r * PAD;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(pr + D));
-                        const float f = exp2_fast(ml.x - base);
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(pr + d));
-                        a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
-                        ls = fmaf(f, ml.y, ls);
+                meet(false);
+                if (tid == 0) {
+                    unsigned* counter = ws.counters + first;  // a CTA starts at most one (sequence, kv head) that it does not end
+                    const bool last = atomicAdd(counter, 1u) == static_cast<unsigned>(parts - 1);
+                    if (last) *counter = 0u;
+                    bar->last = last;
+                }
+                meet(false);
+                if (bar->last) {
+                    __threadfence();
+                    auto part_of = [&](int i) {
+                        // the first CTA's blocks of the pair are its last segment unless the pair starts it
+                        return ws.part + static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * ws.rows * PAD;
+                    };
+                    for (int q = tid; q < rows * (D / 4); q += kDecSoft) {
+                        const int r = q / (D / 4), d = (q % (D / 4)) * 4, token = r / p.G;
+                        float M = -INFINITY;
+#pragma unroll 8
+                        for (int i = 0; i < parts; i++) M = fmaxf(M, __ldcg(part_of(i) + r * PAD + D));
+                        const float b0 = M == -INFINITY ? 0.0f : M;
+                        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        float ls = 0.0f;
+#pragma unroll 8
+                        for (int i = 0; i < parts; i++) {
+                            const float* pr = part_of(i) + r * PAD;
+                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pr + D));
+                            const float4 v = __ldcg(reinterpret_cast<const float4*>(pr + d));
+                            const float f = exp2_fast(ml.x - b0);
+                            a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
+                            ls = fmaf(f, ml.y, ls);
+                        }
+                        const bool sees = sq.len > 0 && sq.len - sq.n + token >= 0;
+                        const float inv = 1.0f / ls;
+                        a = sees ? make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        odd |= !(fabsf(a.x) + fabsf(a.y) + fabsf(a.z) + fabsf(a.w) <= 3.4e38f);
+                        *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(sq.q0 + token) * p.out_stride +
+                                                  static_cast<int64_t>(g.kvh * p.G + r - token * p.G) * D + d) =
+                            make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
                     }
-                    finish(r, d, a, ls);
                 }
             }
-        }
-        // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the
-        // matrix product: then every row is done again in plain loops over what it sees.
-        if (__syncthreads_or(odd) && sq.n > 1) {
-            for (int r = warp; r < rows; r += kDecWarps) {
-                const int token = r / p.G, head = kvh * p.G + r - token * p.G;
-                const int see = max(0, min(sq.len, sq.len - sq.n + token + 1));
-                float mm, ll, a[D / 32];
-                attend_row<KIND, D>(p, b, sq.q0, sq.q0 + token, head, 0, see, lane, mm, ll, a);
-                uint16_t* o = p.out + static_cast<int64_t>(sq.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D + lane * (D / 32);
-                const float inv = see > 0 ? 1.0f / ll : 0.0f;
+            // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the products (and e4m3
+            // and e5m2 terms have no infinity): then every row is done again in plain loops over what it sees.
+            if (meet(odd)) {
+                for (int r = warp; r < rows; r += 4) {
+                    const int token = r / p.G, head = g.kvh * p.G + r - token * p.G;
+                    const int see = max(0, min(sq.len, sq.len - sq.n + token + 1));
+                    float mm, ll, a[D / 32];
+                    attend_row<KIND, D>(p, g.b, sq.q0, sq.q0 + token, head, 0, see, lane, mm, ll, a);
+                    uint16_t* to = p.out + static_cast<int64_t>(sq.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D + lane * (D / 32);
+                    const float inv = see > 0 ? 1.0f / ll : 0.0f;
 #pragma unroll
-                for (int i = 0; i < D / 32; i += 2) *reinterpret_cast<unsigned*>(o + i) = pack_bf16(a[i] * inv, a[i + 1] * inv);
+                    for (int i = 0; i < D / 32; i += 2) *reinterpret_cast<unsigned*>(to + i) = pack_bf16(a[i] * inv, a[i + 1] * inv);
+                }
             }
+            tc_fence_before();
         }
-        lo = seg_end;
+    }
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem) : "memory");
     }
 }
 
