@@ -223,8 +223,9 @@ int launch_decode(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream
     CUtensorMap km, vm;
     if (!encode_pool(&km, p.kv.k, p.kv, D, KIND == KV_E4M3, true) || !encode_pool(&vm, p.kv.v, p.kv, D, KIND == KV_E4M3, true))
         return OOMB_E_LAUNCH;
-    // never more CTAs than there can be blocks
+    // never more CTAs than there can be blocks, which the kernel counts in 32 bits
     const int64_t most = static_cast<int64_t>(p.B) * p.Hkv * (p.kv_max / kDecBlock + 1);
+    if (most > (1 << 30)) return OOMB_E_SHAPE;
     const int grid = most < w.grid ? static_cast<int>(most) : w.grid;
     return launch(decode_rows_kernel<KIND, D, R>, dim3(grid), dim3(kDecThreads), DecodeGeo<KIND, D, R>::TOTAL, s, p, dw, km, vm);
 }

@@ -10,7 +10,7 @@
 // HBM rate, and one thread per position has all rows' scores: its maximum over the
 // positions is needed only when a score passes the running one, which one barrier with
 // an "or" finds out.  A first version on warp-level matrix instructions with the rows as
-// M = 16 spent 437 instructions per 16 positions and head, and took 228 us where this takes 106
+// M = 16 spent 437 instructions per 16 positions and head, and took 228 us where this takes 101
 // (32 sequences of 1,001 to 16,098 positions, 32 heads over 8, e4m3 pages).
 //
 // e4m3 codes are multiplied as they are.  A row of queries, scaled by a power of two into
@@ -39,6 +39,9 @@ constexpr int kDecThreads = kDecSoft + 64;
 constexpr int kDecBlock = 128;              // positions of a work block: one tile
 constexpr int kDecRows = 16;
 constexpr int kDecCtas = 2;                 // CTAs of an SM
+// Parts of a (sequence, kv head), on average, at most: one sequence of 4096 positions over 8 kv heads takes 14.2 us with 8,
+// 11.8 with 16 (one trip to L2 joins them), 12.4 with 32 or more.
+constexpr int kDecParts = 16;
 
 enum : unsigned {
     ERR_DEC_WAIT = 0xb00,  // a decode pipeline wait ran out (+ the waiting role)
@@ -84,18 +87,20 @@ struct DecodeBars {
     float red[4][kDecRows];
     int redx[4];
     unsigned last;
-    int start_b;
-    long long start_prefix, sum[kDecThreads / 32];
+    int4 start;               // the CTA's first sequence, its first block, its blocks
+    Seq start_seq;
+    int2 sum[kDecThreads / 32];
 };
 
-// First block of CTA c of n over `total` blocks, and the CTA that owns a block.
-__device__ __forceinline__ int64_t dec_lo(int64_t total, int c, int n) { return total * c / n; }
-__device__ __forceinline__ int dec_owner(int64_t total, int64_t block, int n) {
-    int c = static_cast<int>(block * n / total);
-    while (c + 1 < n && dec_lo(total, c + 1, n) <= block) c++;
-    while (c > 0 && dec_lo(total, c, n) > block) c--;
-    return c;
-}
+// Blocks dealt to CTAs in order: the first `more` of them get `each` + 1, the others `each`.
+struct DecodeDeal {
+    int each, more;
+    __device__ int lo(int c) const { return c * each + min(c, more); }
+    __device__ int owner(int block) const {
+        const int cut = more * (each + 1);
+        return block < cut ? block / (each + 1) : more + (block - cut) / each;
+    }
+};
 
 // Descriptors' high words: 128-byte rows in the 128-byte swizzle (8-row groups 1024 bytes apart), or 64-byte rows in the
 // 64-byte one (512).
@@ -155,45 +160,39 @@ __device__ __forceinline__ unsigned split_e4m3(float& lo, float& hi) {
     return c;
 }
 
-// One CTA's place in the batch's blocks.
-struct DecodeSpan {
-    int64_t W, lo, hi, b_first;  // all blocks; this CTA's [lo, hi); the first block of sequence b
-    int b, S;                    // CTAs with work
-};
 // A run of blocks of one (sequence, kv head).
 struct DecodeSeg {
     Seq sq;
     int b, kvh, tok0, tok1, tiles;
-    int64_t pair_first, pair_end, lo;
+    int pair_first, pair_end, lo;
 };
 
 // Walks a CTA's segments in order; every role does so on its own.
 struct DecodeWalk {
-    DecodeSpan sp;
+    DecodeDeal deal;
+    int lo, hi;      // this CTA's blocks yet to come
+    int b, b_first;  // a sequence and its first block
     Seq sq;
-    int nb;
-    __device__ void open(const PattnParams& p) {
-        sq = read_seq(p.q_start, p.kv_len, sp.b, p.T, p.kv_max, nullptr);
-        nb = sq.n == 0 || sq.n > p.max_q ? 0 : max(1, (sq.len + kDecBlock - 1) / kDecBlock);
-    }
+    int nb;          // its blocks of one kv head
     __device__ bool next(const PattnParams& p, DecodeSeg& g) {
-        if (sp.lo >= sp.hi) return false;
-        while (sp.lo >= sp.b_first + static_cast<int64_t>(nb) * p.Hkv) {
-            sp.b_first += static_cast<int64_t>(nb) * p.Hkv;
-            sp.b++;
-            open(p);
+        if (lo >= hi) return false;
+        while (lo >= b_first + nb * p.Hkv) {
+            b_first += nb * p.Hkv;
+            b++;
+            sq = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, nullptr);
+            nb = sq.n == 0 || sq.n > p.max_q ? 0 : max(1, (sq.len + kDecBlock - 1) / kDecBlock);
         }
         g.sq = sq;
-        g.b = sp.b;
-        g.kvh = static_cast<int>((sp.lo - sp.b_first) / nb);
-        g.pair_first = sp.b_first + static_cast<int64_t>(g.kvh) * nb;
+        g.b = b;
+        g.kvh = (lo - b_first) / nb;
+        g.pair_first = b_first + g.kvh * nb;
         g.pair_end = g.pair_first + nb;
-        g.lo = sp.lo;
-        const int64_t end = g.pair_end < sp.hi ? g.pair_end : sp.hi;
-        g.tok0 = static_cast<int>(sp.lo - g.pair_first) * kDecBlock;
-        g.tok1 = min(sq.len, static_cast<int>(end - g.pair_first) * kDecBlock);
+        g.lo = lo;
+        const int end = min(g.pair_end, hi);
+        g.tok0 = (lo - g.pair_first) * kDecBlock;
+        g.tok1 = min(sq.len, (end - g.pair_first) * kDecBlock);
         g.tiles = g.tok1 > g.tok0 ? (g.tok1 - g.tok0 + kDecBlock - 1) / kDecBlock : 0;
-        sp.lo = end;
+        lo = end;
         return true;
     }
 };
@@ -242,32 +241,35 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
     // ---- this CTA's blocks of the batch ----
     DecodeWalk walk{};
     {
+        Seq seen{};
         auto blocks_of = [&](int b) {
             if (b >= p.B) return 0;
-            const Seq s = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, p.err);
-            if (s.n > p.max_q) record_error(p.err, ERR_KV_SEQ);
-            if (s.n == 0 || s.n > p.max_q) return 0;
-            return max(1, (s.len + kDecBlock - 1) / kDecBlock);  // a sequence without positions still gets its zeros
+            seen = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, p.err);
+            if (seen.n > p.max_q) record_error(p.err, ERR_KV_SEQ);
+            if (seen.n == 0 || seen.n > p.max_q) return 0;
+            return max(1, (seen.len + kDecBlock - 1) / kDecBlock);  // a sequence without positions still gets its zeros
         };
-        int64_t total = 0;
-        int mine = 0;
+        int total = 0, pairs = 0, mine = 0;
         for (int b0 = 0; b0 < p.B; b0 += kDecThreads) {
             mine = blocks_of(b0 + tid);
-            const int v = __reduce_add_sync(0xffffffffu, mine);
-            if (lane == 0) bar->sum[warp] = v;
+            const int v = __reduce_add_sync(0xffffffffu, mine), n = __popc(__ballot_sync(0xffffffffu, mine > 0));
+            if (lane == 0) bar->sum[warp] = make_int2(v, n);
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < kDecThreads / 32; w++) total += bar->sum[w];
+            for (int w = 0; w < kDecThreads / 32; w++) {
+                total += bar->sum[w].x;
+                pairs += bar->sum[w].y;
+            }
             __syncthreads();
         }
-        DecodeSpan& sp = walk.sp;
-        sp.W = total * p.Hkv;
-        sp.S = static_cast<int>(sp.W < static_cast<int64_t>(gridDim.x) ? sp.W : static_cast<int64_t>(gridDim.x));
-        const bool idle = static_cast<int>(blockIdx.x) >= sp.S;
-        if (!idle) {
-            sp.lo = dec_lo(sp.W, blockIdx.x, sp.S);
-            sp.hi = dec_lo(sp.W, blockIdx.x + 1, sp.S);
-            int64_t prefix = 0;
+        const int W = total * p.Hkv;  // fits: checked by the caller for the longest sequences
+        const int S = min(min(W, static_cast<int>(gridDim.x)), max(1, pairs * p.Hkv * kDecParts));
+        if (static_cast<int>(blockIdx.x) < S) {
+            walk.deal.each = W / S;
+            walk.deal.more = W - walk.deal.each * S;
+            walk.lo = walk.deal.lo(blockIdx.x);
+            walk.hi = walk.deal.lo(blockIdx.x + 1);
+            int prefix = 0;
             for (int b0 = 0; b0 < p.B; b0 += kDecThreads) {
                 if (p.B > kDecThreads) mine = blocks_of(b0 + tid);
                 int inc = mine;
@@ -276,22 +278,22 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     const int u = __shfl_up_sync(0xffffffffu, inc, o);
                     if (lane >= o) inc += u;
                 }
-                if (lane == 31) bar->sum[warp] = inc;
+                if (lane == 31) bar->sum[warp].x = inc;
                 __syncthreads();
-                int64_t before = prefix;
-                for (int w = 0; w < warp; w++) before += bar->sum[w];
-                const int64_t end = before + inc;
-                if (mine > 0 && (end - mine) * p.Hkv <= sp.lo && sp.lo < end * p.Hkv) {
-                    bar->start_b = b0 + tid;
-                    bar->start_prefix = end - mine;
+                int end = prefix + inc;
+                for (int w = 0; w < warp; w++) end += bar->sum[w].x;
+                if (mine > 0 && (end - mine) * p.Hkv <= walk.lo && walk.lo < end * p.Hkv) {
+                    bar->start = make_int4(b0 + tid, (end - mine) * p.Hkv, mine, 0);
+                    bar->start_seq = seen;
                 }
 #pragma unroll
-                for (int w = 0; w < kDecThreads / 32; w++) prefix += bar->sum[w];
+                for (int w = 0; w < kDecThreads / 32; w++) prefix += bar->sum[w].x;
                 __syncthreads();
             }
-            sp.b = bar->start_b;
-            sp.b_first = bar->start_prefix * p.Hkv;
-            walk.open(p);
+            walk.b = bar->start.x;
+            walk.b_first = bar->start.y;
+            walk.nb = bar->start.z;
+            walk.sq = bar->start_seq;
         }
     }
     DecodeSeg g;
@@ -671,7 +673,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
             meet(false);
             if (dead()) break;
             const float unit = F8 ? exp_byte(static_cast<unsigned>(X)) : 1.0f;
-            const int first = dec_owner(walk.sp.W, g.pair_first, walk.sp.S), final_cta = dec_owner(walk.sp.W, g.pair_end - 1, walk.sp.S);
+            const int first = walk.deal.owner(g.pair_first), final_cta = walk.deal.owner(g.pair_end - 1);
             const int parts = final_cta - first + 1;
             float* my_part = ws.part + static_cast<int64_t>(2 * blockIdx.x + (g.lo == g.pair_first ? 1 : 0)) * ws.rows * PAD;
             bool odd = false;
@@ -711,20 +713,33 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     };
                     for (int q = tid; q < rows * (D / 4); q += kDecSoft) {
                         const int r = q / (D / 4), d = (q % (D / 4)) * 4, token = r / p.G;
-                        float M = -INFINITY;
-#pragma unroll 8
-                        for (int i = 0; i < parts; i++) M = fmaxf(M, __ldcg(part_of(i) + r * PAD + D));
-                        const float b0 = M == -INFINITY ? 0.0f : M;
+                        // sixteen parts' loads under way at once: a pass over them is a few trips to L2
+                        float M = -INFINITY, ls = 0.0f;
                         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        float ls = 0.0f;
-#pragma unroll 8
-                        for (int i = 0; i < parts; i++) {
-                            const float* pr = part_of(i) + r * PAD;
-                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pr + D));
-                            const float4 v = __ldcg(reinterpret_cast<const float4*>(pr + d));
-                            const float f = exp2_fast(ml.x - b0);
-                            a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
-                            ls = fmaf(f, ml.y, ls);
+                        for (int i0 = 0; i0 < parts; i0 += 16) {
+                            float2 ml[16];
+                            float4 v[16];
+                            float mn = M;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const float* pr = part_of(i0 + i) + r * PAD;
+                                const bool in = i0 + i < parts;
+                                ml[i] = in ? __ldcg(reinterpret_cast<const float2*>(pr + D)) : make_float2(-INFINITY, 0.0f);
+                                v[i] = in ? __ldcg(reinterpret_cast<const float4*>(pr + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; i++) mn = fmaxf(mn, ml[i].x);
+                            const float b0 = mn == -INFINITY ? 0.0f : mn;
+                            const float c = exp2_fast(M - b0);
+                            M = mn;
+                            ls *= c;
+                            a.x *= c, a.y *= c, a.z *= c, a.w *= c;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const float f = exp2_fast(ml[i].x - b0);
+                                a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
+                                ls = fmaf(f, ml[i].y, ls);
+                            }
                         }
                         const bool sees = sq.len > 0 && sq.len - sq.n + token >= 0;
                         const float inv = 1.0f / ls;

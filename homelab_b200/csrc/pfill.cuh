@@ -49,20 +49,23 @@ constexpr int kFaSoft = 8;         // softmax warps
 constexpr int kFaMinPart = 4;      // key tiles of a part at least
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBuckets = 1024;
+constexpr int kPlanSeqs = 1024;    // sequences whose numbers are kept in shared memory
 
 enum : unsigned {
     ERR_FA_WAIT = 0xa00,  // a prefill pipeline wait ran out (+ the waiting role)
 };
 
-struct FaUnit {
+struct __align__(16) FaUnit {
+    Seq s;
     int b, i0;     // sequence, first new token (of the sequence)
     int kv0, kv1;  // key tiles
     int slot;      // partial outputs' slot, or -1: the unit is its tile's only one
-    int pad[3];
 };
-struct FaSplit {
-    int b, i0, slot, parts;
+struct __align__(16) FaSplit {
+    Seq s;
+    int i0, b, slot, parts, pad;
 };
+static_assert(sizeof(FaUnit) == 32 && sizeof(FaSplit) == 32, "read as two int4");
 struct FaHead {
     int units, splits, slots, pad;
 };
@@ -85,21 +88,23 @@ __device__ __forceinline__ int fa_key_tiles(const Seq& s, int i1) {
     return (vis + kFaTile - 1) / kFaTile;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PattnParams p, const FaWs ws) {
+// One CTA.  The sequences' numbers are read once (up to kPlanSeqs of them) and a warp takes a sequence, a lane a
+// tile.  Up to as many units as SMs are listed as they come; more are sorted by a counting sort on their length.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PattnParams p, const __grid_constant__ FaWs ws) {
     __shared__ int hist[kPlanBuckets];
+    __shared__ Seq seqs[kPlanSeqs];
     __shared__ unsigned long long total_s;
-    __shared__ int slots_s, splits_s, warp_sum[32];
+    __shared__ int slots_s, splits_s, units_s, warp_sum[32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = kPlanThreads / 32;
-    pdl_wait();
-    pdl_launch_dependents();
     if (tid == 0) {
         total_s = 0;
-        slots_s = splits_s = 0;
+        slots_s = splits_s = units_s = 0;
     }
     for (int i = tid; i < kPlanBuckets; i += kPlanThreads) hist[i] = 0;
-    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
     const int tq = fa_tokens(p.G);
-    auto seq_of = [&](int b, unsigned* err) {
+    auto read = [&](int b, unsigned* err) {
         Seq s = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, err);
         if (s.n > p.max_q) {
             record_error(err, ERR_KV_SEQ);
@@ -107,9 +112,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         }
         return s;
     };
+    for (int b = tid; b < p.B; b += kPlanThreads) {
+        const Seq s = read(b, p.err);
+        if (b < kPlanSeqs) seqs[b] = s;
+    }
+    __syncthreads();
+    auto seq_of = [&](int b) { return b < kPlanSeqs ? seqs[b] : read(b, nullptr); };
     unsigned long long work = 0;
     for (int b = warp; b < p.B; b += warps) {
-        const Seq s = seq_of(b, p.err);
+        const Seq s = seq_of(b);
         const int nt = fa_tiles_of(s, tq);
         for (int i = lane; i < nt; i += 32) work += max(1, fa_key_tiles(s, (i + 1) * 2 * tq));
     }
@@ -120,72 +131,79 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     // a part is at least an SM's even share of the step, so there are at most two parts an SM
     const unsigned long long share = (total_s * p.Hkv + ws.sms - 1) / ws.sms;
     const int chunk = share > (1u << 30) ? (1 << 30) : max(kFaMinPart, static_cast<int>(share));
-    for (int pass = 0; pass < 2; pass++) {
-        for (int b = warp; b < p.B; b += warps) {
-            const Seq s = seq_of(b, nullptr);
-            const int nt = fa_tiles_of(s, tq);
-            for (int i = lane; i < nt; i += 32) {
-                const int keys = fa_key_tiles(s, (i + 1) * 2 * tq);
-                const int parts = max(1, (keys + chunk - 1) / chunk);
-                int slot = -1;
-                if (pass == 1 && parts > 1) {
-                    slot = atomicAdd(&slots_s, parts);
-                    const int at = atomicAdd(&splits_s, 1);
-                    ws.splits[at] = FaSplit{b, i * 2 * tq, slot, parts};
-                }
-                for (int j = 0; j < parts; j++) {
-                    const int k0 = static_cast<int>(static_cast<int64_t>(keys) * j / parts);
-                    const int k1 = static_cast<int>(static_cast<int64_t>(keys) * (j + 1) / parts);
-                    const int at = atomicAdd(&hist[kPlanBuckets - 1 - min(k1 - k0, kPlanBuckets - 1)], 1);
-                    if (pass == 1) {
-                        FaUnit u{};
-                        u.b = b;
-                        u.i0 = i * 2 * tq;
-                        u.kv0 = k0;
-                        u.kv1 = k1;
-                        u.slot = slot < 0 ? -1 : slot + j;
-                        ws.units[at] = u;
-                    }
-                }
-            }
+    auto parts_of = [&](int keys) { return max(1, (keys + chunk - 1) / chunk); };
+    auto bucket_of = [&](int k) { return kPlanBuckets - 1 - min(k, kPlanBuckets - 1); };
+    // how many units, and of what length
+    int mine = 0;
+    for (int b = warp; b < p.B; b += warps) {
+        const Seq s = seq_of(b);
+        const int nt = fa_tiles_of(s, tq);
+        for (int i = lane; i < nt; i += 32) {
+            const int keys = fa_key_tiles(s, (i + 1) * 2 * tq), parts = parts_of(keys);
+            mine += parts;
+            // a tile's parts differ by one key tile at most
+            const int each = keys / parts, more = keys - each * parts;
+            if (more) atomicAdd(&hist[bucket_of(each + 1)], more);
+            atomicAdd(&hist[bucket_of(each)], parts - more);
         }
-        __syncthreads();
-        if (pass == 0) {  // exclusive scan of the buckets, longest units first
-            const int v = hist[tid];
-            int inc = v;
+    }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0 && mine) atomicAdd(&units_s, mine);
+    __syncthreads();
+    const int units = units_s;
+    // more units than the workspace holds: only sequences that overlap each other make so many
+    if (units > ws.max_units) {
+        if (tid == 0) {
+            record_error(p.err, ERR_KV_SEQ);
+            *ws.head = FaHead{};
+        }
+        return;
+    }
+    const bool sorted = units * p.Hkv > ws.sms;
+    if (sorted) {  // where each length's units begin, the longest first
+        const int v = hist[tid];
+        int inc = v;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += u;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane == 31) warp_sum[warp] = inc;
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < warp; w++) before += warp_sum[w];
+        hist[tid] = before + inc - v;
+    } else if (tid == 0) {
+        hist[0] = 0;
+    }
+    __syncthreads();
+    for (int b = warp; b < p.B; b += warps) {
+        const Seq s = seq_of(b);
+        const int nt = fa_tiles_of(s, tq);
+        for (int i = lane; i < nt; i += 32) {
+            const int keys = fa_key_tiles(s, (i + 1) * 2 * tq), parts = parts_of(keys);
+            int slot = -1;
+            if (parts > 1) {
+                slot = atomicAdd(&slots_s, parts);
+                ws.splits[atomicAdd(&splits_s, 1)] = FaSplit{s, i * 2 * tq, b, slot, parts, 0};
             }
-            if (lane == 31) warp_sum[warp] = inc;
-            __syncthreads();
-            int before = 0;
-            for (int w = 0; w < warp; w++) before += warp_sum[w];
-            hist[tid] = before + inc - v;
-            if (tid == kPlanThreads - 1) slots_s = before + inc;
-            __syncthreads();
-            // more units than the workspace holds: only sequences that overlap each other make so many
-            const int units = slots_s;
-            if (units > ws.max_units) {
-                if (tid == 0) {
-                    record_error(p.err, ERR_KV_SEQ);
-                    *ws.head = FaHead{};
-                }
-                return;
+            const int each = keys / parts, more = keys - each * parts;
+            for (int j = 0; j < parts; j++) {
+                const int k0 = j * each + min(j, more), k1 = k0 + each + (j < more ? 1 : 0);
+                const int at = atomicAdd(&hist[sorted ? bucket_of(k1 - k0) : 0], 1);
+                FaUnit u;
+                u.s = s;
+                u.b = b;
+                u.i0 = i * 2 * tq;
+                u.kv0 = k0;
+                u.kv1 = k1;
+                u.slot = slot < 0 ? -1 : slot + j;
+                ws.units[at] = u;
             }
-            __syncthreads();
-            if (tid == 0) {
-                ws.head->units = units;
-                slots_s = 0;
-            }
-            __syncthreads();
         }
     }
-    if (tid == 0) {
-        ws.head->splits = splits_s;
-        ws.head->slots = slots_s;
-    }
+    __syncthreads();
+    if (tid == 0) *ws.head = FaHead{units, splits_s, slots_s, 0};
 }
 
 // ---- PTX ------------------------------------------------------------------------------
@@ -361,14 +379,17 @@ struct FaWork {
 
 __device__ __forceinline__ FaWork fa_work(const PattnParams& p, const FaWs& ws, int u, int tq) {
     FaWork w;
-    const int4 a = __ldcg(reinterpret_cast<const int4*>(ws.units + u / p.Hkv));
-    w.slot = __ldcg(&ws.units[u / p.Hkv].slot);
+    const int4* at = reinterpret_cast<const int4*>(ws.units + u / p.Hkv);
+    const int4 a = __ldcg(at), c = __ldcg(at + 1);
+    w.s.q0 = a.x;
+    w.s.n = a.y;
+    w.s.len = a.z;
+    w.b = a.w;
+    w.i0 = c.x;
+    w.kv0 = c.y;
+    w.keys = c.z - c.y;
+    w.slot = c.w;
     w.kvh = u % p.Hkv;
-    w.b = a.x;
-    w.i0 = a.y;
-    w.kv0 = a.z;
-    w.keys = a.w - a.z;
-    w.s = read_seq(p.q_start, p.kv_len, w.b, p.T, p.kv_max, nullptr);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int i = w.i0 + h * tq;
@@ -882,34 +903,48 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Pattn
         const int r = static_cast<int>(i % kFaRows);
         const int64_t tile = i / kFaRows;
         const int kvh = static_cast<int>(tile % p.Hkv);
-        const int4 sp = __ldcg(reinterpret_cast<const int4*>(ws.splits + tile / p.Hkv));
+        const int4* at = reinterpret_cast<const int4*>(ws.splits + tile / p.Hkv);
+        const int4 sa = __ldcg(at), sb = __ldcg(at + 1);  // q0, n, len, i0; b, slot, parts
         const int hr = r % kFaTile;
-        const int token = sp.y + (r / kFaTile) * tq + hr / p.G, head = kvh * p.G + hr % p.G;
-        const Seq s = read_seq(p.q_start, p.kv_len, sp.x, p.T, p.kv_max, nullptr);
-        if (hr / p.G >= tq || token >= s.n) continue;
-        const int vis = max(0, min(s.len, s.len - s.n + token + 1));
-        const float* base = ws.part + ((static_cast<int64_t>(sp.z) * p.Hkv + kvh) * kFaRows + r) * (D + 4);
+        const int token = sa.w + (r / kFaTile) * tq + hr / p.G, head = kvh * p.G + hr % p.G;
+        if (hr / p.G >= tq || token >= sa.y) continue;
+        const int vis = max(0, min(sa.z, sa.z - sa.y + token + 1));
+        const float* base = ws.part + ((static_cast<int64_t>(sb.y) * p.Hkv + kvh) * kFaRows + r) * (D + 4);
         const int64_t step = static_cast<int64_t>(p.Hkv) * kFaRows * (D + 4);
-        float M = -INFINITY;
-        for (int j = lane; j < sp.w; j += 32) M = fmaxf(M, __ldcg(base + j * step + D));
+        // eight parts' loads under way at once
+        float M = -INFINITY, a[E] = {}, l = 0.0f;
+        for (int j0 = 0; j0 < sb.z; j0 += 8) {
+            float2 ml[8], v[8][E / 2];
+            float mn = M;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float b0 = M == -INFINITY ? 0.0f : M;
-        float a[E] = {}, l = 0.0f;
-#pragma unroll 4
-        for (int j = 0; j < sp.w; j++) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(base + j * step + D));
-            const float f = exp2_fast(ml.x - b0);
-            l = fmaf(f, ml.y, l);
+            for (int j = 0; j < 8; j++) {
+                const bool in = j0 + j < sb.z;
+                const float* pr = base + (j0 + j) * step;
+                ml[j] = in ? __ldcg(reinterpret_cast<const float2*>(pr + D)) : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(base + j * step + lane * E + e));
-                a[e] = fmaf(f, v.x, a[e]);
-                a[e + 1] = fmaf(f, v.y, a[e + 1]);
+                for (int e = 0; e < E / 2; e++)
+                    v[j][e] = in ? __ldcg(reinterpret_cast<const float2*>(pr + lane * E + 2 * e)) : make_float2(0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) mn = fmaxf(mn, ml[j].x);
+            const float b0 = mn == -INFINITY ? 0.0f : mn, c = exp2_fast(M - b0);
+            M = mn;
+            l *= c;
+#pragma unroll
+            for (int e = 0; e < E; e++) a[e] *= c;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float f = exp2_fast(ml[j].x - b0);
+                l = fmaf(f, ml[j].y, l);
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    a[e] = fmaf(f, v[j][e / 2].x, a[e]);
+                    a[e + 1] = fmaf(f, v[j][e / 2].y, a[e + 1]);
+                }
             }
         }
         const float inv = vis > 0 ? 1.0f / l : 0.0f;
-        uint16_t* o = p.out + static_cast<int64_t>(s.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D + lane * E;
+        uint16_t* o = p.out + static_cast<int64_t>(sa.x + token) * p.out_stride + static_cast<int64_t>(head) * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
             const __nv_bfloat162 b2 = __floats2bfloat162_rn(a[e] * inv, a[e + 1] * inv);
