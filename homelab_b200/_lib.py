@@ -27,6 +27,7 @@ SCALE_1X128 = 0
 SCALE_128X128 = 1
 KV_BF16 = 0
 KV_E4M3 = 1
+ATTENTION_ZERO_BYTES = 4096
 TABLES_READY = 1
 NOALLOC_SCRATCH_BYTES = 8 * 1024 * 1024
 PART_ALIGN = 256

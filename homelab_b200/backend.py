@@ -61,6 +61,7 @@ def _ptr_or_host(t) -> int:
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda i: torch.cuda.current_stream(i).cuda_stream)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 _ANY, _BF16 = (torch.float32, torch.bfloat16), (torch.bfloat16,)
 
 
@@ -69,6 +70,7 @@ class Gpu:
 
     def __init__(self, device: int = 0):
         self.device = torch.device("cuda", device)
+        self.index = device
         self.L = _lib.lib()
         self._tiled_ws = None  # grown on demand by moe_tiled calls without a workspace
         # paged and prompt attention without a workspace: one per stream, grown on demand, and the shapes known to fit it
@@ -79,12 +81,14 @@ class Gpu:
 
     def _launch(self, fn, what: str, *args):
         """fn(*args, current stream of this device), with this device the current one."""
-        i = self.device.index
-        if torch.cuda.is_initialized() and _current_device() == i:
-            check(fn(*args, _raw_stream(i)), what)
-            return
-        with torch.cuda.device(self.device):
-            check(fn(*args, self._stream()), what)
+        i = self.index
+        if _current_device() == i:
+            st = fn(*args, _raw_stream(i))
+        else:
+            with torch.cuda.device(self.device):
+                st = fn(*args, self._stream())
+        if st:
+            check(st, what)
 
     # ---- Linear -------------------------------------------------------------------------
     def gemm_fp8(self, x, q, scale, y, t: int, n: int, k: int, layout: int = SCALE_128X128, workspace=None):
@@ -273,7 +277,7 @@ class Gpu:
     def _rows(self, x, heads: int, dim: int, t: int, what: str, dtypes=_ANY):
         """Checks a [t, heads, dim] tensor on this device with contiguous rows; its address and token stride."""
         st = x.stride()
-        if x.dtype in dtypes and x.shape == (t, heads, dim) and x.device == self.device:
+        if x.dtype in dtypes and x.shape == (t, heads, dim) and x.get_device() == self.index:
             if t > 1 and st[1] == dim and st[2] == 1:
                 return x.data_ptr(), st[0]
             if t == 0 or (st[2] == 1 and (heads == 1 or st[1] == dim)):
@@ -288,7 +292,7 @@ class Gpu:
     def _index(self, x, n, what: str):
         if x is None:
             return None
-        if x.dtype != torch.int32 or x.device != self.device or x.dim() != 1 or not x.is_contiguous() or (
+        if x.dtype is not torch.int32 or x.get_device() != self.index or x.dim() != 1 or not x.is_contiguous() or (
                 n is not None and x.shape[0] != n):
             raise ValueError(f"{what} must be a contiguous int32 [{'B' if n is None else n}] tensor on {self.device}")
         return x.data_ptr()
@@ -364,11 +368,11 @@ class Gpu:
             raise ValueError("unsupported attention shape")
         return torch.zeros(n, dtype=torch.uint8, device=self.device)
 
-    def _attention_ws(self, paged: bool, *shape) -> torch.Tensor:
+    def _attention_ws(self, paged: bool, shape) -> torch.Tensor:
         """A workspace of this object's for a call of this shape on the current stream.  A graph gets one of its
         own, so that graphs (and eager calls beside them) never share one."""
-        capturing = torch.cuda.is_current_stream_capturing()
-        key = (_raw_stream(self.device.index), paged, *shape)
+        capturing = _capturing()
+        key = (_raw_stream(self.index), paged, shape)
         if not capturing and key in self._attn_ws:
             return self._attn_ws[key]
         with torch.cuda.device(self.device):
@@ -377,7 +381,9 @@ class Gpu:
             if need == 0:
                 raise ValueError("unsupported attention shape")
             if capturing:
-                return torch.zeros(need, dtype=torch.uint8, device=self.device)
+                ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+                ws[:_lib.ATTENTION_ZERO_BYTES].zero_()
+                return ws
             ws = self._attn_ws.get(key[0])
             if ws is None or ws.numel() < need:
                 self._attn_ws = {k: w for k, w in self._attn_ws.items() if k != key[0] and (
@@ -400,9 +406,9 @@ class Gpu:
         B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
         if T == 0 or B == 0:
             return
-        ws = self._attention_ws(True, B, T, max_q, H, cache.kv_heads, D) if workspace is None else workspace
+        ws = self._attention_ws(True, (B, T, max_q, H, cache.kv_heads, D)) if workspace is None else workspace
         self._launch(self.L.oomb_attention_paged, "attention_paged", cache.ref, qp, qs, op, os_, H, qs_p, len_p, B, T, max_q,
-                     scale, _ptr(ws), ws.numel())
+                     scale, ws.data_ptr(), ws.numel())
 
     def attention_prompt(self, q, k, v, out, q_start, max_q: int, scale: float, workspace=None):
         """Causal attention over packed whole prompts (oomb_attention_prompt): q, out bf16 [T, H, D],
@@ -417,9 +423,9 @@ class Gpu:
         B = q_start.numel() - 1
         if T == 0 or B <= 0:
             return
-        ws = self._attention_ws(False, B, T, max_q, H, Hkv, D) if workspace is None else workspace
+        ws = self._attention_ws(False, (B, T, max_q, H, Hkv, D)) if workspace is None else workspace
         self._launch(self.L.oomb_attention_prompt, "attention_prompt", qp, qs, kp, ks, vp, vs, op, os_, H, Hkv, D, qs_p, B, T,
-                     max_q, scale, _ptr(ws), ws.numel())
+                     max_q, scale, ws.data_ptr(), ws.numel())
 
     def device_error(self, clear: bool = True) -> int:
         code = C.c_int(0)

@@ -117,8 +117,10 @@ AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int
     const int64_t rows = static_cast<int64_t>(max_q) * G;
     w.few = paged && rows <= kDecRows;
     w.grid = kDecCtas * d->sms;
+    if (w.grid > OOMB_ATTENTION_ZERO_BYTES / 4) w.grid = OOMB_ATTENTION_ZERO_BYTES / 4;
     // the counters keep their place, and nothing else comes there, whatever the calls that share a workspace
-    const size_t base = align256(static_cast<size_t>(w.grid) * 4);
+    const size_t base = OOMB_ATTENTION_ZERO_BYTES;
+    static_assert(OOMB_ATTENTION_ZERO_BYTES % 256 == 0, "aligned regions");
     w.bytes = base;
     if (paged) {
         w.part_off = base;
@@ -188,7 +190,7 @@ bool encode_pool(CUtensorMap* map, const void* base, const KvView& kv, int D, bo
 }
 
 template <int KIND, int D>
-int launch_fa(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream_t s) {
+int launch_fa(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, cudaStream_t s) {
     FaWs fw{};
     fw.head = reinterpret_cast<FaHead*>(ws + w.head_off);
     fw.units = reinterpret_cast<FaUnit*>(ws + w.unit_off);
@@ -196,7 +198,7 @@ int launch_fa(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream_t s
     fw.part = reinterpret_cast<float*>(ws + w.fa_part_off);
     fw.max_units = w.max_units;
     fw.max_slots = w.max_slots;
-    fw.sms = w.grid / kDecCtas;
+    fw.sms = sms;
     CUtensorMap qm, km, vm;
     if (!encode_rows(&qm, p.q, p.T, p.q_stride, p.H, D, p.G, fa_tokens(p.G))) return OOMB_E_LAUNCH;
     if (KIND == KV_ROWS) {
@@ -210,7 +212,9 @@ int launch_fa(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream_t s
     int st = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, fw);
     if (st == OOMB_OK)
         st = launch(fa_kernel<KIND, D>, dim3(fw.sms), dim3(FaGeo<KIND, D>::THREADS), FaGeo<KIND, D>::TOTAL, s, p, fw, qm, km, vm);
-    if (st == OOMB_OK) st = launch(join_kernel<KIND, D>, dim3(2 * fw.sms), dim3(256), 0, s, p, fw);
+    // no tile has more keys than a part takes: nothing was split
+    const int most = KIND == KV_ROWS ? p.max_q : p.kv_max;
+    if (st == OOMB_OK && most > kFaMinPart * kFaTile) st = launch(join_kernel<KIND, D>, dim3(2 * fw.sms), dim3(256), 0, s, p, fw);
     return st;
 }
 
@@ -231,7 +235,7 @@ int launch_decode(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream
 }
 
 template <int KIND, int D>
-int launch_attn_d(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream_t s) {
+int launch_attn_d(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, cudaStream_t s) {
     if constexpr (KIND != KV_ROWS) {
         const int rows = p.max_q * p.G;
         if (w.few)
@@ -239,13 +243,13 @@ int launch_attn_d(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream
                    : rows <= 8 ? launch_decode<KIND, D, 8>(p, w, ws, s)
                                : launch_decode<KIND, D, 16>(p, w, ws, s);
     }
-    return launch_fa<KIND, D>(p, w, ws, s);
+    return launch_fa<KIND, D>(p, w, sms, ws, s);
 }
 
 template <int KIND>
-int launch_attn(const PattnParams& p, int head_dim, const AttnWs& w, void* ws, cudaStream_t s) {
-    return head_dim == 128 ? launch_attn_d<KIND, 128>(p, w, static_cast<uint8_t*>(ws), s)
-                           : launch_attn_d<KIND, 64>(p, w, static_cast<uint8_t*>(ws), s);
+int launch_attn(const PattnParams& p, int head_dim, const AttnWs& w, int sms, void* ws, cudaStream_t s) {
+    return head_dim == 128 ? launch_attn_d<KIND, 128>(p, w, sms, static_cast<uint8_t*>(ws), s)
+                           : launch_attn_d<KIND, 64>(p, w, sms, static_cast<uint8_t*>(ws), s);
 }
 
 bool attn_shape_ok(int batch, int t, int max_q, int heads, int kv_heads, int head_dim) {
@@ -441,8 +445,8 @@ int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_st
     p.kv_max = cache->max_pages * cache->page_size;
     p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
     p.err = d->err;
-    return cache->dtype == OOMB_KV_E4M3 ? launch_attn<KV_E4M3>(p, cache->head_dim, w, workspace, stream)
-                                        : launch_attn<KV_BF16>(p, cache->head_dim, w, workspace, stream);
+    return cache->dtype == OOMB_KV_E4M3 ? launch_attn<KV_E4M3>(p, cache->head_dim, w, d->sms, workspace, stream)
+                                        : launch_attn<KV_BF16>(p, cache->head_dim, w, d->sms, workspace, stream);
 }
 
 size_t oomb_attention_prompt_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim) {
@@ -487,7 +491,7 @@ int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_
     p.kv.v_stride = v_stride;
     p.kv.Hkv = kv_heads;
     p.err = d->err;
-    return launch_attn<KV_ROWS>(p, head_dim, w, workspace, stream);
+    return launch_attn<KV_ROWS>(p, head_dim, w, d->sms, workspace, stream);
 }
 
 }  // extern "C"

@@ -54,36 +54,39 @@ class PagedKv:
 
     def __init__(self, k_pages, v_pages, block_table, k_exp=None, v_exp=None):
         fp8 = k_exp is not None or v_exp is not None
-        kind, shape, ks, device = k_pages.dtype, k_pages.shape, k_pages.stride(), k_pages.device
+        kind, shape, ks, place = k_pages.dtype, k_pages.shape, k_pages.stride(), k_pages.get_device()
         if (kind not in _CODES if fp8 else kind is not torch.bfloat16) or v_pages.dtype is not kind:
             raise TypeError(f"pages must both be {'e4m3 codes' if fp8 else 'bf16'}, got {kind} and {v_pages.dtype}")
         if len(shape) != 4 or v_pages.shape != shape:
             raise ValueError("k_pages and v_pages must be [pages, kv_heads, page_size, head_dim], of one shape")
         pages, heads, size, dim = shape
-        if ks[1:] != (size * dim, dim, 1) or v_pages.stride() != ks:
+        row = size * dim
+        if ks[1] != row or ks[2] != dim or ks[3] != 1 or v_pages.stride() != ks:
             raise ValueError("the rows of a page must be contiguous, and both pools strided alike")
-        es = (0, 0, 0)
+        same = v_pages.get_device() == place == block_table.get_device()
+        exps = (None, None, 0)
         if fp8:
+            want = shape[:3]
             for x in (k_exp, v_exp):
-                if x is None or x.dtype is not torch.uint8 or x.shape != (pages, heads, size):
+                if x is None or x.dtype is not torch.uint8 or x.shape != want:
                     raise ValueError("k_exp and v_exp must be uint8 [pages, kv_heads, page_size]")
             es = k_exp.stride()
-            if es[1:] != (size, 1) or v_exp.stride() != es:
+            if es[1] != size or es[2] != 1 or v_exp.stride() != es:
                 raise ValueError("the exponents of a page must be contiguous, and both strided alike")
-            if k_exp.device != device or v_exp.device != device:
-                raise ValueError("the pages, exponents and block table must live on one device")
-        ts = block_table.stride()
-        if block_table.dtype is not torch.int32 or len(ts) != 2 or (ts[1] != 1 and block_table.shape[1] > 1):
-            raise ValueError("block_table must be int32 [batch, max_pages] with contiguous rows")
-        if v_pages.device != device or block_table.device != device:
+            same = same and k_exp.get_device() == place == v_exp.get_device()
+            exps = (k_exp.data_ptr(), v_exp.data_ptr(), es[0] if pages > 1 else heads * size)
+        if not same:
             raise ValueError("the pages, exponents and block table must live on one device")
+        ts, tsh = block_table.stride(), block_table.shape
+        if block_table.dtype is not torch.int32 or len(ts) != 2 or (ts[1] != 1 and tsh[1] > 1):
+            raise ValueError("block_table must be int32 [batch, max_pages] with contiguous rows")
         self.k_pages, self.v_pages, self.k_exp, self.v_exp, self.block_table = k_pages, v_pages, k_exp, v_exp, block_table
-        self.kv_heads, self.page_size, self.head_dim, self.fp8, self.device = heads, size, dim, fp8, device
-        self.batch, self.max_pages = block_table.shape
+        self.kv_heads, self.page_size, self.head_dim, self.fp8, self.device = heads, size, dim, fp8, k_pages.device
+        self.batch, width = tsh
+        self.max_pages = width
         self.struct = PagedKvStruct(
-            KV_E4M3 if fp8 else KV_BF16, heads, dim, size, pages, self.max_pages, max(ts[0], self.max_pages), 0,
-            k_pages.data_ptr(), v_pages.data_ptr(), k_exp.data_ptr() if fp8 else None, v_exp.data_ptr() if fp8 else None,
-            ks[0] if pages > 1 else heads * size * dim, (es[0] if pages > 1 else heads * size) if fp8 else 0,
+            KV_E4M3 if fp8 else KV_BF16, heads, dim, size, pages, width, ts[0] if ts[0] > width else width, 0,
+            k_pages.data_ptr(), v_pages.data_ptr(), exps[0], exps[1], ks[0] if pages > 1 else heads * row, exps[2],
             block_table.data_ptr())
         self.ref = C.byref(self.struct)
 

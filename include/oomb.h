@@ -341,8 +341,10 @@ int oomb_kv_read_paged(const oomb_paged_kv* cache, const int32_t* q_start, const
  * 64 heads a kv head.  A token at position p sees positions 0 .. p below kv_len (a token that sees none gets zeros);
  * what it does not see never reaches its output, infinities and NaN included.
  * max_q bounds the tokens of a sequence (a longer one sets the device error word and is left out).  The workspace
- * holds oomb_attention_paged_workspace_bytes(...) bytes, zeroed once before first use (and after a device
- * error); calls that share it must be ordered on one stream. */
+ * holds oomb_attention_paged_workspace_bytes(...) bytes (0: unsupported shape, or no device), enough for every call of at
+ * most this batch, t and max_q with these heads; its first OOMB_ATTENTION_ZERO_BYTES are zero before first use
+ * (and again after a device error).  Calls that share it must be ordered on one stream. */
+#define OOMB_ATTENTION_ZERO_BYTES 4096
 size_t oomb_attention_paged_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim);
 int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_stride, void* out, int64_t out_stride,
                          int heads, const int32_t* q_start, const int32_t* kv_len, int batch, int t, int max_q, float scale,
