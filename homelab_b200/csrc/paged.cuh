@@ -387,22 +387,47 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) 
         }
     }
     __syncthreads();
-    const int per_row = p.kv.Hkv * (D / 8), per_tok = 2 * per_row;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nt * per_tok; i += kReadThreads) {
-        const int a = i / per_tok, rest = i - a * per_tok;
-        const bool is_v = rest >= per_row;
-        const int c = is_v ? rest - per_row : rest, h = c / (D / 8), c8 = (c % (D / 8)) * 8;
-        const int64_t row = tok_row[a];
-        if (row == -2) continue;
-        float f[8] = {};
-        if (row >= 0) {
+    // Chunks of 8 values, four under way at once: (token, keys or values, head, chunk).
+    const int per_row = p.kv.Hkv * (D / 8), per_tok = 2 * per_row, total = nt * per_tok;
+    constexpr int N = 4;
+    for (int i0 = threadIdx.x; i0 < total; i0 += N * kReadThreads) {
+        uint4 w[N];
+        unsigned e[N];
+        int64_t to[N];
+        bool is_v[N], leave[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int i = i0 + k * kReadThreads;
+            w[k] = make_uint4(0u, 0u, 0u, 0u);
+            e[k] = 127u;
+            leave[k] = true;
+            if (i >= total) continue;
+            const int a = i / per_tok, rest = i - a * per_tok;
+            is_v[k] = rest >= per_row;
+            const int c = is_v[k] ? rest - per_row : rest, h = c / (D / 8), c8 = (c % (D / 8)) * 8;
+            const int64_t row = tok_row[a];
+            if (row == -2) continue;
+            leave[k] = false;
+            to[k] = static_cast<int64_t>(t0 + a) * p.out_stride + h * D + c8;
+            if (row < 0) continue;
             const int64_t o = row + (static_cast<int64_t>(h) * D << p.kv.page_log2) + c8;
-            const uint8_t* pool = is_v ? p.kv.v : p.kv.k;
+            const uint8_t* pool = is_v[k] ? p.kv.v : p.kv.k;
             if constexpr (FP8) {
-                const uint2 w = __ldcs(reinterpret_cast<const uint2*>(pool + o));
-                const float s = exp_byte((is_v ? p.kv.ve : p.kv.ke)[tok_exp[a] + (static_cast<int64_t>(h) << p.kv.page_log2)]);
-                const unsigned u[2] = {w.x, w.y};
+                const uint2 u = __ldcs(reinterpret_cast<const uint2*>(pool + o));
+                w[k].x = u.x;
+                w[k].y = u.y;
+                e[k] = (is_v[k] ? p.kv.ve : p.kv.ke)[tok_exp[a] + (static_cast<int64_t>(h) << p.kv.page_log2)];
+            } else {
+                w[k] = __ldcs(reinterpret_cast<const uint4*>(pool + 2 * o));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            if (leave[k]) continue;
+            float f[8];
+            if constexpr (FP8) {
+                const float s = exp_byte(e[k]);
+                const unsigned u[2] = {w[k].x, w[k].y};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float2 d = e4m3x2_to_float2(static_cast<unsigned short>(u[j / 2] >> (16 * (j & 1))));
@@ -410,10 +435,19 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) 
                     f[2 * j + 1] = d.y * s;
                 }
             } else {
-                load8<true>(pool, o, f);
+                if (p.out_bf16) {
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(is_v[k] ? p.vo : p.ko) + to[k]) = w[k];
+                    continue;
+                }
+                const unsigned u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    f[2 * j] = __uint_as_float(u[j] << 16);
+                    f[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                }
             }
+            store8(is_v[k] ? p.vo : p.ko, to[k], p.out_bf16, f);
         }
-        store8(is_v ? p.vo : p.ko, static_cast<int64_t>(t0 + a) * p.out_stride + h * D + c8, p.out_bf16, f);
     }
 }
 
