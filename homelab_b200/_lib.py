@@ -182,7 +182,7 @@ SIGNATURES = [
     ("oomb_kv_append_paged", I, [C.POINTER(PagedKvStruct), C.POINTER(RopeStruct), P, C.c_int64, P, C.c_int64, I, P,
                                  C.c_int64, P, C.c_int64, I, P, P, I, I, S]),
     ("oomb_kv_read_paged", I, [C.POINTER(PagedKvStruct), P, P, I, I, P, P, I, C.c_int64, S]),
-    ("oomb_attention_paged_workspace_bytes", Z, [I, I, I, I, I, I]),
+    ("oomb_attention_paged_workspace_bytes", Z, [C.POINTER(PagedKvStruct), I, I, I, I]),
     ("oomb_attention_paged", I, [C.POINTER(PagedKvStruct), P, C.c_int64, P, C.c_int64, I, P, P, I, I, I, C.c_float,
                                  P, Z, S]),
     ("oomb_attention_prompt_workspace_bytes", Z, [I, I, I, I, I, I]),

@@ -358,37 +358,43 @@ class Gpu:
             return
         self._launch(self.L.oomb_kv_read_paged, "kv_read_paged", cache.ref, qs_p, len_p, B, T, kp, vp, _dtype_code(k_out), ks)
 
-    def attention_paged_workspace(self, batch: int, t: int, max_q: int, heads: int, kv_heads: int,
-                                  head_dim: int) -> torch.Tensor:
-        """A zeroed workspace for attention_paged and attention_prompt calls of at most these sizes."""
+    def attention_paged_workspace(self, cache: PagedKv, batch: int, t: int, max_q: int, heads: int) -> torch.Tensor:
+        """A workspace for attention_paged calls of at most these sizes over a cache of this shape."""
         with torch.cuda.device(self.device):
-            n = max(int(f(batch, t, max_q, heads, kv_heads, head_dim)) for f in
-                    (self.L.oomb_attention_paged_workspace_bytes, self.L.oomb_attention_prompt_workspace_bytes))
-        if n == 0:
-            raise ValueError("unsupported attention shape")
-        return torch.zeros(n, dtype=torch.uint8, device=self.device)
+            return self._new_ws(int(self.L.oomb_attention_paged_workspace_bytes(cache.ref, batch, t, max_q, heads)))
 
-    def _attention_ws(self, paged: bool, shape) -> torch.Tensor:
+    def attention_prompt_workspace(self, batch: int, t: int, max_q: int, heads: int, kv_heads: int,
+                                   head_dim: int) -> torch.Tensor:
+        """A workspace for attention_prompt calls of at most these sizes."""
+        with torch.cuda.device(self.device):
+            return self._new_ws(int(self.L.oomb_attention_prompt_workspace_bytes(batch, t, max_q, heads, kv_heads,
+                                                                                 head_dim)))
+
+    def _new_ws(self, need: int) -> torch.Tensor:
+        if need == 0:
+            raise ValueError("unsupported attention shape")
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        ws[:_lib.ATTENTION_ZERO_BYTES].zero_()
+        return ws
+
+    def _attention_ws(self, cache, shape) -> torch.Tensor:
         """A workspace of this object's for a call of this shape on the current stream.  A graph gets one of its
         own, so that graphs (and eager calls beside them) never share one."""
         capturing = _capturing()
-        key = (_raw_stream(self.index), paged, shape)
+        key = (_raw_stream(self.index), shape) if cache is None else (
+            _raw_stream(self.index), shape, cache.max_pages, cache.page_size, cache.kv_heads, cache.head_dim, cache.fp8)
         if not capturing and key in self._attn_ws:
             return self._attn_ws[key]
         with torch.cuda.device(self.device):
-            need = int((self.L.oomb_attention_paged_workspace_bytes if paged else
-                        self.L.oomb_attention_prompt_workspace_bytes)(*shape))
-            if need == 0:
-                raise ValueError("unsupported attention shape")
+            need = int(self.L.oomb_attention_prompt_workspace_bytes(*shape) if cache is None else
+                       self.L.oomb_attention_paged_workspace_bytes(cache.ref, *shape))
             if capturing:
-                ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-                ws[:_lib.ATTENTION_ZERO_BYTES].zero_()
-                return ws
+                return self._new_ws(need)
             ws = self._attn_ws.get(key[0])
-            if ws is None or ws.numel() < need:
+            if ws is None or ws.numel() < need or need == 0:
                 self._attn_ws = {k: w for k, w in self._attn_ws.items() if k != key[0] and (
                     isinstance(k, int) or k[0] != key[0])}
-                ws = self._attn_ws[key[0]] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+                ws = self._attn_ws[key[0]] = self._new_ws(need)
         if len(self._attn_ws) < 4096:
             self._attn_ws[key] = ws
         return ws
@@ -406,7 +412,7 @@ class Gpu:
         B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
         if T == 0 or B == 0:
             return
-        ws = self._attention_ws(True, (B, T, max_q, H, cache.kv_heads, D)) if workspace is None else workspace
+        ws = self._attention_ws(cache, (B, T, max_q, H)) if workspace is None else workspace
         self._launch(self.L.oomb_attention_paged, "attention_paged", cache.ref, qp, qs, op, os_, H, qs_p, len_p, B, T, max_q,
                      scale, ws.data_ptr(), ws.numel())
 
@@ -423,7 +429,7 @@ class Gpu:
         B = q_start.numel() - 1
         if T == 0 or B <= 0:
             return
-        ws = self._attention_ws(False, (B, T, max_q, H, Hkv, D)) if workspace is None else workspace
+        ws = self._attention_ws(None, (B, T, max_q, H, Hkv, D)) if workspace is None else workspace
         self._launch(self.L.oomb_attention_prompt, "attention_prompt", qp, qs, kp, ks, vp, vs, op, os_, H, Hkv, D, qs_p, B, T,
                      max_q, scale, ws.data_ptr(), ws.numel())
 

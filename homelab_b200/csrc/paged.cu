@@ -108,11 +108,21 @@ struct AttnWs {
     size_t part_off;  // few
     size_t head_off, unit_off, split_off, fa_part_off;
     int max_units, max_slots;
+    bool expand;  // e4m3: the codes are converted once, to bf16 rows in the workspace
+    size_t k_off, v_off;
     size_t bytes;
 };
 
-AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int kv_heads, int head_dim, bool paged) {
+// Above so many query rows a kv head (each pair of tiles would convert every code again) an 8-bit cache is
+// converted once before the attention, where the copy stays below this many bytes.  Measured over 16,000 positions of 8 kv
+// heads, D = 128, in the attention / before it: 512 rows 73 / 93 us (32 heads), 109 / 114 (8 heads); 768 rows 150 / 141; 1024
+// rows 186 / 163 and 187 / 167; 4096 rows 449 / 320.
+constexpr int kExpandRows = 640;
+constexpr int64_t kExpandBytes = int64_t{1} << 30;
+
+AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int kv_heads, int head_dim, const oomb_paged_kv* cache) {
     AttnWs w{};
+    const bool paged = cache != nullptr;
     const int G = heads / kv_heads;
     const int64_t rows = static_cast<int64_t>(max_q) * G;
     w.few = paged && rows <= kDecRows;
@@ -138,6 +148,15 @@ AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int
         w.fa_part_off = align256(w.split_off + static_cast<size_t>(w.max_slots) * sizeof(FaSplit));
         const size_t end = w.fa_part_off + static_cast<size_t>(w.max_slots) * kv_heads * kFaRows * (head_dim + 4) * 4;
         if (end > w.bytes) w.bytes = end;
+        if (cache && cache->dtype == OOMB_KV_E4M3 && rows > kExpandRows) {
+            const int64_t copy = static_cast<int64_t>(batch) * cache->max_pages * cache->page_size * kv_heads * head_dim * 2;
+            if (2 * copy <= kExpandBytes && static_cast<int64_t>(batch) * cache->max_pages * cache->page_size < (1 << 30)) {
+                w.expand = true;
+                w.k_off = align256(end);
+                w.v_off = align256(w.k_off + static_cast<size_t>(copy));
+                if (w.v_off + static_cast<size_t>(copy) > w.bytes) w.bytes = w.v_off + static_cast<size_t>(copy);
+            }
+        }
     }
     return w;
 }
@@ -202,8 +221,9 @@ int launch_fa(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, cudaS
     CUtensorMap qm, km, vm;
     if (!encode_rows(&qm, p.q, p.T, p.q_stride, p.H, D, p.G, fa_tokens(p.G))) return OOMB_E_LAUNCH;
     if (KIND == KV_ROWS) {
-        if (!encode_rows(&km, p.kv.k, p.T, p.kv.k_stride, p.Hkv, D, 1, kFaTile) ||
-            !encode_rows(&vm, p.kv.v, p.T, p.kv.v_stride, p.Hkv, D, 1, kFaTile))
+        const int64_t n = p.kv.seq_rows ? static_cast<int64_t>(p.B) * p.kv.seq_rows : p.T;
+        if (!encode_rows(&km, p.kv.k, n, p.kv.k_stride, p.Hkv, D, 1, kFaTile) ||
+            !encode_rows(&vm, p.kv.v, n, p.kv.v_stride, p.Hkv, D, 1, kFaTile))
             return OOMB_E_LAUNCH;
     } else if (!encode_pool(&km, p.kv.k, p.kv, D, KIND == KV_E4M3, KIND != KV_E4M3) ||
                !encode_pool(&vm, p.kv.v, p.kv, D, KIND == KV_E4M3, KIND != KV_E4M3)) {
@@ -213,7 +233,7 @@ int launch_fa(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, cudaS
     if (st == OOMB_OK)
         st = launch(fa_kernel<KIND, D>, dim3(fw.sms), dim3(FaGeo<KIND, D>::THREADS), FaGeo<KIND, D>::TOTAL, s, p, fw, qm, km, vm);
     // no tile has more keys than a part takes: nothing was split
-    const int most = KIND == KV_ROWS ? p.max_q : p.kv_max;
+    const int most = KIND == KV_ROWS && !p.kv.seq_rows ? p.max_q : p.kv_max;
     if (st == OOMB_OK && most > kFaMinPart * kFaTile) st = launch(join_kernel<KIND, D>, dim3(2 * fw.sms), dim3(256), 0, s, p, fw);
     return st;
 }
@@ -242,6 +262,30 @@ int launch_attn_d(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, c
             return rows <= 4   ? launch_decode<KIND, D, 4>(p, w, ws, s)
                    : rows <= 8 ? launch_decode<KIND, D, 8>(p, w, ws, s)
                                : launch_decode<KIND, D, 16>(p, w, ws, s);
+    }
+    if constexpr (KIND == KV_E4M3) {
+        if (w.expand) {
+            ExpandParams e{};
+            e.kv = p.kv;
+            e.q_start = p.q_start;
+            e.kv_len = p.kv_len;
+            e.B = p.B;
+            e.T = p.T;
+            e.kv_max = p.kv_max;
+            e.ko = reinterpret_cast<uint16_t*>(ws + w.k_off);
+            e.vo = reinterpret_cast<uint16_t*>(ws + w.v_off);
+            e.err = p.err;
+            if (p.B > 65535) return OOMB_E_SHAPE;
+            const dim3 grid(static_cast<unsigned>((p.kv_max + kExpandTokens - 1) / kExpandTokens), static_cast<unsigned>(p.B));
+            const int st = grid.x ? launch(expand_kernel<D>, grid, dim3(kReadThreads), 0, s, e) : OOMB_OK;
+            if (st != OOMB_OK) return st;
+            PattnParams r = p;
+            r.kv.k = ws + w.k_off;
+            r.kv.v = ws + w.v_off;
+            r.kv.k_stride = r.kv.v_stride = static_cast<int64_t>(p.Hkv) * D;
+            r.kv.seq_rows = p.kv_max;
+            return p.kv_max ? launch_fa<KV_ROWS, D>(r, w, sms, ws, s) : launch_fa<KIND, D>(p, w, sms, ws, s);
+        }
     }
     return launch_fa<KIND, D>(p, w, sms, ws, s);
 }
@@ -408,10 +452,11 @@ int oomb_kv_read_paged(const oomb_paged_kv* cache, const int32_t* q_start, const
                : launch(read_kernel<false, 64>, grid, dim3(kReadThreads), 0, stream, p);
 }
 
-size_t oomb_attention_paged_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim) {
+size_t oomb_attention_paged_workspace_bytes(const oomb_paged_kv* cache, int batch, int t, int max_q, int heads) {
+    KvView v;
+    if (check_cache(cache, v) != OOMB_OK || !attn_shape_ok(batch, t, max_q, heads, cache->kv_heads, cache->head_dim)) return 0;
     const DeviceState* d = device_state();
-    if (!d || !attn_shape_ok(batch, t, max_q, heads, kv_heads, head_dim)) return 0;
-    return attn_ws(d, batch, t, max_q, heads, kv_heads, head_dim, true).bytes;
+    return d ? attn_ws(d, batch, t, max_q, heads, cache->kv_heads, cache->head_dim, cache).bytes : 0;
 }
 
 int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_stride, void* out, int64_t out_stride,
@@ -428,7 +473,7 @@ int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_st
     if (batch == 0 || t == 0 || max_q == 0) return OOMB_OK;
     const DeviceState* d = device_state();
     if (!d) return OOMB_E_DEVICE;
-    const AttnWs w = attn_ws(d, batch, t, max_q, heads, cache->kv_heads, cache->head_dim, true);
+    const AttnWs w = attn_ws(d, batch, t, max_q, heads, cache->kv_heads, cache->head_dim, cache);
     if (workspace_bytes < w.bytes) return OOMB_E_WORKSPACE;
     p.q = static_cast<const uint16_t*>(q);
     p.q_stride = q_stride;
@@ -452,7 +497,7 @@ int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_st
 size_t oomb_attention_prompt_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim) {
     const DeviceState* d = device_state();
     if (!d || !attn_shape_ok(batch, t, max_q, heads, kv_heads, head_dim)) return 0;
-    return attn_ws(d, batch, t, max_q, heads, kv_heads, head_dim, false).bytes;
+    return attn_ws(d, batch, t, max_q, heads, kv_heads, head_dim, nullptr).bytes;
 }
 
 int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
@@ -469,7 +514,7 @@ int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_
     if (batch == 0 || t == 0 || max_q == 0) return OOMB_OK;
     const DeviceState* d = device_state();
     if (!d) return OOMB_E_DEVICE;
-    const AttnWs w = attn_ws(d, batch, t, max_q, heads, kv_heads, head_dim, false);
+    const AttnWs w = attn_ws(d, batch, t, max_q, heads, kv_heads, head_dim, nullptr);
     if (workspace_bytes < w.bytes) return OOMB_E_WORKSPACE;
     PattnParams p{};
     p.q = static_cast<const uint16_t*>(q);

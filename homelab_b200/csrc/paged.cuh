@@ -54,6 +54,7 @@ struct KvView {
     int page_log2;
     int Hkv;
     int64_t k_stride, v_stride;  // packed rows: elements from token to token
+    int seq_rows;                // packed rows: sequence b's keys begin at row b * seq_rows; 0: at its first token
 };
 
 // The sequence that token t belongs to: the number of b with q_start[b + 1] <= t, by a
@@ -447,6 +448,77 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) 
                 }
             }
             store8(is_v[k] ? p.vo : p.ko, to[k], p.out_bf16, f);
+        }
+    }
+}
+
+// ---- conversion of a call's codes ------------------------------------------------------
+
+constexpr int kExpandTokens = 16;  // positions of a CTA
+
+struct ExpandParams {
+    KvView kv;
+    const int32_t* q_start;
+    const int32_t* kv_len;
+    int B, T, kv_max;
+    uint16_t *ko, *vo;  // [B * kv_max][kv_heads][D]
+    unsigned* err;
+};
+
+// The cached rows of every sequence as bf16 (a code times a power of two is exact there), position j of sequence b at row
+// b * kv_max + j: for attention whose query tiles would each convert them again.  A position's page is looked up once a
+// CTA; eight values a thread, four loads under way.
+template <int D>
+__global__ void __launch_bounds__(kReadThreads) expand_kernel(const ExpandParams p) {
+    __shared__ int64_t row[kExpandTokens], ex[kExpandTokens];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int b = blockIdx.y, j0 = blockIdx.x * kExpandTokens;
+    const Seq s = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, nullptr);
+    const int nt = s.n > 0 ? min(kExpandTokens, s.len - j0) : 0;
+    if (nt <= 0) return;
+    if (static_cast<int>(threadIdx.x) < nt) {
+        const int j = j0 + threadIdx.x;
+        const int page = __ldcg(p.kv.table + static_cast<int64_t>(b) * p.kv.table_stride + (j >> p.kv.page_log2));
+        const int slot = j & ((1 << p.kv.page_log2) - 1);
+        const bool good = page >= 0 && page < p.kv.num_pages;
+        if (!good) record_error(p.err, ERR_KV_TABLE);
+        row[threadIdx.x] = good ? page * p.kv.page_stride + static_cast<int64_t>(slot) * D : -1;
+        ex[threadIdx.x] = good ? page * p.kv.exp_stride + slot : 0;
+    }
+    __syncthreads();
+    const int per_row = p.kv.Hkv * (D / 8), per_tok = 2 * per_row, total = nt * per_tok;
+    constexpr int N = 4;
+    for (int i0 = threadIdx.x; i0 < total; i0 += N * kReadThreads) {
+        uint2 w[N];
+        unsigned e[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int i = i0 + k * kReadThreads;
+            w[k] = make_uint2(0u, 0u);
+            e[k] = 127u;
+            if (i >= total) continue;
+            const int a = i / per_tok, rest = i - a * per_tok, c = rest % per_row, h = c / (D / 8), c8 = (c % (D / 8)) * 8;
+            if (row[a] < 0) continue;
+            const bool v = rest >= per_row;
+            w[k] = __ldcs(reinterpret_cast<const uint2*>((v ? p.kv.v : p.kv.k) + row[a] + (static_cast<int64_t>(h) * D << p.kv.page_log2) + c8));
+            e[k] = (v ? p.kv.ve : p.kv.ke)[ex[a] + (static_cast<int64_t>(h) << p.kv.page_log2)];
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int i = i0 + k * kReadThreads;
+            if (i >= total) continue;
+            const int a = i / per_tok, rest = i - a * per_tok, c = rest % per_row;
+            const float sc = exp_byte(e[k]);
+            const unsigned u[2] = {w[k].x, w[k].y};
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 d = e4m3x2_to_float2(static_cast<unsigned short>(u[j / 2] >> (16 * (j & 1))));
+                f[2 * j] = d.x * sc;
+                f[2 * j + 1] = d.y * sc;
+            }
+            store8(rest >= per_row ? p.vo : p.ko, (static_cast<int64_t>(b) * p.kv_max + j0 + a) * p.kv.Hkv * D + c * 8, true, f);
         }
     }
 }

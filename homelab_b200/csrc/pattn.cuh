@@ -40,13 +40,13 @@ __device__ __forceinline__ float power_of(int e) { return __int_as_float((e + 12
 // Lane's D / 32 values of key (or value) row j of sequence b, kv head h, as fp32; a bad
 // block table entry reads as zeros.
 template <int KIND, int D>
-__device__ __forceinline__ void kv_row(const PattnParams& p, bool value, int b, int q0, int h, int j, int lane, float (&f)[D / 32]) {
+__device__ __forceinline__ void kv_row(const PattnParams& p, bool value, int b, int base_row, int h, int j, int lane, float (&f)[D / 32]) {
     constexpr int E = D / 32;
     const uint8_t* base = value ? p.kv.v : p.kv.k;
     int64_t o;
     float s = 1.0f;
     if constexpr (KIND == KV_ROWS) {
-        o = static_cast<int64_t>(q0 + j) * (value ? p.kv.v_stride : p.kv.k_stride) + static_cast<int64_t>(h) * D;
+        o = static_cast<int64_t>(base_row + j) * (value ? p.kv.v_stride : p.kv.k_stride) + static_cast<int64_t>(h) * D;
     } else {
         const int page = __ldcg(p.kv.table + static_cast<int64_t>(b) * p.kv.table_stride + (j >> p.kv.page_log2));
         const int slot = j & ((1 << p.kv.page_log2) - 1);
@@ -75,10 +75,10 @@ __device__ __forceinline__ void kv_row(const PattnParams& p, bool value, int b, 
     }
 }
 
-// One query row over positions [j0, j1) by one warp, in plain fp32 loops: the running
+// One query row over positions [j0, j1) (of packed rows from base_row on, or of sequence b's pages) by one warp, in plain fp32 loops: the running
 // maximum m (in units of log2), sum l and unnormalised output acc of the row.
 template <int KIND, int D>
-__device__ __noinline__ void attend_row(const PattnParams& p, int b, int q0, int token, int head, int j0, int j1, int lane, float& m,
+__device__ __noinline__ void attend_row(const PattnParams& p, int b, int base_row, int token, int head, int j0, int j1, int lane, float& m,
                                         float& l, float (&acc)[D / 32]) {
     constexpr int E = D / 32;
     float q[E];
@@ -92,8 +92,8 @@ __device__ __noinline__ void attend_row(const PattnParams& p, int b, int q0, int
     l = 0.0f;
     for (int j = j0; j < j1; j++) {
         float k[E], v[E];
-        kv_row<KIND, D>(p, false, b, q0, head / p.G, j, lane, k);
-        kv_row<KIND, D>(p, true, b, q0, head / p.G, j, lane, v);
+        kv_row<KIND, D>(p, false, b, base_row, head / p.G, j, lane, k);
+        kv_row<KIND, D>(p, true, b, base_row, head / p.G, j, lane, v);
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < E; i++) s = fmaf(q[i], k[i], s);

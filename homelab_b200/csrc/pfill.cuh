@@ -30,8 +30,8 @@
 // paged cache (a page of 16 or more rows keeps the swizzle's 8-row pattern); for an e4m3 cache 12-15
 // turn the loaded codes into bf16 tiles on the way (once per tile, for all 256 rows).
 //
-// Work: plan_kernel lists the units (a tile, or a part of its positions when there are fewer
-// tiles than SMs), longest first; the CTAs take them in turn.  Parts leave (acc, m, l) in the
+// Work: plan_kernel lists the units (a tile, or a part of its positions when there are too few
+// tiles to fill the SMs), longest first; a CTA takes the next when it is through with one.  Parts leave (acc, m, l) in the
 // workspace, joined in order by join_kernel.  Every wait is bounded.
 #pragma once
 
@@ -67,7 +67,8 @@ struct __align__(16) FaSplit {
 };
 static_assert(sizeof(FaUnit) == 32 && sizeof(FaSplit) == 32, "read as two int4");
 struct FaHead {
-    int units, splits, slots, pad;
+    int units, splits, slots;
+    int next;  // units dealt out beyond the CTAs' first
 };
 
 struct FaWs {
@@ -94,11 +95,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     __shared__ int hist[kPlanBuckets];
     __shared__ Seq seqs[kPlanSeqs];
     __shared__ unsigned long long total_s;
-    __shared__ int slots_s, splits_s, units_s, warp_sum[32];
+    __shared__ int slots_s, splits_s, units_s, longest_s, shortest_s, count_s[6], warp_sum[32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = kPlanThreads / 32;
     if (tid == 0) {
         total_s = 0;
-        slots_s = splits_s = units_s = 0;
+        slots_s = splits_s = units_s = longest_s = 0;
+        shortest_s = 1 << 30;
+        for (int k = 0; k < 6; k++) count_s[k] = 0;
     }
     for (int i = tid; i < kPlanBuckets; i += kPlanThreads) hist[i] = 0;
     pdl_wait();
@@ -119,18 +122,65 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     __syncthreads();
     auto seq_of = [&](int b) { return b < kPlanSeqs ? seqs[b] : read(b, nullptr); };
     unsigned long long work = 0;
+    int longest = 1, shortest = 1 << 30;
     for (int b = warp; b < p.B; b += warps) {
         const Seq s = seq_of(b);
         const int nt = fa_tiles_of(s, tq);
-        for (int i = lane; i < nt; i += 32) work += max(1, fa_key_tiles(s, (i + 1) * 2 * tq));
+        for (int i = lane; i < nt; i += 32) {
+            const int keys = max(1, fa_key_tiles(s, (i + 1) * 2 * tq));
+            work += keys;
+            longest = max(longest, keys);
+            shortest = min(shortest, keys);
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-    if (lane == 0 && work) atomicAdd(&total_s, work);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    shortest = __reduce_min_sync(0xffffffffu, shortest);
+    if (lane == 0 && work) {
+        atomicAdd(&total_s, work);
+        atomicMax(&longest_s, longest);
+        atomicMin(&shortest_s, shortest);
+    }
     __syncthreads();
-    // a part is at least an SM's even share of the step, so there are at most two parts an SM
-    const unsigned long long share = (total_s * p.Hkv + ws.sms - 1) / ws.sms;
-    const int chunk = share > (1u << 30) ? (1 << 30) : max(kFaMinPart, static_cast<int>(share));
+    // How long a part may be: an SM's even share of the step or more (so that there are at most two parts an SM), or a whole
+    // tile.  Of a few lengths the one whose last CTA should finish first: with at most a unit an SM that is the
+    // longest unit, else (the longest go first) the share and half of the shortest; writing and joining parts costs about two
+    // key tiles.
+    const unsigned long long share64 = (total_s * p.Hkv + ws.sms - 1) / ws.sms;
+    const int share = share64 > (1u << 28) ? (1 << 28) : max(kFaMinPart, static_cast<int>(share64));
+    longest = longest_s;
+    int chunk = longest;
+    if (longest > share) {
+        constexpr int N = 6;
+        const int len[N] = {share, share + (share + 7) / 8, share + (share + 3) / 4, share + (share + 1) / 2, 2 * share, longest};
+        int units[N] = {};
+        for (int b = warp; b < p.B; b += warps) {
+            const Seq s = seq_of(b);
+            const int nt = fa_tiles_of(s, tq);
+            for (int i = lane; i < nt; i += 32) {
+                const int keys = max(1, fa_key_tiles(s, (i + 1) * 2 * tq));
+#pragma unroll
+                for (int k = 0; k < N; k++) units[k] += (keys + len[k] - 1) / len[k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int u = __reduce_add_sync(0xffffffffu, units[k]);
+            if (lane == 0 && u) atomicAdd(&count_s[k], u);
+        }
+        __syncthreads();
+        int best = 1 << 30;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int parts = (longest + len[k] - 1) / len[k], unit = (longest + parts - 1) / parts;
+            const int cost = (count_s[k] * p.Hkv <= ws.sms ? unit : max(unit, share + min(unit, shortest_s) / 2)) + (parts > 1 ? 2 : 0);
+            if (cost < best) {
+                best = cost;
+                chunk = len[k];
+            }
+        }
+    }
     auto parts_of = [&](int keys) { return max(1, (keys + chunk - 1) / chunk); };
     auto bucket_of = [&](int k) { return kPlanBuckets - 1 - min(k, kPlanBuckets - 1); };
     // how many units, and of what length
@@ -298,7 +348,7 @@ struct FaGeo {
     static constexpr int RAW_OFF = KV_OFF + STAGES * TILE;
     static constexpr int EXP_OFF = RAW_OFF + RAW * CODES;
     static constexpr int BAR_OFF = EXP_OFF + RAW * kFaTile;
-    static constexpr int TOTAL = BAR_OFF + 320;
+    static constexpr int TOTAL = BAR_OFF + 384;
     // registers: the softmax threads hold a row of scores; the rest give theirs up (the sums equal the launch's)
     static constexpr int THREADS = kFaSoft * 32 + (F8 ? 256 : 128);
     static constexpr int SOFT_REGS = F8 ? 192 : 208;
@@ -308,8 +358,9 @@ struct FaGeo {
 };
 
 struct FaBars {
-    uint64_t q_full[2], q_empty, s_full[2], p_ready[2][kFaParts], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2];
+    uint64_t q_full[2], q_empty, s_full[2], p_ready[2][kFaParts], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2], u_full[2], u_empty[2];
     uint32_t tmem;
+    int unit[2];  // the CTA's current and next unit
 };
 
 // The value of lane 0 in every lane: the compiler then keeps it, and what it makes of it, in uniform
@@ -375,6 +426,7 @@ struct FaWork {
     int b, i0, kvh, kv0, keys;  // keys: tiles of the unit
     int nh[2];                  // tiles that half h multiplies (the first of the unit's)
     int slot;
+    int base;                   // packed rows: the sequence's first
 };
 
 __device__ __forceinline__ FaWork fa_work(const PattnParams& p, const FaWs& ws, int u, int tq) {
@@ -390,6 +442,7 @@ __device__ __forceinline__ FaWork fa_work(const PattnParams& p, const FaWs& ws, 
     w.keys = c.z - c.y;
     w.slot = c.w;
     w.kvh = u % p.Hkv;
+    w.base = p.kv.seq_rows ? w.b * p.kv.seq_rows : w.s.q0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int i = w.i0 + h * tq;
@@ -427,6 +480,8 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             mbar_init(&bar->kv_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
+            mbar_init(&bar->u_full[i], 1);
+            mbar_init(&bar->u_empty[i], kFaSoft + 1 + (F8 ? 4 : 0));
             mbar_init(&bar->raw_full[i], 1);
             mbar_init(&bar->raw_empty[i], 4);
         }
@@ -443,6 +498,16 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
     pdl_wait();
     pdl_launch_dependents();
     const int units = __ldcg(&ws.head->units) * p.Hkv;
+    // The loader deals the CTA its units (the first by its index, then whichever is next) and tells the other warps.
+    Ring<2> feed;
+    auto take = [&](int& u) {
+        if (!fa_wait(&bar->u_full[feed.i], feed.phase, p.err, ERR_FA_WAIT + 12)) return false;
+        u = *static_cast<volatile int*>(&bar->unit[feed.i]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->u_empty[feed.i]);
+        feed.next();
+        return u < units;
+    };
     // the register split stands inside the roles' branches: behind a join the smaller share would bind them all
     if (warp < kFaSoft) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Geo::SOFT_REGS));
@@ -456,7 +521,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         const bool negate = p.scale_log2 < 0.0f;
         const int token_of = row / p.G, head_of = row - token_of * p.G;
         const bool row_in = token_of < tq;
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        for (int u; ok && take(u);) {
             const FaWork w = fa_work(p, ws, u, tq);
             const int token = w.i0 + h * tq + token_of;
             const bool valid = row_in && token < w.s.n;
@@ -597,7 +662,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 const int see = __shfl_sync(0xffffffffu, vis, src);
                 const int j0 = w.kv0 * kFaTile, j1 = min(see, (w.kv0 + w.keys) * kFaTile);
                 float mm, ll, a[D / 32];
-                attend_row<KIND, D>(p, w.b, w.s.q0, w.s.q0 + tk, hd, j0, j1, lane, mm, ll, a);
+                attend_row<KIND, D>(p, w.b, w.base, w.s.q0 + tk, hd, j0, j1, lane, mm, ll, a);
                 if (w.slot < 0) {
                     uint16_t* o = p.out + static_cast<int64_t>(w.s.q0 + tk) * p.out_stride + static_cast<int64_t>(hd) * D + lane * (D / 32);
                     const float iv = see > 0 ? 1.0f / ll : 0.0f;
@@ -633,8 +698,19 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 if (lane < per_tile && at < p.kv.max_pages) id = __ldcg(table + at);
                 return id;
             };
-            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            int next = blockIdx.x;
+            while (ok) {
+                const int u = next;
+                if (!fa_wait(&bar->u_empty[feed.i], feed.phase ^ 1, p.err, ERR_FA_WAIT + 13)) break;
+                if (lane == 0) {
+                    *static_cast<volatile int*>(&bar->unit[feed.i]) = u;
+                    mbar_arrive(&bar->u_full[feed.i]);
+                    if (u < units) next = gridDim.x + atomicAdd(&ws.head->next, 1);
+                }
+                feed.next();
+                if (u >= units) break;
                 const FaWork w = fa_work(p, ws, u, tq);
+                next = __shfl_sync(0xffffffffu, next, 0);
                 if (w.keys == 0) continue;
                 if constexpr (KIND != KV_ROWS) {
                     table = p.kv.table + static_cast<int64_t>(w.b) * p.kv.table_stride;
@@ -655,7 +731,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                             mbar_arrive_expect_tx(full, Geo::TILE);
 #pragma unroll
                             for (int c = 0; c < CH; c++)
-                                tma_load_3d(dst + c * Geo::HALF, map, c * 64, w.kvh, w.s.q0 + tile * kFaTile, full);
+                                tma_load_3d(dst + c * Geo::HALF, map, c * 64, w.kvh, w.base + tile * kFaTile, full);
                         }
                     } else {
                         const int page = 1 << p.kv.page_log2;
@@ -768,7 +844,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 rr.next();
                 r.next();
             };
-            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            for (int u; ok && take(u);) {
                 const FaWork w = fa_work(p, ws, u, tq);
                 if (w.keys == 0) continue;
                 convert(w.s.len - w.kv0 * kFaTile);
@@ -829,7 +905,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 if (elect_one()) tc_commit(b);
                 __syncwarp();
             };
-            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            for (int u; ok && take(u);) {
                 const FaWork w = fa_work(p, ws, u, tq);
                 if (w.keys == 0) continue;
                 if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;

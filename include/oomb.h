@@ -342,10 +342,11 @@ int oomb_kv_read_paged(const oomb_paged_kv* cache, const int32_t* q_start, const
  * what it does not see never reaches its output, infinities and NaN included.
  * max_q bounds the tokens of a sequence (a longer one sets the device error word and is left out).  The workspace
  * holds oomb_attention_paged_workspace_bytes(...) bytes (0: unsupported shape, or no device), enough for every call of at
- * most this batch, t and max_q with these heads; its first OOMB_ATTENTION_ZERO_BYTES are zero before first use
+ * most this batch, t and max_q with these heads and a cache of this shape (for long chunks over an e4m3 cache it holds a bf16
+ * copy of up to batch * max_pages pages, 1 GiB at most); its first OOMB_ATTENTION_ZERO_BYTES are zero before first use
  * (and again after a device error).  Calls that share it must be ordered on one stream. */
 #define OOMB_ATTENTION_ZERO_BYTES 4096
-size_t oomb_attention_paged_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim);
+size_t oomb_attention_paged_workspace_bytes(const oomb_paged_kv* cache, int batch, int t, int max_q, int heads);
 int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_stride, void* out, int64_t out_stride,
                          int heads, const int32_t* q_start, const int32_t* kv_len, int batch, int t, int max_q, float scale,
                          void* workspace, size_t workspace_bytes, oomb_stream stream);

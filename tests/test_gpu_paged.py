@@ -461,7 +461,7 @@ def test_many_sequences(gpu):
 
 
 def test_repeats_give_the_same_bits_on_one_workspace(gpu):
-    ws = gpu.attention_paged_workspace(8, 4000, 1000, 32, 8, 128)
+    ws = gpu.attention_paged_workspace(Batch(80, [0, 1], [4100], 2, 128, 16, False).cache, 8, 4000, 1000, 32)
     for new, cached in (([1] * 4, [4000, 3, 900, 0]), ([100, 3], [3000, 9]), ([600], [0])):
         B, q, out = paged_case(gpu, 81, new, cached, 8, 2, 128, 16, False, workspace=ws, behind=0)
         for _ in range(3):
