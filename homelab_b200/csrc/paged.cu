@@ -234,7 +234,7 @@ int launch_fa(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, cudaS
         st = launch(fa_kernel<KIND, D>, dim3(fw.sms), dim3(FaGeo<KIND, D>::THREADS), FaGeo<KIND, D>::TOTAL, s, p, fw, qm, km, vm);
     // no tile has more keys than a part takes: nothing was split
     const int most = KIND == KV_ROWS && !p.kv.seq_rows ? p.max_q : p.kv_max;
-    if (st == OOMB_OK && most > kFaMinPart * kFaTile) st = launch(join_kernel<KIND, D>, dim3(2 * fw.sms), dim3(256), 0, s, p, fw);
+    if (st == OOMB_OK && most > kFaMinPart * kFaTile) st = launch(join_kernel<KIND, D>, dim3(4 * fw.sms), dim3(256), 0, s, p, fw);
     return st;
 }
 

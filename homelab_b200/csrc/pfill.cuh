@@ -47,8 +47,8 @@ constexpr int kFaRows = 256;       // rows of a tile pair
 constexpr int kFaParts = 2;
 constexpr int kFaSoft = 8;         // softmax warps
 constexpr int kFaMinPart = 4;      // key tiles of a part at least
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanBuckets = 1024;
+constexpr int kPlanThreads = 256;
+constexpr int kPlanBuckets = 512;
 constexpr int kPlanSeqs = 1024;    // sequences whose numbers are kept in shared memory
 
 enum : unsigned {
@@ -148,41 +148,33 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     // longest unit, else (the longest go first) the share and half of the shortest; writing and joining parts costs about two
     // key tiles.
     const unsigned long long share64 = (total_s * p.Hkv + ws.sms - 1) / ws.sms;
-    const int share = share64 > (1u << 28) ? (1 << 28) : max(kFaMinPart, static_cast<int>(share64));
+    const int share = share64 > (1u << 24) ? (1 << 24) : max(kFaMinPart, static_cast<int>(share64));
     longest = longest_s;
     int chunk = longest;
     if (longest > share) {
-        constexpr int N = 6;
-        const int len[N] = {share, share + (share + 7) / 8, share + (share + 3) / 4, share + (share + 1) / 2, 2 * share, longest};
-        int units[N] = {};
+        // lane k tries the k-th length: 1, 1 1/8, 1 1/4, 1 1/2, 2 shares, a whole tile
+        const int eighths = lane == 0 ? 8 : lane == 1 ? 9 : lane == 2 ? 10 : lane == 3 ? 12 : 16;
+        const int len = lane < 5 ? (share * eighths + 7) / 8 : longest;
+        int units = 0;
         for (int b = warp; b < p.B; b += warps) {
             const Seq s = seq_of(b);
             const int nt = fa_tiles_of(s, tq);
-            for (int i = lane; i < nt; i += 32) {
-                const int keys = max(1, fa_key_tiles(s, (i + 1) * 2 * tq));
-#pragma unroll
-                for (int k = 0; k < N; k++) units[k] += (keys + len[k] - 1) / len[k];
-            }
+#pragma unroll 1
+            for (int i = 0; i < nt; i++) units += (max(1, fa_key_tiles(s, (i + 1) * 2 * tq)) + len - 1) / len;
         }
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-            const int u = __reduce_add_sync(0xffffffffu, units[k]);
-            if (lane == 0 && u) atomicAdd(&count_s[k], u);
-        }
+        if (lane < 6 && units) atomicAdd(&count_s[lane], units);
         __syncthreads();
-        int best = 1 << 30;
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-            const int parts = (longest + len[k] - 1) / len[k], unit = (longest + parts - 1) / parts;
-            const int cost = (count_s[k] * p.Hkv <= ws.sms ? unit : max(unit, share + min(unit, shortest_s) / 2)) + (parts > 1 ? 2 : 0);
-            if (cost < best) {
-                best = cost;
-                chunk = len[k];
-            }
-        }
+        const int parts = (longest + len - 1) / len, unit = (longest + parts - 1) / parts;
+        const int cost = (count_s[min(lane, 5)] * p.Hkv <= ws.sms ? unit : max(unit, share + min(unit, shortest_s) / 2)) + (parts > 1 ? 2 : 0);
+        const int best = __reduce_min_sync(0xffffffffu, lane < 6 ? cost : 1 << 30);
+        chunk = __shfl_sync(0xffffffffu, len, __ffs(__ballot_sync(0xffffffffu, lane < 6 && cost == best)) - 1);
     }
     auto parts_of = [&](int keys) { return max(1, (keys + chunk - 1) / chunk); };
-    auto bucket_of = [&](int k) { return kPlanBuckets - 1 - min(k, kPlanBuckets - 1); };
+    // lengths up to 128 apart, longer ones to a sixteenth
+    auto bucket_of = [&](int k) {
+        const int e = 31 - __clz(max(k, 1));
+        return kPlanBuckets - 1 - (k < 128 ? k : min(128 + (e - 7) * 16 + ((k >> (e - 4)) & 15), kPlanBuckets - 1));
+    };
     // how many units, and of what length
     int mine = 0;
     for (int b = warp; b < p.B; b += warps) {
@@ -211,7 +203,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     }
     const bool sorted = units * p.Hkv > ws.sms;
     if (sorted) {  // where each length's units begin, the longest first
-        const int v = hist[tid];
+        static_assert(kPlanBuckets == 2 * kPlanThreads, "two buckets a thread");
+        const int v0 = hist[2 * tid], v = v0 + hist[2 * tid + 1];
         int inc = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -222,7 +215,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         __syncthreads();
         int before = 0;
         for (int w = 0; w < warp; w++) before += warp_sum[w];
-        hist[tid] = before + inc - v;
+        hist[2 * tid] = before + inc - v;
+        hist[2 * tid + 1] = before + inc - v + v0;
     } else if (tid == 0) {
         hist[0] = 0;
     }
@@ -348,7 +342,7 @@ struct FaGeo {
     static constexpr int RAW_OFF = KV_OFF + STAGES * TILE;
     static constexpr int EXP_OFF = RAW_OFF + RAW * CODES;
     static constexpr int BAR_OFF = EXP_OFF + RAW * kFaTile;
-    static constexpr int TOTAL = BAR_OFF + 384;
+    static constexpr int TOTAL = BAR_OFF + 448;
     // registers: the softmax threads hold a row of scores; the rest give theirs up (the sums equal the launch's)
     static constexpr int THREADS = kFaSoft * 32 + (F8 ? 256 : 128);
     static constexpr int SOFT_REGS = F8 ? 192 : 208;
@@ -360,7 +354,8 @@ struct FaGeo {
 struct FaBars {
     uint64_t q_full[2], q_empty, s_full[2], p_ready[2][kFaParts], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2], u_full[2], u_empty[2];
     uint32_t tmem;
-    int unit[2];  // the CTA's current and next unit
+    int kvh[2];  // the CTA's current and next unit: kv head (-1: no more), and the rest
+    __align__(16) FaUnit unit[2];
 };
 
 // The value of lane 0 in every lane: the compiler then keeps it, and what it makes of it, in uniform
@@ -429,19 +424,15 @@ struct FaWork {
     int base;                   // packed rows: the sequence's first
 };
 
-__device__ __forceinline__ FaWork fa_work(const PattnParams& p, const FaWs& ws, int u, int tq) {
+__device__ __forceinline__ FaWork fa_work(const PattnParams& p, const FaUnit& u, int kvh, int tq) {
     FaWork w;
-    const int4* at = reinterpret_cast<const int4*>(ws.units + u / p.Hkv);
-    const int4 a = __ldcg(at), c = __ldcg(at + 1);
-    w.s.q0 = a.x;
-    w.s.n = a.y;
-    w.s.len = a.z;
-    w.b = a.w;
-    w.i0 = c.x;
-    w.kv0 = c.y;
-    w.keys = c.z - c.y;
-    w.slot = c.w;
-    w.kvh = u % p.Hkv;
+    w.s = u.s;
+    w.b = u.b;
+    w.i0 = u.i0;
+    w.kv0 = u.kv0;
+    w.keys = u.kv1 - u.kv0;
+    w.slot = u.slot;
+    w.kvh = kvh;
     w.base = p.kv.seq_rows ? w.b * p.kv.seq_rows : w.s.q0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -497,16 +488,16 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
     const uint32_t tmem = bar->tmem;
     pdl_wait();
     pdl_launch_dependents();
-    const int units = __ldcg(&ws.head->units) * p.Hkv;
     // The loader deals the CTA its units (the first by its index, then whichever is next) and tells the other warps.
     Ring<2> feed;
-    auto take = [&](int& u) {
+    auto take = [&](FaWork& w) {
         if (!fa_wait(&bar->u_full[feed.i], feed.phase, p.err, ERR_FA_WAIT + 12)) return false;
-        u = *static_cast<volatile int*>(&bar->unit[feed.i]);
+        const int kvh = *static_cast<volatile int*>(&bar->kvh[feed.i]);
+        if (kvh >= 0) w = fa_work(p, bar->unit[feed.i], kvh, tq);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar->u_empty[feed.i]);
         feed.next();
-        return u < units;
+        return kvh >= 0;
     };
     // the register split stands inside the roles' branches: behind a join the smaller share would bind them all
     if (warp < kFaSoft) {
@@ -521,8 +512,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         const bool negate = p.scale_log2 < 0.0f;
         const int token_of = row / p.G, head_of = row - token_of * p.G;
         const bool row_in = token_of < tq;
-        for (int u; ok && take(u);) {
-            const FaWork w = fa_work(p, ws, u, tq);
+        for (FaWork w; ok && take(w);) {
             const int token = w.i0 + h * tq + token_of;
             const bool valid = row_in && token < w.s.n;
             const int vis = valid ? max(0, min(w.s.len, w.s.len - w.s.n + token + 1)) : 0;
@@ -698,19 +688,26 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 if (lane < per_tile && at < p.kv.max_pages) id = __ldcg(table + at);
                 return id;
             };
+            // the next unit's record is fetched while the current one is loaded
+            auto record = [&](int u) {  // lanes 0 and 1: its two halves
+                return lane < 2 && u / p.Hkv < ws.max_units ? __ldcg(reinterpret_cast<const int4*>(ws.units + u / p.Hkv) + lane) : make_int4(0, 0, 0, 0);
+            };
             int next = blockIdx.x;
+            int4 rec = record(next);
+            const int units = __ldcg(&ws.head->units) * p.Hkv;
             while (ok) {
                 const int u = next;
                 if (!fa_wait(&bar->u_empty[feed.i], feed.phase ^ 1, p.err, ERR_FA_WAIT + 13)) break;
-                if (lane == 0) {
-                    *static_cast<volatile int*>(&bar->unit[feed.i]) = u;
-                    mbar_arrive(&bar->u_full[feed.i]);
-                    if (u < units) next = gridDim.x + atomicAdd(&ws.head->next, 1);
-                }
+                if (lane < 2) reinterpret_cast<int4*>(&bar->unit[feed.i])[lane] = rec;
+                if (lane == 0) bar->kvh[feed.i] = u < units ? u % p.Hkv : -1;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->u_full[feed.i]);
+                const FaWork w = fa_work(p, bar->unit[feed.i], u % p.Hkv, tq);
                 feed.next();
                 if (u >= units) break;
-                const FaWork w = fa_work(p, ws, u, tq);
+                if (lane == 0) next = gridDim.x + atomicAdd(&ws.head->next, 1);
                 next = __shfl_sync(0xffffffffu, next, 0);
+                rec = record(next);
                 if (w.keys == 0) continue;
                 if constexpr (KIND != KV_ROWS) {
                     table = p.kv.table + static_cast<int64_t>(w.b) * p.kv.table_stride;
@@ -844,8 +841,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 rr.next();
                 r.next();
             };
-            for (int u; ok && take(u);) {
-                const FaWork w = fa_work(p, ws, u, tq);
+            for (FaWork w; ok && take(w);) {
                 if (w.keys == 0) continue;
                 convert(w.s.len - w.kv0 * kFaTile);
                 for (int i = 0; i < w.keys && ok; i++) {
@@ -905,8 +901,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 if (elect_one()) tc_commit(b);
                 __syncwarp();
             };
-            for (int u; ok && take(u);) {
-                const FaWork w = fa_work(p, ws, u, tq);
+            for (FaWork w; ok && take(w);) {
                 if (w.keys == 0) continue;
                 if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
 #pragma unroll
