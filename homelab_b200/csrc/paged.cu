@@ -103,7 +103,7 @@ float rotated_limit(float mscale) {
 // rows a kv head) the plan's head, its units and split tiles, partial outputs.  The bytes cover every call of at
 // most this batch, t and max_q.
 struct AttnWs {
-    bool few;  // up to kDecRows query rows a kv head: decode_rows_kernel
+    bool few;  // few query rows a kv head: decode_rows_kernel
     int grid;  // of the decode kernel
     size_t part_off;  // few
     size_t head_off, unit_off, split_off, fa_part_off;
@@ -125,7 +125,8 @@ AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int
     const bool paged = cache != nullptr;
     const int G = heads / kv_heads;
     const int64_t rows = static_cast<int64_t>(max_q) * G;
-    w.few = paged && rows <= kDecRows;
+    const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * ((rows + kDecRows - 1) / kDecRows);
+    w.few = paged && (rows <= kDecRowsAlways || (rows <= kDecRowsFew && pairs <= d->sms));
     w.grid = kDecCtas * d->sms;
     if (w.grid > OOMB_ATTENTION_ZERO_BYTES / 4) w.grid = OOMB_ATTENTION_ZERO_BYTES / 4;
     // the counters keep their place, and nothing else comes there, whatever the calls that share a workspace
@@ -243,12 +244,12 @@ int launch_decode(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream
     DecodeWs dw{};
     dw.counters = reinterpret_cast<unsigned*>(ws);
     dw.part = reinterpret_cast<float*>(ws + w.part_off);
-    dw.rows = p.max_q * p.G;
+    dw.rows = p.max_q * p.G < kDecRows ? p.max_q * p.G : kDecRows;
     CUtensorMap km, vm;
     if (!encode_pool(&km, p.kv.k, p.kv, D, KIND == KV_E4M3, true) || !encode_pool(&vm, p.kv.v, p.kv, D, KIND == KV_E4M3, true))
         return OOMB_E_LAUNCH;
     // never more CTAs than there can be blocks, which the kernel counts in 32 bits
-    const int64_t most = static_cast<int64_t>(p.B) * p.Hkv * (p.kv_max / kDecBlock + 1);
+    const int64_t most = static_cast<int64_t>(p.B) * p.Hkv * (p.kv_max / kDecBlock + 1) * ((p.max_q * p.G + kDecRows - 1) / kDecRows);
     if (most > (1 << 30)) return OOMB_E_SHAPE;
     const int grid = most < w.grid ? static_cast<int>(most) : w.grid;
     return launch(decode_rows_kernel<KIND, D, R>, dim3(grid), dim3(kDecThreads), DecodeGeo<KIND, D, R>::TOTAL, s, p, dw, km, vm);

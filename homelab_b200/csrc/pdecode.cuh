@@ -1,5 +1,5 @@
 // pdecode.cuh - attention of a few query rows per kv head over a paged cache: decode
-// steps and short drafts, up to 16 rows (new tokens x query heads of a kv head).
+// steps and short drafts, in groups of up to 16 rows (new tokens x query heads of a kv head).
 //
 // Bound: HBM; every key and value byte is read once and used for all rows at once.  The
 // positions, not the rows, fill the 128 rows of the tensor cores' tile:
@@ -10,19 +10,19 @@
 // HBM rate, and one thread per position has all rows' scores: its maximum over the
 // positions is needed only when a score passes the running one, which one barrier with
 // an "or" finds out.  A first version on warp-level matrix instructions with the rows as
-// M = 16 spent 437 instructions per 16 positions and head, and took 228 us where this takes 101
+// M = 16 spent 437 instructions per 16 positions and head, and took 228 us where this takes 102
 // (32 sequences of 1,001 to 16,098 positions, 32 heads over 8, e4m3 pages).
 //
-// e4m3 codes are multiplied as they are.  A row of queries, scaled by a power of two into
-// [128, 256), is two e4m3 rows q1 = rn(q), q2 = rn(q - q1): a bf16 value's eight bits, exact
-// down to 2^-9 of the scaled row (beyond, off by 2^-10 of it, 2^-18 of the row's largest).  A weight
+// e4m3 codes are multiplied as they are.  A row of queries, scaled by a power of two so that its largest value lies
+// in [128, 256), is two e4m3 rows q1 = rn(q), q2 = rn(q - q1), which hold a bf16 value's eight bits down to
+// 2^-9 of 256 (smaller values are off by 2^-10 at most, 2^-17 of the row's largest).  A weight
 // w = 2^(x - m + 11) 2^(e - X), e its value row's exponent and X the largest met, is three e5m2 rows of
-// three bits each: off by at most 2^-9 of itself, or by 2^-28 of 2^-... of the largest: e5m2 reaches
-// from 2^15 down to 2^-16.
+// three significant bits each: off by at most 2^-9 of itself, down to 2^-16, which is 2^-27 of the
+// weight that m stands for.
 //
-// Work split: the batch's positions are cut into blocks of 128 (per sequence and kv head)
-// and the blocks, laid end to end, evenly over the CTAs, whatever the lengths;
-// a (sequence, kv head) spread over several CTAs is joined by the last of them
+// Work split: the batch's positions are cut into blocks of 128 for each (sequence, kv head, group of
+// 16 rows), a "pair" below, and the blocks, laid end to end, dealt evenly to the CTAs, whatever the
+// lengths; a pair spread over several CTAs is joined by the last of them
 // to finish, in order, so a call's bits do not depend on timing.
 //
 // Warps: 0-3 softmax, one thread per position of a tile and then per output dimension; 4
@@ -39,9 +39,16 @@ constexpr int kDecThreads = kDecSoft + 64;
 constexpr int kDecBlock = 128;              // positions of a work block: one tile
 constexpr int kDecRows = 16;
 constexpr int kDecCtas = 2;                 // CTAs of an SM
-// Parts of a (sequence, kv head), on average, at most: one sequence of 4096 positions over 8 kv heads takes 14.2 us with 8,
-// 11.8 with 16 (one trip to L2 joins them), 12.4 with 32 or more.
-constexpr int kDecParts = 16;
+// Rows up to which a call comes here rather than to the 128-row tiles of prefill: two groups always, four while the pairs
+// are no more than the SMs.  Over pages of 8 kv heads, here and there, in us: 32 rows 19 / 21 (one sequence of 2,000
+// positions), 29 / 36 (one of 16,000), 38 / 50 (eight of 4,000) in bf16, 21 / 28, 29 / 43, 39 / 68 in e4m3; 64 rows 19 / 22,
+// 34 / 37, 63 / 52 and 20 / 29, 36 / 43, 73 / 70; 128 rows 20 / 23, 51 / 38, 116 / 56.
+constexpr int kDecRowsAlways = 32, kDecRowsFew = 64;
+
+// Parts of a pair that one trip to L2 joins, and the blocks of a run that make more of them worth it: one sequence of 4,096
+// bf16 positions over 8 kv heads takes 14.2 us in 8 parts, 11.8 in 16, 12.4 in 32; one of 16,000 takes 20.1 us in the 16
+// that runs of 8 blocks make, 20.6 in 21 and 22.3 in 31; one of 60,000 48 us in the 37 that fill the SMs.
+constexpr int kDecParts = 16, kDecRun = 8;
 
 enum : unsigned {
     ERR_DEC_WAIT = 0xb00,  // a decode pipeline wait ran out (+ the waiting role)
@@ -87,19 +94,18 @@ struct DecodeBars {
     float red[4][kDecRows];
     int redx[4];
     unsigned last;
-    int4 start;               // the CTA's first sequence, its first block, its blocks
+    int4 start;               // the CTA's first sequence, its first block, the blocks of its pairs, its groups
     Seq start_seq;
     int2 sum[kDecThreads / 32];
 };
 
-// Blocks dealt to CTAs in order: the first `more` of them get `each` + 1, the others `each`.
+// W blocks dealt to S CTAs in proportion: CTA c begins at W c / S, so that with as many CTAs for each of equally long pairs
+// none has parts of two.
 struct DecodeDeal {
-    int each, more;
-    __device__ int lo(int c) const { return c * each + min(c, more); }
-    __device__ int owner(int block) const {
-        const int cut = more * (each + 1);
-        return block < cut ? block / (each + 1) : more + (block - cut) / each;
-    }
+    unsigned W, S;
+    __device__ int lo(int c) const { return static_cast<int>(static_cast<unsigned long long>(W) * c / S); }
+    // the last CTA that begins at or before the block
+    __device__ int owner(int block) const { return static_cast<int>(((block + 1ull) * S - 1) / W); }
 };
 
 // Descriptors' high words: 128-byte rows in the 128-byte swizzle (8-row groups 1024 bytes apart), or 64-byte rows in the
@@ -160,10 +166,17 @@ __device__ __forceinline__ unsigned split_e4m3(float& lo, float& hi) {
     return c;
 }
 
-// A run of blocks of one (sequence, kv head).
+// A sequence's rows of a kv head go in groups of kDecRows, each with the blocks of its own: a "pair" below is one
+// (sequence, kv head, group).
+__device__ __forceinline__ int dec_groups(const Seq& s, int G) { return (s.n * G + kDecRows - 1) / kDecRows; }
+__device__ __forceinline__ int dec_blocks(const Seq& s, int max_q) {
+    return s.n == 0 || s.n > max_q ? 0 : max(1, (s.len + kDecBlock - 1) / kDecBlock);  // without positions, still its zeros
+}
+
+// A run of blocks of one pair.
 struct DecodeSeg {
     Seq sq;
-    int b, kvh, tok0, tok1, tiles;
+    int b, kvh, row0, rows, tok0, tok1, tiles;
     int pair_first, pair_end, lo;
 };
 
@@ -173,19 +186,23 @@ struct DecodeWalk {
     int lo, hi;      // this CTA's blocks yet to come
     int b, b_first;  // a sequence and its first block
     Seq sq;
-    int nb;          // its blocks of one kv head
+    int nb, groups;  // its blocks of a pair, its groups
     __device__ bool next(const PattnParams& p, DecodeSeg& g) {
         if (lo >= hi) return false;
-        while (lo >= b_first + nb * p.Hkv) {
-            b_first += nb * p.Hkv;
+        while (lo >= b_first + nb * groups * p.Hkv) {
+            b_first += nb * groups * p.Hkv;
             b++;
             sq = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, nullptr);
-            nb = sq.n == 0 || sq.n > p.max_q ? 0 : max(1, (sq.len + kDecBlock - 1) / kDecBlock);
+            nb = dec_blocks(sq, p.max_q);
+            groups = dec_groups(sq, p.G);
         }
+        const int pair = (lo - b_first) / nb;
         g.sq = sq;
         g.b = b;
-        g.kvh = (lo - b_first) / nb;
-        g.pair_first = b_first + g.kvh * nb;
+        g.kvh = pair / groups;
+        g.row0 = (pair - g.kvh * groups) * kDecRows;
+        g.rows = min(kDecRows, sq.n * p.G - g.row0);
+        g.pair_first = b_first + pair * nb;
         g.pair_end = g.pair_first + nb;
         g.lo = lo;
         const int end = min(g.pair_end, hi);
@@ -242,17 +259,19 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
     DecodeWalk walk{};
     {
         Seq seen{};
+        int pairs_of = 0;  // a sequence's pairs
         auto blocks_of = [&](int b) {
+            pairs_of = 0;
             if (b >= p.B) return 0;
             seen = read_seq(p.q_start, p.kv_len, b, p.T, p.kv_max, p.err);
             if (seen.n > p.max_q) record_error(p.err, ERR_KV_SEQ);
-            if (seen.n == 0 || seen.n > p.max_q) return 0;
-            return max(1, (seen.len + kDecBlock - 1) / kDecBlock);  // a sequence without positions still gets its zeros
+            pairs_of = dec_groups(seen, p.G) * p.Hkv;
+            return dec_blocks(seen, p.max_q) * pairs_of;
         };
         int total = 0, pairs = 0, mine = 0;
         for (int b0 = 0; b0 < p.B; b0 += kDecThreads) {
             mine = blocks_of(b0 + tid);
-            const int v = __reduce_add_sync(0xffffffffu, mine), n = __popc(__ballot_sync(0xffffffffu, mine > 0));
+            const int v = __reduce_add_sync(0xffffffffu, mine), n = __reduce_add_sync(0xffffffffu, mine > 0 ? pairs_of : 0);
             if (lane == 0) bar->sum[warp] = make_int2(v, n);
             __syncthreads();
 #pragma unroll
@@ -262,11 +281,16 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
             }
             __syncthreads();
         }
-        const int W = total * p.Hkv;  // fits: checked by the caller for the longest sequences
-        const int S = min(min(W, static_cast<int>(gridDim.x)), max(1, pairs * p.Hkv * kDecParts));
+        // As many CTAs as blocks, or as are resident.  Few pairs: equally many CTAs each, at least kDecParts, and more only for
+        // kDecRun blocks a CTA or more (the end and the beginning of a run cost as much as three or four blocks, and a
+        // launch that leaves room lets the next begin beside it).
+        const int W = total, grid = gridDim.x;  // fits: checked by the caller for the longest sequences
+        int S = min(W, grid);
+        if (pairs > 0 && 2 * pairs <= grid)
+            S = min(S, pairs * min(grid / pairs, max(kDecParts, W / (pairs * kDecRun))));
         if (static_cast<int>(blockIdx.x) < S) {
-            walk.deal.each = W / S;
-            walk.deal.more = W - walk.deal.each * S;
+            walk.deal.W = W;
+            walk.deal.S = S;
             walk.lo = walk.deal.lo(blockIdx.x);
             walk.hi = walk.deal.lo(blockIdx.x + 1);
             int prefix = 0;
@@ -282,8 +306,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 __syncthreads();
                 int end = prefix + inc;
                 for (int w = 0; w < warp; w++) end += bar->sum[w].x;
-                if (mine > 0 && (end - mine) * p.Hkv <= walk.lo && walk.lo < end * p.Hkv) {
-                    bar->start = make_int4(b0 + tid, (end - mine) * p.Hkv, mine, 0);
+                if (mine > 0 && end - mine <= walk.lo && walk.lo < end) {
+                    bar->start = make_int4(b0 + tid, end - mine, mine / pairs_of, pairs_of / p.Hkv);
                     bar->start_seq = seen;
                 }
 #pragma unroll
@@ -293,6 +317,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
             walk.b = bar->start.x;
             walk.b_first = bar->start.y;
             walk.nb = bar->start.z;
+            walk.groups = bar->start.w;
             walk.sq = bar->start_seq;
         }
     }
@@ -472,7 +497,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         auto dead = [&]() { return *static_cast<volatile int*>(&bar->dead) != 0; };
         while (!stop && walk.next(p, g)) {
             const Seq sq = g.sq;
-            const int rows = sq.n * p.G;
+            const int rows = g.rows, row0 = g.row0;
             float m[R], l[R], scale[R];
             int vis[R];
 #pragma unroll
@@ -480,7 +505,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 m[r] = -INFINITY;
                 l[r] = 0.0f;
                 scale[r] = p.scale_log2;
-                vis[r] = r < rows ? max(0, min(sq.len, sq.len - sq.n + r / p.G + 1)) : 0;
+                vis[r] = r < rows ? max(0, min(sq.len, sq.len - sq.n + (row0 + r) / p.G + 1)) : 0;
             }
             int X = 0;  // e4m3: the exponent byte that the outputs are counted in
             if (g.tiles > 0) {
@@ -490,8 +515,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         const int r = o / (D / 8), c = o % (D / 8);
                         uint4 x = make_uint4(0u, 0u, 0u, 0u);
                         if (r < rows)
-                            x = __ldcg(reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(sq.q0 + r / p.G) * p.q_stride +
-                                                                      static_cast<int64_t>(g.kvh * p.G + r % p.G) * D + c * 8));
+                            x = __ldcg(reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(sq.q0 + (row0 + r) / p.G) * p.q_stride +
+                                                                      static_cast<int64_t>(g.kvh * p.G + (row0 + r) % p.G) * D + c * 8));
                         *reinterpret_cast<uint4*>(smem + Geo::Q_OFF + (c / 8) * Geo::NQ * 128 + dec_swizzle(128, r, c % 8)) = x;
                     }
                 } else {
@@ -502,8 +527,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         float f[V];
                         float big = 0.0f;
                         const bool in = r < rows;
-                        const uint16_t* q = p.q + static_cast<int64_t>(sq.q0 + (in ? r / p.G : 0)) * p.q_stride +
-                                            static_cast<int64_t>(g.kvh * p.G + (in ? r % p.G : 0)) * D + c * V;
+                        const uint16_t* q = p.q + static_cast<int64_t>(sq.q0 + (in ? (row0 + r) / p.G : 0)) * p.q_stride +
+                                            static_cast<int64_t>(g.kvh * p.G + (in ? (row0 + r) % p.G : 0)) * D + c * V;
 #pragma unroll
                         for (int i = 0; i < V; i += 8) {
                             const uint4 x = in ? __ldcg(reinterpret_cast<const uint4*>(q + i)) : make_uint4(0u, 0u, 0u, 0u);
@@ -579,9 +604,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     // the tile's maxima over its positions, and the outputs so far brought to them
 #pragma unroll
                     for (int r = 0; r < R; r++) {
-                        float x = s[r];
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                        float x;
+                        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(x) : "f"(s[r]));
                         if (lane == 0) bar->red[warp][r] = x;
                     }
                     if constexpr (F8) {
@@ -663,13 +687,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 for (int c = 0; c < Geo::NP; c++) o[c] = 0.0f;
             }
             meet(false);  // the last maxima are read
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                float x = l[r];
-#pragma unroll
-                for (int k = 16; k > 0; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
-                if (lane == 0) bar->red[warp][r] = x;
-            }
+            warp_reduce_multi<R>(l, lane);  // the lane's l[0] is the warp's sum of row reduce_index
+            bar->red[warp][reduce_index<R>(lane, 0)] = l[0];
             meet(false);
             if (dead()) break;
             const float unit = F8 ? exp_byte(static_cast<unsigned>(X)) : 1.0f;
@@ -688,8 +707,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     odd |= tid < D && !(fabsf(x) <= 3.4e38f);
                     const __nv_bfloat16 v = __float2bfloat16_rn(x);
                     if (tid < D)
-                        *reinterpret_cast<__nv_bfloat16*>(p.out + static_cast<int64_t>(sq.q0 + r / p.G) * p.out_stride +
-                                                          static_cast<int64_t>(g.kvh * p.G + r % p.G) * D + tid) = v;
+                        *reinterpret_cast<__nv_bfloat16*>(p.out + static_cast<int64_t>(sq.q0 + (row0 + r) / p.G) * p.out_stride +
+                                                          static_cast<int64_t>(g.kvh * p.G + (row0 + r) % p.G) * D + tid) = v;
                 } else {
                     if (tid < D) my_part[r * PAD + tid] = x;
                     if (tid == 0) *reinterpret_cast<float2*>(my_part + r * PAD + D) = make_float2(m[r], ls);
@@ -712,7 +731,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         return ws.part + static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * ws.rows * PAD;
                     };
                     for (int q = tid; q < rows * (D / 4); q += kDecSoft) {
-                        const int r = q / (D / 4), d = (q % (D / 4)) * 4, token = r / p.G;
+                        const int r = q / (D / 4), d = (q % (D / 4)) * 4, token = (row0 + r) / p.G;
                         // sixteen parts' loads under way at once: a pass over them is a few trips to L2
                         float M = -INFINITY, ls = 0.0f;
                         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -746,7 +765,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         a = sees ? make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         odd |= !(fabsf(a.x) + fabsf(a.y) + fabsf(a.z) + fabsf(a.w) <= 3.4e38f);
                         *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(sq.q0 + token) * p.out_stride +
-                                                  static_cast<int64_t>(g.kvh * p.G + r - token * p.G) * D + d) =
+                                                  static_cast<int64_t>(g.kvh * p.G + row0 + r - token * p.G) * D + d) =
                             make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
                     }
                 }
@@ -755,7 +774,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
             // and e5m2 terms have no infinity): then every row is done again in plain loops over what it sees.
             if (meet(odd)) {
                 for (int r = warp; r < rows; r += 4) {
-                    const int token = r / p.G, head = g.kvh * p.G + r - token * p.G;
+                    const int token = (row0 + r) / p.G, head = g.kvh * p.G + row0 + r - token * p.G;
                     const int see = max(0, min(sq.len, sq.len - sq.n + token + 1));
                     float mm, ll, a[D / 32];
                     attend_row<KIND, D>(p, g.b, sq.q0, sq.q0 + token, head, 0, see, lane, mm, ll, a);
