@@ -306,7 +306,7 @@ bool attn_shape_ok(int batch, int t, int max_q, int heads, int kv_heads, int hea
 int check_attn(const void* q, int64_t q_stride, const void* out, int64_t out_stride, int heads, int kv_heads, int head_dim,
                int batch, int t, int max_q, float scale) {
     if (!q || !out) return OOMB_E_ARG;
-    if (!isfinite(scale)) return OOMB_E_ARG;
+    if (!(fabsf(scale) <= 1e37f)) return OOMB_E_ARG;  // its product with log2(e) is an fp32 number
     if (!attn_shape_ok(batch, t, max_q, heads, kv_heads, head_dim)) return OOMB_E_SHAPE;
     const int64_t row = static_cast<int64_t>(heads) * head_dim;
     const int st = check_rows(q, q_stride, row, OOMB_BF16);

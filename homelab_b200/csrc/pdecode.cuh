@@ -90,7 +90,6 @@ struct DecodeWs {
 struct DecodeBars {
     uint64_t kv_full[8], kv_empty[8], s_full[2], p_ready[2], p_free[2], q_ready, e_full[8];
     uint32_t tmem;
-    int dead;                 // a softmax thread's wait ran out
     float red[4][kDecRows];
     int redx[4];
     unsigned last;
@@ -241,7 +240,6 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         }
         for (int i = 0; i < Geo::EXPS; i++) mbar_init(&bar->e_full[i], 1);
         mbar_init(&bar->q_ready, 4);
-        bar->dead = 0;
         fence_barrier_init();
     }
     if (warp == 4) {
@@ -490,11 +488,11 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                          : "memory");
             return x != 0;
         };
-        // a wait that ran out is told to all at the next meeting: none leaves the loop alone
+        // A thread whose wait ran out goes on to the next meeting, where all learn of it: none leaves the others waiting there.
+        bool gone = false;
         auto wait = [&](uint64_t* b, unsigned ph, int role) {
-            if (!fa_wait(b, ph, p.err, ERR_DEC_WAIT + role)) *static_cast<volatile int*>(&bar->dead) = 1;
+            if (!fa_wait(b, ph, p.err, ERR_DEC_WAIT + role)) gone = true;
         };
-        auto dead = [&]() { return *static_cast<volatile int*>(&bar->dead) != 0; };
         while (!stop && walk.next(p, g)) {
             const Seq sq = g.sq;
             const int rows = g.rows, row0 = g.row0;
@@ -595,12 +593,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     s[r] = x;
                     over |= x > m[r] + kSlack || (m[r] == -INFINITY && x != -INFINITY);
                 }
-                const bool update = meet(over);
-                if (dead()) {
-                    stop = true;
-                    break;
-                }
-                if (update) {
+                if (meet(over || gone)) {
                     // the tile's maxima over its positions, and the outputs so far brought to them
 #pragma unroll
                     for (int r = 0; r < R; r++) {
@@ -613,8 +606,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         if (lane == 0) bar->redx[warp] = x;
                     }
                     if (i > 0) wait(&bar->p_free[(t - 1) & 1], ((t - 1) >> 1) & 1, 8);  // the outputs are at rest
-                    meet(false);
-                    if (dead()) {
+                    if (meet(gone)) {
                         stop = true;
                         break;
                     }
@@ -686,11 +678,10 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
 #pragma unroll
                 for (int c = 0; c < Geo::NP; c++) o[c] = 0.0f;
             }
-            meet(false);  // the last maxima are read
+            if (meet(gone)) break;  // and the last maxima are read
             warp_reduce_multi<R>(l, lane);  // the lane's l[0] is the warp's sum of row reduce_index
             bar->red[warp][reduce_index<R>(lane, 0)] = l[0];
             meet(false);
-            if (dead()) break;
             const float unit = F8 ? exp_byte(static_cast<unsigned>(X)) : 1.0f;
             const int first = walk.deal.owner(g.pair_first), final_cta = walk.deal.owner(g.pair_end - 1);
             const int parts = final_cta - first + 1;
@@ -770,9 +761,9 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     }
                 }
             }
-            // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the products (and e4m3
-            // and e5m2 terms have no infinity): then every row is done again in plain loops over what it sees.
-            if (meet(odd)) {
+            // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the products: then every
+            // row is done again in plain loops over what it sees.  (A single new token sees everything.)
+            if (meet(odd) && sq.n > 1) {
                 for (int r = warp; r < rows; r += 4) {
                     const int token = (row0 + r) / p.G, head = g.kvh * p.G + row0 + r - token * p.G;
                     const int see = max(0, min(sq.len, sq.len - sq.n + token + 1));

@@ -376,7 +376,7 @@ def test_scales(gpu, fp8, scale):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-@pytest.mark.parametrize("new", [[3], [1], [70]])
+@pytest.mark.parametrize("new", [[3], [1], [13], [70], [200]])
 def test_values_behind_the_mask_never_reach_a_row(gpu, fp8, new):
     """NaN keys and infinite values at a later new token: earlier rows are finite and right, later ones follow the
     arithmetic (NaN)."""
@@ -505,6 +505,136 @@ def test_attention_refuses(gpu):
         gpu.attention_paged(q[:, :7], B.cache, out[:, :7], B.q_start, B.kv_len, 1, 0.1)
 
 
+def attend_on_gpu(q, k, v, n_before, scale):
+    """R.attend for larger cases: float64 matrices on the GPU, a head at a time."""
+    n, H, D = q.shape
+    L, K, _ = k.shape
+    q, k, v = (x.to(DEV).double() for x in (q, k, v))
+    later = torch.arange(L, device=DEV)[None] > torch.arange(n_before, n_before + n, device=DEV)[:, None]
+    out, mag, big = (torch.empty(n, H, d, dtype=torch.float64, device=DEV) for d in (D, D, 1))
+    for h in range(H):
+        kk, vv = k[:, h // (H // K)], v[:, h // (H // K)]
+        p = (q[:, h] @ kk.T * scale).masked_fill(later, float("-inf")).softmax(-1)
+        out[:, h], mag[:, h] = p @ vv, p @ vv.abs()
+        big[:, h, 0] = (q[:, h].abs() @ kk.abs().T).masked_fill(later, 0.0).amax(-1) * abs(scale)
+    return out.cpu(), mag.cpu(), big.cpu()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new,cached,H,K,D,page", [
+    ([40], [20001], 8, 2, 128, 64),              # a long cache split over the SMs
+    ([700, 33], [5000, 2500], 8, 2, 128, 32),    # chunks of several tiles beside a short one
+    ([3, 1, 2], [15000, 60, 9000], 16, 1, 64, 16),
+    ([1500], [0], 4, 1, 64, 128),
+])
+def test_larger_chunks(gpu, fp8, new, cached, H, K, D, page):
+    q_start = [0]
+    for n in new:
+        q_start.append(q_start[-1] + n)
+    B = Batch(300 + sum(new), q_start, [a + n for a, n in zip(cached, new)], K, D, page, fp8)
+    vals = B.values()
+    B.poison_unused()
+    q = normal(301, q_start[-1], H, D, scale=1.3).to(torch.bfloat16)
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=DEV)
+    gpu.attention_paged(q.to(DEV), B.cache, out, B.q_start, B.kv_len, max(new), 1 / math.sqrt(D))
+    for b, (n, a) in enumerate(zip(new, cached)):
+        k, v = (R.gather(x, B.table_cpu, b, a + n) for x in vals)
+        s = slice(q_start[b], q_start[b + 1])
+        want, mag, big = attend_on_gpu(q[s], k, v, a, 1 / math.sqrt(D))
+        err = (out[s].cpu().double() - want).abs()
+        bound = R.attention_bound(want, mag, big, D)
+        assert (err <= bound).all(), (b, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new", [1, 3, 30, 200])
+def test_scores_that_keep_rising(gpu, fp8, new):
+    """Every tile passes the running maximum by far: the outputs so far are scaled down again and again."""
+    H, K, D, page, a = 8, 2, 128, 32, 900
+    B = Batch(310, [0, new], [a + new], K, D, page, fp8)
+    g = normal(311, D)
+    for j in range(a + new):  # keys along one direction, longer and longer
+        row = (g * (0.02 + j / 300.0))
+        pg, slot = int(B.table_cpu[0, j // page]), j % page
+        if fp8:
+            e = R.exponent(float(row.abs().max()), 448.0)
+            B.cache.k_pages[pg, :, slot] = (row * 2.0 ** -e).to(torch.float8_e4m3fn).view(torch.uint8).to(DEV)
+            B.cache.k_exp[pg, :, slot] = e + 127
+        else:
+            B.cache.k_pages[pg, :, slot] = row.to(torch.bfloat16).to(DEV)
+    vals = B.values()
+    q = (g + normal(312, new, H, D, scale=0.3)).to(torch.bfloat16)
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=DEV)
+    gpu.attention_paged(q.to(DEV), B.cache, out, B.q_start, B.kv_len, new, 0.3)
+    k, v = (R.gather(x, B.table_cpu, 0, a + new) for x in vals)
+    want, mag, big = R.attend(q.double(), k, v, a, 0.3)
+    err = (out.cpu().double() - want).abs()
+    assert (err <= R.attention_bound(want, mag, big, D)).all()
+
+
+@pytest.mark.parametrize("new", [1, 3, 30, 200])
+@pytest.mark.parametrize("rising", [False, True])
+def test_rows_of_very_unlike_exponents(gpu, new, rising):
+    """e4m3 rows whose powers of two span 2^24, in no order and growing along the sequence."""
+    H, K, D, page, a = 8, 2, 128, 16, 700
+    B = Batch(320, [0, new], [a + new], K, D, page, True)
+    gen = torch.Generator().manual_seed(5)
+    for j in range(a + new):
+        pg, slot = int(B.table_cpu[0, j // page]), j % page
+        for exp in (B.cache.k_exp, B.cache.v_exp):
+            e = 110 + 24 * j // (a + new) if rising else int(torch.randint(110, 134, (1,), generator=gen))
+            exp[pg, :, slot] = e
+    vals = B.values()
+    q = normal(321, new, H, D).to(torch.bfloat16)
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=DEV)
+    scale = 1e-4
+    gpu.attention_paged(q.to(DEV), B.cache, out, B.q_start, B.kv_len, new, scale)
+    k, v = (R.gather(x, B.table_cpu, 0, a + new) for x in vals)
+    want, mag, big = R.attend(q.double(), k, v, a, scale)
+    err = (out.cpu().double() - want).abs()
+    bound = R.attention_bound(want, mag, big, D)
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new", [[1] * 1100, [1, 0, 2] * 400, [40] + [1] * 1100])
+def test_more_sequences_than_any_list_holds(gpu, fp8, new):
+    cached = [(7 * i) % 45 for i in range(len(new))]
+    paged_case(gpu, 330, new, cached, 2, 1, 64, 16, fp8)
+
+
+def test_sequences_that_share_pages(gpu):
+    """Two sequences with a common prefix: the same pages in both rows of the table."""
+    K, D, page = 2, 128, 16
+    B = Batch(340, [0, 1, 41], [100, 140], K, D, page, False)
+    B.table_cpu[1, :6] = B.table_cpu[0, :6]
+    B.cache.block_table.copy_(B.table_cpu)
+    vals = B.values()
+    q = normal(341, 41, 8, D).to(torch.bfloat16).to(DEV)
+    out = torch.empty_like(q)
+    gpu.attention_paged(q, B.cache, out, B.q_start, B.kv_len, 40, 0.1)
+    check_attention(B, vals, q, out, [1, 40], [99, 100], 0.1, D)
+
+
+def test_wide_and_strided_tables(gpu):
+    """A block table cut out of a wider one, its unused entries out of range: never read past a sequence's length."""
+    K, D, page = 2, 128, 16
+    B = Batch(350, [0, 1, 2], [100, 33], K, D, page, True)
+    vals = B.values()
+    wide = torch.full((2, 50), -7, dtype=torch.int32)
+    for b, n in enumerate((7, 3)):
+        wide[b, 5:5 + n] = B.table_cpu[b, :n]
+    cache = PagedKv(B.cache.k_pages, B.cache.v_pages, wide.to(DEV)[:, 5:45], B.cache.k_exp, B.cache.v_exp)
+    for n in (1, 30):
+        q_start = [0, 1, 1 + n]
+        lens = [100, 33]
+        q = normal(351, 1 + n, 8, D).to(torch.bfloat16).to(DEV)
+        out = torch.empty_like(q)
+        gpu.attention_paged(q, cache, out, i32(q_start), i32(lens), n, 0.1)
+        B.q_start_list, B.kv_len_list = q_start, lens
+        check_attention(B, vals, q, out, [1, n], [99, 33 - n], 0.1, D)
+
+
 # ---- attention over prompts ----------------------------------------------------------------
 
 
@@ -557,6 +687,22 @@ def test_prompt_neighbours_never_mix(gpu):
     gpu.attention_prompt(*split(bad), out, i32([0, 70, 160, 200]), 90, 0.1)
     assert torch.equal(out[:70], clean[:70]) and torch.equal(out[160:], clean[160:])
     assert torch.isnan(out[70:160]).all()
+
+
+@pytest.mark.parametrize("new,H,K,D", [([3000, 1501], 4, 1, 128), ([2200], 3, 3, 64), ([700] * 5, 12, 2, 128)])
+def test_larger_prompts(gpu, new, H, K, D):
+    q_start = [0]
+    for n in new:
+        q_start.append(q_start[-1] + n)
+    rows = normal(400, q_start[-1], (H + 2 * K) * D).to(torch.bfloat16).to(DEV)
+    q, k, v = (rows[:, a * D:b * D].unflatten(1, (-1, D)) for a, b in ((0, H), (H, H + K), (H + K, H + 2 * K)))
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=DEV)
+    gpu.attention_prompt(q, k, v, out, i32(q_start), max(new), 0.1)
+    for b in range(len(new)):
+        s = slice(q_start[b], q_start[b + 1])
+        want, mag, big = attend_on_gpu(q[s], k[s], v[s], 0, 0.1)
+        err = (out[s].cpu().double() - want).abs()
+        assert (err <= R.attention_bound(want, mag, big, D)).all()
 
 
 # ---- together ------------------------------------------------------------------------------
@@ -657,3 +803,30 @@ def test_two_streams_at_once(gpu):
     torch.cuda.synchronize()
     for i, (_, _, _, want) in enumerate(cases):
         assert all(torch.equal(o, want) for o in outs[i])
+
+
+def test_two_graphs_at_once(gpu):
+    """Graphs captured from calls without a workspace have their own, so they may replay at the same time."""
+    made = []
+    for i, (new, cached) in enumerate((([1, 1, 1], [4000, 90, 2000]), ([120, 3], [900, 2000]))):
+        q_start = [0]
+        for n in new:
+            q_start.append(q_start[-1] + n)
+        B = Batch(500 + i, q_start, [a + n for a, n in zip(cached, new)], 2, 128, 16, True)
+        q = normal(510 + i, sum(new), 8, 128).to(torch.bfloat16).to(DEV)
+        want, out = torch.empty_like(q), torch.zeros_like(q)
+        gpu.attention_paged(q, B.cache, want, B.q_start, B.kv_len, max(new), 0.1)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(10):
+                gpu.attention_paged(q, B.cache, out, B.q_start, B.kv_len, max(new), 0.1)
+        made.append((g, B, q, want, out, torch.cuda.Stream()))
+    for _ in range(5):
+        for g, _, _, _, out, stream in made:
+            with torch.cuda.stream(stream):
+                out.zero_()
+                g.replay()
+        torch.cuda.synchronize()
+        for _, _, _, want, out, _ in made:
+            assert torch.equal(out, want)

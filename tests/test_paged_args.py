@@ -129,6 +129,7 @@ def test_rope_read_and_attention_refusals():
     assert call(q=None) == _lib.E_ARG
     assert call(ws=None) == _lib.E_ARG
     assert call(scale=float("nan")) == _lib.E_ARG
+    assert call(scale=-3e38) == _lib.E_ARG
     assert call(heads=30) == _lib.E_SHAPE       # heads % kv_heads
     assert call(heads=8 * 65, qs=1 << 20, os=1 << 20) == _lib.E_SHAPE
     assert call(qs=4088) == _lib.E_SHAPE
