@@ -230,7 +230,8 @@ int launch_fa(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, cudaS
                !encode_pool(&vm, p.kv.v, p.kv, D, KIND == KV_E4M3, KIND != KV_E4M3)) {
         return OOMB_E_LAUNCH;
     }
-    int st = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, fw);
+    fw.direct = p.B <= 32 && p.T / (2 * fa_tokens(p.G)) + (p.B < p.T ? p.B : p.T) <= 32;
+    int st = fw.direct ? OOMB_OK : launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, fw);
     if (st == OOMB_OK)
         st = launch(fa_kernel<KIND, D>, dim3(fw.sms), dim3(FaGeo<KIND, D>::THREADS), FaGeo<KIND, D>::TOTAL, s, p, fw, qm, km, vm);
     // no tile has more keys than a part takes: nothing was split

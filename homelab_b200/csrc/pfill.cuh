@@ -77,6 +77,7 @@ struct FaWs {
     FaSplit* splits;
     float* part;  // [slot][kv head][256][D + 4]: acc, m, l
     int max_units, max_slots, sms;
+    int direct;  // few sequences and tiles: every CTA plans by itself
 };
 
 // Tokens of a half tile.
@@ -87,6 +88,14 @@ __device__ __forceinline__ int fa_tiles_of(const Seq& s, int tq) { return (s.n +
 __device__ __forceinline__ int fa_key_tiles(const Seq& s, int i1) {
     const int vis = max(0, min(s.len, s.len - s.n + min(i1, s.n)));
     return (vis + kFaTile - 1) / kFaTile;
+}
+
+// When the last CTA should finish, in key tiles, with parts of `len` at most: with at most a unit an SM that is the
+// longest unit, else (the longest go first) the share and half of the shortest; writing and joining parts costs about
+// two.
+__device__ __forceinline__ int fa_cost(int longest, int shortest, int share, int len, int units, int sms) {
+    const int parts = (longest + len - 1) / len, unit = (longest + parts - 1) / parts;
+    return (units <= sms ? unit : max(unit, share + min(unit, shortest) / 2)) + (parts > 1 ? 2 : 0);
 }
 
 // One CTA.  The sequences' numbers are read once (up to kPlanSeqs of them) and a warp takes a sequence, a lane a
@@ -144,9 +153,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     }
     __syncthreads();
     // How long a part may be: an SM's even share of the step or more (so that there are at most two parts an SM), or a whole
-    // tile.  Of a few lengths the one whose last CTA should finish first: with at most a unit an SM that is the
-    // longest unit, else (the longest go first) the share and half of the shortest; writing and joining parts costs about two
-    // key tiles.
+    // tile.  Of a few lengths the one whose last CTA should finish first.
     const unsigned long long share64 = (total_s * p.Hkv + ws.sms - 1) / ws.sms;
     const int share = share64 > (1u << 24) ? (1 << 24) : max(kFaMinPart, static_cast<int>(share64));
     longest = longest_s;
@@ -164,8 +171,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         }
         if (lane < 6 && units) atomicAdd(&count_s[lane], units);
         __syncthreads();
-        const int parts = (longest + len - 1) / len, unit = (longest + parts - 1) / parts;
-        const int cost = (count_s[min(lane, 5)] * p.Hkv <= ws.sms ? unit : max(unit, share + min(unit, shortest_s) / 2)) + (parts > 1 ? 2 : 0);
+        const int cost = fa_cost(longest, shortest_s, share, len, count_s[min(lane, 5)] * p.Hkv, ws.sms);
         const int best = __reduce_min_sync(0xffffffffu, lane < 6 ? cost : 1 << 30);
         chunk = __shfl_sync(0xffffffffu, len, __ffs(__ballot_sync(0xffffffffu, lane < 6 && cost == best)) - 1);
     }
@@ -413,6 +419,90 @@ __device__ __forceinline__ bool fa_wait(uint64_t* bar, unsigned parity, unsigned
     for (int i = 0; i < 64; i++)
         if (mbar_try_wait(bar, parity)) return true;
     return mbar_wait(bar, parity, err, code);
+}
+
+// The plan of up to 32 sequences with up to 32 tiles together, by one warp and without a launch of its own (which takes four
+// us of a step of short prompts or drafts): lane i keeps tile i.
+struct FaTiles {
+    Seq s;
+    int b, i0, keys, parts;  // the lane's tile
+    int first, slot;         // its first unit, its first slot
+    int units;
+    // The two halves (lanes 0 and 1) of unit v's record.
+    __device__ __forceinline__ int4 unit(int v, int lane) const {
+        const int t = min(31, __popc(__ballot_sync(0xffffffffu, first + parts <= v)));
+        auto of = [&](int x) { return __shfl_sync(0xffffffffu, x, t); };
+        const int j = v - of(first), k = of(keys), n = max(1, of(parts)), each = k / n, more = k - each * n;
+        const int k0 = j * each + min(j, more);
+        const int4 lo = make_int4(of(s.q0), of(s.n), of(s.len), of(b));
+        const int4 hi = make_int4(of(i0), k0, k0 + each + (j < more ? 1 : 0), n > 1 ? of(slot) + j : -1);
+        return lane == 0 ? lo : hi;
+    }
+};
+
+__device__ __noinline__ FaTiles fa_plan_tiles(const PattnParams& p, const FaWs& ws, int tq, int lane) {
+    unsigned* const err = blockIdx.x == 0 ? p.err : nullptr;
+    Seq s{};
+    if (lane < p.B) {
+        s = read_seq(p.q_start, p.kv_len, lane, p.T, p.kv_max, err);
+        if (s.n > p.max_q) {
+            record_error(err, ERR_KV_SEQ);
+            s.n = 0;
+        }
+    }
+    auto scan = [&](int v) {  // inclusive
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        return v;
+    };
+    const int mine = lane < p.B ? fa_tiles_of(s, tq) : 0, ends = scan(mine);
+    int tiles = __shfl_sync(0xffffffffu, ends, 31);
+    if (tiles > 32) {  // only sequences that overlap each other make so many
+        record_error(err, ERR_KV_SEQ);
+        tiles = 0;
+    }
+    FaTiles t{};
+    for (int k = 0; k < p.B; k++) t.b += __shfl_sync(0xffffffffu, ends, k) <= lane;
+    t.b = min(t.b, 31);
+    t.s.q0 = __shfl_sync(0xffffffffu, s.q0, t.b);
+    t.s.n = __shfl_sync(0xffffffffu, s.n, t.b);
+    t.s.len = __shfl_sync(0xffffffffu, s.len, t.b);
+    const bool has = lane < tiles;
+    t.i0 = (lane - __shfl_sync(0xffffffffu, ends - mine, t.b)) * 2 * tq;
+    t.keys = has ? fa_key_tiles(t.s, t.i0 + 2 * tq) : 0;
+    const int work = has ? max(1, t.keys) : 0;
+    const unsigned long long all = static_cast<unsigned long long>(__reduce_add_sync(0xffffffffu, work));
+    const int share = max(kFaMinPart, static_cast<int>(min((all * p.Hkv + ws.sms - 1) / ws.sms, 1ull << 24)));
+    const int longest = max(1, __reduce_max_sync(0xffffffffu, work)), shortest = __reduce_min_sync(0xffffffffu, has ? work : 1 << 30);
+    int chunk = longest;
+    if (longest > share) {  // as plan_kernel chooses
+        int best = 1 << 30;
+#pragma unroll 1
+        for (int k = 0; k < 6; k++) {
+            const int eighths = k == 0 ? 8 : k == 1 ? 9 : k == 2 ? 10 : k == 3 ? 12 : 16;
+            const int len = k < 5 ? (share * eighths + 7) / 8 : longest;
+            const int units = __reduce_add_sync(0xffffffffu, (work + len - 1) / len);
+            const int cost = fa_cost(longest, shortest, share, len, units * p.Hkv, ws.sms);
+            if (cost < best) {
+                best = cost;
+                chunk = len;
+            }
+        }
+    }
+    t.parts = has ? (work + chunk - 1) / chunk : 0;
+    const int ue = scan(t.parts), split = t.parts > 1 ? t.parts : 0;
+    t.first = ue - t.parts;
+    t.slot = scan(split) - split;
+    t.units = __shfl_sync(0xffffffffu, ue, 31);
+    if (blockIdx.x == 0) {  // for the join
+        const unsigned m = __ballot_sync(0xffffffffu, split > 0);
+        if (split) ws.splits[__popc(m & ((1u << lane) - 1))] = FaSplit{t.s, t.i0, t.b, t.slot, t.parts, 0};
+        if (lane == 0) ws.head->splits = __popc(m);
+    }
+    return t;
 }
 
 // What every role derives from a unit: the sequence and each half's key tiles.
@@ -688,13 +778,16 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 if (lane < per_tile && at < p.kv.max_pages) id = __ldcg(table + at);
                 return id;
             };
-            // the next unit's record is fetched while the current one is loaded
-            auto record = [&](int u) {  // lanes 0 and 1: its two halves
+            // Planned before: the next unit's record is fetched while the current one is loaded.
+            auto listed = [&](int u) {  // lanes 0 and 1: its two halves
                 return lane < 2 && u / p.Hkv < ws.max_units ? __ldcg(reinterpret_cast<const int4*>(ws.units + u / p.Hkv) + lane) : make_int4(0, 0, 0, 0);
             };
+            FaTiles own;
+            if (ws.direct) own = fa_plan_tiles(p, ws, tq, lane);
+            auto record = [&](int u) { return ws.direct ? own.unit(u / p.Hkv, lane) : listed(u); };
             int next = blockIdx.x;
             int4 rec = record(next);
-            const int units = __ldcg(&ws.head->units) * p.Hkv;
+            const int units = (ws.direct ? own.units : __ldcg(&ws.head->units)) * p.Hkv;
             while (ok) {
                 const int u = next;
                 if (!fa_wait(&bar->u_empty[feed.i], feed.phase ^ 1, p.err, ERR_FA_WAIT + 13)) break;
@@ -705,7 +798,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 const FaWork w = fa_work(p, bar->unit[feed.i], u % p.Hkv, tq);
                 feed.next();
                 if (u >= units) break;
-                if (lane == 0) next = gridDim.x + atomicAdd(&ws.head->next, 1);
+                if (lane == 0) next = ws.direct ? u + gridDim.x : gridDim.x + atomicAdd(&ws.head->next, 1);
                 next = __shfl_sync(0xffffffffu, next, 0);
                 rec = record(next);
                 if (w.keys == 0) continue;
