@@ -147,7 +147,7 @@ AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int
         w.unit_off = base + 256;
         w.split_off = align256(w.unit_off + static_cast<size_t>(w.max_units) * sizeof(FaUnit));
         w.fa_part_off = align256(w.split_off + static_cast<size_t>(w.max_slots) * sizeof(FaSplit));
-        const size_t end = w.fa_part_off + static_cast<size_t>(w.max_slots) * kv_heads * kFaRows * (head_dim + 4) * 4;
+        const size_t end = w.fa_part_off + static_cast<size_t>(w.max_slots) * kv_heads * kFaRows * fa_line(head_dim) * 4;
         if (end > w.bytes) w.bytes = end;
         if (cache && cache->dtype == OOMB_KV_E4M3 && rows > kExpandRows) {
             const int64_t copy = static_cast<int64_t>(batch) * cache->max_pages * cache->page_size * kv_heads * head_dim * 2;

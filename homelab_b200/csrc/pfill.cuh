@@ -75,10 +75,13 @@ struct FaWs {
     FaHead* head;
     FaUnit* units;
     FaSplit* splits;
-    float* part;  // [slot][kv head][256][D + 4]: acc, m, l
+    float* part;  // [slot][kv head][256][fa_line(D)]: acc, m, l
     int max_units, max_slots, sms;
     int direct;  // few sequences and tiles: every CTA plans by itself
 };
+
+// Floats of a partial row: acc, m, l, 32-byte aligned.
+__host__ __device__ constexpr int fa_line(int D) { return D + 8; }
 
 // Tokens of a half tile.
 __host__ __device__ inline int fa_tokens(int G) { return kFaTile / G; }
@@ -329,6 +332,12 @@ __device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t* r) {
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+// 32 bytes (32-byte aligned): a thread that owns a row writes whole sectors, in half the trips of 16-byte stores.
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&r)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -602,6 +611,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         const bool negate = p.scale_log2 < 0.0f;
         const int token_of = row / p.G, head_of = row - token_of * p.G;
         const bool row_in = token_of < tq;
+        const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | (static_cast<uintptr_t>(p.out_stride) * 2)) & 31u) == 0;
         for (FaWork w; ok && take(w);) {
             const int token = w.i0 + h * tq + token_of;
             const bool valid = row_in && token < w.s.n;
@@ -694,7 +704,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             const float inv = w.slot >= 0 ? 1.0f : vis > 0 ? 1.0f / l : 0.0f;
             const int head = w.kvh * p.G + head_of;
             uint16_t* out = p.out + static_cast<int64_t>(w.s.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D;
-            float* line = ws.part + ((static_cast<int64_t>(max(w.slot, 0)) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + row) * (D + 4);
+            float* line = ws.part + ((static_cast<int64_t>(max(w.slot, 0)) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + row) * fa_line(D);
             bool odd = !(l <= 3.4e38f);
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
@@ -716,19 +726,24 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 if (!valid) continue;
                 if (w.slot < 0) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t v[4];
+                    for (int e = 0; e < 32; e += 16) {
+                        uint32_t v[8];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
+                        for (int k = 0; k < 8; k++) {
                             const __nv_bfloat162 b2 = __floats2bfloat162_rn(o[e + 2 * k], o[e + 2 * k + 1]);
                             v[k] = *reinterpret_cast<const uint32_t*>(&b2);
                         }
-                        *reinterpret_cast<uint4*>(out + 32 * c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+                        if (wide) {
+                            st_global_v8(out + 32 * c + e, v);
+                        } else {
+                            *reinterpret_cast<uint4*>(out + 32 * c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+                            *reinterpret_cast<uint4*>(out + 32 * c + e + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                        }
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4*>(line + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 32; e += 8)
+                        st_global_v8(line + 32 * c + e, *reinterpret_cast<const uint32_t(*)[8]>(&o[e]));
                 }
             }
             if (w.slot >= 0 && valid) *reinterpret_cast<float2*>(line + D) = make_float2(m == -INFINITY ? m : m * scale, l);
@@ -752,7 +767,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                         *reinterpret_cast<__nv_bfloat162*>(o + e) = b2;
                     }
                 } else {
-                    float* o = ws.part + ((static_cast<int64_t>(w.slot) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + (warp & 3) * 32 + src) * (D + 4);
+                    float* o = ws.part + ((static_cast<int64_t>(w.slot) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + (warp & 3) * 32 + src) * fa_line(D);
 #pragma unroll
                     for (int e = 0; e < D / 32; e++) o[lane * (D / 32) + e] = a[e];
                     if (lane == 0) *reinterpret_cast<float2*>(o + D) = make_float2(mm, ll);
@@ -1062,26 +1077,28 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Pattn
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int tq = fa_tokens(p.G);
-    const int64_t rows = static_cast<int64_t>(__ldcg(&ws.head->splits)) * p.Hkv * kFaRows;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < rows; i += static_cast<int64_t>(gridDim.x) * 8) {
+    // a split tile's record and how many there are, read at once (the list is longer than the tiles can be)
+    const int64_t most = static_cast<int64_t>(ws.max_slots) * p.Hkv * kFaRows;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < most; i += static_cast<int64_t>(gridDim.x) * 8) {
         const int r = static_cast<int>(i % kFaRows);
         const int64_t tile = i / kFaRows;
         const int kvh = static_cast<int>(tile % p.Hkv);
         const int4* at = reinterpret_cast<const int4*>(ws.splits + tile / p.Hkv);
         const int4 sa = __ldcg(at), sb = __ldcg(at + 1);  // q0, n, len, i0; b, slot, parts
+        if (tile / p.Hkv >= __ldcg(&ws.head->splits)) break;
         const int hr = r % kFaTile;
         const int token = sa.w + (r / kFaTile) * tq + hr / p.G, head = kvh * p.G + hr % p.G;
         if (hr / p.G >= tq || token >= sa.y) continue;
         const int vis = max(0, min(sa.z, sa.z - sa.y + token + 1));
-        const float* base = ws.part + ((static_cast<int64_t>(sb.y) * p.Hkv + kvh) * kFaRows + r) * (D + 4);
-        const int64_t step = static_cast<int64_t>(p.Hkv) * kFaRows * (D + 4);
-        // eight parts' loads under way at once
+        const float* base = ws.part + ((static_cast<int64_t>(sb.y) * p.Hkv + kvh) * kFaRows + r) * fa_line(D);
+        const int64_t step = static_cast<int64_t>(p.Hkv) * kFaRows * fa_line(D);
+        // sixteen parts' loads under way at once
         float M = -INFINITY, a[E] = {}, l = 0.0f;
-        for (int j0 = 0; j0 < sb.z; j0 += 8) {
-            float2 ml[8], v[8][E / 2];
+        for (int j0 = 0; j0 < sb.z; j0 += 16) {
+            float2 ml[16], v[16][E / 2];
             float mn = M;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < 16; j++) {
                 const bool in = j0 + j < sb.z;
                 const float* pr = base + (j0 + j) * step;
                 ml[j] = in ? __ldcg(reinterpret_cast<const float2*>(pr + D)) : make_float2(-INFINITY, 0.0f);
@@ -1090,14 +1107,14 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Pattn
                     v[j][e] = in ? __ldcg(reinterpret_cast<const float2*>(pr + lane * E + 2 * e)) : make_float2(0.0f, 0.0f);
             }
 #pragma unroll
-            for (int j = 0; j < 8; j++) mn = fmaxf(mn, ml[j].x);
+            for (int j = 0; j < 16; j++) mn = fmaxf(mn, ml[j].x);
             const float b0 = mn == -INFINITY ? 0.0f : mn, c = exp2_fast(M - b0);
             M = mn;
             l *= c;
 #pragma unroll
             for (int e = 0; e < E; e++) a[e] *= c;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < 16; j++) {
                 const float f = exp2_fast(ml[j].x - b0);
                 l = fmaf(f, ml[j].y, l);
 #pragma unroll
