@@ -78,7 +78,8 @@ int launch_rows_d(bool xb, const RowsParams& p, cudaStream_t s) {
 
 template <int CACHE>
 int launch_rows(const DeviceState* d, int head_dim, bool xb, RowsParams& p, cudaStream_t s) {
-    // one token a CTA while that leaves SMs idle, else four: the angles of four tokens fill the CTA's threads
+    // one token a CTA while that leaves SMs idle, else two: the angles of two tokens of 128 fill half the CTA's threads,
+    // and the look-up of a token's sequence is paid once for both
     p.tpb = p.T <= 4 * d->sms ? 1 : kRowsMaxTpb;
     return head_dim == 128 ? launch_rows_d<128, CACHE>(xb, p, s) : launch_rows_d<64, CACHE>(xb, p, s);
 }

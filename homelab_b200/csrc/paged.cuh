@@ -96,7 +96,9 @@ __device__ __forceinline__ Seq read_seq(const int32_t* q_start, const int32_t* k
 // ---- rotation and append -------------------------------------------------------------
 
 constexpr int kRowsThreads = 256;
-constexpr int kRowsMaxTpb = 4;    // tokens of a CTA
+// Tokens of a CTA.  8,192 new tokens of 32 query heads over 8, D = 128 (101 MB read, 101 written), take 46.0 us with one,
+// 38.8 with two and 40.0 with three or four; rotation alone of 9,391 fp32 tokens of 32 heads (308 MB) 47.7, 49.2, 50.4 and 51.8.
+constexpr int kRowsMaxTpb = 2;
 constexpr int kRopeMaxPairs = 64;  // head_dim / 2
 
 struct RowsParams {
@@ -180,9 +182,10 @@ __device__ __forceinline__ uint2 codes8(const float (&f)[8], float inv) {
     return make_uint2(w[0], w[1]);
 }
 
-// CACHE: -1 rotation alone, 0 bf16 pool, 1 e4m3 pool.
+// CACHE: -1 rotation alone, 0 bf16 pool, 1 e4m3 pool.  Six CTAs to an SM (40 registers): the append above takes 45 us with
+// five of 48 registers and 41 with seven of 36.
 template <bool XBF16, int D, int CACHE>
-__global__ void __launch_bounds__(kRowsThreads) rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kRowsThreads, 6) rows_kernel(const RowsParams p) {
     constexpr int TEAM = D / 16;  // threads of a row
     constexpr int SLOTS = kRowsThreads / TEAM;
     __shared__ __align__(16) float cs[kRowsMaxTpb][2][kRopeMaxPairs];
@@ -244,10 +247,13 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const RowsParams p) 
 
     const int R = p.Hq + 2 * p.Hkv, slot = threadIdx.x / TEAM, t8 = threadIdx.x % TEAM;
     const int total = nt * R;
-    for (int r0 = 0; r0 < total; r0 += SLOTS) {
-        const int r = r0 + slot;
-        const bool in = r < total;
-        const int a = in ? r / R : 0, rr = in ? r - a * R : 0;
+    int a = slot / R, rr = slot - a * R;  // token of the CTA, row of the token
+    for (int r0 = 0; r0 < total; r0 += SLOTS, rr += SLOTS) {
+        const bool in = r0 + slot < total;
+        while (rr >= R) {
+            rr -= R;
+            a = min(a + 1, kRowsMaxTpb - 1);  // past the last token nothing is done, but its flag is read
+        }
         const bool is_q = rr < p.Hq, is_k = !is_q && rr < p.Hq + p.Hkv;
         const int h = is_q ? rr : is_k ? rr - p.Hq : rr - p.Hq - p.Hkv;
         const bool ok = in && tok_ok[a];
@@ -286,26 +292,34 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const RowsParams p) 
             const float* c = cs[a][0];
             const float* s = cs[a][1];
             if (p.interleaved) {
+                const float4 ca4 = *reinterpret_cast<const float4*>(c + ca * 4), sa4 = *reinterpret_cast<const float4*>(s + ca * 4);
+                const float4 cb4 = *reinterpret_cast<const float4*>(c + cb * 4), sb4 = *reinterpret_cast<const float4*>(s + cb * 4);
+                const float c1[4] = {ca4.x, ca4.y, ca4.z, ca4.w}, s1[4] = {sa4.x, sa4.y, sa4.z, sa4.w};
+                const float c2[4] = {cb4.x, cb4.y, cb4.z, cb4.w}, s2[4] = {sb4.x, sb4.y, sb4.z, sb4.w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int fa = ca * 4 + i, fb = cb * 4 + i;
-                    if (2 * fa < p.rot) {
+                    if (ca * 8 < p.rot) {  // rot is a multiple of 16: a chunk turns as a whole
                         const float u = x[2 * i], w = x[2 * i + 1];
-                        x[2 * i] = u * c[fa] - w * s[fa];
-                        x[2 * i + 1] = w * c[fa] + u * s[fa];
+                        x[2 * i] = u * c1[i] - w * s1[i];
+                        x[2 * i + 1] = w * c1[i] + u * s1[i];
                     }
-                    if (2 * fb < p.rot) {
+                    if (cb * 8 < p.rot) {
                         const float u = y[2 * i], w = y[2 * i + 1];
-                        y[2 * i] = u * c[fb] - w * s[fb];
-                        y[2 * i + 1] = w * c[fb] + u * s[fb];
+                        y[2 * i] = u * c2[i] - w * s2[i];
+                        y[2 * i + 1] = w * c2[i] + u * s2[i];
                     }
                 }
             } else if (t8 < nr) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float cc = c[t8 * 8 + i], ss = s[t8 * 8 + i], u = x[i], w = y[i];
-                    x[i] = u * cc - w * ss;
-                    y[i] = w * cc + u * ss;
+                for (int i = 0; i < 8; i += 4) {
+                    const float4 c4 = *reinterpret_cast<const float4*>(c + t8 * 8 + i), s4 = *reinterpret_cast<const float4*>(s + t8 * 8 + i);
+                    const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float u = x[i + k], w = y[i + k];
+                        x[i + k] = u * cc[k] - w * ss[k];
+                        y[i + k] = w * cc[k] + u * ss[k];
+                    }
                 }
             }
         }
