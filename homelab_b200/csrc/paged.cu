@@ -121,7 +121,10 @@ struct AttnWs {
 constexpr int kExpandRows = 640;
 constexpr int64_t kExpandBytes = int64_t{1} << 30;
 
-AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int kv_heads, int head_dim, const oomb_paged_kv* cache) {
+// room: the bytes that the caller has.  A workspace for a larger batch, whose copy is past its limit, need not hold a smaller
+// one's: then the codes are converted in the attention.
+AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int kv_heads, int head_dim, const oomb_paged_kv* cache,
+               size_t room = SIZE_MAX) {
     AttnWs w{};
     const bool paged = cache != nullptr;
     const int G = heads / kv_heads;
@@ -152,11 +155,14 @@ AttnWs attn_ws(const DeviceState* d, int batch, int t, int max_q, int heads, int
         if (end > w.bytes) w.bytes = end;
         if (cache && cache->dtype == OOMB_KV_E4M3 && rows > kExpandRows) {
             const int64_t copy = static_cast<int64_t>(batch) * cache->max_pages * cache->page_size * kv_heads * head_dim * 2;
-            if (2 * copy <= kExpandBytes && static_cast<int64_t>(batch) * cache->max_pages * cache->page_size < (1 << 30)) {
-                w.expand = true;
-                w.k_off = align256(end);
-                w.v_off = align256(w.k_off + static_cast<size_t>(copy));
-                if (w.v_off + static_cast<size_t>(copy) > w.bytes) w.bytes = w.v_off + static_cast<size_t>(copy);
+            if (2 * copy <= kExpandBytes && static_cast<int64_t>(batch) * cache->max_pages * cache->page_size < (1 << 30) && batch <= 65535) {
+                const size_t k_off = align256(end), v_off = align256(k_off + static_cast<size_t>(copy)), past = v_off + static_cast<size_t>(copy);
+                if (past <= room) {
+                    w.expand = true;
+                    w.k_off = k_off;
+                    w.v_off = v_off;
+                    if (past > w.bytes) w.bytes = past;
+                }
             }
         }
     }
@@ -260,11 +266,12 @@ int launch_decode(const PattnParams& p, const AttnWs& w, uint8_t* ws, cudaStream
 template <int KIND, int D>
 int launch_attn_d(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, cudaStream_t s) {
     if constexpr (KIND != KV_ROWS) {
-        const int rows = p.max_q * p.G;
-        if (w.few)
+        if (w.few) {
+            const int rows = p.max_q * p.G;
             return rows <= 4   ? launch_decode<KIND, D, 4>(p, w, ws, s)
                    : rows <= 8 ? launch_decode<KIND, D, 8>(p, w, ws, s)
                                : launch_decode<KIND, D, 16>(p, w, ws, s);
+        }
     }
     if constexpr (KIND == KV_E4M3) {
         if (w.expand) {
@@ -278,7 +285,6 @@ int launch_attn_d(const PattnParams& p, const AttnWs& w, int sms, uint8_t* ws, c
             e.ko = reinterpret_cast<uint16_t*>(ws + w.k_off);
             e.vo = reinterpret_cast<uint16_t*>(ws + w.v_off);
             e.err = p.err;
-            if (p.B > 65535) return OOMB_E_SHAPE;
             const dim3 grid(static_cast<unsigned>((p.kv_max + kExpandTokens - 1) / kExpandTokens), static_cast<unsigned>(p.B));
             const int st = grid.x ? launch(expand_kernel<D>, grid, dim3(kReadThreads), 0, s, e) : OOMB_OK;
             if (st != OOMB_OK) return st;
@@ -307,7 +313,7 @@ bool attn_shape_ok(int batch, int t, int max_q, int heads, int kv_heads, int hea
 // The checks that both attentions share.
 int check_attn(const void* q, int64_t q_stride, const void* out, int64_t out_stride, int heads, int kv_heads, int head_dim,
                int batch, int t, int max_q, float scale) {
-    if (!q || !out) return OOMB_E_ARG;
+    if (!q || !out || q == out) return OOMB_E_ARG;
     if (!(fabsf(scale) <= 1e37f)) return OOMB_E_ARG;  // its product with log2(e) is an fp32 number
     if (!attn_shape_ok(batch, t, max_q, heads, kv_heads, head_dim)) return OOMB_E_SHAPE;
     const int64_t row = static_cast<int64_t>(heads) * head_dim;
@@ -472,11 +478,11 @@ int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_st
         st = check_attn(q, q_stride, out, out_stride, heads, cache->kv_heads, cache->head_dim, batch, t, max_q, scale);
     if (st != OOMB_OK) return st;
     if (!q_start && batch != t) return OOMB_E_SHAPE;
-    if (!aligned16(workspace)) return OOMB_E_ALIGN;
+    if (reinterpret_cast<uintptr_t>(workspace) & 31u) return OOMB_E_ALIGN;
     if (batch == 0 || t == 0 || max_q == 0) return OOMB_OK;
     const DeviceState* d = device_state();
     if (!d) return OOMB_E_DEVICE;
-    const AttnWs w = attn_ws(d, batch, t, max_q, heads, cache->kv_heads, cache->head_dim, cache);
+    const AttnWs w = attn_ws(d, batch, t, max_q, heads, cache->kv_heads, cache->head_dim, cache, workspace_bytes);
     if (workspace_bytes < w.bytes) return OOMB_E_WORKSPACE;
     p.q = static_cast<const uint16_t*>(q);
     p.q_stride = q_stride;
@@ -513,7 +519,7 @@ int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_
     if (st == OOMB_OK) st = check_rows(k, k_stride, row, OOMB_BF16);
     if (st == OOMB_OK) st = check_rows(v, v_stride, row, OOMB_BF16);
     if (st != OOMB_OK) return st;
-    if (!aligned16(workspace)) return OOMB_E_ALIGN;
+    if (reinterpret_cast<uintptr_t>(workspace) & 31u) return OOMB_E_ALIGN;
     if (batch == 0 || t == 0 || max_q == 0) return OOMB_OK;
     const DeviceState* d = device_state();
     if (!d) return OOMB_E_DEVICE;

@@ -50,6 +50,10 @@ constexpr int kDecRowsAlways = 32, kDecRowsFew = 64;
 // that runs of 8 blocks make, 20.6 in 21 and 22.3 in 31; one of 60,000 48 us in the 37 that fill the SMs.
 constexpr int kDecParts = 16, kDecRun = 8;
 
+// e4m3: by how many powers of two the value rows hidden from a query row may pass those it sees, the weights' absolute
+// precision of 2^-27 of the largest falling to 2^-23.
+constexpr int kDecUnlike = 4;
+
 enum : unsigned {
     ERR_DEC_WAIT = 0xb00,  // a decode pipeline wait ran out (+ the waiting role)
 };
@@ -506,6 +510,9 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 vis[r] = r < rows ? max(0, min(sq.len, sq.len - sq.n + (row0 + r) / p.G + 1)) : 0;
             }
             int X = 0;  // e4m3: the exponent byte that the outputs are counted in
+            // the largest exponent of the positions that every row sees, or where the segment has none such the least (from 255)
+            const bool shared = g.tok0 < vis[0];
+            int seen = 0;
             if (g.tiles > 0) {
                 // ---- the queries as the scores' second operand; the last segment's scores are all made ----
                 if constexpr (!F8) {
@@ -584,6 +591,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     const uint8_t* ep = smem + Geo::EXP_OFF + e * 2 * kDecBlock;
                     kf = exp_byte(ep[tid]);
                     ve = tok < g.tok1 ? ep[kDecBlock + tid] : 0;
+                    if (tok < (shared ? vis[0] : g.tok1)) seen = max(seen, shared ? ve : 255 - ve);
                 }
                 bool over = ve > X;
 #pragma unroll
@@ -681,8 +689,19 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
             if (meet(gone)) break;  // and the last maxima are read
             warp_reduce_multi<R>(l, lane);  // the lane's l[0] is the warp's sum of row reduce_index
             bar->red[warp][reduce_index<R>(lane, 0)] = l[0];
+            if constexpr (F8) {
+                const int x = __reduce_max_sync(0xffffffffu, seen);
+                if (lane == 0) bar->redx[warp] = x;
+            }
             meet(false);
-            const float unit = F8 ? exp_byte(static_cast<unsigned>(X)) : 1.0f;
+            float unit = 1.0f;
+            if constexpr (F8) {
+                // Value rows that only some of the query rows see, so much larger than what the others do that these lost
+                // their weights' last bits to them: not a number, and done again below.
+                const int x = max(max(bar->redx[0], bar->redx[1]), max(bar->redx[2], bar->redx[3]));
+                const bool lost = sq.n > 1 && X > (shared ? x : 255 - x) + kDecUnlike;
+                unit = lost ? __uint_as_float(0x7fffffffu) : exp_byte(static_cast<unsigned>(X));
+            }
             const int first = walk.deal.owner(g.pair_first), final_cta = walk.deal.owner(g.pair_end - 1);
             const int parts = final_cta - first + 1;
             float* my_part = ws.part + static_cast<int64_t>(2 * blockIdx.x + (g.lo == g.pair_first ? 1 : 0)) * ws.rows * PAD;
@@ -761,8 +780,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     }
                 }
             }
-            // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the products: then every
-            // row is done again in plain loops over what it sees.  (A single new token sees everything.)
+            // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the products: then (and
+            // where a huge one took the weights' bits) every row is done again in plain loops over what it sees.  (A single new token sees everything.)
             if (meet(odd) && sq.n > 1) {
                 for (int r = warp; r < rows; r += 4) {
                     const int token = (row0 + r) / p.G, head = g.kvh * p.G + row0 + r - token * p.G;

@@ -405,6 +405,31 @@ def test_values_behind_the_mask_never_reach_a_row(gpu, fp8, new):
     assert ((rest[:, 4:][..., others] - want[clean:, 4:][..., others]).abs() <= bound[clean:, 4:][..., others]).all()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("H,new,a", [(8, 3, 37), (8, 7, 0), (8, 7, 700), (8, 13, 5), (8, 70, 200), (16, 200, 60), (4, 1000, 100)])
+def test_huge_values_behind_the_mask_never_reach_a_row(gpu, fp8, H, new, a):
+    """Values near the top of the range at the later new tokens: the weights that earlier rows give them are exactly zero,
+    and nothing of the earlier rows' own values is lost to their size."""
+    K, D, page = 2, 128, 16
+    B = Batch(45 + new, [0, new], [a + new], K, D, page, fp8)
+    clean = new // 2
+    vals = [x.clone() for x in B.values()]
+    for j in range(a + clean, a + new):
+        pg, slot = int(B.table_cpu[0, j // page]), j % page
+        if fp8:
+            B.cache.v_exp[pg, :, slot] = 240
+        else:
+            B.cache.v_pages[pg, :, slot] = 1e37
+    q = normal(46, new, H, D).to(torch.bfloat16)
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=DEV)
+    gpu.attention_paged(q.to(DEV), B.cache, out, B.q_start, B.kv_len, new, 0.1)
+    k, v = (R.gather(x, B.table_cpu, 0, a + new) for x in vals)
+    want, mag, big = attend_on_gpu(q[:clean].double(), k[:a + clean], v[:a + clean], a, 0.1)
+    err = (out[:clean].cpu().double() - want).abs()
+    bound = R.attention_bound(want, mag, big, D)
+    assert (err <= bound).all(), float((err / bound).max())
+
+
 def test_infinite_scores_and_masked_extremes(gpu):
     """A largest-value key gives one position all the weight; every score at the type's lowest still averages."""
     K, D, page = 1, 128, 16
@@ -483,6 +508,21 @@ def test_a_sequence_over_max_q_is_left_out_and_recorded(gpu):
         assert not (out[:q_start[1]] == 5.0).all() and not (out[q_start[2]:] == 5.0).all()
 
 
+def test_a_workspace_serves_smaller_batches(gpu):
+    """A cache so wide that the bf16 copy of two sequences' codes is past its limit, and that of one is not."""
+    K, D, page, width, a, n = 8, 128, 64, 2100, 900, 200
+    B = Batch(85, [0, n], [a + n], K, D, page, True)
+    table = torch.zeros((2, width), dtype=torch.int32, device=DEV)
+    table[:1, :B.cache.block_table.shape[1]] = B.cache.block_table
+    B.cache = PagedKv(B.cache.k_pages, B.cache.v_pages, table, B.cache.k_exp, B.cache.v_exp)
+    q = normal(86, n, 32, D).to(torch.bfloat16).to(DEV)
+    ws = gpu.attention_paged_workspace(B.cache, 2, 2 * n, n, 32)
+    for workspace in (ws, None):
+        out = torch.empty_like(q)
+        gpu.attention_paged(q, B.cache, out, B.q_start, B.kv_len, n, 0.1, workspace=workspace)
+        check_attention(B, B.values(), q, out, [n], [a], 0.1, D)
+
+
 def test_attention_refuses(gpu):
     B = Batch(95, [0, 1], [5], 2, 128, 16, False)
     q = torch.zeros(1, 8, 128, dtype=torch.bfloat16, device=DEV)
@@ -503,6 +543,8 @@ def test_attention_refuses(gpu):
         gpu.attention_paged(q, B.cache, out, B.q_start, B.kv_len, 1, 0.1, workspace=torch.zeros(16, dtype=torch.uint8, device=DEV))
     with pytest.raises(Exception):
         gpu.attention_paged(q[:, :7], B.cache, out[:, :7], B.q_start, B.kv_len, 1, 0.1)
+    with pytest.raises(Exception):
+        gpu.attention_paged(q, B.cache, q, B.q_start, B.kv_len, 1, 0.1)  # rows are read again after others are written
 
 
 def attend_on_gpu(q, k, v, n_before, scale):
@@ -687,6 +729,18 @@ def test_prompt_neighbours_never_mix(gpu):
     gpu.attention_prompt(*split(bad), out, i32([0, 70, 160, 200]), 90, 0.1)
     assert torch.equal(out[:70], clean[:70]) and torch.equal(out[160:], clean[160:])
     assert torch.isnan(out[70:160]).all()
+
+
+def test_huge_values_behind_the_mask_of_a_prompt(gpu):
+    H, K, D, n = 8, 2, 128, 300
+    q, k, v = (normal(6 + i, n, h, D).to(torch.bfloat16) for i, h in enumerate((H, K, K)))
+    v[100:] = 1e37
+    out = torch.empty(n, H, D, dtype=torch.bfloat16, device=DEV)
+    gpu.attention_prompt(q.to(DEV), k.to(DEV), v.to(DEV), out, i32([0, n]), n, 0.1)
+    want, mag, big = R.attend(q[:100].double(), k[:100].double(), v[:100].double(), 0, 0.1)
+    err = (out[:100].cpu().double() - want).abs()
+    bound = R.attention_bound(want, mag, big, D)
+    assert (err <= bound).all(), float((err / bound).max())
 
 
 @pytest.mark.parametrize("new,H,K,D", [([3000, 1501], 4, 1, 128), ([2200], 3, 3, 64), ([700] * 5, 12, 2, 128)])

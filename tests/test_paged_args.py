@@ -120,7 +120,7 @@ def test_rope_read_and_attention_refusals():
     assert L.oomb_kv_read_paged(c, FAKE, FAKE, 1, 1, FAKE, None, 1, 1024, None) == _lib.E_ARG
     assert L.oomb_kv_read_paged(c, FAKE, FAKE, 1, 1, FAKE, FAKE, 1, 1000, None) == _lib.E_SHAPE
     assert L.oomb_kv_read_paged(c, None, FAKE, 2, 1, FAKE, FAKE, 1, 1024, None) == _lib.E_SHAPE
-    ok = dict(c=c, q=FAKE, qs=4096, out=FAKE, os=4096, heads=32, q_start=FAKE, kv_len=FAKE, batch=2, t=3, max_q=2,
+    ok = dict(c=c, q=FAKE, qs=4096, out=2 * FAKE, os=4096, heads=32, q_start=FAKE, kv_len=FAKE, batch=2, t=3, max_q=2,
               scale=0.1, ws=FAKE, n=1 << 30)
 
     def call(**kw):
@@ -137,9 +137,11 @@ def test_rope_read_and_attention_refusals():
     assert call(out=FAKE + 2) == _lib.E_ALIGN
     assert call(max_q=-1) == _lib.E_SHAPE
     assert call(q_start=None) == _lib.E_SHAPE
+    assert call(out=FAKE, q=FAKE) == _lib.E_ARG  # the output over the queries
+    assert call(ws=FAKE + 16) == _lib.E_ALIGN
     assert call(t=0) == 0
     assert call(max_q=0) == 0
-    p = dict(q=FAKE, qs=4096, k=FAKE, ks=1024, v=FAKE, vs=1024, out=FAKE, os=4096, heads=32, kv_heads=8, d=128, q_start=FAKE,
+    p = dict(q=FAKE, qs=4096, k=FAKE, ks=1024, v=FAKE, vs=1024, out=2 * FAKE, os=4096, heads=32, kv_heads=8, d=128, q_start=FAKE,
              batch=2, t=3, max_q=2, scale=0.1, ws=FAKE, n=1 << 30)
 
     def prompt(**kw):
@@ -151,6 +153,8 @@ def test_rope_read_and_attention_refusals():
     assert prompt(vs=1028) == _lib.E_ALIGN
     assert prompt(d=96) == _lib.E_SHAPE
     assert prompt(kv_heads=0) == _lib.E_SHAPE
+    assert prompt(out=FAKE) == _lib.E_ARG
+    assert prompt(ws=FAKE + 16) == _lib.E_ALIGN
     assert prompt(batch=0) == 0
 
 
