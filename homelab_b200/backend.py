@@ -297,6 +297,16 @@ class Gpu:
             raise ValueError(f"{what} must be a contiguous int32 [{'B' if n is None else n}] tensor on {self.device}")
         return x.data_ptr()
 
+    def _plan(self, plan: RopePlan):
+        if plan.index != self.index:
+            raise ValueError(f"the rotation's frequencies must live on {self.device}")
+        return plan.ref
+
+    def _ws(self, ws):
+        if ws.dtype is not torch.uint8 or ws.get_device() != self.index or not ws.is_contiguous():
+            raise ValueError(f"a workspace is a contiguous uint8 tensor on {self.device}")
+        return ws
+
     def _step(self, cache: PagedKv, q_start, kv_len, t: int):
         """The batch of a packed step over `cache` and its index addresses."""
         if cache.device != self.device:
@@ -320,7 +330,7 @@ class Gpu:
         pos = self._index(positions, T, "positions")
         if T == 0:
             return out
-        self._launch(self.L.oomb_rope_rows, "rope", plan.ref, xp, _dtype_code(x), xs, pos, op, os_, T, H, D)
+        self._launch(self.L.oomb_rope_rows, "rope", self._plan(plan), xp, _dtype_code(x), xs, pos, op, os_, T, H, D)
         return out
 
     def kv_append_paged(self, cache: PagedKv, k, v, q_start, kv_len, rope: RopePlan = None, q=None, q_out=None):
@@ -342,7 +352,7 @@ class Gpu:
             qo, qos = self._rows(q_out, H, D, T, "q_out", _BF16)
         if T == 0 or B == 0:
             return
-        self._launch(self.L.oomb_kv_append_paged, "kv_append_paged", cache.ref, None if rope is None else rope.ref, qp, qs,
+        self._launch(self.L.oomb_kv_append_paged, "kv_append_paged", cache.ref, None if rope is None else self._plan(rope), qp, qs,
                      qo, qos, H, kp, ks, vp, vs, _dtype_code(k), qs_p, len_p, B, T)
 
     def kv_read_paged(self, cache: PagedKv, q_start, kv_len, k_out, v_out):
@@ -380,6 +390,9 @@ class Gpu:
     def _attention_ws(self, cache, shape) -> torch.Tensor:
         """A workspace of this object's for a call of this shape on the current stream.  A graph gets one of its
         own, so that graphs (and eager calls beside them) never share one."""
+        if _current_device() != self.index:  # whose stream captures is asked of the current device
+            with torch.cuda.device(self.device):
+                return self._attention_ws(cache, shape)
         capturing = _capturing()
         key = (_raw_stream(self.index), shape) if cache is None else (
             _raw_stream(self.index), shape, cache.max_pages, cache.page_size, cache.kv_heads, cache.head_dim, cache.fp8)
@@ -412,7 +425,7 @@ class Gpu:
         B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
         if T == 0 or B == 0:
             return
-        ws = self._attention_ws(cache, (B, T, max_q, H)) if workspace is None else workspace
+        ws = self._attention_ws(cache, (B, T, max_q, H)) if workspace is None else self._ws(workspace)
         self._launch(self.L.oomb_attention_paged, "attention_paged", cache.ref, qp, qs, op, os_, H, qs_p, len_p, B, T, max_q,
                      scale, ws.data_ptr(), ws.numel())
 
@@ -425,11 +438,13 @@ class Gpu:
         kp, ks = self._rows(k, Hkv, D, T, "k", _BF16)
         vp, vs = self._rows(v, Hkv, D, T, "v", _BF16)
         op, os_ = self._rows(out, H, D, T, "out", _BF16)
+        if q_start is None:
+            raise ValueError("prompts need q_start")
         qs_p = self._index(q_start, None, "q_start")
         B = q_start.numel() - 1
         if T == 0 or B <= 0:
             return
-        ws = self._attention_ws(None, (B, T, max_q, H, Hkv, D)) if workspace is None else workspace
+        ws = self._attention_ws(None, (B, T, max_q, H, Hkv, D)) if workspace is None else self._ws(workspace)
         self._launch(self.L.oomb_attention_prompt, "attention_prompt", qp, qs, kp, ks, vp, vs, op, os_, H, Hkv, D, qs_p, B, T,
                      max_q, scale, ws.data_ptr(), ws.numel())
 

@@ -513,7 +513,7 @@ int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_
                           void* out, int64_t out_stride, int heads, int kv_heads, int head_dim, const int32_t* q_start,
                           int batch, int t, int max_q, float scale, void* workspace, size_t workspace_bytes,
                           oomb_stream stream) {
-    if (!k || !v || !q_start || !workspace) return OOMB_E_ARG;
+    if (!k || !v || !q_start || !workspace || out == k || out == v) return OOMB_E_ARG;
     int st = check_attn(q, q_stride, out, out_stride, heads, kv_heads, head_dim, batch, t, max_q, scale);
     const int64_t row = static_cast<int64_t>(kv_heads) * head_dim;
     if (st == OOMB_OK) st = check_rows(k, k_stride, row, OOMB_BF16);

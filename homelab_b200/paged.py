@@ -37,6 +37,7 @@ class RopePlan:
         turns, m = rope_turns(rot_dim, base, scaling, factor, original_len)
         self.rot_dim, self.interleaved, self.mscale = int(rot_dim), bool(interleaved), m
         self.turns = turns.to(device)
+        self.index = self.turns.get_device()
         self.struct = RopeStruct(rot_dim=self.rot_dim, interleaved=int(self.interleaved), mscale=m,
                                  turns=self.turns.data_ptr())
         self.ref = C.byref(self.struct)

@@ -353,7 +353,7 @@ int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_st
                          int heads, const int32_t* q_start, const int32_t* kv_len, int batch, int t, int max_q, float scale,
                          void* workspace, size_t workspace_bytes, oomb_stream stream);
 /* The same over whole prompts whose keys and values are rows of the step itself, bf16
- * [t][kv_heads][head_dim] packed as q: token i of a sequence sees its tokens 0 .. i. */
+ * [t][kv_heads][head_dim] packed as q (out overlaps none of the three): token i of a sequence sees its tokens 0 .. i. */
 size_t oomb_attention_prompt_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim);
 int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                           void* out, int64_t out_stride, int heads, int kv_heads, int head_dim, const int32_t* q_start,

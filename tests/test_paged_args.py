@@ -9,7 +9,8 @@ torch = pytest.importorskip("torch")
 import homelab_b200 as hb  # noqa: E402
 import paged_ref as R  # noqa: E402
 from homelab_b200 import _lib  # noqa: E402
-from homelab_b200.paged import PagedKv, rope_turns  # noqa: E402
+from homelab_b200.backend import Gpu  # noqa: E402
+from homelab_b200.paged import PagedKv, RopePlan, rope_turns  # noqa: E402
 
 FAKE = 0x10000  # never dereferenced: every call below fails its checks first
 
@@ -154,6 +155,7 @@ def test_rope_read_and_attention_refusals():
     assert prompt(d=96) == _lib.E_SHAPE
     assert prompt(kv_heads=0) == _lib.E_SHAPE
     assert prompt(out=FAKE) == _lib.E_ARG
+    assert prompt(k=2 * FAKE) == _lib.E_ARG  # the output over the keys
     assert prompt(ws=FAKE + 16) == _lib.E_ALIGN
     assert prompt(batch=0) == 0
 
@@ -183,3 +185,27 @@ def test_handles_refuse_what_does_not_fit():
         PagedKv(codes, codes.clone(), t, e)
     with pytest.raises(ValueError):
         PagedKv(codes, codes.clone(), t, e, e[:, :1])
+
+
+def test_methods_refuse_what_lives_elsewhere():
+    """A Gpu object that stands on the CPU: every call fails before a launch."""
+    g = Gpu.__new__(Gpu)
+    g.device, g.index, g.L, g._attn_ws = torch.device("cpu"), -1, hb.lib(), {}
+    plan = RopePlan("cpu", 128)
+    plan.index = 3
+    x, pos = torch.zeros(2, 4, 128, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="frequencies"):
+        g.rope(x, pos, plan)
+    k = torch.zeros(4, 2, 16, 128, dtype=torch.bfloat16)
+    cache = PagedKv(k, k.clone(), torch.zeros(2, 3, dtype=torch.int32))
+    kv = torch.zeros(2, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="frequencies"):
+        g.kv_append_paged(cache, kv, kv, None, pos, rope=plan)
+    ws = torch.zeros(1 << 20, dtype=torch.uint8)
+    for bad in (ws.view(torch.int32), ws[:64].expand(4, 64), ws[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            g.attention_paged(x, cache, x.clone(), None, pos, 1, 0.1, workspace=bad)
+        with pytest.raises(ValueError, match="workspace"):
+            g.attention_prompt(x, kv, kv, x.clone(), torch.tensor([0, 2], dtype=torch.int32), 2, 0.1, workspace=bad)
+    with pytest.raises(ValueError, match="q_start"):
+        g.attention_prompt(x, kv, kv, x.clone(), None, 2, 0.1)
