@@ -452,12 +452,13 @@ struct FaTiles {
     }
 };
 
-__device__ __noinline__ FaTiles fa_plan_tiles(const PattnParams& p, const FaWs& ws, int tq, int lane) {
-    unsigned* const err = blockIdx.x == 0 ? p.err : nullptr;
+// (Its arguments come by value: a reference to the kernel's parameters would be read through the caches.)
+__device__ __noinline__ FaTiles fa_plan_tiles(const int32_t* q_start, const int32_t* kv_len, int B, int T, int kv_max, int max_q, int Hkv,
+                                              int sms, int tq, int lane, FaSplit* splits, FaHead* head, unsigned* err) {
     Seq s{};
-    if (lane < p.B) {
-        s = read_seq(p.q_start, p.kv_len, lane, p.T, p.kv_max, err);
-        if (s.n > p.max_q) {
+    if (lane < B) {
+        s = read_seq(q_start, kv_len, lane, T, kv_max, err);
+        if (s.n > max_q) {
             record_error(err, ERR_KV_SEQ);
             s.n = 0;
         }
@@ -470,14 +471,14 @@ __device__ __noinline__ FaTiles fa_plan_tiles(const PattnParams& p, const FaWs& 
         }
         return v;
     };
-    const int mine = lane < p.B ? fa_tiles_of(s, tq) : 0, ends = scan(mine);
+    const int mine = lane < B ? fa_tiles_of(s, tq) : 0, ends = scan(mine);
     int tiles = __shfl_sync(0xffffffffu, ends, 31);
     if (tiles > 32) {  // only sequences that overlap each other make so many
         record_error(err, ERR_KV_SEQ);
         tiles = 0;
     }
     FaTiles t{};
-    for (int k = 0; k < p.B; k++) t.b += __shfl_sync(0xffffffffu, ends, k) <= lane;
+    for (int k = 0; k < B; k++) t.b += __shfl_sync(0xffffffffu, ends, k) <= lane;
     t.b = min(t.b, 31);
     t.s.q0 = __shfl_sync(0xffffffffu, s.q0, t.b);
     t.s.n = __shfl_sync(0xffffffffu, s.n, t.b);
@@ -486,33 +487,35 @@ __device__ __noinline__ FaTiles fa_plan_tiles(const PattnParams& p, const FaWs& 
     t.i0 = (lane - __shfl_sync(0xffffffffu, ends - mine, t.b)) * 2 * tq;
     t.keys = has ? fa_key_tiles(t.s, t.i0 + 2 * tq) : 0;
     const int work = has ? max(1, t.keys) : 0;
-    const unsigned long long all = static_cast<unsigned long long>(__reduce_add_sync(0xffffffffu, work));
-    const int share = max(kFaMinPart, static_cast<int>(min((all * p.Hkv + ws.sms - 1) / ws.sms, 1ull << 24)));
+    // (a 64-bit division would take longer than the rest; 2^28 tiles at most, and the slots have room for a share off by 2^-22)
+    const float even = static_cast<float>(__reduce_add_sync(0xffffffffu, work)) * Hkv * (1.0f / sms);
+    const int share = max(kFaMinPart, static_cast<int>(fminf(ceilf(even), 16777216.0f)));
     const int longest = max(1, __reduce_max_sync(0xffffffffu, work)), shortest = __reduce_min_sync(0xffffffffu, has ? work : 1 << 30);
     int chunk = longest;
     if (longest > share) {  // as plan_kernel chooses
-        int best = 1 << 30;
+        // lane k keeps the k-th length's units and its cost
+        const int eighths = lane == 0 ? 8 : lane == 1 ? 9 : lane == 2 ? 10 : lane == 3 ? 12 : 16;
+        const int len = lane < 5 ? (share * eighths + 7) / 8 : longest;
+        int units = 0;
 #pragma unroll 1
         for (int k = 0; k < 6; k++) {
-            const int eighths = k == 0 ? 8 : k == 1 ? 9 : k == 2 ? 10 : k == 3 ? 12 : 16;
-            const int len = k < 5 ? (share * eighths + 7) / 8 : longest;
-            const int units = __reduce_add_sync(0xffffffffu, (work + len - 1) / len);
-            const int cost = fa_cost(longest, shortest, share, len, units * p.Hkv, ws.sms);
-            if (cost < best) {
-                best = cost;
-                chunk = len;
-            }
+            const int of = __shfl_sync(0xffffffffu, len, k), sum = __reduce_add_sync(0xffffffffu, (work + of - 1) / of);
+            units = lane == k ? sum : units;
         }
+        const int cost = fa_cost(longest, shortest, share, len, units * Hkv, sms);
+        const int best = __reduce_min_sync(0xffffffffu, lane < 6 ? cost : 1 << 30);
+        chunk = __shfl_sync(0xffffffffu, len, __ffs(__ballot_sync(0xffffffffu, lane < 6 && cost == best)) - 1);
     }
     t.parts = has ? (work + chunk - 1) / chunk : 0;
-    const int ue = scan(t.parts), split = t.parts > 1 ? t.parts : 0;
-    t.first = ue - t.parts;
-    t.slot = scan(split) - split;
-    t.units = __shfl_sync(0xffffffffu, ue, 31);
+    // units in the low half, slots in the high one (no more than 32 and twice the SMs)
+    const int split = t.parts > 1 ? t.parts : 0, both = t.parts | split << 16, ue = scan(both);
+    t.first = (ue - both) & 0xffff;
+    t.slot = (ue - both) >> 16;
+    t.units = __shfl_sync(0xffffffffu, ue, 31) & 0xffff;
     if (blockIdx.x == 0) {  // for the join
         const unsigned m = __ballot_sync(0xffffffffu, split > 0);
-        if (split) ws.splits[__popc(m & ((1u << lane) - 1))] = FaSplit{t.s, t.i0, t.b, t.slot, t.parts, 0};
-        if (lane == 0) ws.head->splits = __popc(m);
+        if (split) splits[__popc(m & ((1u << lane) - 1))] = FaSplit{t.s, t.i0, t.b, t.slot, t.parts, 0};
+        if (lane == 0) head->splits = __popc(m);
     }
     return t;
 }
@@ -801,7 +804,9 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 return lane < 2 && u / p.Hkv < ws.max_units ? __ldcg(reinterpret_cast<const int4*>(ws.units + u / p.Hkv) + lane) : make_int4(0, 0, 0, 0);
             };
             FaTiles own;
-            if (ws.direct) own = fa_plan_tiles(p, ws, tq, lane);
+            if (ws.direct)
+                own = fa_plan_tiles(p.q_start, p.kv_len, p.B, p.T, p.kv_max, p.max_q, p.Hkv, ws.sms, tq, lane, ws.splits, ws.head,
+                                    blockIdx.x == 0 ? p.err : nullptr);
             auto record = [&](int u) { return ws.direct ? own.unit(u / p.Hkv, lane) : listed(u); };
             int next = blockIdx.x;
             int4 rec = record(next);
@@ -1081,14 +1086,14 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Pattn
     const int lane = threadIdx.x & 31;
     const int tq = fa_tokens(p.G);
     // a split tile's record and how many there are, read at once (the list is longer than the tiles can be)
-    const int64_t most = static_cast<int64_t>(ws.max_slots) * p.Hkv * kFaRows;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < most; i += static_cast<int64_t>(gridDim.x) * 8) {
-        const int r = static_cast<int>(i % kFaRows);
-        const int64_t tile = i / kFaRows;
-        const int kvh = static_cast<int>(tile % p.Hkv);
-        const int4* at = reinterpret_cast<const int4*>(ws.splits + tile / p.Hkv);
+    int most = ws.max_slots * p.Hkv * kFaRows;  // 512 rows an SM, or two slots
+    const int splits = __ldcg(&ws.head->splits);
+    for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < most; i += gridDim.x * 8) {
+        const int r = i % kFaRows, tile = i / kFaRows, of = tile / p.Hkv, kvh = tile - of * p.Hkv;
+        const int4* at = reinterpret_cast<const int4*>(ws.splits + of);
         const int4 sa = __ldcg(at), sb = __ldcg(at + 1);  // q0, n, len, i0; b, slot, parts
-        if (tile / p.Hkv >= __ldcg(&ws.head->splits)) break;
+        most = splits * p.Hkv * kFaRows;
+        if (i >= most) break;
         const int hr = r % kFaTile;
         const int token = sa.w + (r / kFaTile) * tq + hr / p.G, head = kvh * p.G + hr % p.G;
         if (hr / p.G >= tq || token >= sa.y) continue;
