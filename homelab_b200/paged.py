@@ -50,7 +50,7 @@ class PagedKv:
     (torch.float8_e4m3fn or uint8) with k_exp, v_exp uint8 [pages, kv_heads,
     page_size], a row's value being code * 2^(byte - 127).  Pages may be strided
     (keys and values side by side in one pool); the rows of a page are contiguous.
-    block_table int32 [batch, max_pages] (rows may be strided).
+    block_table int32 [batch, max_pages] (rows may be strided, but not overlap).
     """
 
     def __init__(self, k_pages, v_pages, block_table, k_exp=None, v_exp=None):
@@ -81,12 +81,14 @@ class PagedKv:
         ts, tsh = block_table.stride(), block_table.shape
         if block_table.dtype is not torch.int32 or len(ts) != 2 or (ts[1] != 1 and tsh[1] > 1):
             raise ValueError("block_table must be int32 [batch, max_pages] with contiguous rows")
+        if tsh[0] > 1 and ts[0] < tsh[1]:
+            raise ValueError("the rows of block_table must not overlap: copy a table that is expanded or a sliding view")
         self.k_pages, self.v_pages, self.k_exp, self.v_exp, self.block_table = k_pages, v_pages, k_exp, v_exp, block_table
         self.kv_heads, self.page_size, self.head_dim, self.fp8, self.device = heads, size, dim, fp8, k_pages.device
         self.batch, width = tsh
         self.max_pages = width
         self.struct = PagedKvStruct(
-            KV_E4M3 if fp8 else KV_BF16, heads, dim, size, pages, width, ts[0] if ts[0] > width else width, 0,
+            KV_E4M3 if fp8 else KV_BF16, heads, dim, size, pages, width, ts[0] if self.batch > 1 else width, 0,
             k_pages.data_ptr(), v_pages.data_ptr(), exps[0], exps[1], ks[0] if pages > 1 else heads * row, exps[2],
             block_table.data_ptr())
         self.ref = C.byref(self.struct)
