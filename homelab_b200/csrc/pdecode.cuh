@@ -15,10 +15,13 @@
 //
 // e4m3 codes are multiplied as they are.  A row of queries, scaled by a power of two so that its largest value lies
 // in [128, 256), is two e4m3 rows q1 = rn(q), q2 = rn(q - q1), which hold a bf16 value's eight bits down to
-// 2^-9 of 256 (smaller values are off by 2^-10 at most, 2^-17 of the row's largest).  A weight
-// w = 2^(x - m + 11) 2^(e - X), e its value row's exponent and X the largest met, is three e5m2 rows of
-// three significant bits each: off by at most 2^-9 of itself, down to 2^-16, which is 2^-27 of the
-// weight that m stands for.
+// 2^-9 of 256 (smaller values are off by 2^-10 at most, 2^-17 of the row's largest).  A weight, its value row's exponent e
+// taken into it, 2^(x - m + e - T + 11), is three e5m2 rows of three significant bits each: off by at most 2^-9 of itself, down
+// to 2^-16.  T is a query row's own, the largest x - m + e that it sees (and up to 2^4 below later ones), so what the terms
+// leave out is 2^-28 of the largest weighted value row that the query sees: neither a large row of little weight nor one that
+// is hidden from it costs bits.  While the exponents of a run lie within 2^6, as those of most caches do, T is the largest
+// exponent for all rows (2^-22); else it is found in a second look at the tile, in which rows of zeros do not count,
+// whatever their exponent.
 //
 // Work split: the batch's positions are cut into blocks of 128 for each (sequence, kv head, group of
 // 16 rows), a "pair" below, and the blocks, laid end to end, dealt evenly to the CTAs, whatever the
@@ -50,9 +53,13 @@ constexpr int kDecRowsAlways = 32, kDecRowsFew = 64;
 // that runs of 8 blocks make, 20.6 in 21 and 22.3 in 31; one of 60,000 48 us in the 37 that fill the SMs.
 constexpr int kDecParts = 16, kDecRun = 8;
 
-// e4m3: by how many powers of two the value rows hidden from a query row may pass those it sees, the weights' absolute
-// precision of 2^-27 of the largest falling to 2^-23.
-constexpr int kDecUnlike = 4;
+// e4m3.  Weights are made as 2^(x - n + 11 - 30) 2^(e - X + 30), X the largest exponent byte met and n = m - (X - T): the left
+// factor is what the sum of weights adds up, and stays an fp32 number (2^97 a position) while exponents lie within 2^112.  (n
+// is only a reference: what it loses where m is large cancels, but past 2^20 it could no longer hold X - T.)
+// Over 8 kv heads, eight sequences of 4,000 positions and 16 rows take 29.0 us if every run looks twice, 27.0 if only those past
+// 2^6 do; one of 4,096 and 4 rows 12.3 and 11.3.
+constexpr int kDecUnit = 30, kDecSpread = 112, kDecNear = 6;
+constexpr int kZeroByte = 127;  // the exponent that an append gives a row of zeros
 
 enum : unsigned {
     ERR_DEC_WAIT = 0xb00,  // a decode pipeline wait ran out (+ the waiting role)
@@ -71,14 +78,15 @@ struct DecodeGeo {
     static constexpr int Q_BYTES = (CH * NQ * CHUNK + 1023) / 1024 * 1024;
     static constexpr int P_STEP = (NP * kDecBlock * (F8 ? 1 : 2) + 1023) / 1024 * 1024;
     static constexpr int EXPS = 8;                              // tiles whose exponents are kept
-    static constexpr int REST = Q_BYTES + 2 * P_STEP + (F8 ? EXPS * 2 * kDecBlock : 0) + 1024;
+    static constexpr int BARS = 1280;                           // bytes of the barriers and of what the warps tell one another
+    static constexpr int REST = Q_BYTES + 2 * P_STEP + (F8 ? EXPS * 2 * kDecBlock : 0) + BARS;
     static constexpr int ROOM = 228 * 1024 / kDecCtas - 1024 - REST;
     static constexpr int STAGES = ROOM / TILE < 8 ? ROOM / TILE : 8;
     static constexpr int Q_OFF = STAGES * TILE;
     static constexpr int P_OFF = Q_OFF + Q_BYTES;
     static constexpr int EXP_OFF = P_OFF + 2 * P_STEP;
     static constexpr int BAR_OFF = EXP_OFF + (F8 ? EXPS * 2 * kDecBlock : 0);
-    static constexpr int TOTAL = BAR_OFF + 1024;
+    static constexpr int TOTAL = BAR_OFF + BARS;
     static constexpr int S_COLS = 32;                           // tensor-memory columns of a score buffer
     static constexpr int PAD = D + 4;                           // floats of a partial row
     static_assert(NQ <= S_COLS && NP <= 64, "tensor memory");
@@ -94,8 +102,9 @@ struct DecodeWs {
 struct DecodeBars {
     uint64_t kv_full[8], kv_empty[8], s_full[2], p_ready[2], p_free[2], q_ready, e_full[8];
     uint32_t tmem;
-    float red[4][kDecRows];
-    int redx[4];
+    float red[4][kDecRows], redt[4][kDecRows];
+    float n[kDecRows], top[kDecRows], fl[kDecRows], fo[kDecRows];  // a row's reference, largest score, and factors of a change
+    int redx[4], redn[4], redv[4];
     unsigned last;
     int4 start;               // the CTA's first sequence, its first block, the blocks of its pairs, its groups
     Seq start_seq;
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
     constexpr int ST = Geo::STAGES, CHUNK = Geo::CHUNK, CH = Geo::CH, PAD = Geo::PAD;
     extern __shared__ __align__(1024) uint8_t smem[];
     DecodeBars* bar = reinterpret_cast<DecodeBars*>(smem + Geo::BAR_OFF);
-    static_assert(sizeof(DecodeBars) <= 1024, "barriers");
+    static_assert(sizeof(DecodeBars) <= Geo::BARS, "barriers");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (smem_addr(smem) & 1023u) {  // the swizzle's pattern starts there
         if (tid == 0) record_error(p.err, ERR_DEC_WAIT + 15);
@@ -485,8 +494,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
     } else {
         // ---- softmax: a position's thread, then an output dimension's ----
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-        constexpr float kSlack = F8 ? 4.0f : 8.0f, kLift = F8 ? 11.0f : 0.0f;
-        unsigned t = 0;
+        constexpr float kSlack = F8 ? 4.0f : 8.0f, kBase = F8 ? 11.0f - kDecUnit : 0.0f;
+        unsigned t = 0, v_item = 0;  // tiles so far, and what the loader brought before the segment
         bool stop = false;
         // the four warps meet; whether any says so
         auto meet = [&](bool any) {
@@ -514,10 +523,11 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 scale[r] = p.scale_log2;
                 vis[r] = r < rows ? max(0, min(sq.len, sq.len - sq.n + (row0 + r) / p.G + 1)) : 0;
             }
-            int X = 0;  // e4m3: the exponent byte that the outputs are counted in
-            // the largest exponent of the positions that every row sees, or where the segment has none such the least (from 255)
-            const bool shared = g.tok0 < vis[0];
-            int seen = 0;
+            int X = 0;       // e4m3: the exponent byte that the outputs are counted in
+            int low = 255;   // the least of this thread's positions
+            bool thin = false;  // one of them raised a reference with codes below 2
+            bool wide = false;  // the exponents lie apart
+            if (F8 && tid < R) bar->n[tid] = bar->top[tid] = -INFINITY;
             if (g.tiles > 0) {
                 // ---- the queries as the scores' second operand; the last segment's scores are all made ----
                 if constexpr (!F8) {
@@ -595,16 +605,20 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     wait(&bar->e_full[e], (t / Geo::EXPS) & 1, 7);
                     const uint8_t* ep = smem + Geo::EXP_OFF + e * 2 * kDecBlock;
                     kf = exp_byte(ep[tid]);
-                    ve = tok < g.tok1 ? ep[kDecBlock + tid] : 0;
-                    if (tok < (shared ? vis[0] : g.tok1)) seen = max(seen, shared ? ve : 255 - ve);
+                    if (tok < g.tok1) {
+                        ve = ep[kDecBlock + tid];
+                        low = min(low, ve);
+                    }
                 }
-                bool over = ve > X;
+                // (2^(e - X + 30) is to stay an fp32 number)
+                bool over = F8 && (ve > X + 60 || (!wide && low + kDecNear < X));
+                const float top = kSlack + static_cast<float>(X - ve);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     float x = F8 ? (s[r] + s[R + r]) * (scale[r] * kf) : s[r] * scale[r];
                     if (tok >= vis[r]) x = -INFINITY;
                     s[r] = x;
-                    over |= x > m[r] + kSlack || (m[r] == -INFINITY && x != -INFINITY);
+                    over |= x > m[r] + top || (m[r] == -INFINITY && x != -INFINITY);
                 }
                 if (meet(over || gone)) {
                     // the tile's maxima over its positions, and the outputs so far brought to them
@@ -615,8 +629,12 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         if (lane == 0) bar->red[warp][r] = x;
                     }
                     if constexpr (F8) {
-                        const int x = __reduce_max_sync(0xffffffffu, ve);
-                        if (lane == 0) bar->redx[warp] = x;
+                        const int x = __reduce_max_sync(0xffffffffu, over ? ve : 0), n = __reduce_min_sync(0xffffffffu, low);
+                        const bool none = __any_sync(0xffffffffu, over && ve == kZeroByte);
+                        if (lane == 0) {
+                            bar->redx[warp] = x;
+                            bar->redn[warp] = none ? -1 : n;  // a row of zeros, maybe
+                        }
                     }
                     if (i > 0) wait(&bar->p_free[(t - 1) & 1], ((t - 1) >> 1) & 1, 8);  // the outputs are at rest
                     if (meet(gone)) {
@@ -624,17 +642,72 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         break;
                     }
                     float f[R];
-                    int xn = X;
-                    if constexpr (F8) xn = max(max(X, max(bar->redx[0], bar->redx[1])), max(bar->redx[2], bar->redx[3]));
-                    const float fx = F8 && i > 0 ? exp2_fast(static_cast<float>(X - xn)) : 1.0f;
-                    X = xn;
+                    auto over_warps = [&](const float (&x)[4][kDecRows], int r) { return fmaxf(fmaxf(x[0][r], x[1][r]), fmaxf(x[2][r], x[3][r])); };
+                    if constexpr (F8) {
+                        int xn = max(max(X, max(bar->redx[0], bar->redx[1])), max(bar->redx[2], bar->redx[3]));
+                        const int ln = min(min(bar->redn[0], bar->redn[1]), min(bar->redn[2], bar->redn[3]));
+                        const bool look = wide || ln < 0 || xn - ln > kDecNear;
+                        if (look) {
+                            // ---- the second look: how large this tile's weighted value rows are ----
+                            if (__any_sync(0xffffffffu, over)) {  // what these positions' value rows hold
+                                const unsigned item = v_item + (i + 1 < g.tiles ? 2 * i + 2 : 2 * g.tiles - 1);
+                                wait(&bar->kv_full[item % ST], (item / ST) & 1, 10);
+                                const uint8_t* row = smem + (item % ST) * Geo::TILE + tid * CHUNK;
+                                unsigned bits = 0;
 #pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        const float mn = fmaxf(m[r], fmaxf(fmaxf(bar->red[0][r], bar->red[1][r]), fmaxf(bar->red[2][r], bar->red[3][r])));
-                        const float c = m[r] == -INFINITY ? 0.0f : exp2_fast(m[r] - mn);
-                        l[r] *= c;
-                        f[r] = c * fx;
-                        m[r] = mn;
+                                for (int c = 0; c < CHUNK / 16; c++) {
+                                    const uint4 w = *reinterpret_cast<const uint4*>(row + (((c + tid) % (CHUNK / 16)) << 4));
+                                    bits |= w.x | w.y | w.z | w.w;
+                                }
+                                if (over && (bits & 0x7f7f7f7fu) == 0) ve = 0;
+                                thin |= over && ve > 0 && (bits & 0x40404040u) == 0;
+                            }
+                            const int v = __reduce_max_sync(0xffffffffu, over ? ve : 0);
+                            if (lane == 0) bar->redv[warp] = v;
+#pragma unroll
+                            for (int r = 0; r < R; r++) {
+                                float y = ve == 0 ? -INFINITY : (s[r] - over_warps(bar->red, r)) + static_cast<float>(ve);
+                                asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(y));
+                                if (lane == 0) bar->redt[warp][r] = y;
+                            }
+                            if (meet(gone)) {
+                                stop = true;
+                                break;
+                            }
+                            xn = max(max(X, max(bar->redv[0], bar->redv[1])), max(bar->redv[2], bar->redv[3]));
+                        }
+                        if (tid < R) {  // a row's thread
+                            const float was = bar->n[tid], tile = over_warps(bar->red, tid), mx = fmaxf(bar->top[tid], tile);
+                            const bool first = was == -INFINITY;
+                            float n = mx;
+                            if (look) {
+                                float T = over_warps(bar->redt, tid) + (tile - mx);
+                                // (an X that stood for T may have come from rows of zeros: too low a T costs nothing, the outputs are fp32)
+                                T = ceilf(fmaxf(T, first ? -INFINITY : (was - mx) + static_cast<float>(X) - (wide ? 0.0f : 60.0f)));
+                                n = mx - (static_cast<float>(xn) - fmaxf(T, static_cast<float>(xn - kDecSpread)));
+                            }
+                            bar->n[tid] = n;
+                            bar->top[tid] = mx;
+                            bar->fl[tid] = first ? 0.0f : exp2_fast(was - n);
+                            bar->fo[tid] = first ? 0.0f : exp2_fast((was - n) + static_cast<float>(X - xn));
+                        }
+                        X = xn;
+                        wide |= look;
+                        meet(false);
+#pragma unroll
+                        for (int r = 0; r < R; r++) {
+                            m[r] = bar->n[r];
+                            l[r] *= bar->fl[r];
+                            f[r] = bar->fo[r];
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < R; r++) {
+                            const float mn = fmaxf(m[r], over_warps(bar->red, r));
+                            f[r] = m[r] == -INFINITY ? 0.0f : exp2_fast(m[r] - mn);
+                            l[r] *= f[r];
+                            m[r] = mn;
+                        }
                     }
                     if (i > 0) {
                         tc_fence_after();
@@ -650,11 +723,11 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 // ---- weights, as the outputs' second operand ----
                 wait(&bar->p_free[t & 1], ((t >> 1) & 1) ^ 1, 9);
                 uint8_t* pw = smem + Geo::P_OFF + (t & 1) * Geo::P_STEP;
-                const float vf = F8 ? exp2_fast(static_cast<float>(ve - X)) : 1.0f;
+                const float vf = F8 ? exp2_fast(static_cast<float>(ve - X + kDecUnit)) : 1.0f;
 #pragma unroll
                 for (int r = 0; r < R; r += 2) {
-                    float a = exp2_fast(s[r] - (m[r] == -INFINITY ? 0.0f : m[r]) + kLift);
-                    float b = exp2_fast(s[r + 1] - (m[r + 1] == -INFINITY ? 0.0f : m[r + 1]) + kLift);
+                    float a = exp2_fast(s[r] - (m[r] == -INFINITY ? 0.0f : m[r]) + kBase);
+                    float b = exp2_fast(s[r + 1] - (m[r + 1] == -INFINITY ? 0.0f : m[r + 1]) + kBase);
                     l[r] += a;
                     l[r + 1] += b;
                     if constexpr (F8) {
@@ -695,38 +768,53 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
             warp_reduce_multi<R>(l, lane);  // the lane's l[0] is the warp's sum of row reduce_index
             bar->red[warp][reduce_index<R>(lane, 0)] = l[0];
             if constexpr (F8) {
-                const int x = __reduce_max_sync(0xffffffffu, seen);
-                if (lane == 0) bar->redx[warp] = x;
+                const int x = __reduce_min_sync(0xffffffffu, low);
+                const unsigned y = __ballot_sync(0xffffffffu, thin);
+                if (lane == 0) bar->redx[warp] = y ? x - 256 : x;
             }
             meet(false);
-            float unit = 1.0f;
+            // Exponents further apart than the weights can follow, scores past what a reference holds beside them, or a reference
+            // raised by a row whose codes do not fill its exponent (an append writes none): every row is done again below.
+            bool lost = false;
             if constexpr (F8) {
-                // Value rows that only some of the query rows see, so much larger than what the others do that these lost
-                // their weights' last bits to them: not a number, and done again below.
-                const int x = max(max(bar->redx[0], bar->redx[1]), max(bar->redx[2], bar->redx[3]));
-                const bool lost = sq.n > 1 && X > (shared ? x : 255 - x) + kDecUnlike;
-                unit = lost ? __uint_as_float(0x7fffffffu) : exp_byte(static_cast<unsigned>(X));
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const int x = bar->redx[w];
+                    low = min(low, x < 0 ? x + 256 : x);
+                    thin |= x < 0;
+                }
+                lost = X - low > (thin ? 8 : kDecSpread);
+                for (int r = 0; wide && r < rows; r++) lost |= fabsf(bar->top[r]) > 1048576.0f && bar->top[r] != -INFINITY;
+                v_item += 2 * g.tiles;
             }
             const int first = walk.deal.owner(g.pair_first), final_cta = walk.deal.owner(g.pair_end - 1);
             const int parts = final_cta - first + 1;
             float* my_part = ws.part + static_cast<int64_t>(2 * blockIdx.x + (g.lo == g.pair_first ? 1 : 0)) * ws.rows * PAD;
-            bool odd = false;
+            bool odd = lost;
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 if (r >= rows) continue;
-                const float ls = bar->red[0][r] + bar->red[1][r] + bar->red[2][r] + bar->red[3][r];
+                float ls = bar->red[0][r] + bar->red[1][r] + bar->red[2][r] + bar->red[3][r];
                 float x = o[r];
-                if constexpr (F8) x = (o[r] + o[R + r] + o[2 * R + r]) * unit;
+                if constexpr (F8) x = (o[r] + o[R + r] + o[2 * R + r]) * power_of(-kDecUnit) * exp_byte(static_cast<unsigned>(X));
                 if (parts == 1) {
                     x = vis[r] > 0 ? x / ls : 0.0f;
-                    odd |= tid < D && !(fabsf(x) <= 3.4e38f);
+                    odd |= sq.n > 1 && tid < D && !(fabsf(x) <= 3.4e38f);
                     const __nv_bfloat16 v = __float2bfloat16_rn(x);
                     if (tid < D)
                         *reinterpret_cast<__nv_bfloat16*>(p.out + static_cast<int64_t>(sq.q0 + (row0 + r) / p.G) * p.out_stride +
                                                           static_cast<int64_t>(g.kvh * p.G + (row0 + r) % p.G) * D + tid) = v;
                 } else {
+                    float mx = m[r];
+                    if (wide && mx != -INFINITY) {  // parts are joined by their largest scores
+                        mx = bar->top[r];
+                        const float back = exp2_fast(m[r] - mx);
+                        x *= back;
+                        ls *= back;
+                    }
                     if (tid < D) my_part[r * PAD + tid] = x;
-                    if (tid == 0) *reinterpret_cast<float2*>(my_part + r * PAD + D) = make_float2(m[r], ls);
+                    if (tid == 0)  // a sum below zero says that the range was passed
+                        *reinterpret_cast<float2*>(my_part + r * PAD + D) = make_float2(mx, lost ? -1.0f : ls);
                 }
             }
             if (parts > 1) {
@@ -771,6 +859,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
                                 const float f = exp2_fast(ml[i].x - b0);
+                                odd |= ml[i].y < 0.0f;
                                 a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
                                 ls = fmaf(f, ml[i].y, ls);
                             }
@@ -778,16 +867,17 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         const bool sees = sq.len > 0 && sq.len - sq.n + token >= 0;
                         const float inv = 1.0f / ls;
                         a = sees ? make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        odd |= !(fabsf(a.x) + fabsf(a.y) + fabsf(a.z) + fabsf(a.w) <= 3.4e38f);
+                        odd |= sq.n > 1 && !(fabsf(a.x) + fabsf(a.y) + fabsf(a.z) + fabsf(a.w) <= 3.4e38f);
                         *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(sq.q0 + token) * p.out_stride +
                                                   static_cast<int64_t>(g.kvh * p.G + row0 + r - token * p.G) * D + d) =
                             make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
                     }
                 }
             }
-            // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the products: then (and
-            // where a huge one took the weights' bits) every row is done again in plain loops over what it sees.  (A single new token sees everything.)
-            if (meet(odd) && sq.n > 1) {
+            // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the products (a single new
+            // token sees everything): then, and where the weights' range was passed, every row is done again in plain loops over
+            // what it sees.
+            if (meet(odd)) {
                 for (int r = warp; r < rows; r += 4) {
                     const int token = (row0 + r) / p.G, head = g.kvh * p.G + row0 + r - token * p.G;
                     const int see = max(0, min(sq.len, sq.len - sq.n + token + 1));

@@ -1,0 +1,204 @@
+"""Attention over e4m3 pages whose rows' powers of two lie far apart, on the GPU, against float64 (tests/paged_ref.py)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import paged_ref as R  # noqa: E402
+from homelab_b200.backend import Gpu  # noqa: E402
+from homelab_b200.paged import PagedKv  # noqa: E402
+
+if not torch.cuda.is_available():
+    pytest.skip("needs a GPU", allow_module_level=True)
+
+DEV = torch.device("cuda", 0)
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    g = Gpu(0)
+    yield g
+    torch.cuda.synchronize()
+    assert g.device_error() == 0
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def normal(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
+
+
+def quantise(x):
+    """x [L, K, D] as e4m3 codes and exponent bytes, as the cache's write makes them."""
+    L, K, _ = x.shape
+    e = torch.tensor([[R.exponent(float(x[j, h].abs().max()), 448.0) for h in range(K)] for j in range(L)])
+    codes = (x.double() * torch.exp2(-e.double())[..., None]).float().to(torch.float8_e4m3fn)
+    return codes, (e + 127).to(torch.uint8)
+
+
+def paged(codes_k, ke, codes_v, ve, page):
+    """Rows [L, K, D] as a pool of their own with shuffled pages and a table of one sequence."""
+    L, K, D = codes_k.shape
+    n = -(-L // page)
+    order = torch.randperm(n, generator=torch.Generator().manual_seed(L)).to(torch.int32)
+    pools = []
+    for x in (codes_k.view(torch.uint8), codes_v.view(torch.uint8), ke, ve):
+        full = torch.full((n * page, *x.shape[1:]), 255 if x.dim() == 2 else 0x7f, dtype=torch.uint8)  # behind the end
+        full[:L] = x
+        full = full.unflatten(0, (n, page)).transpose(1, 2)
+        pool = torch.empty_like(full, memory_format=torch.contiguous_format)
+        pool[order.long()] = full
+        pools.append(pool.to(DEV))
+    return PagedKv(pools[0], pools[1], order[None].to(DEV), pools[2], pools[3])
+
+
+def stands_for(codes, e):
+    """A row's values, as fp32 numbers: what passes fp32's range is infinite, and 0 * inf NaN."""
+    return (codes.double() * torch.exp2(e.double() - 127)[..., None]).float().double()
+
+
+def check(gpu, q, ck, ke, cv, ve, page, scale, n_before):
+    """Attention of q's tokens behind n_before positions, within the bound of every row's own magnitudes.  On top comes what
+    the three e5m2 terms of a weight leave out: half of their last unit 2^-16 at a largest weighted row of 2^11, so 2^-28 of
+    that row (codes up to 448) for each position, and 2^-22 where exponents within 2^6 of one another share one reference."""
+    n, H, D = q.shape
+    L, K, _ = ck.shape
+    out = torch.empty(n, H, D, dtype=torch.bfloat16, device=DEV)
+    gpu.attention_paged(q.to(DEV), paged(ck, ke, cv, ve, page), out, i32([0, n]), i32([L]), n, scale)
+    k, v = stands_for(ck, ke), stands_for(cv, ve)
+    want, mag, big = R.attend(q.double(), k, v, n_before, scale)
+    _, least, _ = R.attend(q.double(), k, v.abs().clamp(max=3.4e38).amax(-1, keepdim=True).expand_as(v), n_before, scale)
+    bound = R.attention_bound(want, mag, big, D) + L * 2.0 ** -22 * least
+    out = out.cpu().double()
+    none = torch.isnan(want)
+    assert torch.equal(torch.isnan(out), none)
+    err = torch.where(out == want, 0.0, (out - want).abs())  # infinities among them
+    assert (err <= bound)[~none].all(), float((err / bound)[~none].max())
+    return out
+
+
+def one_loud_row(L, K, D, spread, seed, where):
+    """Keys and values as usual, but for position `where`: its value row is 2^spread larger, its key points away from q."""
+    q = normal(seed, 1, 4 * K, D).to(torch.bfloat16)
+    k, v = normal(seed + 1, L, K, D), normal(seed + 2, L, K, D)
+    k[where] = -2.0 * q[0].float().unflatten(0, (K, 4)).mean(1)
+    v[where] *= 2.0 ** spread
+    return q, k, v
+
+
+@pytest.mark.parametrize("spread", [6, 12, 18, 20, 24, 30, 60, 100])
+@pytest.mark.parametrize("L,where", [(90, 3), (1000, 0), (1000, 700), (1000, 999), (9000, 8000)])
+def test_a_visible_large_row_of_little_weight_costs_no_bits(gpu, spread, L, where):
+    """One new token: a value row up to 2^100 larger, whose weight is too small to count, leaves the others' weights alone."""
+    K, D = 2, 128
+    q, k, v = one_loud_row(L, K, D, spread, 17, where)
+    scale = (spread + 20.0) * math.log(2.0) / float((q[0].float() ** 2).sum(-1).min()) * 4
+    check(gpu, q, *quantise(k), *quantise(v), 16, scale, L - 1)
+
+
+@pytest.mark.parametrize("n,H", [(1, 8), (3, 8), (4, 4), (7, 16), (16, 2), (30, 2), (200, 8)])
+@pytest.mark.parametrize("spread", [18, 30, 70])
+def test_large_rows_seen_by_some(gpu, n, H, spread):
+    """Drafts and chunks: rows of every size among the cached positions and among the new ones, so that some query rows see a
+    large one and some do not, its weight small or whole."""
+    K, D, a = 2, 128, 333
+    L = a + n
+    q = normal(31, n, H, D).to(torch.bfloat16)
+    k, v = normal(32, L, K, D), normal(33, L, K, D)
+    for j in (5, 200, a, a + n // 2, L - 1):
+        v[j] *= 2.0 ** spread
+        if j % 2:
+            k[j] = -20.0 * q[n - 1, :K].float()
+    check(gpu, q, *quantise(k), *quantise(v), 32, 0.09, a)
+
+
+@pytest.mark.parametrize("n,H", [(1, 8), (5, 8), (16, 2), (100, 8)])
+@pytest.mark.parametrize("tiny", [1e-3, 1e-4, 1e-5, 1e-12])
+@pytest.mark.parametrize("zeros", [[0], [7, 130, 131, 400], list(range(0, 420, 3))])
+def test_rows_of_zeros_among_small_values(gpu, n, H, tiny, zeros):
+    """A row of zeros is written with exponent 0, far above the exponents of small values: it must not cost them bits."""
+    K, D, a = 2, 128, 420
+    L = a + n
+    q = normal(41, n, H, D).to(torch.bfloat16)
+    k, v = normal(42, L, K, D), normal(43, L, K, D) * tiny
+    v[zeros] = 0.0
+    check(gpu, q, *quantise(k), *quantise(v), 64, 0.09, a)
+
+
+@pytest.mark.parametrize("n,H", [(1, 8), (6, 8), (90, 8)])
+@pytest.mark.parametrize("size", [300.0, 20.0, 1.0, 0.01])
+@pytest.mark.parametrize("sinks,L", [([0], 400), ([0, 1, 2, 3], 3000), ([260], 300)])
+def test_rows_of_zeros_that_take_the_weight(gpu, n, H, size, sinks, L):
+    """Positions of zero values whose keys draw all but 2^-15 of the weight: the rest keeps its bits."""
+    K, D = 2, 128
+    q = normal(55, n, H, D)
+    q = (q + 2.0).to(torch.bfloat16)  # a direction that all queries share
+    k, v = normal(56, L, K, D), normal(57, L, K, D) * size
+    k[sinks], v[sinks] = 1.0, 0.0
+    scale = 15.0 * math.log(2.0) / float(q.float().sum(-1).mean())
+    check(gpu, q, *quantise(k), *quantise(v), 16, scale, L - n)
+
+
+def test_every_row_is_zero(gpu):
+    K, D, L = 2, 128, 300
+    q, k = normal(51, 1, 8, D).to(torch.bfloat16), normal(52, L, K, D)
+    out = check(gpu, q, *quantise(k), *quantise(torch.zeros(L, K, D)), 16, 0.09, L - 1)
+    assert not out.any()
+    # and zeros in front of the first row that is none, where the others' weights are the larger ones
+    v = torch.zeros(L, K, D)
+    v[250:] = normal(53, 50, K, D) * 1e-6
+    k[:250] = 2.0 * q[0].float().unflatten(0, (K, 4)).mean(1)
+    check(gpu, q, *quantise(k), *quantise(v), 16, 0.09, L - 1)
+
+
+@pytest.mark.parametrize("n,H", [(1, 8), (6, 8), (90, 8)])
+@pytest.mark.parametrize("loud", [250, 245, 240, 200])
+def test_exponents_over_the_whole_range(gpu, n, H, loud):
+    """Bytes from 1 to 254, in pools that no append wrote: codes that do not fill their exponent among them."""
+    K, D, a = 2, 128, 400
+    L = a + n
+    g = torch.Generator().manual_seed(61)
+    q = normal(62, n, H, D).to(torch.bfloat16)
+    ck, ke = quantise(normal(63, L, K, D))
+    cv = (normal(64, L, K, D) * 30).to(torch.float8_e4m3fn)
+    ve = torch.randint(1, 110, (L, K), generator=g, dtype=torch.uint8)
+    ve[50] = loud
+    ck[50] = (-q[0, :K].float() * 100).to(torch.float8_e4m3fn)  # hardly any weight
+    ke[50] = 140
+    check(gpu, q, ck, ke, cv, ve, 16, 0.3, a)
+    cv, ve = (normal(65, L, K, D) * 30).to(torch.float8_e4m3fn), torch.full((L, K), 100, dtype=torch.uint8)
+    cv[77] = (normal(66, K, D) * 2.0 ** -8).to(torch.float8_e4m3fn)  # a few units of the smallest code under a large byte
+    ve[77] = 120
+    check(gpu, q, ck, ke, cv, ve, 16, 0.09, a)
+
+
+@pytest.mark.parametrize("n", [1, 5])
+def test_large_values_do_not_pass_fp32_on_the_way(gpu, n):
+    """Value rows near 2^120 over thousands of positions: their mean is an fp32 number, their sum is none."""
+    K, D, a = 1, 64, 5000
+    L = a + n
+    q = normal(71, n, 8, D).to(torch.bfloat16)
+    k, v = normal(72, L, K, D), normal(73, L, K, D)
+    v = v.clamp(-3, 3) * 2.0 ** 117
+    check(gpu, q, *quantise(k), *quantise(v), 64, 0.05, a)
+
+
+def test_scores_of_a_billion(gpu):
+    """Scores so large that an exponent added to them is rounded away: the largest takes all the weight."""
+    K, D, L = 1, 128, 700
+    q = torch.ones(1, 8, D).to(torch.bfloat16)
+    ck = torch.full((L, K, D), 0.5).to(torch.float8_e4m3fn)
+    ke = torch.full((L, K), 127, dtype=torch.uint8)
+    ck[333] = 1.0
+    cv, ve = quantise(normal(81, L, K, D))
+    ve[::3] -= 40
+    ve[333] = 90
+    out = torch.empty(1, 8, D, dtype=torch.bfloat16, device=DEV)
+    for scale in (1e4, 1e7, 1e12, 1e30):
+        gpu.attention_paged(q.to(DEV), paged(ck, ke, cv, ve, 16), out, i32([0, 1]), i32([L]), 1, scale)
+        want = stands_for(cv, ve)[333, 0].expand(8, D)
+        assert ((out[0].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs()).all()
