@@ -14,8 +14,8 @@
 // (32 sequences of 1,001 to 16,098 positions, 32 heads over 8, e4m3 pages).
 //
 // e4m3 codes are multiplied as they are.  A row of queries, scaled by a power of two so that its largest value lies
-// in [128, 256), is two e4m3 rows q1 = rn(q), q2 = rn(q - q1), which hold a bf16 value's eight bits down to
-// 2^-9 of 256 (smaller values are off by 2^-10 at most, 2^-17 of the row's largest).  A weight, its value row's exponent e
+// in [128, 256), is two e4m3 rows q1 = rn(q), q2 = rn(2^5 (q - q1)) (|q - q1| <= 8), which hold a bf16 value's eight bits down
+// to 2^-7 (smaller values are off by 2^-15 at most, 2^-22 of the row's largest).  A weight, its value row's exponent e
 // taken into it, 2^(x - m + e - T + 11), is three e5m2 rows of three significant bits each: off by at most 2^-9 of itself, down
 // to 2^-16.  T is a query row's own, the largest x - m + e that it sees (and up to 2^4 below later ones), so what the terms
 // leave out is 2^-28 of the largest weighted value row that the query sees: neither a large row of little weight nor one that
@@ -59,6 +59,7 @@ constexpr int kDecParts = 16, kDecRun = 8;
 // Over 8 kv heads, eight sequences of 4,000 positions and 16 rows take 29.0 us if every run looks twice, 27.0 if only those past
 // 2^6 do; one of 4,096 and 4 rows 12.3 and 11.3.
 constexpr int kDecUnit = 30, kDecSpread = 112, kDecNear = 6;
+constexpr float kRestUp = 32.0f;  // what q - q1 is multiplied by
 constexpr int kZeroByte = 127;  // the exponent that an append gives a row of zeros
 
 enum : unsigned {
@@ -574,6 +575,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                                 float a = f[i] * up, b = f[i + 1] * up, d = f[i + 2] * up, e = f[i + 3] * up;
                                 if (a != a || b != b || d != d || e != e || bad) a = __uint_as_float(0x7fffffffu);
                                 const unsigned h0 = split_e4m3(a, b), h1 = split_e4m3(d, e);
+                                a *= kRestUp, b *= kRestUp, d *= kRestUp, e *= kRestUp;
                                 const unsigned l0 = split_e4m3(a, b), l1 = split_e4m3(d, e);
                                 const int at = c * V + i;  // byte of the row
                                 *reinterpret_cast<unsigned*>(q1 + dec_swizzle(CHUNK, r, at / 16) + at % 16) = h0 | (h1 << 16);
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 const float top = kSlack + static_cast<float>(X - ve);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    float x = F8 ? (s[r] + s[R + r]) * (scale[r] * kf) : s[r] * scale[r];
+                    float x = F8 ? fmaf(s[R + r], 1.0f / kRestUp, s[r]) * (scale[r] * kf) : s[r] * scale[r];
                     if (tok >= vis[r]) x = -INFINITY;
                     s[r] = x;
                     over |= x > m[r] + top || (m[r] == -INFINITY && x != -INFINITY);

@@ -61,10 +61,11 @@ def stands_for(codes, e):
     return (codes.double() * torch.exp2(e.double() - 127)[..., None]).float().double()
 
 
-def check(gpu, q, ck, ke, cv, ve, page, scale, n_before):
+def check(gpu, q, ck, ke, cv, ve, page, scale, n_before, score_err=0.0):
     """Attention of q's tokens behind n_before positions, within the bound of every row's own magnitudes.  On top comes what
     the three e5m2 terms of a weight leave out: half of their last unit 2^-16 at a largest weighted row of 2^11, so 2^-28 of
-    that row (codes up to 448) for each position, and 2^-22 where exponents within 2^6 of one another share one reference."""
+    that row (codes up to 448) for each position, and 2^-22 where exponents within 2^6 of one another share one reference.  An
+    error of the scores counts twice, in the weight and in the sum it is divided by."""
     n, H, D = q.shape
     L, K, _ = ck.shape
     out = torch.empty(n, H, D, dtype=torch.bfloat16, device=DEV)
@@ -73,6 +74,8 @@ def check(gpu, q, ck, ke, cv, ve, page, scale, n_before):
     want, mag, big = R.attend(q.double(), k, v, n_before, scale)
     _, least, _ = R.attend(q.double(), k, v.abs().clamp(max=3.4e38).amax(-1, keepdim=True).expand_as(v), n_before, scale)
     bound = R.attention_bound(want, mag, big, D) + L * 2.0 ** -22 * least
+    if score_err:
+        bound = bound + 2 * score_err * mag
     out = out.cpu().double()
     none = torch.isnan(want)
     assert torch.equal(torch.isnan(out), none)
@@ -127,6 +130,25 @@ def test_rows_of_zeros_among_small_values(gpu, n, H, tiny, zeros):
     k, v = normal(42, L, K, D), normal(43, L, K, D) * tiny
     v[zeros] = 0.0
     check(gpu, q, *quantise(k), *quantise(v), 64, 0.09, a)
+
+
+@pytest.mark.parametrize("n,H", [(1, 8), (5, 8), (16, 2), (100, 8)])
+@pytest.mark.parametrize("apart", [6, 10, 13])
+@pytest.mark.parametrize("a", [2, 300])
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_with_channels_of_unlike_size(gpu, n, H, apart, a, D):
+    """A few channels of the queries 2^apart larger than the rest, those of the keys as much smaller: the small ones make
+    most of a score.  A query's two terms are off by 2^-22 of its largest value in each channel."""
+    K = 2
+    L = a + n
+    q, k, v = normal(91, n, H, D), normal(92, L, K, D) * 2.0, normal(93, L, K, D)
+    q[..., 3::40] *= 2.0 ** apart
+    k[..., 3::40] *= 2.0 ** -apart
+    q = q.to(torch.bfloat16)
+    ck, ke = quantise(k)
+    cv, ve = quantise(v)
+    more = 2.0 ** -22 * float(q.float().abs().max()) * stands_for(ck, ke).abs().sum(-1).max() * 0.09
+    check(gpu, q, ck, ke, cv, ve, 16, 0.09, a, score_err=float(more))
 
 
 @pytest.mark.parametrize("n,H", [(1, 8), (6, 8), (90, 8)])
