@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         }
 #pragma unroll
                         for (int o = 1; o < 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                        const int ex = max(-100, min(100, static_cast<int>(__float_as_uint(big) >> 23) - 127 - 7));
+                        const int ex = max(-126, static_cast<int>(__float_as_uint(big) >> 23) - 127 - 7);  // 2^ex and 2^-ex are fp32 numbers
                         const float up = power_of(-ex);
                         if (r < R) {
                             if (c == 0) bar->red[0][r] = power_of(ex);

@@ -151,6 +151,16 @@ def test_queries_with_channels_of_unlike_size(gpu, n, H, apart, a, D):
     check(gpu, q, ck, ke, cv, ve, 16, 0.09, a, score_err=float(more))
 
 
+@pytest.mark.parametrize("n,H", [(1, 8), (5, 8), (16, 2), (100, 8)])
+@pytest.mark.parametrize("power", [120, 112, 95, -95, -112, -118])
+def test_queries_of_any_size(gpu, n, H, power):
+    """Queries near both ends of bf16's range, and a scale that brings their scores back."""
+    K, D, a = 2, 128, 150
+    L = a + n
+    q = (normal(95, n, H, D) * 2.0 ** power).to(torch.bfloat16)
+    check(gpu, q, *quantise(normal(96, L, K, D)), *quantise(normal(97, L, K, D)), 16, 0.09 * 2.0 ** -power, a)
+
+
 @pytest.mark.parametrize("n,H", [(1, 8), (6, 8), (90, 8)])
 @pytest.mark.parametrize("size", [300.0, 20.0, 1.0, 0.01])
 @pytest.mark.parametrize("sinks,L", [([0], 400), ([0, 1, 2, 3], 3000), ([260], 300)])
