@@ -10,6 +10,7 @@ current torch stream; nothing synchronises the host.
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 
 import torch
 
@@ -65,6 +66,9 @@ _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.
 _ANY, _BF16 = (torch.float32, torch.bfloat16), (torch.bfloat16,)
 
 
+_gpus = weakref.WeakSet()  # every Gpu of the process
+
+
 class Gpu:
     """One device's backend (the counterpart of `oominf_cuda::Gpu`)."""
 
@@ -75,6 +79,7 @@ class Gpu:
         self._tiled_ws = None  # grown on demand by moe_tiled calls without a workspace
         # paged and prompt attention without a workspace: one per stream, grown on demand, and the shapes known to fit it
         self._attn_ws = {}
+        _gpus.add(self)
 
     def _stream(self) -> int:
         return torch.cuda.current_stream(self.device).cuda_stream
@@ -449,8 +454,14 @@ class Gpu:
                      max_q, scale, ws.data_ptr(), ws.numel())
 
     def device_error(self, clear: bool = True) -> int:
+        """The device's error word (0: none).  A wait that ran out leaves counts behind in attention workspaces: after an
+        error the ones that this process's Gpu objects keep are made anew; a caller's own is the caller's to zero."""
         code = C.c_int(0)
         self.L.oomb_device_error(C.byref(code), int(clear))
+        if code.value:
+            for g in [self, *_gpus]:
+                if g.index == self.index:
+                    g._attn_ws = {}
         return code.value
 
     def set_wait_limit(self, ns: int = 0) -> None:

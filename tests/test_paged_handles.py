@@ -3,6 +3,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from homelab_b200 import backend  # noqa: E402
+from homelab_b200.backend import Gpu  # noqa: E402
 from homelab_b200.paged import PagedKv  # noqa: E402
 
 
@@ -42,3 +44,86 @@ def test_block_table_rows_are_read_where_they_lie(table):
     k, v = pool()
     rows, want = reach(table, PagedKv(k, v, table))
     assert rows == want
+
+
+class FakeLibrary:
+    """The entry points that the calls below reach, on the CPU: what they were given, and a device error word."""
+
+    def __init__(self):
+        self.error, self.workspaces, self.waits = 0, [], 0.0
+
+    def oomb_device_error(self, code, clear):
+        code._obj.value = self.error
+        if clear:
+            self.error = 0
+        return 0
+
+    def oomb_attention_paged_workspace_bytes(self, *args):
+        return 8192
+
+    def oomb_attention_prompt_workspace_bytes(self, *args):
+        return 8192
+
+    def oomb_attention_paged(self, *args):
+        self.workspaces.append(args[13])
+        return 0
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Gpu objects that stand on the CPU, over one FakeLibrary."""
+    lib = FakeLibrary()
+
+    class Here:
+        def __init__(self, *a):
+            pass
+
+        def __enter__(self):
+            return self
+
+        def __exit__(self, *a):
+            return False
+
+    monkeypatch.setattr(backend, "_current_device", lambda: -1)
+    monkeypatch.setattr(backend, "_raw_stream", lambda i: 77)
+    monkeypatch.setattr(backend, "_capturing", lambda: False)
+    monkeypatch.setattr(backend.torch.cuda, "device", Here)
+    monkeypatch.setattr(backend._lib, "lib", lambda: lib)
+    monkeypatch.setattr(backend.torch, "device", lambda *a: torch.empty(0).device)
+
+    def make():
+        g = Gpu(-1)
+        assert g.L is lib
+        return g
+
+    return lib, make
+
+
+def attend(g):
+    k, v = pool(dim=128)
+    cache = PagedKv(k, v, torch.zeros(2, 3, dtype=torch.int32))
+    x = torch.zeros(2, 4, 128, dtype=torch.bfloat16)
+    g.attention_paged(x, cache, x.clone(), None, torch.ones(2, dtype=torch.int32), 1, 0.1)
+
+
+def counters(g):
+    """The words that have to be zero, of the workspace that the object keeps."""
+    return next(w for k, w in g._attn_ws.items() if isinstance(k, int))[:backend._lib.ATTENTION_ZERO_BYTES]
+
+
+def test_kept_workspaces_are_zero_again_after_a_device_error(host):
+    lib, make = host
+    g, other = make(), make()
+    attend(g), attend(other)
+    attend(g)
+    assert lib.workspaces[0] == lib.workspaces[2] != lib.workspaces[1], "one is kept"
+    for x in (g, other):
+        counters(x)[5] = 1  # an arrival that the call which gave up left behind
+    lib.error = 0xb06
+    assert g.device_error() == 0xb06
+    attend(g), attend(other)
+    assert not counters(g).any() and not counters(other).any()
+    kept = counters(g)
+    assert g.device_error() == 0
+    attend(g)
+    assert counters(g).data_ptr() == kept.data_ptr(), "without an error nothing is made anew"
