@@ -65,7 +65,7 @@ class FakeLibrary:
         return 8192
 
     def oomb_attention_paged(self, *args):
-        self.workspaces.append(args[13])
+        self.workspaces.append(args[12])
         return 0
 
 
