@@ -101,7 +101,7 @@ struct DecodeWs {
 };
 
 struct DecodeBars {
-    uint64_t kv_full[8], kv_empty[8], s_full[2], p_ready[2], p_free[2], q_ready, e_full[8];
+    uint64_t kv_full[8], kv_empty[8], s_full[2], p_ready[2], p_free[2], q_ready, e_full[8], done;
     uint32_t tmem;
     float red[4][kDecRows], redt[4][kDecRows];
     float n[kDecRows], top[kDecRows], fl[kDecRows], fo[kDecRows];  // a row's reference, largest score, and factors of a change
@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         }
         for (int i = 0; i < Geo::EXPS; i++) mbar_init(&bar->e_full[i], 1);
         mbar_init(&bar->q_ready, 4);
+        mbar_init(&bar->done, 1);
         fence_barrier_init();
     }
     if (warp == 4) {
@@ -401,20 +402,21 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 load(true, i, was);
             }
         }
-        // the ring is drained before the CTA ends: nothing may still arrive in its shared memory
+        // the last loads of every slot have landed before the CTA ends, whoever still waited for them: nothing may arrive in its
+        // shared memory later (a slot never loaded counts as landed)
         for (int i = 0; i < ST; i++) {
-            fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_DEC_WAIT + 2);
+            fa_drain(&bar->kv_full[r.i], r.phase ^ 1, p.err, ERR_DEC_WAIT + 2);
             r.next();
         }
+        for (unsigned e = 0; F8 && e < Geo::EXPS && e < tile_no; e++)
+            fa_drain(&bar->e_full[e], ((tile_no - 1 - e) / Geo::EXPS) & 1, p.err, ERR_DEC_WAIT + 2);
     } else if (warp == 4) {
         // ---- the issuing warp ----
         Ring<ST> r;
         unsigned t = 0, q_ph = 0;  // tiles so far
         bool ok = true;
-        auto wait = [&](uint64_t* b, unsigned ph, int role) {
-            if (ok && !fa_wait(b, ph, p.err, ERR_DEC_WAIT + role)) ok = false;
-            return ok;
-        };
+        bool gone = false;  // this lane gave up
+        auto wait = [&](uint64_t* b, unsigned ph, int role) { gone |= !fa_wait_lane(b, ph, p.err, ERR_DEC_WAIT + role); };
         constexpr uint32_t fmt = F8 ? 0u : (1u << 7) | (1u << 10);
         constexpr uint32_t id_s = (1u << 4) | fmt | (static_cast<uint32_t>(Geo::NQ >> 3) << 17) | (8u << 24);
         // A along positions (bit 15); e4m3 values with e5m2 weights
@@ -462,20 +464,20 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         };
         while (ok && walk.next(p, g)) {
             if (g.tiles == 0) continue;
-            if (!wait(&bar->q_ready, q_ph, 3)) break;
+            wait(&bar->q_ready, q_ph, 3);
             q_ph ^= 1;
-            if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+            wait(&bar->kv_full[r.i], r.phase, 4);
             scores(r.i, t);
             release(r.i);
             r.next();
             for (int i = 0; i < g.tiles && ok; i++, t++) {
                 if (i + 1 < g.tiles) {
-                    if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                    wait(&bar->kv_full[r.i], r.phase, 4);
                     scores(r.i, t + 1);
                     release(r.i);
                     r.next();
                 }
-                if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                wait(&bar->kv_full[r.i], r.phase, 4);
                 const int left = g.tok1 - g.tok0 - i * kDecBlock;
                 if (left < kDecBlock) {
                     // rows behind the last position: anything may be there, and 0 * NaN is NaN
@@ -486,12 +488,17 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     fence_async_smem();
                     __syncwarp();
                 }
-                if (!wait(&bar->p_ready[t & 1], (t >> 1) & 1, 5)) break;
+                wait(&bar->p_ready[t & 1], (t >> 1) & 1, 5);
                 outputs(r.i, t, i == 0);
                 release(r.i);
                 r.next();
+                ok = !__any_sync(0xffffffffu, gone);
             }
         }
+        // every product has read its operands before the CTA ends, also where the softmax gave up on one
+        if (elect_one()) tc_commit(&bar->done);
+        __syncwarp();
+        fa_drain(&bar->done, 0, p.err, ERR_DEC_WAIT + 11);
     } else {
         // ---- softmax: a position's thread, then an output dimension's ----
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
@@ -510,7 +517,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         // A thread whose wait ran out goes on to the next meeting, where all learn of it: none leaves the others waiting there.
         bool gone = false;
         auto wait = [&](uint64_t* b, unsigned ph, int role) {
-            if (!fa_wait(b, ph, p.err, ERR_DEC_WAIT + role)) gone = true;
+            if (!fa_wait_lane(b, ph, p.err, ERR_DEC_WAIT + role)) gone = true;
         };
         while (!stop && walk.next(p, g)) {
             const Seq sq = g.sq;

@@ -369,7 +369,7 @@ struct FaGeo {
 };
 
 struct FaBars {
-    uint64_t q_full[2], q_empty, s_full[2], p_ready[2][kFaParts], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2], u_full[2], u_empty[2];
+    uint64_t q_full[2], q_empty, s_full[2], p_ready[2][kFaParts], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2], u_full[2], u_empty[2], done;
     uint32_t tmem;
     int kvh[2];  // the CTA's current and next unit: kv head (-1: no more), and the rest
     __align__(16) FaUnit unit[2];
@@ -427,10 +427,28 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
 
 // As mbar_wait, but the clock and the limit (a load from global memory, some 600 cycles) are read only
 // after many polls: a wait of a tile's length must not pay for them.
-__device__ __forceinline__ bool fa_wait(uint64_t* bar, unsigned parity, unsigned* err, unsigned code) {
+__device__ __forceinline__ bool fa_wait_lane(uint64_t* bar, unsigned parity, unsigned* err, unsigned code) {
     for (int i = 0; i < 64; i++)
         if (mbar_try_wait(bar, parity)) return true;
     return mbar_wait(bar, parity, err, code);
+}
+// The same for a warp whose lanes agree: where one gave up all do, since what follows (tensor memory, votes, the end of the
+// role) takes the warp together.  The warps that pace the products go on after a wait that ran out, over whatever is in their
+// tiles, and agree once a tile (two packed prompts of 8,192 and 3,001 tokens took 524 us without agreeing, 530 with a vote a
+// wait, 527 so).
+__device__ __forceinline__ bool fa_wait(uint64_t* bar, unsigned parity, unsigned* err, unsigned code) {
+    return __all_sync(0xffffffffu, fa_wait_lane(bar, parity, err, code));
+}
+// The waits at a CTA's end for copies and products under way, which end by themselves: the limit that a caller may shorten does
+// not count here, since a CTA that left before them would have its shared memory written after it.
+__device__ __forceinline__ void fa_drain(uint64_t* bar, unsigned parity, unsigned* err, unsigned code) {
+    if (mbar_try_wait(bar, parity)) return;
+    const unsigned long long t0 = global_ns();
+    while (!mbar_try_wait(bar, parity))
+        if (global_ns() - t0 > kWaitLimitNs) {
+            record_error(err, code);
+            return;
+        }
 }
 
 // The plan of up to 32 sequences with up to 32 tiles together, by one warp and without a launch of its own (which takes four
@@ -556,6 +574,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
     constexpr int ST = Geo::STAGES, CH = D / 64;  // 64-column chunks of a tile
     extern __shared__ __align__(1024) uint8_t smem[];
     FaBars* bar = reinterpret_cast<FaBars*>(smem + Geo::BAR_OFF);
+    static_assert(sizeof(FaBars) <= Geo::TOTAL - Geo::BAR_OFF, "barriers");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int tq = fa_tokens(p.G);
 
@@ -571,6 +590,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             mbar_init(&bar->o_full[h], 1);
         }
         mbar_init(&bar->q_empty, 1);
+        mbar_init(&bar->done, 1);
         for (int i = 0; i < ST; i++) {
             mbar_init(&bar->kv_full[i], F8 ? 4 : 1);
             mbar_init(&bar->kv_empty[i], 1);
@@ -624,10 +644,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             const int vis = valid ? max(0, min(w.s.len, w.s.len - w.s.n + token + 1)) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < w.nh[h]; i++) {
-                if (!fa_wait(&bar->s_full[h], s_ph, p.err, ERR_FA_WAIT + 7)) {
-                    ok = false;
-                    break;
-                }
+                const bool there = fa_wait_lane(&bar->s_full[h], s_ph, p.err, ERR_FA_WAIT + 7);
                 s_ph ^= 1;
                 tc_fence_after();
                 float s[128];
@@ -640,7 +657,11 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
 #pragma unroll
                     for (int c = 0; c < 128; c++) s[c] = -s[c];
                 }
-                if (__any_sync(0xffffffffu, lim < kFaTile)) {
+                if (__any_sync(0xffffffffu, lim < kFaTile || !there)) {
+                    if (!__all_sync(0xffffffffu, there)) {
+                        ok = false;
+                        break;
+                    }
 #pragma unroll
                     for (int c = 0; c < 128; c++) s[c] = c < lim ? s[c] : -INFINITY;
                 }
@@ -788,7 +809,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             Ring<F8 ? 2 : ST> r;
             uint64_t* const full_bar = F8 ? bar->raw_full : bar->kv_full;
             uint64_t* const empty_bar = F8 ? bar->raw_empty : bar->kv_empty;
-            unsigned q_phase = 0;
+            unsigned q_phase = 0, q_loads[2] = {0, 0};
             bool ok = true;
             const int32_t* table = nullptr;
             int ids_of = -1, ids = 0, ids_next = 0;
@@ -877,6 +898,8 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 if (ok && !fa_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 2)) ok = false;
                 q_phase ^= 1;
                 if (!ok) break;
+#pragma unroll
+                for (int h = 0; h < 2; h++) q_loads[h] += w.nh[h] > 0;
                 if (lane == 0) {
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -899,12 +922,15 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                     load(true, w.kv0 + i, cur);
                 }
             }
-            // the ring is drained before the CTA ends: nothing may still arrive in its shared memory
+            // the last loads of every slot have landed before the CTA ends, whoever still waited for them: nothing may arrive
+            // in its shared memory later (a slot never loaded counts as landed)
             for (int i = 0; i < (F8 ? 2 : ST); i++) {
-                fa_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
+                fa_drain(&full_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
                 r.next();
             }
-            fa_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 3);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                if (q_loads[h]) fa_drain(&bar->q_full[h], (q_loads[h] - 1) & 1, p.err, ERR_FA_WAIT + 3);
         } else if (F8 && warp >= kFaSoft + 4) {
             // ---- conversion: codes times their row's power of two, exact in bf16, into the swizzled tile ----
             Ring<2> rr;
@@ -913,8 +939,9 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             constexpr int RC = D / 16;  // 16-code chunks of a row
             const int ct = tid - (kFaSoft + 4) * 32;
             auto convert = [&](int left) {
-                if (!ok || !fa_wait(&bar->raw_full[rr.i], rr.phase, p.err, ERR_FA_WAIT + 9) ||
-                    !fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 10)) {
+                if (!ok) return;
+                const bool raw = fa_wait_lane(&bar->raw_full[rr.i], rr.phase, p.err, ERR_FA_WAIT + 9);
+                if (!__all_sync(0xffffffffu, fa_wait_lane(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 10) && raw)) {
                     ok = false;
                     return;
                 }
@@ -966,20 +993,14 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                     convert(left);
                 }
             }
-            for (int i = 0; i < ST; i++) {  // every tile released before the CTA ends
-                fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 3);
-                r.next();
-            }
         } else if (warp == kFaSoft) {
             // ---- the issuing warp ----
             Ring<ST> r;
             unsigned q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
             bool ok = true;
             constexpr uint32_t id_s = fa_idesc(kFaTile, false), id_o = fa_idesc(D, true);
-            auto wait = [&](uint64_t* b, unsigned ph, int role) {
-                if (ok && !fa_wait(b, ph, p.err, ERR_FA_WAIT + role)) ok = false;
-                return ok;
-            };
+            bool gone = false;  // this lane gave up
+            auto wait = [&](uint64_t* b, unsigned ph, int role) { gone |= !fa_wait_lane(b, ph, p.err, ERR_FA_WAIT + role); };
             const uint32_t q_lo = uniform(static_cast<uint32_t>(tc_smem_desc(smem_addr(smem + Geo::Q_OFF))));
             const uint32_t k_lo = uniform(static_cast<uint32_t>(tc_smem_desc(smem_addr(smem + Geo::KV_OFF))));
             const uint32_t v_lo = uniform(static_cast<uint32_t>(fa_desc_mn(smem_addr(smem + Geo::KV_OFF), Geo::HALF)));
@@ -1019,15 +1040,14 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             };
             for (FaWork w; ok && take(w);) {
                 if (w.keys == 0) continue;
-                if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                wait(&bar->kv_full[r.i], r.phase, 4);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     if (w.nh[h] == 0) continue;
-                    if (!wait(&bar->q_full[h], q_ph[h], 5)) break;
+                    wait(&bar->q_full[h], q_ph[h], 5);
                     q_ph[h] ^= 1;
                     scores(h, r.i);
                 }
-                if (!ok) break;
                 release(&bar->kv_empty[r.i]);
                 r.next();
                 if (w.keys == 1) release(&bar->q_empty);
@@ -1036,11 +1056,11 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                     int k_stage = 0;
                     if (more) {
                         k_stage = r.i;
-                        if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                        wait(&bar->kv_full[r.i], r.phase, 4);
                         r.next();
                     }
                     const int v_stage = r.i;
-                    if (!wait(&bar->kv_full[r.i], r.phase, 4)) break;
+                    wait(&bar->kv_full[r.i], r.phase, 4);
                     r.next();
                     const int left = w.s.len - (w.kv0 + i) * kFaTile;  // positions of the tile
                     if (!F8 && left < kFaTile) {
@@ -1054,20 +1074,24 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                     }
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        if (!ok || i >= w.nh[h]) continue;
+                        if (i >= w.nh[h]) continue;
                         for (int part = 0; part < kFaParts; part++) {
-                            if (!wait(&bar->p_ready[h][part], p_ph[h], 6)) break;
+                            wait(&bar->p_ready[h][part], p_ph[h], 6);
                             outputs(h, v_stage, part, i == 0, part + 1 == kFaParts && i + 1 == w.nh[h]);
                         }
                         p_ph[h] ^= 1;
-                        if (ok && i + 1 < w.nh[h]) scores(h, k_stage);
+                        if (i + 1 < w.nh[h]) scores(h, k_stage);
                     }
+                    ok = !__any_sync(0xffffffffu, gone);
                     if (!ok) break;
                     release(&bar->kv_empty[v_stage]);
                     if (more) release(&bar->kv_empty[k_stage]);
                     if (i + 2 == w.keys) release(&bar->q_empty);
                 }
             }
+            // every product has read its operands before the CTA ends, also where the softmax gave up on one
+            release(&bar->done);
+            fa_drain(&bar->done, 0, p.err, ERR_FA_WAIT + 14);
         }
     }
     __syncthreads();
