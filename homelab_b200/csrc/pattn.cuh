@@ -75,10 +75,23 @@ __device__ __forceinline__ void kv_row(const PattnParams& p, bool value, int b, 
     }
 }
 
-// One query row over positions [j0, j1) (of packed rows from base_row on, or of sequence b's pages) by one warp, in plain fp32 loops: the running
-// maximum m (in units of log2), sum l and unnormalised output acc of the row.
+// Whether a value row of the positions [j0, j1) holds something that is not finite (for the whole warp).
 template <int KIND, int D>
-__device__ __noinline__ void attend_row(const PattnParams& p, int b, int base_row, int token, int head, int j0, int j1, int lane, float& m,
+__device__ __noinline__ bool odd_values(const PattnParams& p, int b, int base_row, int h, int j0, int j1, int lane) {
+    bool odd = false;
+    for (int j = j0; j < j1; j++) {
+        float f[D / 32];
+        kv_row<KIND, D>(p, true, b, base_row, h, j, lane, f);
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) odd |= !(fabsf(f[i]) <= 3.4e38f);
+    }
+    return __any_sync(0xffffffffu, odd);
+}
+
+// One query row over positions [j0, j1) (of packed rows from base_row on, or of sequence b's pages) by one warp, in plain fp32 loops: the running
+// maximum m (in units of log2), sum l and unnormalised output acc of the row.  `beat` moves on the way, for those who wait.
+template <int KIND, int D>
+__device__ __noinline__ void attend_row(const PattnParams& p, int b, int base_row, int token, int head, int j0, int j1, int lane, unsigned* beat, float& m,
                                         float& l, float (&acc)[D / 32]) {
     constexpr int E = D / 32;
     float q[E];
@@ -91,6 +104,9 @@ __device__ __noinline__ void attend_row(const PattnParams& p, int b, int base_ro
     m = -INFINITY;
     l = 0.0f;
     for (int j = j0; j < j1; j++) {
+        if ((j & 1023) == 0 || j == j0) {
+            if (lane == 0) atomicAdd(beat, 1u);
+        }
         float k[E], v[E];
         kv_row<KIND, D>(p, false, b, base_row, head / p.G, j, lane, k);
         kv_row<KIND, D>(p, true, b, base_row, head / p.G, j, lane, v);

@@ -103,6 +103,7 @@ struct DecodeWs {
 struct DecodeBars {
     uint64_t kv_full[8], kv_empty[8], s_full[2], p_ready[2], p_free[2], q_ready, e_full[8], done;
     uint32_t tmem;
+    unsigned beat;  // moves while rows are done again
     float red[4][kDecRows], redt[4][kDecRows];
     float n[kDecRows], top[kDecRows], fl[kDecRows], fo[kDecRows];  // a row's reference, largest score, and factors of a change
     int redx[4], redn[4], redv[4];
@@ -260,6 +261,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         for (int i = 0; i < Geo::EXPS; i++) mbar_init(&bar->e_full[i], 1);
         mbar_init(&bar->q_ready, 4);
         mbar_init(&bar->done, 1);
+        bar->beat = 0;
         fence_barrier_init();
     }
     if (warp == 4) {
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 return i < g.tiles && lane < per_tile && at < p.kv.max_pages ? __ldcg(table + at) : 0;
             };
             auto load = [&](bool value, int i, int id) {
-                if (!ok || !fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_DEC_WAIT + 1)) {
+                if (!ok || !fa_wait(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_DEC_WAIT + 1, &bar->beat)) {
                     ok = false;
                     return;
                 }
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         unsigned t = 0, q_ph = 0;  // tiles so far
         bool ok = true;
         bool gone = false;  // this lane gave up
-        auto wait = [&](uint64_t* b, unsigned ph, int role) { gone |= !fa_wait_lane(b, ph, p.err, ERR_DEC_WAIT + role); };
+        auto wait = [&](uint64_t* b, unsigned ph, int role) { gone |= !fa_wait_lane(b, ph, p.err, ERR_DEC_WAIT + role, &bar->beat); };
         constexpr uint32_t fmt = F8 ? 0u : (1u << 7) | (1u << 10);
         constexpr uint32_t id_s = (1u << 4) | fmt | (static_cast<uint32_t>(Geo::NQ >> 3) << 17) | (8u << 24);
         // A along positions (bit 15); e4m3 values with e5m2 weights
@@ -502,7 +504,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
     } else {
         // ---- softmax: a position's thread, then an output dimension's ----
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-        constexpr float kSlack = F8 ? 4.0f : 8.0f, kBase = F8 ? 11.0f - kDecUnit : 0.0f;
+        constexpr float kSlack = F8 ? 4.0f : 8.0f, kBase = F8 ? 11.0f - kDecUnit : -kFaDown;
         unsigned t = 0, v_item = 0;  // tiles so far, and what the loader brought before the segment
         bool stop = false;
         // the four warps meet; whether any says so
@@ -517,7 +519,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         // A thread whose wait ran out goes on to the next meeting, where all learn of it: none leaves the others waiting there.
         bool gone = false;
         auto wait = [&](uint64_t* b, unsigned ph, int role) {
-            if (!fa_wait_lane(b, ph, p.err, ERR_DEC_WAIT + role)) gone = true;
+            if (!fa_wait_lane(b, ph, p.err, ERR_DEC_WAIT + role, &bar->beat)) gone = true;
         };
         while (!stop && walk.next(p, g)) {
             const Seq sq = g.sq;
@@ -799,7 +801,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
             const int first = walk.deal.owner(g.pair_first), final_cta = walk.deal.owner(g.pair_end - 1);
             const int parts = final_cta - first + 1;
             float* my_part = ws.part + static_cast<int64_t>(2 * blockIdx.x + (g.lo == g.pair_first ? 1 : 0)) * ws.rows * PAD;
-            bool odd = lost;
+            bool odd = false;
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 if (r >= rows) continue;
@@ -827,6 +829,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 }
             }
             if (parts > 1) {
+                lost = false;  // the CTA that joins the parts learns it from them
                 __threadfence();
                 meet(false);
                 if (tid == 0) {
@@ -868,7 +871,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
                                 const float f = exp2_fast(ml[i].x - b0);
-                                odd |= ml[i].y < 0.0f;
+                                lost |= ml[i].y < 0.0f;
                                 a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
                                 ls = fmaf(f, ml[i].y, ls);
                             }
@@ -884,14 +887,17 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 }
             }
             // A value that is not finite, behind some row's mask, reaches that row as 0 * inf through the products (a single new
-            // token sees everything): then, and where the weights' range was passed, every row is done again in plain loops over
-            // what it sees.
-            if (meet(odd)) {
+            // token sees everything): where there is one, and where the weights' range was passed, every row is done again in
+            // plain loops over what it sees.
+            bool redo = meet(odd || lost);
+            if (redo && !meet(lost))
+                redo = odd_values<KIND, D>(p, g.b, sq.q0, g.kvh, max(0, min(sq.len, sq.len - sq.n + row0 / p.G + 1)), sq.len, lane);
+            if (redo) {
                 for (int r = warp; r < rows; r += 4) {
                     const int token = (row0 + r) / p.G, head = g.kvh * p.G + row0 + r - token * p.G;
                     const int see = max(0, min(sq.len, sq.len - sq.n + token + 1));
                     float mm, ll, a[D / 32];
-                    attend_row<KIND, D>(p, g.b, sq.q0, sq.q0 + token, head, 0, see, lane, mm, ll, a);
+                    attend_row<KIND, D>(p, g.b, sq.q0, sq.q0 + token, head, 0, see, lane, &bar->beat, mm, ll, a);
                     uint16_t* to = p.out + static_cast<int64_t>(sq.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D + lane * (D / 32);
                     const float inv = see > 0 ? 1.0f / ll : 0.0f;
 #pragma unroll

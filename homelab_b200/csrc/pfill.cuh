@@ -48,6 +48,9 @@ constexpr int kFaRows = 256;       // rows of a tile pair
 // tokens (32 heads over 8, D = 128): one part 610 us, two 569-600, four 601-625 (each hand-over waits for its stores).
 constexpr int kFaParts = 2;
 constexpr int kFaSoft = 8;         // softmax warps
+// Weights are made, and summed, as 2^-16 of what they are: with the 2^8 that a row's maximum may lag behind, no product with a
+// value passes what fp32 holds that the value itself does not.
+constexpr float kFaDown = 16.0f;
 constexpr int kFaMinPart = 4;      // key tiles of a part at least
 constexpr int kPlanThreads = 256;
 constexpr int kPlanBuckets = 512;
@@ -371,6 +374,7 @@ struct FaGeo {
 struct FaBars {
     uint64_t q_full[2], q_empty, s_full[2], p_ready[2][kFaParts], o_full[2], kv_full[8], kv_empty[8], raw_full[2], raw_empty[2], u_full[2], u_empty[2], done;
     uint32_t tmem;
+    unsigned beat;  // moves while rows are done again
     int kvh[2];  // the CTA's current and next unit: kv head (-1: no more), and the rest
     __align__(16) FaUnit unit[2];
 };
@@ -426,18 +430,34 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
 }
 
 // As mbar_wait, but the clock and the limit (a load from global memory, some 600 cycles) are read only
-// after many polls: a wait of a tile's length must not pay for them.
-__device__ __forceinline__ bool fa_wait_lane(uint64_t* bar, unsigned parity, unsigned* err, unsigned code) {
+// after many polls: a wait of a tile's length must not pay for them.  While `beat` moves a warp of the CTA does rows again
+// (attend_row), which takes as long as it takes, and the limit begins anew.
+__device__ __forceinline__ bool fa_wait_lane(uint64_t* bar, unsigned parity, unsigned* err, unsigned code, const unsigned* beat) {
     for (int i = 0; i < 64; i++)
         if (mbar_try_wait(bar, parity)) return true;
-    return mbar_wait(bar, parity, err, code);
+    const volatile unsigned* at = beat;
+    unsigned long long t0 = global_ns();
+    const unsigned long long limit = wait_limit();
+    unsigned seen = *at;
+    for (;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        const unsigned long long now = global_ns();
+        if (now - t0 <= limit) continue;
+        const unsigned b = *at;
+        if (b == seen) {
+            record_error(err, code);
+            return false;
+        }
+        seen = b;
+        t0 = now;
+    }
 }
 // The same for a warp whose lanes agree: where one gave up all do, since what follows (tensor memory, votes, the end of the
 // role) takes the warp together.  The warps that pace the products go on after a wait that ran out, over whatever is in their
 // tiles, and agree once a tile (two packed prompts of 8,192 and 3,001 tokens took 524 us without agreeing, 530 with a vote a
 // wait, 527 so).
-__device__ __forceinline__ bool fa_wait(uint64_t* bar, unsigned parity, unsigned* err, unsigned code) {
-    return __all_sync(0xffffffffu, fa_wait_lane(bar, parity, err, code));
+__device__ __forceinline__ bool fa_wait(uint64_t* bar, unsigned parity, unsigned* err, unsigned code, const unsigned* beat) {
+    return __all_sync(0xffffffffu, fa_wait_lane(bar, parity, err, code, beat));
 }
 // The waits at a CTA's end for copies and products under way, which end by themselves: the limit that a caller may shorten does
 // not count here, since a CTA that left before them would have its shared memory written after it.
@@ -565,6 +585,38 @@ __device__ __forceinline__ FaWork fa_work(const PattnParams& p, const FaUnit& u,
     return w;
 }
 
+// Values that are not finite, behind some row's mask, reach that row as 0 * inf through the products: the rows `again` of a
+// warp (a lane's token, head, positions seen and partial row are its own) are done again in plain loops over what they see of
+// the positions [j0, j1) that were multiplied, if there is such a value (else what they see is not finite).
+template <int KIND, int D>
+__device__ __noinline__ void fa_redo(const PattnParams& p, int b, int base, int kvh, int j0, int j1, unsigned again, int token, int head, int vis,
+                                     float* line, int lane, unsigned* beat) {
+    const bool mine = again >> lane & 1;
+    const int hidden = __reduce_min_sync(0xffffffffu, mine ? max(vis, j0) : j1);
+    if (!odd_values<KIND, D>(p, b, base, kvh, hidden, j1, lane)) return;
+    while (again) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1;
+        const int tk = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src), see = __shfl_sync(0xffffffffu, vis, src);
+        float* const to = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(line), src));
+        float mm, ll, a[D / 32];
+        attend_row<KIND, D>(p, b, base, tk, hd, j0, min(see, j1), lane, beat, mm, ll, a);
+        if (to == nullptr) {
+            uint16_t* o = p.out + static_cast<int64_t>(tk) * p.out_stride + static_cast<int64_t>(hd) * D + lane * (D / 32);
+            const float iv = see > 0 ? 1.0f / ll : 0.0f;
+#pragma unroll
+            for (int e = 0; e < D / 32; e += 2) {
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(a[e] * iv, a[e + 1] * iv);
+                *reinterpret_cast<__nv_bfloat162*>(o + e) = b2;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < D / 32; e++) to[lane * (D / 32) + e] = a[e];
+            if (lane == 0) *reinterpret_cast<float2*>(to + D) = make_float2(mm - kFaDown, ll);
+        }
+    }
+}
+
 template <int KIND, int D>
 __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
     fa_kernel(const __grid_constant__ PattnParams p, const __grid_constant__ FaWs ws, const __grid_constant__ CUtensorMap qmap,
@@ -591,6 +643,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         }
         mbar_init(&bar->q_empty, 1);
         mbar_init(&bar->done, 1);
+        bar->beat = 0;
         for (int i = 0; i < ST; i++) {
             mbar_init(&bar->kv_full[i], F8 ? 4 : 1);
             mbar_init(&bar->kv_empty[i], 1);
@@ -616,7 +669,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
     // The loader deals the CTA its units (the first by its index, then whichever is next) and tells the other warps.
     Ring<2> feed;
     auto take = [&](FaWork& w) {
-        if (!fa_wait(&bar->u_full[feed.i], feed.phase, p.err, ERR_FA_WAIT + 12)) return false;
+        if (!fa_wait(&bar->u_full[feed.i], feed.phase, p.err, ERR_FA_WAIT + 12, &bar->beat)) return false;
         const int kvh = *static_cast<volatile int*>(&bar->kvh[feed.i]);
         if (kvh >= 0) w = fa_work(p, bar->unit[feed.i], kvh, tq);
         __syncwarp();
@@ -633,8 +686,9 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         const uint32_t ts = tmem + lane_base + h * 128, to = tmem + lane_base + 256 + h * 128;
         unsigned s_ph = 0, o_ph = 0;
         bool ok = true;
-        const float scale = fabsf(p.scale_log2);
-        const bool negate = p.scale_log2 < 0.0f;
+        // a scale below zero turns the scores' sign, and one of zero makes them zero (before the mask: 0 * -inf is NaN)
+        const float turn = p.scale_log2 > 0.0f ? 1.0f : p.scale_log2 < 0.0f ? -1.0f : 0.0f;
+        const float scale = turn == 0.0f ? 1.0f : fabsf(p.scale_log2);
         const int token_of = row / p.G, head_of = row - token_of * p.G;
         const bool row_in = token_of < tq;
         const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | (static_cast<uintptr_t>(p.out_stride) * 2)) & 31u) == 0;
@@ -644,7 +698,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             const int vis = valid ? max(0, min(w.s.len, w.s.len - w.s.n + token + 1)) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < w.nh[h]; i++) {
-                const bool there = fa_wait_lane(&bar->s_full[h], s_ph, p.err, ERR_FA_WAIT + 7);
+                const bool there = fa_wait_lane(&bar->s_full[h], s_ph, p.err, ERR_FA_WAIT + 7, &bar->beat);
                 s_ph ^= 1;
                 tc_fence_after();
                 float s[128];
@@ -653,9 +707,9 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 tc_wait_ld();
                 // rows that are no query's (and the next sequence's) are not masked: nobody reads them
                 const int lim = valid ? vis - (w.kv0 + i) * kFaTile : kFaTile;
-                if (negate) {
+                if (turn != 1.0f) {
 #pragma unroll
-                    for (int c = 0; c < 128; c++) s[c] = -s[c];
+                    for (int c = 0; c < 128; c++) s[c] *= turn;
                 }
                 if (__any_sync(0xffffffffu, lim < kFaTile || !there)) {
                     if (!__all_sync(0xffffffffu, there)) {
@@ -691,7 +745,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : m * scale;
+                const float base = m == -INFINITY ? 0.0f : fmaf(m, scale, kFaDown);
                 float2 ls = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
@@ -721,7 +775,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             // ---- the row's output ----
             const bool any = w.nh[h] > 0;
             if (any) {
-                if (!fa_wait(&bar->o_full[h], o_ph, p.err, ERR_FA_WAIT + 8)) {
+                if (!fa_wait(&bar->o_full[h], o_ph, p.err, ERR_FA_WAIT + 8, &bar->beat)) {
                     ok = false;
                     break;
                 }
@@ -774,32 +828,10 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 }
             }
             if (w.slot >= 0 && valid) *reinterpret_cast<float2*>(line + D) = make_float2(m == -INFINITY ? m : m * scale, l);
-            // Values that are not finite, behind some row's mask, reach that row as 0 * inf through the products: such rows
-            // are done again in plain loops over what they see.
-            unsigned again = __ballot_sync(0xffffffffu, valid && odd);
-            while (again) {
-                const int src = __ffs(again) - 1;
-                again &= again - 1;
-                const int tk = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
-                const int see = __shfl_sync(0xffffffffu, vis, src);
-                const int j0 = w.kv0 * kFaTile, j1 = min(see, (w.kv0 + w.keys) * kFaTile);
-                float mm, ll, a[D / 32];
-                attend_row<KIND, D>(p, w.b, w.base, w.s.q0 + tk, hd, j0, j1, lane, mm, ll, a);
-                if (w.slot < 0) {
-                    uint16_t* o = p.out + static_cast<int64_t>(w.s.q0 + tk) * p.out_stride + static_cast<int64_t>(hd) * D + lane * (D / 32);
-                    const float iv = see > 0 ? 1.0f / ll : 0.0f;
-#pragma unroll
-                    for (int e = 0; e < D / 32; e += 2) {
-                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(a[e] * iv, a[e + 1] * iv);
-                        *reinterpret_cast<__nv_bfloat162*>(o + e) = b2;
-                    }
-                } else {
-                    float* o = ws.part + ((static_cast<int64_t>(w.slot) * p.Hkv + w.kvh) * kFaRows + h * kFaTile + (warp & 3) * 32 + src) * fa_line(D);
-#pragma unroll
-                    for (int e = 0; e < D / 32; e++) o[lane * (D / 32) + e] = a[e];
-                    if (lane == 0) *reinterpret_cast<float2*>(o + D) = make_float2(mm, ll);
-                }
-            }
+            const unsigned again = __ballot_sync(0xffffffffu, valid && odd);
+            if (again)
+                fa_redo<KIND, D>(p, w.b, w.base, w.kvh, w.kv0 * kFaTile, min(w.s.len, (w.kv0 + w.nh[h]) * kFaTile), again, w.s.q0 + token, head, vis,
+                                 w.slot < 0 ? nullptr : line, lane, &bar->beat);
             tc_fence_before();
         }
     } else {
@@ -834,7 +866,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             const int units = (ws.direct ? own.units : __ldcg(&ws.head->units)) * p.Hkv;
             while (ok) {
                 const int u = next;
-                if (!fa_wait(&bar->u_empty[feed.i], feed.phase ^ 1, p.err, ERR_FA_WAIT + 13)) break;
+                if (!fa_wait(&bar->u_empty[feed.i], feed.phase ^ 1, p.err, ERR_FA_WAIT + 13, &bar->beat)) break;
                 if (lane < 2) reinterpret_cast<int4*>(&bar->unit[feed.i])[lane] = rec;
                 if (lane == 0) bar->kvh[feed.i] = u < units ? u % p.Hkv : -1;
                 __syncwarp();
@@ -853,7 +885,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                     ids_next = w.keys > 1 ? lookup(ids_of + 1) : 0;
                 }
                 auto load = [&](bool value, int tile, int page_ids) {
-                    if (!ok || !fa_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 1)) {
+                    if (!ok || !fa_wait(&empty_bar[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 1, &bar->beat)) {
                         ok = false;
                         return;
                     }
@@ -895,7 +927,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 };
                 load(false, w.kv0, ids);
                 // the queries, once the previous unit's last scores are multiplied
-                if (ok && !fa_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 2)) ok = false;
+                if (ok && !fa_wait(&bar->q_empty, q_phase ^ 1, p.err, ERR_FA_WAIT + 2, &bar->beat)) ok = false;
                 q_phase ^= 1;
                 if (!ok) break;
 #pragma unroll
@@ -940,8 +972,8 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             const int ct = tid - (kFaSoft + 4) * 32;
             auto convert = [&](int left) {
                 if (!ok) return;
-                const bool raw = fa_wait_lane(&bar->raw_full[rr.i], rr.phase, p.err, ERR_FA_WAIT + 9);
-                if (!__all_sync(0xffffffffu, fa_wait_lane(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 10) && raw)) {
+                const bool raw = fa_wait_lane(&bar->raw_full[rr.i], rr.phase, p.err, ERR_FA_WAIT + 9, &bar->beat);
+                if (!__all_sync(0xffffffffu, fa_wait_lane(&bar->kv_empty[r.i], r.phase ^ 1, p.err, ERR_FA_WAIT + 10, &bar->beat) && raw)) {
                     ok = false;
                     return;
                 }
@@ -1000,7 +1032,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
             bool ok = true;
             constexpr uint32_t id_s = fa_idesc(kFaTile, false), id_o = fa_idesc(D, true);
             bool gone = false;  // this lane gave up
-            auto wait = [&](uint64_t* b, unsigned ph, int role) { gone |= !fa_wait_lane(b, ph, p.err, ERR_FA_WAIT + role); };
+            auto wait = [&](uint64_t* b, unsigned ph, int role) { gone |= !fa_wait_lane(b, ph, p.err, ERR_FA_WAIT + role, &bar->beat); };
             const uint32_t q_lo = uniform(static_cast<uint32_t>(tc_smem_desc(smem_addr(smem + Geo::Q_OFF))));
             const uint32_t k_lo = uniform(static_cast<uint32_t>(tc_smem_desc(smem_addr(smem + Geo::KV_OFF))));
             const uint32_t v_lo = uniform(static_cast<uint32_t>(fa_desc_mn(smem_addr(smem + Geo::KV_OFF), Geo::HALF)));

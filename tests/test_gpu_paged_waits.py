@@ -6,6 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
+import paged_ref as R  # noqa: E402
 from homelab_b200.backend import Gpu  # noqa: E402
 from homelab_b200.paged import PagedKv  # noqa: E402
 
@@ -86,3 +87,99 @@ def test_a_wait_that_runs_out_ends_the_call_with_an_error(gpu, path, fp8):
             assert torch.equal(out, want)
         assert torch.equal(call(), want)
         assert gpu.device_error() == 0
+
+
+def exact(cache, q, b, at, n, a, scale):
+    """The rows of sequence b in float64 on the GPU, a head at a time, and the bound of their error."""
+    K, D, L = cache.kv_heads, cache.head_dim, a + n
+    ids = cache.block_table[b, :-(-L // cache.page_size)].long()
+    k, v = (x[ids].double().transpose(1, 2).flatten(0, 1)[:L] for x in (cache.k_pages, cache.v_pages))
+    if cache.fp8:
+        k, v = (x * torch.exp2(e[ids].double() - 127).transpose(1, 2).flatten(0, 1)[:L][..., None]
+                for x, e in ((k, cache.k_exp), (v, cache.v_exp)))
+    later = torch.arange(L, device=DEV)[None] > torch.arange(a, a + n, device=DEV)[:, None]
+    x = q[at:at + n].double()
+    H = x.shape[1]
+    out, mag, big = (torch.empty(n, H, d, dtype=torch.float64, device=DEV) for d in (D, D, 1))
+    for h in range(H):
+        kk, vv = k[:, h // (H // K)], v[:, h // (H // K)]
+        p = (x[:, h] @ kk.T * scale).masked_fill(later, float("-inf")).softmax(-1)
+        seen = torch.where(torch.isfinite(vv), vv, 0.0)  # what is hidden has no weight
+        out[:, h], mag[:, h] = p @ seen, p @ seen.abs()
+        big[:, h, 0] = (x[:, h].abs() @ kk.abs().T).masked_fill(later, 0.0).amax(-1) * abs(scale)
+    return out, R.attention_bound(out, mag, big, D)
+
+
+def plant(cache, b, j):
+    """A value that is not finite at position j of sequence b, in every kv head's dimension 7."""
+    page, slot = int(cache.block_table[b, j // cache.page_size]), j % cache.page_size
+    v = cache.v_pages.view(torch.uint8) if cache.fp8 else cache.v_pages
+    v[page, :, slot, 7] = 0x7f if cache.fp8 else float("inf")
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new,cached", [([300, 40], [60000, 5]), ([100, 20], [60000, 5]), ([4] * 30, [9000] * 30)])
+def test_a_visible_value_that_is_not_finite_costs_nothing(gpu, fp8, new, cached):
+    """Position 0 of the first sequence: its rows are what the arithmetic makes of it, at once, and the others are as ever."""
+    call, cache, _ = step(gpu, new, cached, fp8, seed=3)
+    want = call().clone()
+    plant(cache, 0, 0)
+    try:
+        gpu.set_wait_limit(2_000_000)  # 2 ms: one warp over 32 rows of 60,000 positions takes some 150
+        got = call().clone()
+        torch.cuda.synchronize()
+    finally:
+        gpu.set_wait_limit(0)
+    assert gpu.device_error() == 0
+    n = new[0]
+    assert torch.equal(got[n:], want[n:])
+    hit = got[:n, :, 7].float()
+    assert (torch.isnan(hit) if fp8 else torch.isnan(hit) | torch.isinf(hit)).all()
+    others = [d for d in range(128) if d != 7]
+    assert torch.equal(got[:n][..., others], want[:n][..., others])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new,cached", [([300, 40], [60000, 5]), ([100, 20], [60000, 5]), ([4, 4], [200000, 3])])
+def test_rows_that_are_done_again_outlast_the_waits(gpu, fp8, new, cached):
+    """A value that is not finite at the last new token: rows of its tile are done again over the whole cache, which takes far
+    longer than the limit, while the other warps wait."""
+    call, cache, q = step(gpu, new, cached, fp8, seed=5)
+    n, a = new[0], cached[0]
+    want, bound = exact(cache, q, 0, 0, n, a, 1 / math.sqrt(128))
+    clean = call().clone()
+    plant(cache, 0, a + n - 1)
+    try:
+        gpu.set_wait_limit(2_000_000)
+        got = call().clone()
+        torch.cuda.synchronize()
+    finally:
+        gpu.set_wait_limit(0)
+    assert gpu.device_error() == 0
+    assert torch.equal(got[n:], clean[n:])
+    err = (got[:n - 1].double() - want[:n - 1]).abs()
+    assert (err <= bound[:n - 1]).all(), float((err / bound[:n - 1]).max())
+    hit = got[n - 1, :, 7].float()
+    assert (torch.isnan(hit) if fp8 else hit == float("inf")).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", [1, 5, 60, 200])
+@pytest.mark.parametrize("rising", [False, True])
+def test_sums_of_large_values_stay_in_range(gpu, fp8, n, rising):
+    """Values of 2^112 whose weights may stand 2^8 above one while a maximum lags behind: 2,000 of them pass fp32's range
+    unless the weights are held lower."""
+    call, cache, q = step(gpu, [n], [2000], fp8, seed=7)
+    if fp8:
+        cache.v_exp.fill_(121 + 112)
+    else:
+        cache.v_pages.mul_(2.0 ** 112)
+    if rising:  # scores that grow along the cache, by less than the 2^8 (2^4) that a maximum may lag behind a tile
+        ramp = torch.arange(cache.k_pages.shape[0] * cache.page_size, device=DEV).view(-1, 1, cache.page_size, 1) / 2200.0
+        q.copy_(q.abs())
+        k = cache.k_pages.float() * 0.1 + ramp * (28.0 if fp8 else 0.5)
+        cache.k_pages.copy_(k.to(cache.k_pages.dtype))
+    got = call()
+    want, bound = exact(cache, q, 0, 0, n, 2000, 1 / math.sqrt(128))
+    err = (got.double() - want).abs()
+    assert (err <= bound).all(), float((err / bound).max())
