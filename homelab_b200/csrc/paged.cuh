@@ -17,7 +17,7 @@
 // by at most sqrt(2)) and 1 otherwise: comparing the input's largest value with a
 // constant is exact, so the byte does not depend on how the angles were rounded.
 // e4m3 being a floating type, the factor sqrt(2) costs no precision above 2^-6 * 2^e.
-// Infinities and NaN become the NaN code; e is clamped to [-100, 120].
+// Infinities and NaN become the NaN code; e is clamped to [-100, 120], and codes to what an fp32 number can stand for.
 //
 // Angles: the frequency of a pair is kept as turns per position in units of 2^-64; a
 // position times it modulo 2^64 is the exact phase, of which 32 bits go to sincospif:
@@ -160,6 +160,15 @@ __device__ __forceinline__ int row_exponent(float amax, float limit) {
     const unsigned a = __float_as_uint(amax), l = __float_as_uint(limit);
     const int e = static_cast<int>(a >> 23) - static_cast<int>(l >> 23) + ((a & 0x7fffffu) > (l & 0x7fffffu) ? 1 : 0);
     return amax > 0.0f ? max(-100, min(120, e)) : 0;
+}
+
+// Finite values of a row with the largest exponent, 120, held within 240 * 2^120: the codes above stand for 2^128 and more, which no
+// fp32 number is (2^128 itself is off by 2^-4 so, a rounding's most).
+__device__ __forceinline__ void hold_finite(float (&f)[8]) {
+    constexpr float kTop = 3.1901471898837980e38f;  // 15 * 2^124
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (fabsf(f[i]) > kTop && fabsf(f[i]) <= 3.4028235e38f) f[i] = copysignf(kTop, f[i]);
 }
 
 // Eight values times 2^-e as e4m3 codes; non-finite values become the NaN code.
@@ -337,6 +346,10 @@ __global__ void __launch_bounds__(kRowsThreads, 6) rows_kernel(const RowsParams 
             } else {
                 const int e = row_exponent(amax, is_k ? p.k_limit : 448.0f);
                 const float inv = __int_as_float((127 - e) << 23);
+                if (e == 120) {
+                    hold_finite(x);
+                    hold_finite(y);
+                }
                 *reinterpret_cast<uint2*>(pool + o + ca * 8) = codes8(x, inv);
                 *reinterpret_cast<uint2*>(pool + o + cb * 8) = codes8(y, inv);
                 if (t8 == 0)

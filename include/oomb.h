@@ -326,7 +326,8 @@ typedef struct {
  * rotated queries [t][heads][head_dim] to q_out in bf16 (q_out may be q when that is bf16).
  * An e4m3 row takes the least e with amax * r <= 448 * 2^e over its finite values before rotation
  * (r = sqrt(2) * mscale for rotated keys, else 1), clamped to [-100, 120], its values
- * rounded to nearest even; infinities and NaN become the NaN code.  Two tokens of one call must not share a
+ * rounded to nearest even (at e = 120 to 240 * 2^120 at most, the largest that an fp32 number holds); infinities and NaN,
+ * rotated values past fp32's range among them, become the NaN code.  Two tokens of one call must not share a
  * position of a page. */
 int oomb_kv_append_paged(const oomb_paged_kv* cache, const oomb_rope* rope, const void* q, int64_t q_stride, void* q_out,
                          int64_t q_out_stride, int heads, const void* k, int64_t k_stride, const void* v, int64_t v_stride,

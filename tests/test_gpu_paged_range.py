@@ -234,3 +234,34 @@ def test_scores_of_a_billion(gpu):
         gpu.attention_paged(q.to(DEV), paged(ck, ke, cv, ve, 16), out, i32([0, 1]), i32([L]), 1, scale)
         want = stands_for(cv, ve)[333, 0].expand(8, D)
         assert ((out[0].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs()).all()
+
+
+@pytest.mark.parametrize("src", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rotated", [False, True])
+def test_the_largest_finite_values_come_back_finite(gpu, src, rotated):
+    """Rows that hold a type's largest values: their codes stand for fp32 numbers, off by 2^-4 of the value at most."""
+    K, D, page, L = 1, 64, 16, 8
+    v = normal(101, L, K, D)
+    v[0, 0, 3], v[1, 0, 5] = torch.finfo(src).max, -torch.finfo(src).max
+    v[2] = torch.finfo(src).max
+    v[3, 0, ::2] = -torch.finfo(src).max
+    v[4] *= 2.0 ** 125
+    v[5, 0, 7] = 248.0 * 2.0 ** 120
+    v[6, 0, 8] = 247.0 * 2.0 ** 120
+    v[7, 0, 1], v[7, 0, 2] = torch.finfo(src).max, float("inf")
+    v = v.to(src).to(DEV)
+    cache = PagedKv.empty(2, K, page, D, i32([[1, 0]]), fp8=True)
+    plan = gpu.rope_plan(16) if rotated else None  # position 0 turns by nothing
+    for j in range(L):
+        gpu.kv_append_paged(cache, v[j:j + 1], v[j:j + 1], i32([0, 1]), i32([1]), rope=plan)
+        k_out, v_out = (torch.empty(1, K, D, dtype=torch.float32, device=DEV) for _ in range(2))
+        gpu.kv_read_paged(cache, i32([0, 1]), i32([1]), k_out, v_out)
+        turned = v[j].double()
+        if rotated:  # 0 * inf reaches the other half of its pair
+            turned = torch.from_numpy(R.rotate(v[j:j + 1].double().cpu().numpy(), [0], 16, False, *R.inv_freq(16))[0][0]).to(DEV)
+        for got, want in ((k_out[0].double(), turned), (v_out[0].double(), v[j].double())):
+            finite = torch.isfinite(want)
+            assert torch.equal(torch.isfinite(got), finite)
+            e = cache.v_exp[1, 0, 0].double() - 127
+            bound = torch.maximum(2.0 ** -4 * want.abs(), torch.exp2(e - 10))
+            assert ((got - want).abs() <= bound)[finite].all(), j
