@@ -25,6 +25,16 @@ int check_rows(const void* p, int64_t stride, int64_t row, int dtype) {
     return OOMB_OK;
 }
 
+// Whether two sets of t rows (strides and rows in bytes, rows no longer than strides) share memory.  Rows side by side in
+// wider ones, with one stride, do not; rows of unlike strides in one stretch of memory count as if they did.
+bool rows_meet(const void* a, int64_t stride_a, int64_t row_a, const void* b, int64_t stride_b, int64_t row_b, int64_t t) {
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+    if (t <= 0 || pa >= pb + (t - 1) * stride_b + row_b || pb >= pa + (t - 1) * stride_a + row_a) return false;
+    if (t == 1 || stride_a != stride_b) return true;
+    const int64_t apart = static_cast<int64_t>(pb - pa) % stride_a, at = apart < 0 ? apart + stride_a : apart;
+    return at < row_a || at + row_b > stride_a;
+}
+
 int check_rope(const oomb_rope* r, int head_dim) {
     if (!r->turns || (r->interleaved != 0 && r->interleaved != 1)) return OOMB_E_ARG;
     if (!(r->mscale > 0.0f) || !(r->mscale <= 1024.0f)) return OOMB_E_ARG;
@@ -313,12 +323,14 @@ bool attn_shape_ok(int batch, int t, int max_q, int heads, int kv_heads, int hea
 // The checks that both attentions share.
 int check_attn(const void* q, int64_t q_stride, const void* out, int64_t out_stride, int heads, int kv_heads, int head_dim,
                int batch, int t, int max_q, float scale) {
-    if (!q || !out || q == out) return OOMB_E_ARG;
+    if (!q || !out) return OOMB_E_ARG;
     if (!(fabsf(scale) <= 1e37f)) return OOMB_E_ARG;  // its product with log2(e) is an fp32 number
     if (!attn_shape_ok(batch, t, max_q, heads, kv_heads, head_dim)) return OOMB_E_SHAPE;
     const int64_t row = static_cast<int64_t>(heads) * head_dim;
-    const int st = check_rows(q, q_stride, row, OOMB_BF16);
-    return st != OOMB_OK ? st : check_rows(out, out_stride, row, OOMB_BF16);
+    int st = check_rows(q, q_stride, row, OOMB_BF16);
+    if (st == OOMB_OK) st = check_rows(out, out_stride, row, OOMB_BF16);
+    if (st != OOMB_OK) return st;
+    return rows_meet(q, 2 * q_stride, 2 * row, out, 2 * out_stride, 2 * row, t) ? OOMB_E_ARG : OOMB_OK;
 }
 
 }  // namespace
@@ -369,6 +381,8 @@ int oomb_rope_rows(const oomb_rope* rope, const void* x, int x_dtype, int64_t x_
     if (st == OOMB_OK) st = check_rows(x, x_stride, row, x_dtype);
     if (st == OOMB_OK) st = check_rows(out, out_stride, row, x_dtype);
     if (st != OOMB_OK) return st;
+    const int64_t es = x_dtype == OOMB_BF16 ? 2 : 4;
+    if (!(out == x && out_stride == x_stride) && rows_meet(x, es * x_stride, es * row, out, es * out_stride, es * row, t)) return OOMB_E_ARG;
     if (t == 0) return OOMB_OK;
     const DeviceState* d = device_state();
     if (!d) return OOMB_E_DEVICE;
@@ -401,6 +415,14 @@ int oomb_kv_append_paged(const oomb_paged_kv* cache, const oomb_rope* rope, cons
     if (st == OOMB_OK && q) st = check_rows(q, q_stride, static_cast<int64_t>(heads) * cache->head_dim, src_dtype);
     if (st == OOMB_OK && q) st = check_rows(q_out, q_out_stride, static_cast<int64_t>(heads) * cache->head_dim, OOMB_BF16);
     if (st != OOMB_OK) return st;
+    if (q) {
+        const int64_t es = src_dtype == OOMB_BF16 ? 2 : 4, q_row = static_cast<int64_t>(heads) * cache->head_dim;
+        auto over = [&](const void* x, int64_t stride, int64_t x_row) {
+            return rows_meet(x, es * stride, es * x_row, q_out, 2 * q_out_stride, 2 * q_row, t);
+        };
+        const bool in_place = src_dtype == OOMB_BF16 && q_out == q && q_out_stride == q_stride;
+        if ((!in_place && over(q, q_stride, q_row)) || over(k, k_stride, row) || over(v, v_stride, row)) return OOMB_E_ARG;
+    }
     if (batch == 0 || t == 0) return OOMB_OK;
     const DeviceState* d = device_state();
     if (!d) return OOMB_E_DEVICE;
@@ -440,6 +462,8 @@ int oomb_kv_read_paged(const oomb_paged_kv* cache, const int32_t* q_start, const
     if (st == OOMB_OK) st = check_rows(k_out, out_stride, row, out_dtype);
     if (st == OOMB_OK) st = check_rows(v_out, out_stride, row, out_dtype);
     if (st != OOMB_OK) return st;
+    const int64_t es = out_dtype == OOMB_BF16 ? 2 : 4;
+    if (rows_meet(k_out, es * out_stride, es * row, v_out, es * out_stride, es * row, t)) return OOMB_E_ARG;
     if (batch == 0 || t == 0) return OOMB_OK;
     const DeviceState* d = device_state();
     if (!d) return OOMB_E_DEVICE;
@@ -513,12 +537,16 @@ int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_
                           void* out, int64_t out_stride, int heads, int kv_heads, int head_dim, const int32_t* q_start,
                           int batch, int t, int max_q, float scale, void* workspace, size_t workspace_bytes,
                           oomb_stream stream) {
-    if (!k || !v || !q_start || !workspace || out == k || out == v) return OOMB_E_ARG;
+    if (!k || !v || !q_start || !workspace) return OOMB_E_ARG;
     int st = check_attn(q, q_stride, out, out_stride, heads, kv_heads, head_dim, batch, t, max_q, scale);
     const int64_t row = static_cast<int64_t>(kv_heads) * head_dim;
     if (st == OOMB_OK) st = check_rows(k, k_stride, row, OOMB_BF16);
     if (st == OOMB_OK) st = check_rows(v, v_stride, row, OOMB_BF16);
     if (st != OOMB_OK) return st;
+    const int64_t out_row = static_cast<int64_t>(heads) * head_dim;
+    if (rows_meet(k, 2 * k_stride, 2 * row, out, 2 * out_stride, 2 * out_row, t) ||
+        rows_meet(v, 2 * v_stride, 2 * row, out, 2 * out_stride, 2 * out_row, t))
+        return OOMB_E_ARG;
     if (reinterpret_cast<uintptr_t>(workspace) & 31u) return OOMB_E_ALIGN;
     if (batch == 0 || t == 0 || max_q == 0) return OOMB_OK;
     const DeviceState* d = device_state();

@@ -291,7 +291,7 @@ typedef struct {
 int oomb_rope_turns(int rot_dim, double base, int scaling, double factor, int64_t original_len, uint64_t* turns,
                     float* mscale);
 /* out[t][h][:] = rotated x[t][h][:] at positions[t] (device int32 [t], any sign), x and out [t][heads][head_dim] of x_dtype
- * with token strides in elements; out may be x.  head_dim 64 or 128. */
+ * with token strides in elements; out is x, with its stride, or shares no memory with it.  head_dim 64 or 128. */
 int oomb_rope_rows(const oomb_rope* rope, const void* x, int x_dtype, int64_t x_stride, const int32_t* positions, void* out,
                    int64_t out_stride, int t, int heads, int head_dim, oomb_stream stream);
 
@@ -323,7 +323,8 @@ typedef struct {
 } oomb_paged_kv;
 /* Writes a step's keys and values (fp32 or bf16 [t][kv_heads][head_dim], token strides in
  * elements) into their pages, the keys rotated first when `rope` is given; with q, also writes the step's
- * rotated queries [t][heads][head_dim] to q_out in bf16 (q_out may be q when that is bf16).
+ * rotated queries [t][heads][head_dim] to q_out in bf16 (which is q, with its stride, if that is bf16, or shares no memory with
+ * q, and none with k and v).
  * An e4m3 row takes the least e with amax * r <= 448 * 2^e over its finite values before rotation
  * (r = sqrt(2) * mscale for rotated keys, else 1), clamped to [-100, 120], its values
  * rounded to nearest even (at e = 120 to 240 * 2^120 at most, the largest that an fp32 number holds); infinities and NaN,
@@ -334,14 +335,14 @@ int oomb_kv_append_paged(const oomb_paged_kv* cache, const oomb_rope* rope, cons
                          int src_dtype, const int32_t* q_start, const int32_t* kv_len, int batch, int t,
                          oomb_stream stream);
 /* The inverse: k_out, v_out [t][kv_heads][head_dim] (out_dtype, token stride out_stride) get the
- * rows at the packed positions. */
+ * rows at the packed positions; the two share no memory. */
 int oomb_kv_read_paged(const oomb_paged_kv* cache, const int32_t* q_start, const int32_t* kv_len, int batch, int t,
                        void* k_out, void* v_out, int out_dtype, int64_t out_stride, oomb_stream stream);
 /* Causal attention of the packed new tokens over their sequences' pages: q, out bf16
  * [t][heads][head_dim] (token strides in elements), query head h reading kv head h / (heads / kv_heads), at most
  * 64 heads a kv head.  A token at position p sees positions 0 .. p below kv_len (a token that sees none gets zeros);
  * what it does not see never reaches its output, infinities and NaN included.
- * |scale| <= 1e37; out does not overlap q; at most 2^30 blocks of 128 positions over all sequences at max_pages, kv heads and
+ * |scale| <= 1e37; out shares no memory with q (rows side by side in wider rows of one stride do not); at most 2^30 blocks of 128 positions over all sequences at max_pages, kv heads and
  * groups of 16 rows where a kv head has 64 rows or fewer.  max_q bounds the tokens of a sequence (a longer one sets the device error word and is left out).  The workspace
  * holds oomb_attention_paged_workspace_bytes(...) bytes (0: unsupported shape, or no device), enough for every call of at
  * most this batch, t and max_q with these heads and a cache of this shape (for long chunks over an e4m3 cache it holds a bf16
@@ -354,7 +355,7 @@ int oomb_attention_paged(const oomb_paged_kv* cache, const void* q, int64_t q_st
                          int heads, const int32_t* q_start, const int32_t* kv_len, int batch, int t, int max_q, float scale,
                          void* workspace, size_t workspace_bytes, oomb_stream stream);
 /* The same over whole prompts whose keys and values are rows of the step itself, bf16
- * [t][kv_heads][head_dim] packed as q (out overlaps none of the three): token i of a sequence sees its tokens 0 .. i. */
+ * [t][kv_heads][head_dim] packed as q (out shares memory with none of the three): token i of a sequence sees its tokens 0 .. i. */
 size_t oomb_attention_prompt_workspace_bytes(int batch, int t, int max_q, int heads, int kv_heads, int head_dim);
 int oomb_attention_prompt(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                           void* out, int64_t out_stride, int heads, int kv_heads, int head_dim, const int32_t* q_start,

@@ -127,3 +127,76 @@ def test_kept_workspaces_are_zero_again_after_a_device_error(host):
     assert g.device_error() == 0
     attend(g)
     assert counters(g).data_ptr() == kept.data_ptr(), "without an error nothing is made anew"
+
+
+# ---- operands that share memory: refused before any launch ----------------------------------
+
+HERE = 1 << 20  # an address that is never followed
+
+
+@pytest.mark.parametrize("x,sx,y,sy,t,meet", [
+    (0, 512, 3 * 1024, 512, 3, False),      # one behind the other (bytes apart; strides in elements of 2 bytes)
+    (0, 512, 3 * 1024 - 16, 512, 3, True),
+    (0, 512, 1024, 512, 3, True),           # shifted by a token
+    (0, 512, -2 * 1024, 512, 3, True),
+    (0, 512, -3 * 1024, 512, 3, False),
+    (0, 512, 16, 512, 3, True),
+    (0, 1024, 1024, 1024, 3, False),        # side by side in rows of 2,048 bytes
+    (0, 1024, 1024 - 16, 1024, 3, True),
+    (1024, 1024, 0, 1024, 3, False),
+    (1024, 1024, 2 * 2048, 1024, 3, False),
+    (1024, 1024, 2 * 2048 + 16, 1024, 3, True),
+    (0, 512, 1024, 1024, 1, False),         # a single row has no stride
+    (0, 512, 1024 - 16, 1024, 1, True),
+    (0, 512, 2048, 1024, 4, True),          # unlike strides in one stretch
+    (0, 512, 0, 512, 0, False),
+])
+def test_operands_that_share_memory_are_refused(x, sx, y, sy, t, meet):
+    """Rows of 8 heads of 64 bf16 values, 1,024 bytes."""
+    import ctypes as C
+
+    from homelab_b200 import _lib
+    L = _lib.lib()
+    far = HERE + (1 << 24)
+    X, Y = HERE + x, HERE + y
+    passes = (0,) if t == 0 else (_lib.E_DEVICE,)  # all checks passed: nothing to do, or no device here
+    if torch.cuda.is_available():
+        pytest.skip("calls that pass their checks would launch")
+    want = (_lib.E_ARG,) if meet else passes
+    rope = C.byref(_lib.RopeStruct(rot_dim=64, interleaved=0, mscale=1.0, turns=far))
+    cache = C.byref(_lib.PagedKvStruct(dtype=0, kv_heads=8, head_dim=64, page_size=16, num_pages=10, max_pages=4, table_stride=4,
+                                       k=far, v=far, page_stride=8 * 16 * 64, block_table=far))
+    assert L.oomb_rope_rows(rope, X, 1, sx, far, Y, sy, t, 8, 64, None) in want
+    B = t
+    assert L.oomb_attention_paged(cache, X, sx, Y, sy, 8, None, far, B, t, 1, 0.1, far, 1 << 40, None) in want
+    # queries, keys or values of a prompt under its output
+    for a in range(3):
+        rows = [(far + (1 << 22) * i, 512) for i in range(3)]
+        rows[a] = (X, sx)
+        (q, qs), (k, ks), (v, vs) = rows
+        assert L.oomb_attention_prompt(q, qs, k, ks, v, vs, Y, sy, 8, 8, 64, far, 1, t, 1, 0.1, far, 1 << 40, None) in want, a
+        assert L.oomb_kv_append_paged(cache, rope, q, qs, Y, sy, 8, k, ks, v, vs, 1, None, far, B, t, None) in want, a
+    if sx == sy:
+        assert L.oomb_kv_read_paged(cache, None, far, B, t, X, Y, 1, sx, None) in want
+
+
+def test_operations_in_place():
+    import ctypes as C
+
+    from homelab_b200 import _lib
+    if torch.cuda.is_available():
+        pytest.skip("calls that pass their checks would launch")
+    L = _lib.lib()
+    far = HERE + (1 << 24)
+    rope = C.byref(_lib.RopeStruct(rot_dim=64, interleaved=0, mscale=1.0, turns=far))
+    cache = C.byref(_lib.PagedKvStruct(dtype=0, kv_heads=8, head_dim=64, page_size=16, num_pages=10, max_pages=4, table_stride=4,
+                                       k=far, v=far, page_stride=8 * 16 * 64, block_table=far))
+    assert L.oomb_rope_rows(rope, HERE, 0, 512, far, HERE, 512, 3, 8, 64, None) == _lib.E_DEVICE
+    assert L.oomb_rope_rows(rope, HERE, 0, 512, far, HERE, 520, 3, 8, 64, None) == _lib.E_ARG  # the same rows, another stride
+    append = lambda dt, qs, qos, qo: L.oomb_kv_append_paged(  # noqa: E731
+        cache, rope, HERE, qs, qo, qos, 8, HERE + 1024, 1536, HERE + 2048, 1536, dt, None, far, 3, 3, None)
+    assert append(1, 1536, 1536, HERE) == _lib.E_DEVICE   # the queries of a fused projection's rows, in place
+    assert append(1, 1536, 1544, HERE) == _lib.E_ARG
+    assert append(1, 1536, 1536, HERE + 1024) == _lib.E_ARG  # over the keys
+    assert L.oomb_kv_append_paged(cache, rope, HERE, 1536, HERE, 3072, 8, HERE + 2048, 1536, HERE + 4096, 1536, 0, None, far, 3, 3,
+                                  None) == _lib.E_ARG     # fp32 rows are not written over in bf16
