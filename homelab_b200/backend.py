@@ -10,6 +10,7 @@ current torch stream; nothing synchronises the host.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 import weakref
 
 import torch
@@ -79,6 +80,7 @@ class Gpu:
         self._tiled_ws = None  # grown on demand by moe_tiled calls without a workspace
         # paged and prompt attention without a workspace: one per stream, grown on demand, and the shapes known to fit it
         self._attn_ws = {}
+        self._attn_lock = threading.Lock()  # a call's launches over a kept workspace stay together on their stream
         _gpus.add(self)
 
     def _stream(self) -> int:
@@ -417,6 +419,16 @@ class Gpu:
             self._attn_ws[key] = ws
         return ws
 
+    def _attend(self, workspace, cache, shape, fn, what: str, *args):
+        """fn(*args, workspace, its bytes, stream) over the caller's workspace, or over one that this object keeps: then one
+        thread's launches at a time, since threads may share a stream and with it the workspace."""
+        if workspace is not None:
+            ws = self._ws(workspace)
+            return self._launch(fn, what, *args, ws.data_ptr(), ws.numel())
+        with self._attn_lock:
+            ws = self._attention_ws(cache, shape)
+            return self._launch(fn, what, *args, ws.data_ptr(), ws.numel())
+
     def attention_paged(self, q, cache: PagedKv, out, q_start, kv_len, max_q: int, scale: float, workspace=None):
         """Causal attention of the packed new tokens over their sequences' pages (oomb_attention_paged):
         q, out bf16 [T, H, D]; q_start int32 [B + 1] or None (one token a sequence); kv_len int32 [B]
@@ -430,9 +442,8 @@ class Gpu:
         B, qs_p, len_p = self._step(cache, q_start, kv_len, T)
         if T == 0 or B == 0:
             return
-        ws = self._attention_ws(cache, (B, T, max_q, H)) if workspace is None else self._ws(workspace)
-        self._launch(self.L.oomb_attention_paged, "attention_paged", cache.ref, qp, qs, op, os_, H, qs_p, len_p, B, T, max_q,
-                     scale, ws.data_ptr(), ws.numel())
+        self._attend(workspace, cache, (B, T, max_q, H), self.L.oomb_attention_paged, "attention_paged", cache.ref, qp, qs, op,
+                     os_, H, qs_p, len_p, B, T, max_q, scale)
 
     def attention_prompt(self, q, k, v, out, q_start, max_q: int, scale: float, workspace=None):
         """Causal attention over packed whole prompts (oomb_attention_prompt): q, out bf16 [T, H, D],
@@ -449,9 +460,8 @@ class Gpu:
         B = q_start.numel() - 1
         if T == 0 or B <= 0:
             return
-        ws = self._attention_ws(None, (B, T, max_q, H, Hkv, D)) if workspace is None else self._ws(workspace)
-        self._launch(self.L.oomb_attention_prompt, "attention_prompt", qp, qs, kp, ks, vp, vs, op, os_, H, Hkv, D, qs_p, B, T,
-                     max_q, scale, ws.data_ptr(), ws.numel())
+        self._attend(workspace, None, (B, T, max_q, H, Hkv, D), self.L.oomb_attention_prompt, "attention_prompt", qp, qs, kp, ks,
+                     vp, vs, op, os_, H, Hkv, D, qs_p, B, T, max_q, scale)
 
     def device_error(self, clear: bool = True) -> int:
         """The device's error word (0: none).  A wait that ran out leaves counts behind in attention workspaces: after an
@@ -461,7 +471,8 @@ class Gpu:
         if code.value:
             for g in [self, *_gpus]:
                 if g.index == self.index:
-                    g._attn_ws = {}
+                    with g._attn_lock:
+                        g._attn_ws = {}
         return code.value
 
     def set_wait_limit(self, ns: int = 0) -> None:

@@ -1,4 +1,7 @@
 """Handles and workspaces of the paged cache's calls on the host: what they refuse, keep and hand on.  No GPU."""
+import threading
+import time
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -51,6 +54,7 @@ class FakeLibrary:
 
     def __init__(self):
         self.error, self.workspaces, self.waits = 0, [], 0.0
+        self.inside, self.shared = set(), False
 
     def oomb_device_error(self, code, clear):
         code._obj.value = self.error
@@ -66,6 +70,10 @@ class FakeLibrary:
 
     def oomb_attention_paged(self, *args):
         self.workspaces.append(args[12])
+        self.shared |= args[12] in self.inside
+        self.inside.add(args[12])
+        time.sleep(self.waits)  # a call's several launches
+        self.inside.discard(args[12])
         return 0
 
 
@@ -127,6 +135,21 @@ def test_kept_workspaces_are_zero_again_after_a_device_error(host):
     assert g.device_error() == 0
     attend(g)
     assert counters(g).data_ptr() == kept.data_ptr(), "without an error nothing is made anew"
+
+
+def test_threads_on_one_stream_take_turns(host):
+    """Two threads' calls over one kept workspace: the launches of one do not come between those of the other."""
+    lib, make = host
+    g = make()
+    attend(g)
+    lib.waits = 0.005
+    threads = [threading.Thread(target=lambda: [attend(g) for _ in range(5)]) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(lib.workspaces) == 21 and len(set(lib.workspaces)) == 1
+    assert not lib.shared
 
 
 # ---- operands that share memory: refused before any launch ----------------------------------
