@@ -94,10 +94,11 @@ def one_loud_row(L, K, D, spread, seed, where):
 
 
 @pytest.mark.parametrize("spread", [6, 12, 18, 20, 24, 30, 60, 100])
-@pytest.mark.parametrize("L,where", [(90, 3), (1000, 0), (1000, 700), (1000, 999), (9000, 8000)])
-def test_a_visible_large_row_of_little_weight_costs_no_bits(gpu, spread, L, where):
+@pytest.mark.parametrize("L,where,D", [(90, 3, 128), (1000, 0, 128), (1000, 700, 128), (1000, 999, 128), (9000, 8000, 128),
+                                       (1000, 130, 64), (5000, 4999, 64)])
+def test_a_visible_large_row_of_little_weight_costs_no_bits(gpu, spread, L, where, D):
     """One new token: a value row up to 2^100 larger, whose weight is too small to count, leaves the others' weights alone."""
-    K, D = 2, 128
+    K = 2
     q, k, v = one_loud_row(L, K, D, spread, 17, where)
     scale = (spread + 20.0) * math.log(2.0) / float((q[0].float() ** 2).sum(-1).min()) * 4
     check(gpu, q, *quantise(k), *quantise(v), 16, scale, L - 1)
@@ -122,9 +123,10 @@ def test_large_rows_seen_by_some(gpu, n, H, spread):
 @pytest.mark.parametrize("n,H", [(1, 8), (5, 8), (16, 2), (100, 8)])
 @pytest.mark.parametrize("tiny", [1e-3, 1e-4, 1e-5, 1e-12])
 @pytest.mark.parametrize("zeros", [[0], [7, 130, 131, 400], list(range(0, 420, 3))])
-def test_rows_of_zeros_among_small_values(gpu, n, H, tiny, zeros):
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_of_zeros_among_small_values(gpu, n, H, tiny, zeros, D):
     """A row of zeros is written with exponent 0, far above the exponents of small values: it must not cost them bits."""
-    K, D, a = 2, 128, 420
+    K, a = 2, 420
     L = a + n
     q = normal(41, n, H, D).to(torch.bfloat16)
     k, v = normal(42, L, K, D), normal(43, L, K, D) * tiny
@@ -265,3 +267,45 @@ def test_the_largest_finite_values_come_back_finite(gpu, src, rotated):
             e = cache.v_exp[1, 0, 0].double() - 127
             bound = torch.maximum(2.0 ** -4 * want.abs(), torch.exp2(e - 10))
             assert ((got - want).abs() <= bound)[finite].all(), j
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 1, 3]])
+@pytest.mark.parametrize("repeat", [False, True])
+def test_a_batch_of_unlike_caches_repeats_its_bits(gpu, new, repeat):
+    """Sequences whose exponents lie close and far apart, side by side: right, and the same bits every time."""
+    K, D, page = 2, 128, 16
+    lens = [700, 130, 2500]
+    rows = []
+    for b, (n, L) in enumerate(zip(new, lens)):
+        v = normal(112 + b, L, K, D)
+        if b != 1:
+            v[::7] *= 2.0 ** 25
+            v[::5] = 0.0
+        rows.append((*quantise(normal(110 + b, L, K, D)), *quantise(v)))
+    caches = [paged(*r, page) for r in rows]
+    pools = [torch.cat([getattr(c, name) for c in caches]) for name in ("k_pages", "v_pages", "k_exp", "v_exp")]
+    width, at = max(c.max_pages for c in caches), 0
+    table = torch.zeros(3, width, dtype=torch.int32, device=DEV)
+    for b, c in enumerate(caches):
+        table[b, :c.max_pages] = c.block_table[0] + at
+        at += c.k_pages.shape[0]
+    cache = PagedKv(pools[0], pools[1], table, pools[2], pools[3])
+    q = normal(119, sum(new), 8, D).to(torch.bfloat16)
+    q_start, at = [0], 0
+    for n in new:
+        q_start.append(q_start[-1] + n)
+    out = torch.empty(sum(new), 8, D, dtype=torch.bfloat16, device=DEV)
+    gpu.attention_paged(q.to(DEV), cache, out, i32(q_start), i32(lens), max(new), 0.09)
+    for b, (n, L) in enumerate(zip(new, lens)):
+        s = slice(q_start[b], q_start[b + 1])
+        k, v = stands_for(*rows[b][:2]), stands_for(*rows[b][2:])
+        want, mag, big = R.attend(q[s].double(), k, v, L - n, 0.09)
+        _, least, _ = R.attend(q[s].double(), k, v.abs().amax(-1, keepdim=True).expand_as(v), L - n, 0.09)
+        err = (out[s].cpu().double() - want).abs()
+        bound = R.attention_bound(want, mag, big, D) + L * 2.0 ** -22 * least
+        assert (err <= bound).all(), (b, float((err / bound).max()))
+    if repeat:
+        for _ in range(20):
+            again = torch.empty_like(out)
+            gpu.attention_paged(q.to(DEV), cache, again, i32(q_start), i32(lens), max(new), 0.09)
+            assert torch.equal(again, out)
