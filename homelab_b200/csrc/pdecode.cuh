@@ -74,7 +74,9 @@ struct DecodeGeo {
     static constexpr int CHUNK = ROW < 128 ? ROW : 128;         // bytes of a swizzled row
     static constexpr int CH = ROW / CHUNK;
     static constexpr int TILE = kDecBlock * ROW;
-    static constexpr int QT = F8 ? 2 : 1, PT = F8 ? 3 : 1;      // terms of a query and of a weight
+    // terms of a query and of a weight: a product takes 16 columns whatever their number, so bf16 weights of up to 8 rows are two
+    // bf16 terms (off by 2^-15) for nothing; with 16 rows the second would take the third tile's room, and they are one (2^-8)
+    static constexpr int QT = F8 ? 2 : 1, PT = F8 ? 3 : R <= 8 ? 2 : 1;
     static constexpr int NQ = (R * QT + 15) / 16 * 16, NP = (R * PT + 15) / 16 * 16;
     static constexpr int Q_BYTES = (CH * NQ * CHUNK + 1023) / 1024 * 1024;
     static constexpr int P_STEP = (NP * kDecBlock * (F8 ? 1 : 2) + 1023) / 1024 * 1024;
@@ -752,11 +754,21 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                             pw[dec_swizzle(128, n0 + 1, tid / 16) + tid % 16] = static_cast<uint8_t>(c >> 8);
                         }
                     } else {
-                        const unsigned c = pack_bf16(a, b);  // weights in 8 bits' mantissa, as the tensor cores take bf16
                         uint8_t* at = pw + (tid / 64) * Geo::NP * 128;
                         const int k = tid % 64;
-                        *reinterpret_cast<uint16_t*>(at + dec_swizzle(128, r, k / 8) + (k % 8) * 2) = static_cast<uint16_t>(c);
-                        *reinterpret_cast<uint16_t*>(at + dec_swizzle(128, r + 1, k / 8) + (k % 8) * 2) = static_cast<uint16_t>(c >> 16);
+                        auto put = [&](int n, unsigned c) {
+                            *reinterpret_cast<uint16_t*>(at + dec_swizzle(128, n, k / 8) + (k % 8) * 2) = static_cast<uint16_t>(c);
+                            *reinterpret_cast<uint16_t*>(at + dec_swizzle(128, n + 1, k / 8) + (k % 8) * 2) = static_cast<uint16_t>(c >> 16);
+                        };
+                        if constexpr (Geo::PT == 1) {
+                            put(r, pack_bf16(a, b));
+                        } else {
+                            // the first term is cut off and the second a little larger than what is left: neither is zero or of
+                            // the other sign, so that an infinite value stays one
+                            const unsigned ha = __float_as_uint(a) & 0xffff0000u, hb = __float_as_uint(b) & 0xffff0000u;
+                            put(r, ha >> 16 | hb);
+                            put(R + r, pack_bf16(fmaf(a, 0x1p-20f, a - __uint_as_float(ha)), fmaf(b, 0x1p-20f, b - __uint_as_float(hb))));
+                        }
                     }
                 }
                 fence_async_smem();
@@ -807,6 +819,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 if (r >= rows) continue;
                 float ls = bar->red[0][r] + bar->red[1][r] + bar->red[2][r] + bar->red[3][r];
                 float x = o[r];
+                if constexpr (!F8 && Geo::PT == 2) x += o[R + r];
                 if constexpr (F8) x = (o[r] + o[R + r] + o[2 * R + r]) * power_of(-kDecUnit) * exp_byte(static_cast<unsigned>(X));
                 if (parts == 1) {
                     x = vis[r] > 0 ? x / ls : 0.0f;

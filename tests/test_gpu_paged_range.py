@@ -309,3 +309,31 @@ def test_a_batch_of_unlike_caches_repeats_its_bits(gpu, new, repeat):
             again = torch.empty_like(out)
             gpu.attention_paged(q.to(DEV), cache, again, i32(q_start), i32(lens), max(new), 0.09)
             assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("n,H", [(1, 8), (1, 16), (2, 8), (1, 2), (3, 4)])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("L,D", [(33, 128), (700, 128), (5000, 128), (400, 64)])
+def test_few_rows_are_rounded_once(gpu, n, H, fp8, L, D):
+    """Up to 8 query rows a kv head: the weights keep 15 bits (9 over e4m3 pages), so that over bf16 pages an output is the
+    formula's, rounded once: 2^-8 of it; and of the magnitudes 2^-15 for the weights' terms (the first is cut off, so that the
+    second is 2^-7 of the weight at most and off by 2^-8 of that), 2^-20 for what is added to the second, 2^-18 for exponentials
+    and sums."""
+    K, a = 2, L - n
+    q = normal(131, n, H, D).to(torch.bfloat16)
+    k, v = normal(132, L, K, D), normal(133, L, K, D)
+    if fp8:
+        check(gpu, q, *quantise(k), *quantise(v), 16, 0.09, a)
+        return
+    k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+    pages = -(-L // 16)
+    pool = torch.full((2, pages * 16, K, D), float("nan"), dtype=torch.bfloat16)
+    pool[0, :L], pool[1, :L] = k, v
+    pool = pool.unflatten(1, (pages, 16)).transpose(2, 3).contiguous().to(DEV)
+    cache = PagedKv(pool[0], pool[1], torch.arange(pages, dtype=torch.int32, device=DEV)[None])
+    out = torch.empty(n, H, D, dtype=torch.bfloat16, device=DEV)
+    gpu.attention_paged(q.to(DEV), cache, out, i32([0, n]), i32([L]), n, 0.09)
+    want, mag, big = R.attend(q.double(), k.double(), v.double(), a, 0.09)
+    err = (out.cpu().double() - want).abs()
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -15 + 2.0 ** -20 + 2.0 ** -18 + 4 * D * 2.0 ** -24 * big) * mag + 1e-30
+    assert (err <= bound).all(), float((err / bound).max())
