@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     kf = exp_byte(ep[tid]);
                     if (tok < g.tok1) {
                         ve = ep[kDecBlock + tid];
-                        low = min(low, ve);
+                        if (ve) low = min(low, ve);  // 0: a bad table entry's zeros
                     }
                 }
                 // (2^(e - X + 30) is to stay an fp32 number)
