@@ -687,14 +687,11 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
         unsigned s_ph = 0, o_ph = 0;
         bool ok = true;
         // a scale below zero turns the scores' sign, and one of zero makes them zero (before the mask: 0 * -inf is NaN)
-        const float turn = p.scale_log2 > 0.0f ? 1.0f : p.scale_log2 < 0.0f ? -1.0f : 0.0f;
-        const float scale = turn == 0.0f ? 1.0f : fabsf(p.scale_log2);
-        const int token_of = row / p.G, head_of = row - token_of * p.G;
-        const bool row_in = token_of < tq;
-        const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | (static_cast<uintptr_t>(p.out_stride) * 2)) & 31u) == 0;
+        const float scale = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
         for (FaWork w; ok && take(w);) {
+            const int token_of = row / p.G, head_of = row - token_of * p.G;
             const int token = w.i0 + h * tq + token_of;
-            const bool valid = row_in && token < w.s.n;
+            const bool valid = token_of < tq && token < w.s.n;
             const int vis = valid ? max(0, min(w.s.len, w.s.len - w.s.n + token + 1)) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < w.nh[h]; i++) {
@@ -707,7 +704,8 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 tc_wait_ld();
                 // rows that are no query's (and the next sequence's) are not masked: nobody reads them
                 const int lim = valid ? vis - (w.kv0 + i) * kFaTile : kFaTile;
-                if (turn != 1.0f) {
+                if (!(p.scale_log2 > 0.0f)) {
+                    const float turn = p.scale_log2 < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
                     for (int c = 0; c < 128; c++) s[c] *= turn;
                 }
@@ -782,6 +780,7 @@ __global__ void __launch_bounds__(FaGeo<KIND, D>::THREADS, 1)
                 o_ph ^= 1;
                 tc_fence_after();
             }
+            const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | (static_cast<uintptr_t>(p.out_stride) * 2)) & 31u) == 0;
             const float inv = w.slot >= 0 ? 1.0f : vis > 0 ? 1.0f / l : 0.0f;
             const int head = w.kvh * p.G + head_of;
             uint16_t* out = p.out + static_cast<int64_t>(w.s.q0 + token) * p.out_stride + static_cast<int64_t>(head) * D;
