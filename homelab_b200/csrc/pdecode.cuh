@@ -107,6 +107,7 @@ struct DecodeBars {
     uint32_t tmem;
     unsigned beat;  // moves while rows are done again
     float red[4][kDecRows], redt[4][kDecRows];
+    float scale[kDecRows];    // e4m3: a row's scale, its power of two in it
     float n[kDecRows], top[kDecRows], fl[kDecRows], fo[kDecRows];  // a row's reference, largest score, and factors of a change
     int redx[4], redn[4], redv[4];
     unsigned last;
@@ -526,13 +527,12 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         while (!stop && walk.next(p, g)) {
             const Seq sq = g.sq;
             const int rows = g.rows, row0 = g.row0;
-            float m[R], l[R], scale[R];
+            float m[R], l[R];
             int vis[R];
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 m[r] = -INFINITY;
                 l[r] = 0.0f;
-                scale[r] = p.scale_log2;
                 vis[r] = r < rows ? max(0, min(sq.len, sq.len - sq.n + (row0 + r) / p.G + 1)) : 0;
             }
             int X = 0;       // e4m3: the exponent byte that the outputs are counted in
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                         const int ex = max(-126, static_cast<int>(__float_as_uint(big) >> 23) - 127 - 7);  // 2^ex and 2^-ex are fp32 numbers
                         const float up = power_of(-ex);
                         if (r < R) {
-                            if (c == 0) bar->red[0][r] = power_of(ex);
+                            if (c == 0) bar->scale[r] = p.scale_log2 * power_of(ex);
                             // a value that is not finite has no code: its row's scores become NaN
                             const bool bad = !(big <= 3.4e38f);
                             uint8_t* q1 = smem + Geo::Q_OFF;
@@ -599,11 +599,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar->q_ready);
-                if constexpr (F8) {
-                    meet(false);
-#pragma unroll
-                    for (int r = 0; r < R; r++) scale[r] *= bar->red[0][r];
-                }
+                if constexpr (F8) meet(false);  // the rows' scales are there
             }
             for (int i = 0; i < g.tiles; i++, t++) {
                 wait(&bar->s_full[t & 1], (t >> 1) & 1, 6);
@@ -628,7 +624,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 const float top = kSlack + static_cast<float>(X - ve);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    float x = F8 ? fmaf(s[R + r], 1.0f / kRestUp, s[r]) * (scale[r] * kf) : s[r] * scale[r];
+                    float x = F8 ? fmaf(s[R + r], 1.0f / kRestUp, s[r]) * (bar->scale[r] * kf) : s[r] * p.scale_log2;
                     if (tok >= vis[r]) x = -INFINITY;
                     s[r] = x;
                     over |= x > m[r] + top || (m[r] == -INFINITY && x != -INFINITY);
