@@ -56,8 +56,8 @@ constexpr int kDecParts = 16, kDecRun = 8;
 // e4m3.  Weights are made as 2^(x - n + 11 - 30) 2^(e - X + 30), X the largest exponent byte met and n = m - (X - T): the left
 // factor is what the sum of weights adds up, and stays an fp32 number (2^97 a position) while exponents lie within 2^112.  (n
 // is only a reference: what it loses where m is large cancels, but past 2^20 it could no longer hold X - T.)
-// Over 8 kv heads, eight sequences of 4,000 positions and 16 rows take 29.0 us if every run looks twice, 27.0 if only those past
-// 2^6 do; one of 4,096 and 4 rows 12.3 and 11.3.
+// Over 8 kv heads, eight sequences of 4,000 positions and 16 rows take 29.2 us if every run looks twice, 26.8 if only those past
+// 2^6 do; one of 4,096 and 4 rows 12.6 and 11.4.
 constexpr int kDecUnit = 30, kDecSpread = 112, kDecNear = 6;
 constexpr float kRestUp = 32.0f;  // what q - q1 is multiplied by
 constexpr int kZeroByte = 127;  // the exponent that an append gives a row of zeros
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
         while (!stop && walk.next(p, g)) {
             const Seq sq = g.sq;
             const int rows = g.rows, row0 = g.row0;
-            float m[R], l[R];
+            float m[R], l[R], sc[R];  // sc: e4m3, up to 8 rows (16 read it from shared memory, 84 bytes of spills less)
             int vis[R];
 #pragma unroll
             for (int r = 0; r < R; r++) {
@@ -599,7 +599,11 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar->q_ready);
-                if constexpr (F8) meet(false);  // the rows' scales are there
+                if constexpr (F8) {
+                    meet(false);
+#pragma unroll
+                    for (int r = 0; r < R; r++) sc[r] = R <= 8 ? bar->scale[r] : 0.0f;
+                }
             }
             for (int i = 0; i < g.tiles; i++, t++) {
                 wait(&bar->s_full[t & 1], (t >> 1) & 1, 6);
@@ -624,7 +628,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 const float top = kSlack + static_cast<float>(X - ve);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    float x = F8 ? fmaf(s[R + r], 1.0f / kRestUp, s[r]) * (bar->scale[r] * kf) : s[r] * p.scale_log2;
+                    float x = F8 ? fmaf(s[R + r], 1.0f / kRestUp, s[r]) * ((R <= 8 ? sc[r] : bar->scale[r]) * kf) : s[r] * p.scale_log2;
                     if (tok >= vis[r]) x = -INFINITY;
                     s[r] = x;
                     over |= x > m[r] + top || (m[r] == -INFINITY && x != -INFINITY);

@@ -22,7 +22,8 @@
 // P was consumed.  Scores, maxima, exponentials and products of one half still follow one
 // another (tensor memory has no room for second scores beside two outputs of 128 columns), which leaves
 // the tensor pipe active 58 % of the time.  Prompts of 8,192 and 3,001 tokens
-// (32 heads over 8, D = 128) take 522 us, 1,195 TFLOP/s.
+// (32 heads over 8, D = 128) take 515-524 us, 1,190-1,210 TFLOP/s, in short bursts, and 608 us, 1,026, called on end for a
+// second, when the power limit lowers the clock.
 // Tried when this stood at 569 us, and no faster: two threads a row (619 us), scores of 64 positions at a time, made
 // ahead (633 us: the products cost the same at N = 64).
 //
