@@ -343,10 +343,10 @@ int oomb_kv_read_paged(const oomb_paged_kv* cache, const int32_t* q_start, const
  * 64 heads a kv head.  A token at position p sees positions 0 .. p below kv_len (a token that sees none gets zeros);
  * what it does not see never reaches its output, infinities and NaN included.
  * |scale| <= 1e37; out shares no memory with q (rows side by side in wider rows of one stride do not); at most 2^30 blocks of 128 positions over all sequences at max_pages, kv heads and
- * groups of 16 rows where a kv head has 64 rows or fewer.  max_q bounds the tokens of a sequence (a longer one sets the device error word and is left out).  The workspace
+ * groups of 16 rows where a kv head has 64 rows or fewer.  max_q bounds the tokens of a sequence (a longer one sets the device error word and is left out; 0: nothing is done).  The workspace
  * holds oomb_attention_paged_workspace_bytes(...) bytes (0: unsupported shape, or no device), enough for every call of at
  * most this batch, t and max_q with these heads and a cache of this shape (for long chunks over an e4m3 cache it holds a bf16
- * copy of up to batch * max_pages pages, 1 GiB at most; a call whose copy has no room in it does without one, in other bits
+ * copy of up to batch * max_pages pages, 1 GiB at most; a call whose copy has no room in it, or would pass the limit, does without one, in other last bits
  * and more time); it is 32-byte aligned, and its first OOMB_ATTENTION_ZERO_BYTES are zero before first use
  * (and again after a device error).  Calls that share it must be ordered on one stream. */
 #define OOMB_ATTENTION_ZERO_BYTES 4096
