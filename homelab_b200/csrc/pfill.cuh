@@ -49,9 +49,10 @@ constexpr int kFaRows = 256;       // rows of a tile pair
 // tokens (32 heads over 8, D = 128): one part 610 us, two 569-600, four 601-625 (each hand-over waits for its stores).
 constexpr int kFaParts = 2;
 constexpr int kFaSoft = 8;         // softmax warps
-// Weights are made, and summed, as 2^-16 of what they are: with the 2^8 that a row's maximum may lag behind, no product with a
-// value passes what fp32 holds that the value itself does not.
-constexpr float kFaDown = 16.0f;
+// Weights are made, and summed, as 2^-8 of what they are: with the 2^8 that a row's maximum may lag behind they are one at most,
+// and no product with a value passes what fp32 holds that the value itself does not.  (Those below 2^-118 of the row's largest
+// are zero, where fp32's own range would end at 2^-126.)
+constexpr float kFaDown = 8.0f;
 constexpr int kFaMinPart = 4;      // key tiles of a part at least
 constexpr int kPlanThreads = 256;
 constexpr int kPlanBuckets = 512;

@@ -65,7 +65,8 @@ def check(gpu, q, ck, ke, cv, ve, page, scale, n_before, score_err=0.0):
     """Attention of q's tokens behind n_before positions, within the bound of every row's own magnitudes.  On top comes what
     the three e5m2 terms of a weight leave out: half of their last unit 2^-16 at a largest weighted row of 2^11, so 2^-28 of
     that row (codes up to 448) for each position, and 2^-22 where exponents within 2^6 of one another share one reference.  An
-    error of the scores counts twice, in the weight and in the sum it is divided by."""
+    error of the scores counts twice, in the weight and in the sum it is divided by.  Weights below 2^-118 of a row's largest
+    may be zero: exponentials end at 2^-126 in fp32, and are made 2^-8 lower."""
     n, H, D = q.shape
     L, K, _ = ck.shape
     out = torch.empty(n, H, D, dtype=torch.bfloat16, device=DEV)
@@ -74,6 +75,14 @@ def check(gpu, q, ck, ke, cv, ve, page, scale, n_before, score_err=0.0):
     want, mag, big = R.attend(q.double(), k, v, n_before, scale)
     _, least, _ = R.attend(q.double(), k, v.abs().clamp(max=3.4e38).amax(-1, keepdim=True).expand_as(v), n_before, scale)
     bound = R.attention_bound(want, mag, big, D) + L * 2.0 ** -22 * least
+    for i in range(n):
+        for h in range(H):
+            x = (k[:n_before + i + 1, h // (H // K)] @ q[i, h].double()) * scale
+            gone = x < x.max() - 118.0 * math.log(2.0)
+            if gone.any():
+                p = torch.softmax(x, 0)
+                bound[i, h] += torch.where(gone[:, None] & torch.isfinite(v[:n_before + i + 1, h // (H // K)]),
+                                           p[:, None] * v[:n_before + i + 1, h // (H // K)].abs(), 0.0).sum(0)
     if score_err:
         bound = bound + 2 * score_err * mag
     out = out.cpu().double()
@@ -337,3 +346,22 @@ def test_few_rows_are_rounded_once(gpu, n, H, fp8, L, D):
     err = (out.cpu().double() - want).abs()
     bound = 2.0 ** -8 * want.abs() + (2.0 ** -15 + 2.0 ** -20 + 2.0 ** -18 + 4 * D * 2.0 ** -24 * big) * mag + 1e-30
     assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("n,H", [(1, 8), (4, 8), (16, 2), (70, 8)])
+@pytest.mark.parametrize("L", [100, 900])
+@pytest.mark.parametrize("spread", [40, 90, 105])
+@pytest.mark.parametrize("first", [0, 20, 400])
+@pytest.mark.parametrize("down", [60])
+def test_zeros_that_take_the_weight_beside_a_large_row(gpu, n, H, L, spread, first, down):
+    """Rows of zeros draw all but 2^-down of the weight, from the start or from some position on, and a row 2^spread larger as
+    little of the rest: what is left, 2^-down of the weight each, makes the output, or the large row does."""
+    K, D = 2, 128
+    q = (normal(141, n, H, D) + 2.0).to(torch.bfloat16)  # a direction that all queries share
+    k, v = normal(142, L, K, D) * 0.2, normal(143, L, K, D)
+    k[min(first, L // 2)] = 1.0
+    v[min(first, L // 2)] = 0.0
+    loud = L - n - 1
+    k[loud], v[loud] = -1.0, v[loud] * 2.0 ** spread
+    scale = down * math.log(2.0) / float(q.float().sum(-1).mean())
+    check(gpu, q, *quantise(k), *quantise(v), 16, scale, L - n)
