@@ -81,7 +81,7 @@ struct DecodeGeo {
     static constexpr int Q_BYTES = (CH * NQ * CHUNK + 1023) / 1024 * 1024;
     static constexpr int P_STEP = (NP * kDecBlock * (F8 ? 1 : 2) + 1023) / 1024 * 1024;
     static constexpr int EXPS = 8;                              // tiles whose exponents are kept
-    static constexpr int BARS = 1280;                           // bytes of the barriers and of what the warps tell one another
+    static constexpr int BARS = 1408;                           // bytes of the barriers and of what the warps tell one another
     static constexpr int REST = Q_BYTES + 2 * P_STEP + (F8 ? EXPS * 2 * kDecBlock : 0) + BARS;
     static constexpr int ROOM = 228 * 1024 / kDecCtas - 1024 - REST;
     static constexpr int STAGES = ROOM / TILE < 8 ? ROOM / TILE : 8;
@@ -108,7 +108,7 @@ struct DecodeBars {
     unsigned beat;  // moves while rows are done again
     float red[4][kDecRows], redt[4][kDecRows];
     float scale[kDecRows];    // e4m3: a row's scale, its power of two in it
-    float n[kDecRows], top[kDecRows], fl[kDecRows], fo[kDecRows];  // a row's reference, largest score, and factors of a change
+    float n[kDecRows], top[kDecRows], T[kDecRows], fl[kDecRows], fo[kDecRows];  // a row's reference, largest score, T, and factors of a change
     int redx[4], redn[4], redv[4];
     unsigned last;
     int4 start;               // the CTA's first sequence, its first block, the blocks of its pairs, its groups
@@ -694,10 +694,11 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                             const bool first = was == -INFINITY;
                             float n = mx;
                             if (look) {
-                                float T = over_warps(bar->redt, tid) + (tile - mx);
                                 // (an X that stood for T may have come from rows of zeros: too low a T costs nothing, the outputs are fp32)
-                                T = ceilf(fmaxf(T, first ? -INFINITY : (was - mx) + static_cast<float>(X) - (wide ? 0.0f : 60.0f)));
+                                const float old = first ? -INFINITY : wide ? bar->T[tid] + (bar->top[tid] - mx) : (was - mx) + static_cast<float>(X) - 60.0f;
+                                const float T = ceilf(fmaxf(over_warps(bar->redt, tid) + (tile - mx), old));
                                 n = mx - (static_cast<float>(xn) - fmaxf(T, static_cast<float>(xn - kDecSpread)));
+                                bar->T[tid] = T;
                             }
                             bar->n[tid] = n;
                             bar->top[tid] = mx;
@@ -796,8 +797,9 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                 if (lane == 0) bar->redx[warp] = y ? x - 256 : x;
             }
             meet(false);
-            // Exponents further apart than the weights can follow, scores past what a reference holds beside them, or a reference
-            // raised by a row whose codes do not fill its exponent (an append writes none): every row is done again below.
+            // Exponents, or all that a query row sees and the largest exponent, further apart than the weights can follow, scores past
+            // what a reference holds beside them, or a reference raised by a row whose codes do not fill its exponent (an append
+            // writes none): every row is done again below.
             bool lost = false;
             if constexpr (F8) {
 #pragma unroll
@@ -807,7 +809,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas)
                     thin |= x < 0;
                 }
                 lost = X - low > (thin ? 8 : kDecSpread);
-                for (int r = 0; wide && r < rows; r++) lost |= fabsf(bar->top[r]) > 1048576.0f && bar->top[r] != -INFINITY;
+                for (int r = 0; wide && r < rows; r++)
+                    lost |= bar->top[r] != -INFINITY && (fabsf(bar->top[r]) > 1048576.0f || (X > 0 && bar->T[r] < static_cast<float>(X - kDecSpread - 8)));
                 v_item += 2 * g.tiles;
             }
             const int first = walk.deal.owner(g.pair_first), final_cta = walk.deal.owner(g.pair_end - 1);

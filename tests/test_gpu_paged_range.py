@@ -352,7 +352,7 @@ def test_few_rows_are_rounded_once(gpu, n, H, fp8, L, D):
 @pytest.mark.parametrize("L", [100, 900])
 @pytest.mark.parametrize("spread", [40, 90, 105])
 @pytest.mark.parametrize("first", [0, 20, 400])
-@pytest.mark.parametrize("down", [60])
+@pytest.mark.parametrize("down", [60, 95])
 def test_zeros_that_take_the_weight_beside_a_large_row(gpu, n, H, L, spread, first, down):
     """Rows of zeros draw all but 2^-down of the weight, from the start or from some position on, and a row 2^spread larger as
     little of the rest: what is left, 2^-down of the weight each, makes the output, or the large row does."""
