@@ -412,13 +412,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // 2^x of two values on the FMA units: x = r + f, r the nearest integer, 2^f by a polynomial of degree 4
 // fitted to it on [-1/2, 1/2] (Remez exchange on the relative error: 2.7e-6, an 800th of the weights'
-// rounding to bf16), r added to the exponent.  Below -126 it is 0, as a hidden position's weight has to be; NaN gives a huge
-// value, which the epilogue's check for values that are not finite finds.  -inf < x < 128.
+// rounding to bf16), r added to the exponent.  Below -126 it is 0, as a hidden position's weight has to be, and NaN is NaN
+// (the larger of x and 0 is that, where x is not at least -126).  x < 128.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
-    const bool none_x = x.x < -126.0f, none_y = x.y < -126.0f;
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.0f));
+    const bool in_x = x.x >= -126.0f, in_y = x.y >= -126.0f;
+    float2 out;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(out.x) : "f"(x.x), "f"(0.0f));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(out.y) : "f"(x.y), "f"(0.0f));
     const float2 one = make_float2(1.0f, 1.0f);
     const float2 t = ffma2(x, one, make_float2(kMagic, kMagic));
     const float2 r = ffma2(t, one, make_float2(-kMagic, -kMagic));
@@ -427,8 +428,8 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
     y = ffma2(y, f, make_float2(2.402474433e-01f, 2.402474433e-01f));
     y = ffma2(y, f, make_float2(6.931217909e-01f, 6.931217909e-01f));
     y = ffma2(y, f, make_float2(9.999992847e-01f, 9.999992847e-01f));
-    return make_float2(none_x ? 0.0f : __int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
-                       none_y ? 0.0f : __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+    return make_float2(in_x ? __int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)) : out.x,
+                       in_y ? __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)) : out.y);
 }
 
 // As mbar_wait, but the clock and the limit (a load from global memory, some 600 cycles) are read only

@@ -183,3 +183,43 @@ def test_sums_of_large_values_stay_in_range(gpu, fp8, n, rising):
     want, bound = exact(cache, q, 0, 0, n, 2000, 1 / math.sqrt(128))
     err = (got.double() - want).abs()
     assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new,cached", [([1, 2], [300, 40]), ([5, 3], [300, 2]), ([200, 9], [77, 300]), ([70, 40], [1000, 5])])
+@pytest.mark.parametrize("at", list(range(0, 32, 3)) + [129])
+def test_a_key_that_is_not_finite_makes_its_rows_nan(gpu, fp8, new, cached, at):
+    """At any position of a tile, with no value beside it that is not finite: every row of its kv head that sees it is NaN, the
+    other kv head's and the other sequence's rows are as ever."""
+    call, cache, _ = step(gpu, new, cached, fp8, seed=9)
+    want = call().clone()
+    page, slot = int(cache.block_table[0, at // cache.page_size]), at % cache.page_size
+    for bad in ((0x7f,) if fp8 else (float("nan"), float("inf"))):
+        k = cache.k_pages.view(torch.uint8) if fp8 else cache.k_pages
+        keep = k[page, 1, slot, 5].clone()
+        k[page, 1, slot, 5] = bad
+        got = call().clone()
+        k[page, 1, slot, 5] = keep
+        n, first = new[0], max(0, at - cached[0])  # the first new token that sees it
+        assert torch.equal(got[n:], want[n:]) and torch.equal(got[:n, :4], want[:n, :4])
+        assert torch.equal(got[:min(first, n), 4:], want[:min(first, n), 4:])
+        rows = got[first:n, 4:]
+        if bad == float("inf"):  # a score of +inf makes NaN, one of -inf no weight
+            q = step(gpu, new, cached, fp8, seed=9)[2][first:n, 4:, 5]
+            up = q > 0
+            assert torch.isnan(rows[up]).all() and torch.isfinite(rows[q < 0].float()).all()
+        else:
+            assert torch.isnan(rows).all()
+
+
+@pytest.mark.parametrize("at", list(range(0, 32, 3)) + [129])
+def test_a_key_of_a_prompt_that_is_not_finite(gpu, at):
+    H, K, D, n = 8, 2, 128, 200
+    g = torch.Generator(device=DEV).manual_seed(11)
+    q, k, v = (torch.randn(n + 30, h, D, generator=g, device=DEV).to(torch.bfloat16) for h in (H, K, K))
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    gpu.attention_prompt(q, k, v, want, i32([0, n, n + 30]), n, 0.09)
+    k[at, 1, 7] = float("nan")
+    gpu.attention_prompt(q, k, v, got, i32([0, n, n + 30]), n, 0.09)
+    assert torch.isnan(got[at:n, 4:]).all()
+    assert torch.equal(got[:, :4], want[:, :4]) and torch.equal(got[:at], want[:at]) and torch.equal(got[n:], want[n:])
