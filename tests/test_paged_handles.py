@@ -221,5 +221,5 @@ def test_operations_in_place():
     assert append(1, 1536, 1536, HERE) == _lib.E_DEVICE   # the queries of a fused projection's rows, in place
     assert append(1, 1536, 1544, HERE) == _lib.E_ARG
     assert append(1, 1536, 1536, HERE + 1024) == _lib.E_ARG  # over the keys
-    assert L.oomb_kv_append_paged(cache, rope, HERE, 1536, HERE, 3072, 8, HERE + 2048, 1536, HERE + 4096, 1536, 0, None, far, 3, 3,
+    assert L.oomb_kv_append_paged(cache, rope, HERE, 1536, HERE, 3080, 8, HERE + 2048, 1536, HERE + 4096, 1536, 0, None, far, 3, 3,
                                   None) == _lib.E_ARG     # fp32 rows are not written over in bf16
